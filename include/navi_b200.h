@@ -363,6 +363,128 @@ typedef struct navi_conv_args {
 } navi_conv_args;
 int navi_conv1d(navi_device * dev, const navi_conv_args * a);
 
+/* ---- paged KV cache and drafted trees (no counterpart in the reference, which keeps one
+ *      contiguous cache per stream, talker.h:20-24, and decodes one row per step) ----
+ * One pool of pages holds the keys and values of many requests. A page is page_size tokens of
+ * one layer's K or V, laid out [n_kv_head][page_size][head_dim]; the same page ids serve every
+ * layer. Row r of the block table lists the pages of request r in order; pages no request
+ * holds lie on a stack. A step adds n_new[i] rows to each of its requests: one decoded token, a
+ * tree of drafted tokens (each row names its parent row) or a chunk of a prompt (a chain).
+ *
+ *   navi_pages_plan     pages for the step's rows, and each row's request, position, slot and ancestors
+ *   navi_pages_store    q/k RMSNorm and RoPE of the rows, K and V into their slots      (per layer)
+ *   navi_pages_attend   attention of the rows over their request's tokens and ancestors (per layer)
+ *   navi_pages_commit   the branch that agrees with the model's choices, its K/V moved to the front
+ *
+ * Every call only enqueues work on `stream` (a cudaStream_t, as everywhere in CUDA NULL is the
+ * legacy default stream; navi_device_stream gives the engine's) and returns. A device's first
+ * plan or attend on each stream takes that stream's scratch (make it before capturing the
+ * stream); nothing else allocates. The calls of one cache are ordered by the caller: on one
+ * stream, or by events between streams. */
+#define NAVI_PAGES_MAX_LAYERS 128
+enum { NAVI_F32 = 0, NAVI_F16 = 1, NAVI_BF16 = 2 };   /* the .navi type codes */
+#define NAVI_PAGES_MAX_REQUESTS 8192
+#define NAVI_STEP_MAX_TREE 256                         /* most nodes of one request's tree */
+
+typedef struct navi_pages navi_pages;
+
+typedef struct navi_pages_desc {
+    int n_layer, n_pages;
+    int page_size;                 /* tokens: 16, 32, 64 or 128 */
+    int n_kv_head;
+    int head_dim;                  /* 64 or 128 */
+    int dtype;                     /* of the cache: NAVI_F16 or NAVI_BF16 */
+    int max_requests, max_blocks;  /* the block table's rows (<= NAVI_PAGES_MAX_REQUESTS) and columns */
+    void ** k, ** v;               /* host arrays of n_layer device pools [n_pages][n_kv_head][page_size][head_dim],
+                                      16-byte aligned; both NULL: the library allocates them (zeroed) */
+    int32_t * table;               /* device [max_requests][max_blocks] */
+    int32_t * held;                /* device [max_requests]: pages that each request holds */
+    int32_t * free_pages;          /* device [n_pages]: the stack of free pages, its top at n_free - 1 */
+    int32_t * n_free;              /* device [1] */
+                                   /* all four NULL: the library allocates them, every page free, page 0 on top */
+} navi_pages_desc;
+
+int navi_pages_create(navi_device * dev, const navi_pages_desc * desc, navi_pages ** out);
+/* The cache's shape and the pointers it uses (its own or the caller's). */
+int navi_pages_get(const navi_pages * p, navi_pages_desc * out);
+void navi_pages_destroy(navi_pages * p);
+
+typedef struct navi_step {
+    int n_req;                     /* requests of the step, 0..max_requests */
+    int max_rows;                  /* room of the row arrays; the rows of the step may be fewer */
+    int max_new;                   /* no request has more new rows (NAVI_STEP_MAX_TREE with parent) */
+    int mask_words;                /* with parent: 64-bit words of a row of mask, 64 * mask_words >= max_new */
+    const int32_t * req;           /* device [n_req]: the table row of each, all different; NULL: i */
+    const int32_t * ctx_len;       /* device [n_req]: tokens cached before the step */
+    const int32_t * n_new;         /* device [n_req]: rows added; 0 is allowed */
+    const int32_t * parent;        /* device [max_rows]: each row's parent among its request's rows, below its own
+                                      number, or -1 (the last cached token); NULL: row j follows row j - 1 */
+    /* written by navi_pages_plan (device), read by the other calls */
+    int32_t * cu_rows;             /* [n_req + 1]: first row of each request */
+    int32_t * row_req;             /* [max_rows]: index 0..n_req-1 of the row's request */
+    int32_t * pos;                 /* [max_rows]: ctx_len + depth, the RoPE position */
+    int64_t * slot;                /* [max_rows]: page * page_size + offset where the row's K/V go, -1: nowhere */
+    uint64_t * mask;               /* [max_rows][mask_words]: bit a = row a of the request is the row itself or an ancestor */
+    int32_t * status;              /* [n_req]: NAVI_OK, or why the request is not served:
+                                      NAVI_E_KV_FULL  too few free pages: it waits, and with it every later request that needs pages
+                                      NAVI_E_SHAPE    longer than the block table, max_new or max_rows allow
+                                      NAVI_E_ARG      a negative length, a table row out of range, a parent not below its row */
+} navi_step;
+
+/* Makes each request hold ceil((ctx_len + n_new) / page_size) pages. Pages above that go back on
+ * the stack (n_new = 0 after a drafted step gives back what the drafts took, ctx_len = 0 frees a
+ * request), the first request's first page on top; then requests take pages from the top in their
+ * order, so that a step that grows and one that undoes it leave the stack as it was. A request
+ * that is not served keeps its pages, and its rows get slot -1. */
+int navi_pages_plan(navi_pages * p, const navi_step * s, void * stream);
+
+typedef struct navi_store_args {
+    const void * qkv;              /* device rows [n_head q heads | n_kv_head k heads | n_kv_head v heads] x head_dim */
+    int64_t qkv_stride;            /* elements between rows; 0: dense */
+    void * q_out;                  /* device rows [n_head][head_dim]; may be the q part of qkv; NULL with n_head 0 */
+    int64_t q_out_stride;          /* 0: dense */
+    int dtype;                     /* of qkv and q_out: NAVI_F32, or the cache's own */
+    int n_head;                    /* q heads in a row, 0 for rows of K and V alone */
+    const float * q_norm, * k_norm;/* device [head_dim]; NULL: no RMSNorm */
+    float eps;
+    const float * rope;            /* device [rope_positions][head_dim]: cos[head_dim / 2], sin[head_dim / 2]; NULL: none */
+    int rope_positions;            /* a row at a position outside the table is not stored, its q is 0 */
+} navi_store_args;
+/* q and k: x * rsqrt(mean(x^2) + eps) * weight, then RoPE of the pairs (i, i + head_dim / 2) at
+ * pos; v as it is; K and V rounded once to the cache's type (NAVI_F32 rows need an f16 cache). */
+int navi_pages_store(navi_pages * p, const navi_step * s, int layer, const navi_store_args * a, void * stream);
+
+typedef struct navi_attend_args {
+    const void * q;                /* device rows [n_head][head_dim] */
+    int64_t q_stride;              /* elements between rows; 0: dense */
+    void * out;                    /* device rows [n_head][head_dim], not overlapping q */
+    int64_t out_stride;            /* 0: dense */
+    float * lse;                   /* device [max_rows][n_head]: log of the softmax sum; NULL: not wanted */
+    int dtype;                     /* of q and out: NAVI_F32 (f16 cache only), or the cache's own */
+    int n_head;                    /* a multiple of n_kv_head */
+    float scale;                   /* of q k, > 0 */
+} navi_attend_args;
+/* out = softmax(scale q k) v over the request's ctx_len cached tokens and, of the step's rows, those in
+ * the row's mask (parent) or up to the row itself (no parent). q head h reads KV head
+ * h / (n_head / n_kv_head). A row that sees no key, and every row of a request that is not
+ * served, gets out 0 and lse -inf. */
+int navi_pages_attend(navi_pages * p, const navi_step * s, int layer, const navi_attend_args * a, void * stream);
+
+typedef struct navi_commit_args {
+    int width;                     /* ids of one node (16 codes of a frame; 1 for plain tokens) */
+    const int32_t * tokens;        /* device [max_rows][width]: what each row was drafted as */
+    const int32_t * targets;       /* device [max_rows][width]: what the model chose after each row */
+    const int32_t * root_target;   /* device [n_req][width]: what it chose after the last cached token */
+    int32_t * accepted;            /* device [n_req]: rows of the branch that agrees */
+    int32_t * path;                /* device [max_rows]: of each request its accepted rows in order, then -1 */
+    int32_t * new_len;             /* device [n_req]: ctx_len + accepted */
+    int32_t * next_token;          /* device [n_req][width]: the model's choice after the branch */
+} navi_commit_args;
+/* From the root down, the lowest-numbered child whose ids equal the model's choice is accepted.
+ * The accepted rows' K and V move to the tokens ctx_len .. new_len - 1 in every layer, in place.
+ * The step needs parent; a request that is not served accepts nothing. */
+int navi_pages_commit(navi_pages * p, const navi_step * s, const navi_commit_args * a, void * stream);
+
 /* Inspection of the last frame (host copies): the talker's post-norm hidden [hidden],
  * its codec logits [talker vocab], and the 15 code-predictor logit rows [15][cp vocab].
  * Any pointer may be NULL. The reference keeps these in its Work buffers (frame.hip:51-70). */

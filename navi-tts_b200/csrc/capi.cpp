@@ -8,6 +8,7 @@
 #include "graph.hpp"
 #include "vocoder.hpp"
 #include "conv_api.hpp"
+#include "pages.hpp"
 
 #include <algorithm>
 #include <cstring>
@@ -32,6 +33,9 @@ struct navi_talker {
 struct navi_graph {
     std::unique_ptr<navi::qwen3tts::Graph> g;
     int hidden = 0;
+};
+struct navi_pages {
+    std::unique_ptr<navi::Pages> p;
 };
 struct navi_vocoder {
     std::unique_ptr<navi::qwen3tts::Vocoder> v;
@@ -735,6 +739,58 @@ int navi_vocoder_set_stage_hook(navi_vocoder * v, navi_stage_fn fn, void * user)
 }
 
 void navi_vocoder_destroy(navi_vocoder * v) { delete v; }
+
+int navi_pages_create(navi_device * dev, const navi_pages_desc * desc, navi_pages ** out) {
+    return guard([&]() -> int {
+        if (!dev || !desc || !out) return set_err(NAVI_E_ARG, "NULL argument");
+        auto p = std::make_unique<navi_pages>();
+        p->p = navi::Pages::create(*dev->dev, *desc);
+        *out = p.release();
+        return NAVI_OK;
+    });
+}
+
+int navi_pages_get(const navi_pages * p, navi_pages_desc * out) {
+    return guard([&]() -> int {
+        if (!p || !out) return set_err(NAVI_E_ARG, "NULL argument");
+        *out = p->p->desc();
+        return NAVI_OK;
+    });
+}
+
+void navi_pages_destroy(navi_pages * p) { delete p; }
+
+int navi_pages_plan(navi_pages * p, const navi_step * s, void * stream) {
+    return guard([&]() -> int {
+        if (!p || !s) return set_err(NAVI_E_ARG, "NULL argument");
+        p->p->plan(*s, static_cast<cudaStream_t>(stream));
+        return NAVI_OK;
+    });
+}
+
+int navi_pages_store(navi_pages * p, const navi_step * s, int layer, const navi_store_args * a, void * stream) {
+    return guard([&]() -> int {
+        if (!p || !s || !a) return set_err(NAVI_E_ARG, "NULL argument");
+        p->p->store(*s, layer, *a, static_cast<cudaStream_t>(stream));
+        return NAVI_OK;
+    });
+}
+
+int navi_pages_attend(navi_pages * p, const navi_step * s, int layer, const navi_attend_args * a, void * stream) {
+    return guard([&]() -> int {
+        if (!p || !s || !a) return set_err(NAVI_E_ARG, "NULL argument");
+        p->p->attend(*s, layer, *a, static_cast<cudaStream_t>(stream));
+        return NAVI_OK;
+    });
+}
+
+int navi_pages_commit(navi_pages * p, const navi_step * s, const navi_commit_args * a, void * stream) {
+    return guard([&]() -> int {
+        if (!p || !s || !a) return set_err(NAVI_E_ARG, "NULL argument");
+        p->p->commit(*s, *a, static_cast<cudaStream_t>(stream));
+        return NAVI_OK;
+    });
+}
 
 int navi_conv1d(navi_device * dev, const navi_conv_args * a) {
     return guard([&]() -> int {

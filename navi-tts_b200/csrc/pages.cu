@@ -1,0 +1,579 @@
+// The paged KV cache: its pools and block tables, and the operators that plan a step, store its
+// rows and commit the accepted branch of a drafted tree (include/navi_b200.h). The attention
+// over the pages is in paged_attn.cu.
+#include "pages.hpp"
+#include "device.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <climits>
+#include <cstring>
+#include <string>
+
+namespace navi {
+
+namespace {
+
+using namespace navi::dev;
+
+// ---- plan ------------------------------------------------------------------------------------
+
+struct PlanArgs {
+    navi_step s;
+    int32_t * table, * held, * free_pages, * n_free;
+    int * ticket, * broken;
+    int n_pages, shift, max_blocks, max_requests;
+};
+
+constexpr int PLAN_THREADS = 256;
+
+// Exclusive sum of one value per thread over the block, and the total; `red` holds a word per warp.
+template <class T> __device__ __forceinline__ T block_scan(T v, T * red, T & total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    T x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const T y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) red[warp] = x;
+    __syncthreads();
+    T base = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < PLAN_THREADS / 32; ++w) {
+        if (w < warp) base += red[w];
+        total += red[w];
+    }
+    __syncthreads();
+    return base + x - v;
+}
+
+// The last i with a[i] <= e, for a[0] = 0 <= e and a[] not decreasing.
+__device__ __forceinline__ int owner(const int * a, int n, int e) {
+    int lo = 0, hi = n;   // a[lo] <= e < a[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a[mid] <= e) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// One launch. The step is a handful of sums over the requests and then independent items: rows,
+// pages taken, pages given back. Every block does the sums over all requests itself (12 bytes a
+// request, from L2 after the first block) and keeps them in shared memory, which costs less
+// than a second launch or a wait between blocks; then the blocks share the items out. What the
+// sums read (held, n_free) is written by the block that finishes last, so no block can see it
+// half done: an arrival counter, no wait. A page that is taken from above the old stack top is
+// one that this very call gives back; it is read where it still stands, in its owner's table
+// row, whose entries past the need nobody writes.
+__global__ void __launch_bounds__(PLAN_THREADS) k_pages_plan(const __grid_constant__ PlanArgs a) {
+    extern __shared__ int plan_smem[];
+    __shared__ long long red64[PLAN_THREADS / 32];
+    __shared__ int red[PLAN_THREADS / 32];
+    __shared__ int par[2 * PLAN_THREADS];
+    __shared__ int last_block, taken_s;
+    const int B = a.s.n_req, tid = threadIdx.x, MB = a.max_blocks;
+    int * cu = plan_smem, * cg = cu + B + 1, * cs = cg + B, * st = cs + B;
+
+    const int per = (B + PLAN_THREADS - 1) / PLAN_THREADS, i0 = min(B, tid * per), i1 = min(B, i0 + per);
+    const long long cap = a.s.max_rows;
+    long long rows = 0;
+    for (int i = i0; i < i1; ++i) rows += max(a.s.n_new[i], 0);
+    long long total_rows;
+    long long row = block_scan(rows, red64, total_rows);
+    int grow = 0, surplus = 0;
+    for (int i = i0; i < i1; ++i) {
+        const int n = a.s.n_new[i], ctx = a.s.ctx_len[i], tr = a.s.req ? a.s.req[i] : i;
+        cu[i] = static_cast<int>(min(row, cap));
+        row += max(n, 0);
+        int status = NAVI_OK, g = 0, u = 0;
+        if (n < 0 || ctx < 0 || tr < 0 || tr >= a.max_requests) status = NAVI_E_ARG;
+        else {
+            const int held = a.held[tr];
+            const long long need = (static_cast<long long>(ctx) + n + (1 << a.shift) - 1) >> a.shift;
+            if (held < 0 || held > MB) status = NAVI_E_ARG;
+            else if (n > a.s.max_new || need > MB || row > cap) status = NAVI_E_SHAPE;
+            else {
+                g = max(static_cast<int>(need) - held, 0);
+                u = max(held - static_cast<int>(need), 0);
+            }
+        }
+        cg[i] = g;
+        cs[i] = u;
+        st[i] = status;
+        grow += g;
+        surplus += u;
+    }
+    if (tid == 0) {
+        cu[B] = static_cast<int>(min(total_rows, cap));
+        taken_s = 0;
+    }
+    int all_grow, all_surplus;
+    int g = block_scan(grow, red, all_grow);
+    int u = block_scan(surplus, red, all_surplus);
+    const int F = min(max(*a.n_free, 0), a.n_pages);
+    const int top = min(F + all_surplus, a.n_pages);
+    int taken = 0;
+    for (int i = i0; i < i1; ++i) {
+        const int gi = cg[i], ui = cs[i];
+        cg[i] = g;
+        cs[i] = u;
+        g += gi;
+        u += ui;
+        if (gi > 0) {
+            if (g <= top) taken = g;
+            else st[i] = NAVI_E_KV_FULL;
+        }
+    }
+    if (taken > 0) atomicMax(&taken_s, taken);
+    __syncthreads();
+    taken = taken_s;
+
+    const auto need_of = [&](int i) { return (a.s.ctx_len[i] + max(a.s.n_new[i], 0) + (1 << a.shift) - 1) >> a.shift; };
+    const auto table_row = [&](int i) { return a.table + static_cast<size_t>(a.s.req ? a.s.req[i] : i) * MB; };
+    // the e-th page that is given back
+    const auto given = [&](int e) {
+        const int i = owner(cs, B, e);
+        return table_row(i)[need_of(i) + e - cs[i]];
+    };
+    // the e-th page that is taken
+    const auto taken_page = [&](int e) {
+        const int at = top - 1 - e;
+        return at < F ? a.free_pages[at] : given(top - 1 - at);
+    };
+    const int nb = gridDim.x, step = nb * PLAN_THREADS, first = blockIdx.x * PLAN_THREADS + tid;
+    for (int e = first; e < all_surplus; e += step) {
+        const int at = top - 1 - e;
+        if (at >= F) a.free_pages[at] = given(e);
+    }
+    for (int e = first; e < taken; e += step) {
+        const int i = owner(cg, B, e);
+        table_row(i)[a.held[a.s.req ? a.s.req[i] : i] + e - cg[i]] = taken_page(e);
+    }
+    if (blockIdx.x == 0)
+        for (int i = tid; i <= B; i += PLAN_THREADS) a.s.cu_rows[i] = cu[i];
+
+    const int n_rows = cu[B];
+    for (int r0 = blockIdx.x * PLAN_THREADS; r0 < n_rows; r0 += step) {
+        const int r = r0 + tid;
+        int base = 0;
+        if (a.s.parent) {   // the parents of these rows and of the rows before them in the first one's request
+            base = max(cu[owner(cu, B, r0)], r0 - PLAN_THREADS);
+            __syncthreads();
+            for (int k = base + tid; k < min(r0 + PLAN_THREADS, n_rows); k += PLAN_THREADS) par[k - base] = a.s.parent[k];
+            __syncthreads();
+        }
+        if (r >= n_rows) continue;
+        const int i = owner(cu, B, r), j = r - cu[i], ctx = a.s.ctx_len[i];
+        int depth = j;
+        bool whole = true;
+        if (a.s.parent) {
+            uint64_t m[NAVI_STEP_MAX_TREE / 64] = {};
+            depth = -1;
+            int at = j;
+            while (at >= 0) {
+                ++depth;
+#pragma unroll
+                for (int w = 0; w < NAVI_STEP_MAX_TREE / 64; ++w)
+                    if ((at >> 6) == w) m[w] |= 1ull << (at & 63);
+                const int k = cu[i] + at - base;
+                const int up = k >= 0 ? par[k] : at;   // a request refused for its length may begin before the staged rows
+                whole = up >= -1 && up < at;
+                at = whole ? up : -1;
+            }
+            for (int w = 0; w < a.s.mask_words; ++w) {
+                uint64_t v = 0;
+#pragma unroll
+                for (int x = 0; x < NAVI_STEP_MAX_TREE / 64; ++x)
+                    if (x == w) v = m[x];
+                a.s.mask[static_cast<size_t>(r) * a.s.mask_words + w] = whole ? v : 0;
+            }
+        }
+        int64_t slot = -1;
+        if (st[i] == NAVI_OK && whole) {
+            const int held = a.held[a.s.req ? a.s.req[i] : i], blk = (ctx + j) >> a.shift;
+            const int page = blk < held ? table_row(i)[blk] : taken_page(cg[i] + blk - held);
+            if (page >= 0 && page < a.n_pages) slot = (static_cast<int64_t>(page) << a.shift) + ((ctx + j) & ((1 << a.shift) - 1));
+        }
+        if (!whole) a.broken[i] = 1;
+        a.s.row_req[r] = i;
+        a.s.pos[r] = ctx + depth;
+        a.s.slot[r] = slot;
+    }
+
+    if (nb > 1) {
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) last_block = atomicAdd(a.ticket, 1) == nb - 1;
+        __syncthreads();
+        if (!last_block) return;
+        __threadfence();
+    } else {
+        __syncthreads();
+    }
+    for (int i = tid; i < B; i += PLAN_THREADS) {
+        int status = st[i];
+        if (status == NAVI_OK) a.held[a.s.req ? a.s.req[i] : i] = need_of(i);
+        if (a.s.parent && __ldcg(a.broken + i)) {
+            a.broken[i] = 0;
+            if (status == NAVI_OK) status = NAVI_E_ARG;
+        }
+        a.s.status[i] = status;
+    }
+    if (tid == 0) {
+        *a.n_free = top - taken;
+        *a.ticket = 0;
+    }
+}
+
+// ---- store -----------------------------------------------------------------------------------
+
+struct StoreArgs {
+    const void * qkv;
+    void * q_out;
+    int64_t in_stride, out_stride;
+    const int32_t * cu_rows, * pos;
+    const int64_t * slot;
+    const float * q_norm, * k_norm, * rope;
+    uint8_t * k, * v;
+    float eps;
+    int n_req, max_rows, n_head, n_kv, shift, n_pages, rope_positions, parts;
+};
+
+template <class T> __device__ __forceinline__ void load16(const T * p, float * v);
+template <> __device__ __forceinline__ void load16<float>(const float * p, float * v) {
+    const float4 x = *reinterpret_cast<const float4 *>(p);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+}
+template <> __device__ __forceinline__ void load16<__half>(const __half * p, float * v) {
+    const uint4 x = *reinterpret_cast<const uint4 *>(p);
+    const __half2 * h = reinterpret_cast<const __half2 *>(&x);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { const float2 f = __half22float2(h[k]); v[2 * k] = f.x; v[2 * k + 1] = f.y; }
+}
+template <> __device__ __forceinline__ void load16<__nv_bfloat16>(const __nv_bfloat16 * p, float * v) {
+    const uint4 x = *reinterpret_cast<const uint4 *>(p);
+    const __nv_bfloat162 * h = reinterpret_cast<const __nv_bfloat162 *>(&x);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { const float2 f = __bfloat1622float2(h[k]); v[2 * k] = f.x; v[2 * k + 1] = f.y; }
+}
+template <class T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// E values (4 or 8) rounded to T and written with one store
+template <class T, int E> __device__ __forceinline__ void store_vec(T * p, const float * v) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else if constexpr (E == 4) {
+        *reinterpret_cast<uint2 *>(p) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+    } else {
+        *reinterpret_cast<uint4 *>(p) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+    }
+}
+
+// A warp takes a share (1 / parts) of one row's heads. A lane holds 16 bytes of the input, so a
+// head is D * sizeof(T) / 16 lanes and a warp reads 512 bytes at a time; the RoPE partner of
+// element i is i + D / 2, half a head's lanes away.
+template <class T, class C, int D> __global__ void __launch_bounds__(128) k_pages_store(const __grid_constant__ StoreArgs a) {
+    constexpr int E = 16 / sizeof(T), LANES = D / E, HPW = 32 / LANES;   // elements a lane, lanes a head, heads a warp
+    const int w = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+    const int r = w / a.parts, part = w % a.parts;
+    if (r >= a.max_rows || r >= a.cu_rows[a.n_req]) return;
+    const int sub = lane % LANES, e0 = sub * E, H = a.n_head, total = H + 2 * a.n_kv;
+    const int64_t slot = a.slot[r];
+    const int pos = a.pos[r];
+    const bool known = !a.rope || (pos >= 0 && pos < a.rope_positions);
+    const T * in = static_cast<const T *>(a.qkv) + r * a.in_stride + e0;
+    T * qo = static_cast<T *>(a.q_out) + r * a.out_stride + e0;
+    const int64_t page = slot >> a.shift, off = slot & ((1 << a.shift) - 1);
+    const size_t at = ((static_cast<size_t>(page) * a.n_kv << a.shift) + off) * D + e0;   // head 0 of the token
+    C * k = reinterpret_cast<C *>(a.k) + at, * v = reinterpret_cast<C *>(a.v) + at;
+    float qw[E], kw[E], cs[E], sn[E];
+#pragma unroll
+    for (int x = 0; x < E; ++x) { qw[x] = kw[x] = cs[x] = 1.f; sn[x] = 0.f; }
+#pragma unroll
+    for (int x = 0; x < E; ++x) {
+        if (a.q_norm) qw[x] = a.q_norm[e0 + x];
+        if (a.k_norm) kw[x] = a.k_norm[e0 + x];
+        if (a.rope && known) {
+            const float * row = a.rope + static_cast<size_t>(pos) * D;
+            cs[x] = row[(e0 + x) % (D / 2)];
+            sn[x] = e0 < D / 2 ? -row[D / 2 + e0 + x] : row[e0 + x];
+        }
+    }
+    for (int h0 = part * HPW; h0 < total; h0 += a.parts * HPW) {
+        const int h = h0 + lane / LANES;
+        const bool here = h < total;
+        float x[E];
+        load16<T>(in + static_cast<size_t>(here ? h : 0) * D, x);
+        const bool is_q = h < H, is_v = h >= H + a.n_kv;
+        const float * nw = is_q ? a.q_norm : a.k_norm;
+        float ss = 0.f;
+#pragma unroll
+        for (int c = 0; c < E; ++c) ss += x[c] * x[c];
+#pragma unroll
+        for (int o = 1; o < LANES; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float scale = nw ? rsqrtf(ss / static_cast<float>(D) + a.eps) : 1.f;
+        float y[E];
+#pragma unroll
+        for (int c = 0; c < E; ++c) y[c] = x[c] * scale * (is_q ? qw[c] : kw[c]);
+#pragma unroll
+        for (int c = 0; c < E; ++c) {
+            const float z = __shfl_xor_sync(0xffffffffu, y[c], LANES / 2);
+            y[c] = y[c] * cs[c] + z * sn[c];
+        }
+        if (!here) continue;
+        if (is_q) {
+            if (!known) {
+#pragma unroll
+                for (int c = 0; c < E; ++c) y[c] = 0.f;
+            }
+            store_vec<T, E>(qo + static_cast<size_t>(h) * D, y);
+        } else if (slot >= 0 && page < a.n_pages && known) {
+            C * dst = (is_v ? v : k) + (static_cast<size_t>(h - H - (is_v ? a.n_kv : 0)) << a.shift) * D;
+            store_vec<C, E>(dst, is_v ? x : y);
+        }
+    }
+}
+
+// ---- commit ----------------------------------------------------------------------------------
+
+struct CommitArgs {
+    navi_step s;
+    navi_commit_args c;
+    uint8_t * k[NAVI_PAGES_MAX_LAYERS], * v[NAVI_PAGES_MAX_LAYERS];
+    int n_layer, n_kv, shift, chunks;   // chunks: 16-byte pieces of one head's row
+    int n_pages;
+};
+
+constexpr int COMMIT_THREADS = 256;
+
+// Block (i, z) walks request i's tree (every z the same walk: a few hundred ids from L2) and moves
+// its share of the layers. The walk: each row looks whether its ids are the model's choice at its
+// parent, the lowest such child of each node is kept, and one thread follows them from the root.
+// The k-th accepted row is row path[k] >= k, so a thread that owns 16 bytes of a token's row and
+// goes through the path in order never writes a place that a later step still has to read.
+__global__ void __launch_bounds__(COMMIT_THREADS) k_pages_commit(const __grid_constant__ CommitArgs a) {
+    __shared__ int child[NAVI_STEP_MAX_TREE + 1];
+    __shared__ int path[NAVI_STEP_MAX_TREE];
+    __shared__ int64_t from[NAVI_STEP_MAX_TREE], to[NAVI_STEP_MAX_TREE];
+    __shared__ int count, moved;
+    const int i = blockIdx.x, tid = threadIdx.x, W = a.c.width;
+    const int r0 = a.s.cu_rows[i], n = min(a.s.cu_rows[i + 1] - r0, NAVI_STEP_MAX_TREE);
+    const bool served = a.s.status[i] == NAVI_OK;
+    for (int j = tid; j <= n; j += COMMIT_THREADS) child[j] = INT_MAX;
+    __syncthreads();
+    for (int j = tid; j < n; j += COMMIT_THREADS) {
+        const int up = a.s.parent[r0 + j];
+        if (!served || up < -1 || up >= j) continue;
+        const int32_t * want = up >= 0 ? a.c.targets + static_cast<size_t>(r0 + up) * W : a.c.root_target + static_cast<size_t>(i) * W;
+        const int32_t * have = a.c.tokens + static_cast<size_t>(r0 + j) * W;
+        bool same = true;
+        for (int x = 0; x < W; ++x) same = same && want[x] == have[x];
+        if (same) atomicMin(&child[up + 1], j);
+    }
+    __syncthreads();
+    if (tid == 0) {
+        int at = 0, k = 0, m = -1;
+        while (child[at] != INT_MAX) {
+            const int j = child[at];
+            if (j != k && m < 0) m = k;
+            path[k++] = j;
+            at = j + 1;
+        }
+        count = k;
+        moved = m < 0 ? k : m;   // the first of the path that is not in its place
+    }
+    __syncthreads();
+    const int k0 = moved, k1 = count;
+    if (blockIdx.y == 0) {
+        for (int j = tid; j < n; j += COMMIT_THREADS) a.c.path[r0 + j] = j < k1 ? path[j] : -1;
+        const int32_t * nx = k1 > 0 ? a.c.targets + static_cast<size_t>(r0 + path[k1 - 1]) * W : a.c.root_target + static_cast<size_t>(i) * W;
+        for (int x = tid; x < W; x += COMMIT_THREADS) a.c.next_token[static_cast<size_t>(i) * W + x] = nx[x];
+        if (tid == 0) {
+            a.c.accepted[i] = k1;
+            a.c.new_len[i] = a.s.ctx_len[i] + k1;
+        }
+    }
+    if (k0 >= k1) return;
+    // places of the moved rows: byte offset of head 0 in units of 16 bytes
+    for (int k = k0 + tid; k < k1; k += COMMIT_THREADS) {
+        const auto place = [&](int64_t slot) {
+            const int64_t page = slot >> a.shift, off = slot & ((1 << a.shift) - 1);
+            return slot >= 0 && page < a.n_pages ? ((page * a.n_kv << a.shift) + off) * a.chunks : -1;
+        };
+        from[k] = place(a.s.slot[r0 + path[k]]);
+        to[k] = place(a.s.slot[r0 + k]);
+    }
+    __syncthreads();
+    const int per = a.n_kv * a.chunks, items = a.n_layer * 2 * per;
+    for (int x = blockIdx.y * COMMIT_THREADS + tid; x < items; x += gridDim.y * COMMIT_THREADS) {
+        const int l = x / (2 * per), y = x % (2 * per), kv = y / per, z = y % per, h = z / a.chunks, c = z % a.chunks;
+        uint4 * pool = reinterpret_cast<uint4 *>(kv ? a.v[l] : a.k[l]) + (static_cast<size_t>(h) << a.shift) * a.chunks + c;
+        for (int k = k0; k < k1; ++k)
+            if (from[k] >= 0 && to[k] >= 0) pool[to[k]] = pool[from[k]];
+    }
+}
+
+bool aligned16(const void * p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+} // namespace
+
+// ---- host side -------------------------------------------------------------------------------
+
+std::unique_ptr<Pages> Pages::create(const Device & dev, const navi_pages_desc & d) {
+    if (d.n_layer < 1 || d.n_layer > NAVI_PAGES_MAX_LAYERS) fail("pages: n_layer outside 1..NAVI_PAGES_MAX_LAYERS", NAVI_E_ARG);
+    if (d.page_size != 16 && d.page_size != 32 && d.page_size != 64 && d.page_size != 128) fail("pages: page_size must be 16, 32, 64 or 128", NAVI_E_ARG);
+    if (d.head_dim != 64 && d.head_dim != 128) fail("pages: the kernels are built for head_dim 64 and 128", NAVI_E_SHAPE);
+    if (d.dtype != NAVI_F16 && d.dtype != NAVI_BF16) fail("pages: the cache is NAVI_F16 or NAVI_BF16", NAVI_E_ARG);
+    if (d.n_kv_head < 1 || d.n_pages < 1 || d.max_blocks < 1) fail("pages: n_kv_head, n_pages and max_blocks must be positive", NAVI_E_ARG);
+    if (d.max_requests < 1 || d.max_requests > NAVI_PAGES_MAX_REQUESTS) fail("pages: max_requests outside 1..NAVI_PAGES_MAX_REQUESTS", NAVI_E_ARG);
+    // rows of all heads and pages are counted in 31 bits (tensor-map coordinates), a table row's tokens too
+    if (static_cast<int64_t>(d.n_pages) * d.n_kv_head * d.page_size > INT32_MAX) fail("pages: n_pages * n_kv_head * page_size passes 31 bits", NAVI_E_SHAPE);
+    if (static_cast<int64_t>(d.max_blocks) * d.page_size > INT32_MAX / 2) fail("pages: max_blocks * page_size passes 30 bits", NAVI_E_SHAPE);
+    if (!d.k != !d.v) fail("pages: k and v are both given or both NULL", NAVI_E_ARG);
+    const int given = !!d.table + !!d.held + !!d.free_pages + !!d.n_free;
+    if (given != 0 && given != 4) fail("pages: table, held, free_pages and n_free are all given or all NULL", NAVI_E_ARG);
+    if (d.k)
+        for (int l = 0; l < d.n_layer; ++l)
+            if (!aligned16(d.k[l]) || !aligned16(d.v[l])) fail("pages: a layer's pool is not 16-byte aligned", NAVI_E_ARG);
+    std::unique_ptr<Pages> p(new Pages());
+    dev.make_current();
+    p->dev_ = &dev;
+    p->d_ = d;
+    while ((1 << p->shift_) < d.page_size) ++p->shift_;
+    const auto take = [&](size_t bytes) {
+        void * m = nullptr;
+        NAVI_CUDA(cudaMalloc(&m, bytes));
+        p->owned_.push_back(m);
+        NAVI_CUDA(cudaMemset(m, 0, bytes));
+        return m;
+    };
+    if (d.k) {
+        p->k_.assign(d.k, d.k + d.n_layer);
+        p->v_.assign(d.v, d.v + d.n_layer);
+    } else {
+        const size_t bytes = static_cast<size_t>(d.n_pages) * d.n_kv_head * d.page_size * d.head_dim * 2;
+        for (int l = 0; l < d.n_layer; ++l) {
+            p->k_.push_back(take(bytes));
+            p->v_.push_back(take(bytes));
+        }
+    }
+    p->d_.k = p->k_.data();
+    p->d_.v = p->v_.data();
+    if (!given) {
+        std::vector<int32_t> ids(static_cast<size_t>(d.n_pages));
+        for (int i = 0; i < d.n_pages; ++i) ids[static_cast<size_t>(i)] = d.n_pages - 1 - i;
+        p->d_.table = static_cast<int32_t *>(take(static_cast<size_t>(d.max_requests) * d.max_blocks * 4));
+        p->d_.held = static_cast<int32_t *>(take(static_cast<size_t>(d.max_requests) * 4));
+        p->d_.free_pages = static_cast<int32_t *>(take(ids.size() * 4));
+        p->d_.n_free = static_cast<int32_t *>(take(4));
+        NAVI_CUDA(cudaMemcpy(p->d_.free_pages, ids.data(), ids.size() * 4, cudaMemcpyHostToDevice));
+        NAVI_CUDA(cudaMemcpy(p->d_.n_free, &d.n_pages, 4, cudaMemcpyHostToDevice));
+    }
+    return p;
+}
+
+Pages::~Pages() {
+    if (!owned_.empty()) cudaSetDevice(dev_->info().ordinal);
+    for (void * m : owned_) cudaFree(m);
+}
+
+void Pages::check_step(const navi_step & s, const char * who) const {
+    const std::string w(who);
+    if (s.n_req < 0 || s.n_req > d_.max_requests) fail(w + ": n_req outside 0..max_requests", NAVI_E_ARG);
+    if (s.max_rows < 0 || s.max_new < 0) fail(w + ": max_rows and max_new must not be negative", NAVI_E_ARG);
+    if (s.n_req == 0) return;
+    if (!s.ctx_len || !s.n_new || !s.cu_rows || !s.status) fail(w + ": ctx_len, n_new, cu_rows and status are needed", NAVI_E_ARG);
+    if (s.max_rows > 0 && (!s.row_req || !s.pos || !s.slot)) fail(w + ": row_req, pos and slot are needed", NAVI_E_ARG);
+    if (s.parent) {
+        if (s.max_new > NAVI_STEP_MAX_TREE) fail(w + ": a tree has at most NAVI_STEP_MAX_TREE rows", NAVI_E_SHAPE);
+        if (s.mask_words < 0 || s.mask_words > NAVI_STEP_MAX_TREE / 64 || 64 * s.mask_words < s.max_new || (s.max_new > 0 && !s.mask))
+            fail(w + ": mask of 64 * mask_words >= max_new bits is needed with parent", NAVI_E_ARG);
+    }
+}
+
+void Pages::plan(const navi_step & s, cudaStream_t stream) const {
+    check_step(s, "pages plan");
+    if (s.n_req == 0) return;
+    NAVI_CUDA(cudaSetDevice(dev_->info().ordinal));
+    int * scratch = static_cast<int *>(dev_->scratch(stream, PagesScratch::BYTES));
+    PlanArgs a{s, d_.table, d_.held, d_.free_pages, d_.n_free, scratch, scratch + PagesScratch::TICKETS, d_.n_pages, shift_, d_.max_blocks, d_.max_requests};
+    const size_t smem = (4 * static_cast<size_t>(s.n_req) + 1) * sizeof(int);
+    static_assert((4 * static_cast<size_t>(NAVI_PAGES_MAX_REQUESTS) + 1) * sizeof(int) < 200 * 1024);
+    if (smem > 40 * 1024)
+        NAVI_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(&k_pages_plan), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>((4 * NAVI_PAGES_MAX_REQUESTS + 1) * sizeof(int))));
+    const int blocks = std::clamp((s.max_rows + PLAN_THREADS - 1) / PLAN_THREADS, 1, 2 * dev_->info().multiprocessors);
+    k_pages_plan<<<blocks, PLAN_THREADS, smem, stream>>>(a);
+    NAVI_CUDA(cudaGetLastError());
+}
+
+void Pages::store(const navi_step & s, int layer, const navi_store_args & q, cudaStream_t stream) const {
+    check_step(s, "pages store");
+    if (layer < 0 || layer >= d_.n_layer) fail("pages store: layer outside the cache", NAVI_E_ARG);
+    if (q.n_head < 0 || q.n_head > 4096) fail("pages store: n_head outside 0..4096", NAVI_E_ARG);
+    if (!(q.dtype == d_.dtype || (q.dtype == NAVI_F32 && d_.dtype == NAVI_F16))) fail("pages store: rows are of the cache's type, or NAVI_F32 for an f16 cache", NAVI_E_ARG);
+    if (q.rope && q.rope_positions < 1) fail("pages store: rope_positions must be positive", NAVI_E_ARG);
+    if (s.n_req == 0 || s.max_rows == 0) return;
+    const int D = d_.head_dim, heads = q.n_head + 2 * d_.n_kv_head;
+    const int64_t elt = q.dtype == NAVI_F32 ? 4 : 2, in = q.qkv_stride ? q.qkv_stride : static_cast<int64_t>(heads) * D,
+                  out = q.q_out_stride ? q.q_out_stride : static_cast<int64_t>(q.n_head) * D;
+    if (!q.qkv || (q.n_head > 0 && !q.q_out)) fail("pages store: NULL rows", NAVI_E_ARG);
+    if (in < static_cast<int64_t>(heads) * D || out < static_cast<int64_t>(q.n_head) * D) fail("pages store: a row stride is shorter than the row", NAVI_E_ARG);
+    if (!aligned16(q.qkv) || !aligned16(q.q_out) || in * elt % 16 || out * elt % 16) fail("pages store: rows must be 16-byte aligned", NAVI_E_ARG);
+    NAVI_CUDA(cudaSetDevice(dev_->info().ordinal));
+    StoreArgs a{q.qkv, q.q_out, in, out, s.cu_rows, s.pos, s.slot, q.q_norm, q.k_norm, q.rope, static_cast<uint8_t *>(k_[static_cast<size_t>(layer)]),
+                static_cast<uint8_t *>(v_[static_cast<size_t>(layer)]), q.eps, s.n_req, s.max_rows, q.n_head, d_.n_kv_head, shift_, d_.n_pages, q.rope_positions, 1};
+    // few rows: a row's heads go to several warps, down to one pass of a warp each
+    const int per_warp = static_cast<int>(512 / (D * elt)), passes = (heads + per_warp - 1) / per_warp;
+    while (a.parts * 2 <= passes && static_cast<int64_t>(s.max_rows) * a.parts < 16 * 4 * dev_->info().multiprocessors) a.parts *= 2;
+    const int64_t warps = static_cast<int64_t>(s.max_rows) * a.parts;
+    if (warps > INT32_MAX / 32) fail("pages store: too many rows", NAVI_E_SHAPE);
+    const unsigned blocks = static_cast<unsigned>((warps + 3) / 4);
+    const auto go = [&](auto kernel) { kernel<<<blocks, 128, 0, stream>>>(a); };
+    if (q.dtype == NAVI_F32) D == 128 ? go(k_pages_store<float, __half, 128>) : go(k_pages_store<float, __half, 64>);
+    else if (q.dtype == NAVI_F16) D == 128 ? go(k_pages_store<__half, __half, 128>) : go(k_pages_store<__half, __half, 64>);
+    else D == 128 ? go(k_pages_store<__nv_bfloat16, __nv_bfloat16, 128>) : go(k_pages_store<__nv_bfloat16, __nv_bfloat16, 64>);
+    NAVI_CUDA(cudaGetLastError());
+}
+
+void Pages::commit(const navi_step & s, const navi_commit_args & c, cudaStream_t stream) const {
+    check_step(s, "pages commit");
+    if (c.width < 1) fail("pages commit: width must be positive", NAVI_E_ARG);
+    if (s.n_req == 0) return;
+    if (!s.parent) fail("pages commit: the step has no parent (there is no tree to walk)", NAVI_E_ARG);
+    if (!c.root_target || !c.accepted || !c.new_len || !c.next_token) fail("pages commit: NULL argument", NAVI_E_ARG);
+    if (s.max_rows > 0 && (!c.tokens || !c.targets || !c.path)) fail("pages commit: NULL argument", NAVI_E_ARG);
+    NAVI_CUDA(cudaSetDevice(dev_->info().ordinal));
+    CommitArgs a{};
+    a.s = s;
+    a.c = c;
+    for (int l = 0; l < d_.n_layer; ++l) {
+        a.k[l] = static_cast<uint8_t *>(k_[static_cast<size_t>(l)]);
+        a.v[l] = static_cast<uint8_t *>(v_[static_cast<size_t>(l)]);
+    }
+    a.n_layer = d_.n_layer;
+    a.n_kv = d_.n_kv_head;
+    a.shift = shift_;
+    a.chunks = d_.head_dim / 8;
+    a.n_pages = d_.n_pages;
+    const int64_t items = static_cast<int64_t>(d_.n_layer) * 2 * d_.n_kv_head * a.chunks;
+    if (items > INT32_MAX / 2) fail("pages commit: too many heads", NAVI_E_SHAPE);
+    const int most = static_cast<int>((items + COMMIT_THREADS - 1) / COMMIT_THREADS);
+    const int z = std::clamp(4 * dev_->info().multiprocessors / s.n_req, 1, std::min(most, 65535));
+    k_pages_commit<<<dim3(static_cast<unsigned>(s.n_req), static_cast<unsigned>(z)), COMMIT_THREADS, 0, stream>>>(a);
+    NAVI_CUDA(cudaGetLastError());
+}
+
+} // namespace navi

@@ -456,8 +456,23 @@ Device::Device(int ordinal) {
 Device::~Device() {
     if (stream_) {
         cudaSetDevice(info_.ordinal);
+        for (const auto & s : scratch_) cudaFree(s.second);
         cudaStreamDestroy(stream_);
     }
+}
+
+void * Device::scratch(cudaStream_t stream, size_t bytes) const {
+    for (const auto & s : scratch_)
+        if (s.first == stream) return s.second;
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    NAVI_CUDA(cudaStreamIsCapturing(stream, &cap));
+    if (cap != cudaStreamCaptureStatusNone)
+        fail("the stream's scratch must be taken by a call made before the stream is captured", NAVI_E_ARG);
+    void * p = nullptr;
+    NAVI_CUDA(cudaMalloc(&p, bytes));
+    NAVI_CUDA(cudaMemsetAsync(p, 0, bytes, stream));
+    scratch_.emplace_back(stream, p);
+    return p;
 }
 
 void Device::make_current() const { NAVI_CUDA(cudaSetDevice(info_.ordinal)); }

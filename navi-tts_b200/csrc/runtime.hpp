@@ -147,10 +147,15 @@ public:
     const DeviceInfo & info() const { return info_; }
     cudaStream_t stream() const { return stream_; }
     void make_current() const;
+    // `bytes` of device memory for the launches of one stream to hand work to one another: a block
+    // per stream, zeroed when it is taken at the stream's first call and kept until the device
+    // closes. Every caller asks for the same size.
+    void * scratch(cudaStream_t stream, size_t bytes) const;
 
 private:
     DeviceInfo info_;
     cudaStream_t stream_ = nullptr;
+    mutable std::vector<std::pair<cudaStream_t, void *>> scratch_;
 };
 
 // ---- weights arena (reference: runtime/weights/device_weights.cpp:18-72) ----------------------------

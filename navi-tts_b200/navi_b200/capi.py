@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char, c_char_p, c_double, c_float, c_int, c_int32, c_size_t, c_uint8, c_uint16, c_uint64, c_void_p
+from ctypes import POINTER, c_char, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint8, c_uint16, c_uint64, c_void_p
 
 # NAVI_B200_LIB overrides the library path (e.g. a variant build); the default is the in-tree build.
 LIB_PATH = os.environ.get("NAVI_B200_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "libnavi_b200.so")
@@ -16,6 +16,10 @@ NAVI_OK, NAVI_E_ARG, NAVI_E_CUDA, NAVI_E_FORMAT, NAVI_E_TIMEOUT, NAVI_E_KV_FULL,
 NAVI_FRAME_SLOTS = 4
 NAVI_RNG_PCG, NAVI_RNG_PHILOX = 0, 1
 NAVI_SAMPLE_STATIC_MAX_VOCAB = 32768
+NAVI_F32, NAVI_F16, NAVI_BF16 = range(3)
+NAVI_PAGES_MAX_REQUESTS = 8192
+NAVI_PAGES_MAX_LAYERS = 128
+NAVI_STEP_MAX_TREE = 256
 
 
 class DeviceInfo(ctypes.Structure):
@@ -74,6 +78,33 @@ class ConvArgs(ctypes.Structure):
 class SynthRequest(ctypes.Structure):
     _fields_ = [("ids", POINTER(c_int32)), ("n_ids", c_int), ("language", c_char_p), ("speaker", POINTER(c_float)), ("seed", c_uint64),
                 ("max_frames", c_int), ("codes", POINTER(c_int32)), ("codes_cap", c_int)]
+
+
+class PagesDesc(ctypes.Structure):
+    _fields_ = [("n_layer", c_int), ("n_pages", c_int), ("page_size", c_int), ("n_kv_head", c_int), ("head_dim", c_int), ("dtype", c_int),
+                ("max_requests", c_int), ("max_blocks", c_int), ("k", POINTER(c_void_p)), ("v", POINTER(c_void_p)), ("table", c_void_p),
+                ("held", c_void_p), ("free_pages", c_void_p), ("n_free", c_void_p)]
+
+
+class Step(ctypes.Structure):
+    _fields_ = [("n_req", c_int), ("max_rows", c_int), ("max_new", c_int), ("mask_words", c_int), ("req", c_void_p), ("ctx_len", c_void_p),
+                ("n_new", c_void_p), ("parent", c_void_p), ("cu_rows", c_void_p), ("row_req", c_void_p), ("pos", c_void_p),
+                ("slot", c_void_p), ("mask", c_void_p), ("status", c_void_p)]
+
+
+class StoreArgs(ctypes.Structure):
+    _fields_ = [("qkv", c_void_p), ("qkv_stride", c_int64), ("q_out", c_void_p), ("q_out_stride", c_int64), ("dtype", c_int), ("n_head", c_int),
+                ("q_norm", c_void_p), ("k_norm", c_void_p), ("eps", c_float), ("rope", c_void_p), ("rope_positions", c_int)]
+
+
+class AttendArgs(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("q_stride", c_int64), ("out", c_void_p), ("out_stride", c_int64), ("lse", c_void_p), ("dtype", c_int),
+                ("n_head", c_int), ("scale", c_float)]
+
+
+class CommitArgs(ctypes.Structure):
+    _fields_ = [("width", c_int), ("tokens", c_void_p), ("targets", c_void_p), ("root_target", c_void_p), ("accepted", c_void_p),
+                ("path", c_void_p), ("new_len", c_void_p), ("next_token", c_void_p)]
 
 
 STREAM_PCM_FN = ctypes.CFUNCTYPE(None, c_int, POINTER(c_float), c_int, c_void_p)
@@ -157,6 +188,13 @@ SIGNATURES = [
     ("navi_vocoder_last_ms", c_double, [c_void_p]),
     ("navi_vocoder_set_stage_hook", c_int, [c_void_p, STAGE_FN, c_void_p]),
     ("navi_vocoder_destroy", None, [c_void_p]),
+    ("navi_pages_create", c_int, [c_void_p, POINTER(PagesDesc), POINTER(c_void_p)]),
+    ("navi_pages_get", c_int, [c_void_p, POINTER(PagesDesc)]),
+    ("navi_pages_destroy", None, [c_void_p]),
+    ("navi_pages_plan", c_int, [c_void_p, c_void_p, c_void_p]),
+    ("navi_pages_store", c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    ("navi_pages_attend", c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    ("navi_pages_commit", c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),
     ("navi_conv1d", c_int, [c_void_p, POINTER(ConvArgs)]),
     ("navi_frame_inspect", c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),
     ("navi_frame_set_profile", c_int, [c_void_p, c_int, c_int]),

@@ -3,6 +3,7 @@
 Device      <- navi::Device        (runtime/device/device.h:43-66)
 Weights     <- NaviFile + DeviceWeights + Params (runtime/weights/*, model/qwen3tts/params.h)
 KvCache     <- navi::qwen3tts::KvCache (model/qwen3tts/talker.h:20-24)
+PagedKv     (no counterpart): a cache of pages shared by many requests, for drafted trees
 Frame       <- navi::qwen3tts::Frame   (model/qwen3tts/frame.h:46-71)
 
 Same method names and argument meaning; failures raise NaviError carrying the
@@ -208,6 +209,105 @@ class Talker:
         if self.h:
             if _open(self.dev, self.w):
                 lib().navi_talker_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def _record(cls, doc):
+    """A class for one of the C argument structures that is passed by its address, made from
+    keywords (device pointers as integers, 0 for none)."""
+    class Record:
+        __doc__ = doc
+
+        def __init__(self, keepalive=None, **kw):
+            self.s = cls()
+            names = {n for n, _ in cls._fields_}
+            for k, v in kw.items():
+                if k not in names:
+                    raise TypeError(f"{type(self).__name__} has no field {k!r}")
+                setattr(self.s, k, v)
+            self.ptr = ctypes.addressof(self.s)
+            self.keepalive = keepalive
+
+    return Record
+
+
+class TreeStep(_record(capi.Step, "")):
+    """navi_step: the requests of one step, their new rows and, once planned, where these go."""
+
+
+class StoreArgs(_record(capi.StoreArgs, "")):
+    """navi_store_args: a layer's qkv rows and how q and k are normalised and rotated."""
+
+
+class AttendArgs(_record(capi.AttendArgs, "")):
+    """navi_attend_args: a layer's query rows and where the result goes."""
+
+
+class CommitArgs(_record(capi.CommitArgs, "")):
+    """navi_commit_args: the drafted ids, the model's choices and the outcome."""
+
+
+class PagedKv:
+    """The paged KV cache of many requests (navi_pages): create() lets the library allocate the
+    pools and block tables, wrap() uses the caller's. Every call enqueues on `stream` (a
+    cudaStream_t as an integer, 0 the default stream; None: the engine's own)."""
+
+    def __init__(self, dev: Device, desc: capi.PagesDesc, keepalive=None):
+        h = c_void_p()
+        L = lib()
+        check(L.navi_pages_create(dev.h, byref(desc), byref(h)))
+        self.h, self.dev, self._keep = h, dev, keepalive
+        self._stream = dev.stream
+        self._plan, self._store, self._attend, self._commit = L.navi_pages_plan, L.navi_pages_store, L.navi_pages_attend, L.navi_pages_commit
+
+    @staticmethod
+    def create(dev: Device, n_layer: int, n_pages: int, page_size: int, n_kv_head: int, head_dim: int, max_requests: int, max_blocks: int,
+               dtype: int = capi.NAVI_F16) -> "PagedKv":
+        return PagedKv(dev, capi.PagesDesc(n_layer, n_pages, page_size, n_kv_head, head_dim, dtype, max_requests, max_blocks))
+
+    @staticmethod
+    def wrap(dev: Device, k_ptrs, v_ptrs, n_pages: int, page_size: int, n_kv_head: int, head_dim: int, dtype: int, max_requests: int,
+             max_blocks: int, table: int, held: int, free_pages: int, n_free: int, keepalive=None) -> "PagedKv":
+        n = len(k_ptrs)
+        ka, va = (c_void_p * n)(*k_ptrs), (c_void_p * n)(*v_ptrs)
+        return PagedKv(dev, capi.PagesDesc(n, n_pages, page_size, n_kv_head, head_dim, dtype, max_requests, max_blocks, ka, va, table, held,
+                                           free_pages, n_free), keepalive)
+
+    def desc(self) -> capi.PagesDesc:
+        d = capi.PagesDesc()
+        check(lib().navi_pages_get(self.h, byref(d)))
+        return d
+
+    def plan(self, step: TreeStep, stream: int | None = None) -> None:
+        st = self._plan(self.h, step.ptr, self._stream if stream is None else stream)
+        if st:
+            check(st)
+
+    def store(self, step: TreeStep, layer: int, args: StoreArgs, stream: int | None = None) -> None:
+        st = self._store(self.h, step.ptr, layer, args.ptr, self._stream if stream is None else stream)
+        if st:
+            check(st)
+
+    def attend(self, step: TreeStep, layer: int, args: AttendArgs, stream: int | None = None) -> None:
+        st = self._attend(self.h, step.ptr, layer, args.ptr, self._stream if stream is None else stream)
+        if st:
+            check(st)
+
+    def commit(self, step: TreeStep, args: CommitArgs, stream: int | None = None) -> None:
+        st = self._commit(self.h, step.ptr, args.ptr, self._stream if stream is None else stream)
+        if st:
+            check(st)
+
+    def close(self):
+        if self.h:
+            if _open(self.dev):
+                lib().navi_pages_destroy(self.h)
             self.h = None
 
     def __del__(self):
