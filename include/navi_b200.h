@@ -485,6 +485,11 @@ typedef struct navi_commit_args {
  * The step needs parent; a request that is not served accepts nothing. */
 int navi_pages_commit(navi_pages * p, const navi_step * s, const navi_commit_args * a, void * stream);
 
+/* Waits for `stream`. NAVI_E_TIMEOUT when a kernel of these calls on it gave up a wait for a copy
+ * or a matrix product since the last check (its results are then void); the waits are bounded, so
+ * no call hangs the device. */
+int navi_pages_check(navi_pages * p, void * stream);
+
 /* Inspection of the last frame (host copies): the talker's post-norm hidden [hidden],
  * its codec logits [talker vocab], and the 15 code-predictor logit rows [15][cp vocab].
  * Any pointer may be NULL. The reference keeps these in its Work buffers (frame.hip:51-70). */

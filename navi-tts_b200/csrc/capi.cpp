@@ -792,6 +792,14 @@ int navi_pages_commit(navi_pages * p, const navi_step * s, const navi_commit_arg
     });
 }
 
+int navi_pages_check(navi_pages * p, void * stream) {
+    return guard([&]() -> int {
+        if (!p) return set_err(NAVI_E_ARG, "NULL argument");
+        p->p->check(static_cast<cudaStream_t>(stream));
+        return NAVI_OK;
+    });
+}
+
 int navi_conv1d(navi_device * dev, const navi_conv_args * a) {
     return guard([&]() -> int {
         if (!dev || !a || !a->w || !a->x || !a->y) return set_err(NAVI_E_ARG, "NULL argument");

@@ -5,50 +5,16 @@
 // over the request's cached tokens k < ctx and those of the step's rows that row j sees: its
 // ancestors and itself in a drafted tree (a bit mask), rows up to j in a chain. m is a running
 // maximum, so one pass over the keys is enough; m, l and the sums are f32.
-#include "pages.hpp"
-#include "device.cuh"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+#include "paged_attn.hpp"
+#include "paged_attn.cuh"
 
 #include <string>
-#include <type_traits>
 
 namespace navi {
 
 namespace {
 
-using namespace navi::dev;
-
-struct AttendArgs {
-    const void * q;
-    void * out;
-    float * lse;
-    const uint8_t * k, * v;
-    const int32_t * table, * req, * ctx_len, * cu_rows, * status;
-    const uint64_t * mask;       // nullptr: a chain
-    int64_t q_stride, out_stride;
-    float scale;                 // times log2(e)
-    int n_req, max_rows, mask_words, n_head, n_kv, group, shift, n_pages, max_blocks, max_requests;
-};
-
-// What a block needs to know of one request.
-struct Request {
-    int row0, n, ctx, keys;      // first row, rows, cached tokens, tokens in all
-    const int32_t * table;
-};
-__device__ __forceinline__ Request request(const AttendArgs & a, int i) {
-    Request r;
-    r.row0 = a.cu_rows[i];
-    r.n = min(a.cu_rows[i + 1], a.max_rows) - r.row0;
-    r.ctx = a.ctx_len[i];
-    const int tr = a.req ? a.req[i] : i;
-    const bool ok = a.status[i] == NAVI_OK && tr >= 0 && tr < a.max_requests && r.ctx >= 0 &&
-                    static_cast<long long>(r.ctx) + r.n <= (static_cast<long long>(a.max_blocks) << a.shift);
-    r.keys = ok ? r.ctx + r.n : 0;
-    r.table = a.table + static_cast<size_t>(ok ? tr : 0) * a.max_blocks;
-    return r;
-}
+using namespace navi::attn;
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -67,26 +33,6 @@ template <class C> __device__ __forceinline__ void mma(float (&c)[4], const uint
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <class C> __device__ __forceinline__ uint32_t pack(float a, float b) {
-    if constexpr (std::is_same_v<C, __half>) {
-        const __half2 h = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t *>(&h);
-    } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t *>(&h);
-    }
-}
-template <class C> __device__ __forceinline__ float2 unpack(uint32_t v) {
-    if constexpr (std::is_same_v<C, __half>) return __half22float2(*reinterpret_cast<const __half2 *>(&v));
-    else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v));
-}
-// 2^x by the hardware's approximation (two units of the last place); 2^-inf = 0
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 constexpr int ROWS = 64, KEYS = 64, WARPS = 4, THREADS = 128;
 
 // A block takes 64 of a request's rows x heads of one KV head (4 warps of 16, the heads of a row
@@ -95,7 +41,8 @@ constexpr int ROWS = 64, KEYS = 64, WARPS = 4, THREADS = 128;
 // p = hi + lo, against the exact cache values: about 22 bits. 16-bit rows are exact, and p is
 // rounded once to the type that the result has. Shared-memory rows are swizzled by 16-byte
 // pieces so that ldmatrix reads eight different banks.
-template <class T, class C, int D> __global__ void __launch_bounds__(THREADS) k_attend(const __grid_constant__ AttendArgs a) {
+template <class T, class C, int D>
+__global__ void __launch_bounds__(THREADS) k_attend(const __grid_constant__ AttendArgs a, const uint8_t * kpool, const uint8_t * vpool) {
     constexpr bool SPLIT = std::is_same_v<T, float>;
     constexpr int CH = D / 8;                         // 16-byte pieces of a row
     constexpr uint32_t ROW = D * 2, TILE = KEYS * ROW;
@@ -117,8 +64,8 @@ template <class T, class C, int D> __global__ void __launch_bounds__(THREADS) k_
             if (key < n_keys) {
                 const int page = min(max(rq.table[key >> a.shift], 0), a.n_pages - 1);
                 const size_t at = ((((static_cast<size_t>(page) * a.n_kv + g) << a.shift) + (key & ((1 << a.shift) - 1))) * CH + c) * 16;
-                cp_async16(kb + o, a.k + at);
-                cp_async16(vb + o, a.v + at);
+                cp_async16(kb + o, kpool + at);
+                cp_async16(vb + o, vpool + at);
             } else {   // past the request's tokens: zeros, whatever the page holds there
                 *reinterpret_cast<uint4 *>(kb + o) = make_uint4(0, 0, 0, 0);
                 *reinterpret_cast<uint4 *>(vb + o) = make_uint4(0, 0, 0, 0);
@@ -288,15 +235,19 @@ void Pages::attend(const navi_step & s, int layer, const navi_attend_args & q, c
     const auto off16 = [](const void * p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; };
     if (off16(q.q) || off16(q.out) || in * elt % 16 || out * elt % 16) fail("pages attend: rows must be 16-byte aligned", NAVI_E_ARG);
     NAVI_CUDA(cudaSetDevice(dev_->info().ordinal));
-    AttendArgs a{q.q, q.out, q.lse, static_cast<const uint8_t *>(k_[static_cast<size_t>(layer)]), static_cast<const uint8_t *>(v_[static_cast<size_t>(layer)]),
-                 d_.table, s.req, s.ctx_len, s.cu_rows, s.status, s.parent ? s.mask : nullptr, in, out, q.scale * 1.4426950408889634f,
-                 s.n_req, s.max_rows, s.mask_words, q.n_head, d_.n_kv_head, q.n_head / d_.n_kv_head, shift_, d_.n_pages, d_.max_blocks, d_.max_requests};
+    const int sms = dev_->info().multiprocessors;
+    const PagesScratch sc(dev_->scratch(stream, PagesScratch::bytes(sms)), sms);
+    AttendArgs a{q.q, q.out, q.lse, d_.table, s.req, s.ctx_len, s.cu_rows, s.status, s.parent ? s.mask : nullptr, sc.pieces, sc.arrived, sc.err,
+                 in, out, q.scale * 1.4426950408889634f, s.n_req, s.max_rows, s.mask_words, q.n_head, d_.n_kv_head, q.n_head / d_.n_kv_head, D, shift_,
+                 d_.n_pages, d_.max_blocks, d_.max_requests};
+    const CUtensorMap & km = maps_[static_cast<size_t>(2 * layer)], & vm = maps_[static_cast<size_t>(2 * layer + 1)];
     const int64_t m = static_cast<int64_t>(std::min(s.max_new, s.max_rows)) * a.group;
+    if (m <= 32) return attend_few(a, km, vm, q.dtype, d_.dtype, static_cast<int>(m), sms, stream);
     const dim3 grid(static_cast<unsigned>((m + ROWS - 1) / ROWS), static_cast<unsigned>(d_.n_kv_head), static_cast<unsigned>(s.n_req));
     const auto go = [&](auto kernel, bool split) {
         const int smem = static_cast<int>(((split ? 2 : 1) * ROWS + 4 * KEYS) * D * 2);
         NAVI_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        kernel<<<grid, THREADS, static_cast<size_t>(smem), stream>>>(a);
+        kernel<<<grid, THREADS, static_cast<size_t>(smem), stream>>>(a, static_cast<const uint8_t *>(k_[static_cast<size_t>(layer)]), static_cast<const uint8_t *>(v_[static_cast<size_t>(layer)]));
     };
     if (q.dtype == NAVI_F32) D == 128 ? go(k_attend<float, __half, 128>, true) : go(k_attend<float, __half, 64>, true);
     else if (q.dtype == NAVI_F16) D == 128 ? go(k_attend<__half, __half, 128>, false) : go(k_attend<__half, __half, 64>, false);

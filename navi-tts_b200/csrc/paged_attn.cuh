@@ -1,0 +1,299 @@
+// What the attention kernels over the paged KV cache share (paged_attn.cu has the mathematics):
+// the launch's arguments, how the blocks divide ragged requests between them, how the pieces of
+// an item are joined, and how a tile of pages is brought to shared memory.
+#pragma once
+
+#include "device.cuh"
+#include "pages.hpp"
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+namespace navi::attn {
+
+using namespace navi::dev;
+
+struct AttendArgs {
+    const void * q;
+    void * out;
+    float * lse;
+    const int32_t * table, * req, * ctx_len, * cu_rows, * status;
+    const uint64_t * mask;       // nullptr: a chain
+    float * pieces;              // the stream's scratch: unfinished sums, arrival counters, error word
+    int * arrived, * err;
+    int64_t q_stride, out_stride;
+    float scale;                 // times log2(e)
+    int n_req, max_rows, mask_words, n_head, n_kv, group, head_dim, shift, n_pages, max_blocks, max_requests;
+};
+
+// What a block needs to know of one request.
+struct Request {
+    int row0, n, ctx, keys;      // first row, rows, cached tokens, tokens in all
+    const int32_t * table;
+};
+__device__ __forceinline__ Request request(const AttendArgs & a, int i) {
+    Request r;
+    r.row0 = a.cu_rows[i];
+    r.n = max(min(a.cu_rows[i + 1], a.max_rows) - r.row0, 0);
+    r.ctx = a.ctx_len[i];
+    const int tr = a.req ? a.req[i] : i;
+    const bool ok = a.status[i] == NAVI_OK && tr >= 0 && tr < a.max_requests && r.ctx >= 0 &&
+                    static_cast<long long>(r.ctx) + r.n <= (static_cast<long long>(a.max_blocks) << a.shift);
+    r.keys = ok ? r.ctx + r.n : 0;
+    r.table = a.table + static_cast<size_t>(ok ? tr : 0) * a.max_blocks;
+    return r;
+}
+
+template <class C> __device__ __forceinline__ uint32_t pack(float a, float b) {
+    if constexpr (std::is_same_v<C, __half>) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+template <class C> __device__ __forceinline__ float2 unpack(uint32_t v) {
+    if constexpr (std::is_same_v<C, __half>) return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+    else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v));
+}
+// 2^x by the hardware's approximation (two units of the last place); 2^-inf = 0
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// ---- who does what ----------------------------------------------------------------------------
+//
+// The work of a launch is a list of units: for each request, each KV head and each tile of ROWS
+// rows (rows x heads of the KV head, an item), the item's key tiles of KT keys, at least one.
+// Lengths are on the device and ragged, so the blocks divide the list evenly themselves: block c
+// of G takes the units [c W / G, (c + 1) W / G), whatever request they belong to. An item that
+// falls to several blocks leaves its pieces (the sums and each row's maximum and sum, f32) in
+// the stream's scratch, and the block that arrives last joins them in the blocks' order, so
+// the result does not depend on who was last. A block has at most two such pieces: slot 0 for
+// one that begins inside an item, slot 1 for one that only ends inside it.
+
+constexpr int KT = 128;
+
+struct Item {
+    int i, g, rt;                // request, KV head, row tile
+    int tiles, n_keys;           // key tiles (1 at least) and keys that its rows may see
+    int m0, m;                   // its first row x head, and how many
+    long long u0;                // its first unit
+    Request rq;
+};
+
+template <int ROWS> __device__ __forceinline__ int row_tiles(const AttendArgs & a, const Request & r) { return (r.n * a.group + ROWS - 1) / ROWS; }
+template <int ROWS> __device__ __forceinline__ int keys_of(const AttendArgs & a, const Request & r, int rt) {
+    if (a.mask || r.keys == 0) return r.keys;
+    return r.ctx + min(((rt + 1) * ROWS - 1) / a.group + 1, r.n);
+}
+__device__ __forceinline__ int tiles_of(int n_keys) { return max((n_keys + KT - 1) / KT, 1); }
+// the units of one KV head of a request
+template <int ROWS> __device__ __forceinline__ long long units_of(const AttendArgs & a, const Request & r) {
+    const int rts = row_tiles<ROWS>(a, r);
+    if (a.mask || r.keys == 0) return static_cast<long long>(rts) * tiles_of(r.keys);
+    long long n = 0;
+    for (int rt = 0; rt < rts; ++rt) n += tiles_of(keys_of<ROWS>(a, r, rt));
+    return n;
+}
+template <int ROWS> __device__ __forceinline__ void open_tile(const AttendArgs & a, Item & it) {
+    it.n_keys = keys_of<ROWS>(a, it.rq, it.rt);
+    it.tiles = tiles_of(it.n_keys);
+    it.m0 = it.rt * ROWS;
+    it.m = min(it.rq.n * a.group - it.m0, ROWS);
+}
+template <int ROWS> __device__ __forceinline__ void next_item(const AttendArgs & a, Item & it) {
+    it.u0 += it.tiles;
+    if (++it.rt >= row_tiles<ROWS>(a, it.rq)) {
+        it.rt = 0;
+        if (++it.g >= a.n_kv) {
+            it.g = 0;
+            do it.rq = request(a, ++it.i);
+            while (it.rq.n <= 0);   // more units follow, so a later request has rows
+        }
+    }
+    open_tile<ROWS>(a, it);
+}
+
+// This block's units [u, end) of total, and the item that holds the first.
+struct Share {
+    long long u, end, total;
+    int blocks, i;               // blocks that have work; the request of unit u
+    long long base;              // the request's first unit
+};
+
+// Every thread of the block takes part (and passes two block barriers).
+template <int ROWS, int THREADS> __device__ __forceinline__ void share_out(const AttendArgs & a, Share * sh, long long * red) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.n_req;
+    const int per = (B + THREADS - 1) / THREADS, i0 = min(B, tid * per), i1 = min(B, i0 + per);
+    long long mine = 0;
+    for (int i = i0; i < i1; ++i) mine += units_of<ROWS>(a, request(a, i)) * a.n_kv;
+    long long x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) red[warp] = x;
+    __syncthreads();
+    long long base = x - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+        if (w < warp) base += red[w];
+        total += red[w];
+    }
+    const long long G = min(static_cast<long long>(gridDim.x), total), c = blockIdx.x;
+    const long long u = G ? c * total / G : 0, end = G ? (c + 1) * total / G : 0;
+    if (tid == 0) {
+        sh->u = u;
+        sh->end = c < G ? end : u;
+        sh->total = total;
+        sh->blocks = static_cast<int>(G);
+    }
+    if (c < G && u >= base && u < base + mine) {
+        int i = i0;
+        long long b = base;
+        for (;; ++i) {
+            const long long n = units_of<ROWS>(a, request(a, i)) * a.n_kv;
+            if (u < b + n) break;
+            b += n;
+        }
+        sh->i = i;
+        sh->base = b;
+    }
+    __syncthreads();
+}
+template <int ROWS> __device__ __forceinline__ Item first_item(const AttendArgs & a, const Share & sh) {
+    Item it{};
+    it.i = sh.i;
+    it.rq = request(a, it.i);
+    const long long per_head = units_of<ROWS>(a, it.rq);
+    it.g = static_cast<int>((sh.u - sh.base) / per_head);
+    it.u0 = sh.base + it.g * per_head;
+    it.rt = 0;
+    open_tile<ROWS>(a, it);
+    while (it.u0 + it.tiles <= sh.u) {
+        it.u0 += it.tiles;
+        ++it.rt;
+        open_tile<ROWS>(a, it);
+    }
+    return it;
+}
+__device__ __forceinline__ int block_of(const Share & sh, long long unit) { return static_cast<int>(((unit + 1) * sh.blocks - 1) / sh.total); }
+
+// A piece in the scratch: [rows][D] sums, then [rows] maxima and [rows] sums of weights.
+__device__ __forceinline__ float * piece(const AttendArgs & a, int block, int slot) {
+    return a.pieces + (static_cast<size_t>(block) * 2 + slot) * PagesScratch::PIECE_FLOATS;
+}
+
+// Row m of an item: where its q and its result are.
+template <class T> __device__ __forceinline__ T * row_at(const AttendArgs & a, const void * base, int64_t stride, const Item & it, int m) {
+    const int at = it.m0 + m;
+    return static_cast<T *>(const_cast<void *>(base)) + (it.rq.row0 + at / a.group) * stride + static_cast<int64_t>(it.g * a.group + at % a.group) * (a.head_dim);
+}
+__device__ __forceinline__ float * lse_at(const AttendArgs & a, const Item & it, int m) {
+    const int at = it.m0 + m;
+    return a.lse + static_cast<size_t>(it.rq.row0 + at / a.group) * a.n_head + it.g * a.group + at % a.group;
+}
+__device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f; }
+
+// One thread of a block whose piece is written: whether it is the item's last.
+__device__ __forceinline__ bool arrive_piece(const AttendArgs & a, const Share & sh, const Item & it) {
+    const int c0 = block_of(sh, it.u0), c1 = block_of(sh, it.u0 + it.tiles - 1);
+    if (atomicAdd(a.arrived + c0, 1) != c1 - c0) return false;
+    a.arrived[c0] = 0;
+    __threadfence();
+    return true;
+}
+
+// Joins the pieces of an item, in order; THREADS threads of the block, all of them.
+template <class T, class C, int ROWS, int D, int THREADS>
+__device__ __forceinline__ void join(const AttendArgs & a, const Share & sh, const Item & it, int tid) {
+    const int c0 = block_of(sh, it.u0), c1 = block_of(sh, it.u0 + it.tiles - 1);
+    constexpr int Q = D / 4;
+    for (int x = tid; x < it.m * Q; x += THREADS) {
+        const int m = x / Q, q = x % Q;
+        float top = -INFINITY;
+        for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(piece(a, c, c == c0) + ROWS * D + m));
+        const float ref = top == -INFINITY ? 0.f : top;
+        float l = 0.f;
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int c = c0; c <= c1; ++c) {
+            const float * p = piece(a, c, c == c0);
+            const float w = exp2_fast(__ldcg(p + ROWS * D + m) - ref);
+            const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + m * D) + q);
+            l += w * __ldcg(p + ROWS * D + ROWS + m);
+            s.x += w * v.x; s.y += w * v.y; s.z += w * v.z; s.w += w * v.w;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        T * dst = row_at<T>(a, a.out, a.out_stride, it, m) + 4 * q;
+        if constexpr (std::is_same_v<T, float>) *reinterpret_cast<float4 *>(dst) = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
+        else *reinterpret_cast<uint2 *>(dst) = make_uint2(pack<C>(s.x * inv, s.y * inv), pack<C>(s.z * inv, s.w * inv));
+        if (a.lse && q == 0) *lse_at(a, it, m) = lse_of(top, l);
+    }
+}
+
+// ---- waits --------------------------------------------------------------------------------------
+// Every wait for a copy or an MMA is bounded: past the deadline the block raises its abort flag and
+// the scratch's error word (navi_pages_check), and every role leaves its loops.
+
+constexpr unsigned long long DEADLINE_NS = 2000000000ull;
+
+struct Wait {
+    volatile int * abort;
+    int * err;
+    __device__ __forceinline__ bool operator()(uint64_t * bar, uint32_t parity) const {
+        for (int k = 0; k < 64; ++k)
+            if (mbar_try_wait(bar, parity)) return true;
+        const unsigned long long t0 = globaltimer();
+        while (!mbar_try_wait(bar, parity)) {
+            if (*abort) return false;
+            if (globaltimer() - t0 > DEADLINE_NS) {
+                *abort = 1;
+                atomicExch(err, 1);
+                return false;
+            }
+        }
+        return true;
+    }
+};
+
+// The same wait for copies that nothing stops any more, after an abort.
+__device__ __forceinline__ void mbar_drain(uint64_t * bar, uint32_t parity) {
+    const unsigned long long t0 = globaltimer();
+    while (!mbar_try_wait(bar, parity) && globaltimer() - t0 < 2 * DEADLINE_NS) {}
+}
+
+// Whether row j of the item's request sees token `key`.
+__device__ __forceinline__ bool sees(const AttendArgs & a, const Item & it, int key, int j) {
+    if (key >= it.n_keys) return false;
+    const int at = key - it.rq.ctx;
+    if (at < 0) return true;
+    if (!a.mask) return at <= j;
+    return at < 64 * a.mask_words && (__ldg(a.mask + static_cast<size_t>(it.rq.row0 + j) * a.mask_words + (at >> 6)) >> (at & 63) & 1);
+}
+
+// The pages that hold key tile t of an item, and the bytes of them that one pool contributes.
+__device__ __forceinline__ int tile_pages(const AttendArgs & a, const Item & it, int t) {
+    return (min(it.n_keys - t * KT, KT) + (1 << a.shift) - 1) >> a.shift;
+}
+// Those pages from one pool's map into dst: halves of 64 dims, each [KT][64] in 128-byte rows that
+// the copy swizzles; only pages with keys of the item, so rows past them keep what they held. One
+// thread; the bytes (tile_pages * page * D * 2) arrive on `bar`.
+template <int D>
+__device__ __forceinline__ void load_tile(const AttendArgs & a, const CUtensorMap * map, const Item & it, int t, int pages, uint8_t * dst, uint64_t * bar) {
+    for (int p = 0; p < pages; ++p) {
+        const int id = min(max(__ldg(it.rq.table + (t * KT >> a.shift) + p), 0), a.n_pages - 1), y = (id * a.n_kv + it.g) << a.shift;
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h) tma_box_2d(dst + h * (KT * 128) + (p << a.shift) * 128, map, h * 64, y, bar);
+    }
+}
+
+} // namespace navi::attn

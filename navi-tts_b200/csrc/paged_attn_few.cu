@@ -1,0 +1,350 @@
+// Attention over the paged KV cache for few rows of a request (paged_attn.cu): single tokens and
+// small drafted trees, on mma.sync tiles.
+#include "paged_attn.hpp"
+#include "paged_attn.cuh"
+
+namespace navi::attn {
+
+namespace {
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+// c (16x8 f32) += a (16x16, row) b (16x8, col), operands of the cache's type C
+template <class C> __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same_v<C, __half>)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// ---- few rows: mma.sync ------------------------------------------------------------------------
+//
+// RT tiles of 16 rows, 8 / RT warps to each, which divide a key tile of 128 between them, each with
+// a running maximum and sums of its own until the item ends; a ninth warp keeps a ring of tiles
+// full by TMA. K and V are read once however many rows there are, so up to 32 rows the bound is
+// HBM. f32 rows enter the products as two f16 terms, q = hi + lo and p = hi + lo, against the
+// exact cache values, about 22 bits; the tensor cores' sums truncate, so the low terms and each
+// tile's contribution are summed apart and added in f32. 16-bit rows are exact, and p is
+// rounded once to the type that the result has.
+template <int D> struct FewSmem {
+    static constexpr int STAGE = KT * D * 4;                    // K and V of a tile
+    static constexpr int STAGES = D == 128 ? 3 : 6;
+    static constexpr int JOIN = 4 * 16 * D * 4;                 // four warps' sums
+    static constexpr int BYTES = 1024 + STAGES * STAGE + JOIN;  // 1024: to align the ring to the swizzle's 1024 bytes
+};
+
+template <class T, class C, int D, int RT>
+__global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
+                                                       const __grid_constant__ CUtensorMap vmap) {
+    constexpr bool SPLIT = std::is_same_v<T, float>;
+    constexpr int ROWS = 16 * RT, KQ = 8 / RT, WK = KT / KQ;    // WK: keys of a tile that a warp takes
+    using L = FewSmem<D>;
+    extern __shared__ uint8_t raw[];
+    uint8_t * ring = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
+    float * sums = reinterpret_cast<float *>(ring + L::STAGES * L::STAGE);
+    __shared__ __align__(8) uint64_t full[L::STAGES], empty[L::STAGES];
+    __shared__ float stat[8][2][16];
+    __shared__ long long red[9];
+    __shared__ Share sh;
+    __shared__ int abort_flag, is_last;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, tq = lane & 3;
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < L::STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 8);
+        }
+        fence_mbar_init();
+    }
+    share_out<ROWS, 288>(a, &sh, red);
+    if (sh.u >= sh.end) return;
+    const Wait wait{&abort_flag, a.err};
+    Item it = first_item<ROWS>(a, sh);
+
+    if (warp == 8) {
+        if (lane != 0) return;
+        int n = 0;
+        for (long long u = sh.u; u < sh.end;) {
+            const int t0 = static_cast<int>(u - it.u0), t1 = static_cast<int>(min(static_cast<long long>(it.tiles), sh.end - it.u0));
+            if (it.n_keys > 0)
+                for (int t = t0; t < t1; ++t, ++n) {
+                    const int s = n % L::STAGES, pages = tile_pages(a, it, t);
+                    if (n >= L::STAGES && !wait(&empty[s], (n / L::STAGES - 1) & 1)) goto drain;
+                    uint8_t * dst = ring + s * L::STAGE;
+                    mbar_arrive_expect_tx(&full[s], static_cast<uint32_t>(2 * (pages << a.shift) * D * 2));
+                    load_tile<D>(a, &kmap, it, t, pages, dst, &full[s]);
+                    load_tile<D>(a, &vmap, it, t, pages, dst + L::STAGE / 2, &full[s]);
+                }
+            u += t1 - t0;
+            if (u < sh.end) next_item<ROWS>(a, it);
+        }
+    drain:
+        // after an abort the copies still under way land before the block's shared memory goes
+        if (abort_flag)
+            for (int k = max(n - L::STAGES, 0); k < n; ++k) mbar_drain(&full[k % L::STAGES], (k / L::STAGES) & 1);
+        return;
+    }
+
+    const int rt = warp / KQ, kq = warp % KQ, k0 = kq * WK;
+    const uint32_t ring_at = smem_addr(ring);
+    const auto at = [](uint32_t base, int key, int piece) { return base + (piece >> 3) * (KT * 128) + key * 128 + (((piece & 7) ^ (key & 7)) << 4); };
+    int n = 0;
+    for (long long u = sh.u; u < sh.end;) {
+        const int t0 = static_cast<int>(u - it.u0), t1 = static_cast<int>(min(static_cast<long long>(it.tiles), sh.end - it.u0));
+        // this thread's rows: gq and gq + 8 of its warp's 16
+        uint32_t qh[D / 16][4], ql[SPLIT ? D / 16 : 1][4];
+        int row[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int m = rt * 16 + gq + 8 * x;
+            const bool live = m < it.m;
+            row[x] = live ? (it.m0 + m) / a.group : 0;
+            const T * q = row_at<const T>(a, a.q, a.q_stride, it, live ? m : 0) + 2 * tq;
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    if constexpr (SPLIT) {
+                        const float2 f = live ? *reinterpret_cast<const float2 *>(q + ks * 16 + y * 8) : make_float2(0.f, 0.f);
+                        const uint32_t h = pack<C>(f.x, f.y);
+                        const float2 b = unpack<C>(h);
+                        qh[ks][2 * y + x] = h;
+                        ql[ks][2 * y + x] = pack<C>(f.x - b.x, f.y - b.y);
+                    } else {
+                        qh[ks][2 * y + x] = live ? *reinterpret_cast<const uint32_t *>(q + ks * 16 + y * 8) : 0u;
+                    }
+                }
+        }
+        float o[D / 8][4], mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < D / 8; ++x) o[x][0] = o[x][1] = o[x][2] = o[x][3] = 0.f;
+        if (it.n_keys > 0)
+            for (int t = t0; t < t1; ++t, ++n) {
+                const int st = n % L::STAGES;
+                if (!wait(&full[st], (n / L::STAGES) & 1)) break;
+                const uint32_t sk = ring_at + st * L::STAGE, sv = sk + L::STAGE / 2;
+                const int first = t * KT + k0, valid = it.n_keys - first;   // this warp's keys of the tile
+                if (valid > 0) {
+                    if (valid < WK) {   // rows past the item's keys: zeros, whatever the page holds there
+                        for (int x = lane; x < (WK - valid) * (D / 8); x += 32) {
+                            const int key = k0 + valid + x / (D / 8);
+                            *reinterpret_cast<uint4 *>(ring + (at(sv, key, x % (D / 8)) - ring_at)) = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    float s[WK / 8][4];
+#pragma unroll
+                    for (int x = 0; x < WK / 8; ++x) s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
+#pragma unroll
+                    for (int np = 0; np < WK / 16; ++np) {
+                        float low[2][4] = {};
+#pragma unroll
+                        for (int ks = 0; ks < D / 16; ++ks) {
+                            uint32_t b[4];
+                            ldsm4(b, at(sk, k0 + np * 16 + (lane & 7) + (lane >> 4) * 8, ks * 2 + ((lane >> 3) & 1)));
+                            mma<C>(s[2 * np], qh[ks], b[0], b[1]);
+                            mma<C>(s[2 * np + 1], qh[ks], b[2], b[3]);
+                            if constexpr (SPLIT) {
+                                mma<C>(low[0], ql[ks], b[0], b[1]);
+                                mma<C>(low[1], ql[ks], b[2], b[3]);
+                            }
+                        }
+                        if constexpr (SPLIT) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                s[2 * np][e] += low[0][e];
+                                s[2 * np + 1][e] += low[1][e];
+                            }
+                        }
+                    }
+                    if (first + WK > it.rq.ctx) {   // some of these keys are new rows, or past the last
+#pragma unroll
+                        for (int x = 0; x < WK / 8; ++x)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int key = first + x * 8 + 2 * tq + (e & 1);
+                                if (!sees(a, it, key, row[e >> 1])) s[x][e] = -INFINITY;
+                            }
+                    }
+                    float m[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                    for (int x = 0; x < WK / 8; ++x)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) m[e >> 1] = fmaxf(m[e >> 1], s[x][e]);
+                    bool more = false;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        m[x] = fmaxf(m[x], __shfl_xor_sync(0xffffffffu, m[x], 1));
+                        m[x] = fmaxf(m[x], __shfl_xor_sync(0xffffffffu, m[x], 2)) * a.scale;
+                        more = more || m[x] > mx[x];
+                    }
+                    if (__any_sync(0xffffffffu, more)) {
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            m[x] = fmaxf(m[x], mx[x]);
+                            const float w = m[x] == -INFINITY ? 1.f : exp2_fast(mx[x] - m[x]);
+                            mx[x] = m[x];
+                            l[x] *= w;
+#pragma unroll
+                            for (int d = 0; d < D / 8; ++d) {
+                                o[d][2 * x] *= w;
+                                o[d][2 * x + 1] *= w;
+                            }
+                        }
+                    }
+                    const float ref[2] = {mx[0] == -INFINITY ? 0.f : mx[0], mx[1] == -INFINITY ? 0.f : mx[1]};
+#pragma unroll
+                    for (int np = 0; np < WK / 16; ++np) {
+                        uint32_t ph[4], pl[4];
+#pragma unroll
+                        for (int y = 0; y < 2; ++y)
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                const float p0 = exp2_fast(fmaf(s[2 * np + y][2 * x], a.scale, -ref[x]));
+                                const float p1 = exp2_fast(fmaf(s[2 * np + y][2 * x + 1], a.scale, -ref[x]));
+                                l[x] += p0 + p1;
+                                ph[2 * y + x] = pack<C>(p0, p1);
+                                if constexpr (SPLIT) {
+                                    const float2 b = unpack<C>(ph[2 * y + x]);
+                                    pl[2 * y + x] = pack<C>(p0 - b.x, p1 - b.y);
+                                }
+                            }
+#pragma unroll
+                        for (int dp = 0; dp < D / 16; ++dp) {
+                            uint32_t b[4];
+                            ldsm4t(b, at(sv, k0 + np * 16 + (lane & 15), dp * 2 + (lane >> 4)));
+                            if constexpr (SPLIT) {
+                                float c[2][4] = {};
+                                mma<C>(c[0], pl, b[0], b[1]);
+                                mma<C>(c[1], pl, b[2], b[3]);
+                                mma<C>(c[0], ph, b[0], b[1]);
+                                mma<C>(c[1], ph, b[2], b[3]);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    o[2 * dp][e] += c[0][e];
+                                    o[2 * dp + 1][e] += c[1][e];
+                                }
+                            } else {
+                                mma<C>(o[2 * dp], ph, b[0], b[1]);
+                                mma<C>(o[2 * dp + 1], ph, b[2], b[3]);
+                            }
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[st]);
+            }
+
+        // the warps' sums of a row become one
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+            l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+            if (tq == 0) {
+                stat[warp][0][gq + 8 * x] = mx[x];
+                stat[warp][1][gq + 8 * x] = l[x];
+            }
+        }
+        named_sync(1, 256);
+        float top[2], sum[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            top[x] = -INFINITY;
+            sum[x] = 0.f;
+#pragma unroll
+            for (int k = 0; k < KQ; ++k) top[x] = fmaxf(top[x], stat[rt * KQ + k][0][gq + 8 * x]);
+            const float ref = top[x] == -INFINITY ? 0.f : top[x];
+#pragma unroll
+            for (int k = 0; k < KQ; ++k) sum[x] += stat[rt * KQ + k][1][gq + 8 * x] * exp2_fast(stat[rt * KQ + k][0][gq + 8 * x] - ref);
+            const float w = exp2_fast(mx[x] - ref);
+#pragma unroll
+            for (int d = 0; d < D / 8; ++d) {
+                o[d][2 * x] *= w;
+                o[d][2 * x + 1] *= w;
+            }
+        }
+#pragma unroll
+        for (int half = KQ / 2; half >= 1; half /= 2) {
+            float * slot = sums + static_cast<size_t>((kq % half) * RT + rt) * 16 * D + lane;
+            if (kq >= half && kq < 2 * half) {
+#pragma unroll
+                for (int d = 0; d < D / 8; ++d)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) slot[(d * 4 + e) * 32] = o[d][e];
+            }
+            named_sync(1, 256);
+            if (kq < half) {
+#pragma unroll
+                for (int d = 0; d < D / 8; ++d)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[d][e] += slot[(d * 4 + e) * 32];
+            }
+            if (half > 1) named_sync(1, 256);
+        }
+        const bool whole = t0 == 0 && t1 == it.tiles;
+        if (kq == 0) {
+            float * pc = piece(a, blockIdx.x, t0 == 0);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int m = rt * 16 + gq + 8 * x;
+                if (m >= it.m) continue;
+                if (whole) {
+                    const float inv = sum[x] == 0.f ? 0.f : 1.f / sum[x];
+                    T * dst = row_at<T>(a, a.out, a.out_stride, it, m) + 2 * tq;
+#pragma unroll
+                    for (int d = 0; d < D / 8; ++d) {
+                        const float v = o[d][2 * x] * inv, w = o[d][2 * x + 1] * inv;
+                        if constexpr (SPLIT) *reinterpret_cast<float2 *>(dst + d * 8) = make_float2(v, w);
+                        else *reinterpret_cast<uint32_t *>(dst + d * 8) = pack<C>(v, w);
+                    }
+                    if (a.lse && tq == 0) *lse_at(a, it, m) = lse_of(top[x], sum[x]);
+                } else {
+#pragma unroll
+                    for (int d = 0; d < D / 8; ++d) *reinterpret_cast<float2 *>(pc + m * D + d * 8 + 2 * tq) = make_float2(o[d][2 * x], o[d][2 * x + 1]);
+                    if (tq == 0) {
+                        pc[ROWS * D + m] = top[x];
+                        pc[ROWS * D + ROWS + m] = sum[x];
+                    }
+                }
+            }
+        }
+        if (!whole) {
+            __threadfence();
+            named_sync(1, 256);
+            if (tid == 0) is_last = arrive_piece(a, sh, it);
+            named_sync(1, 256);
+            if (is_last) join<T, C, ROWS, D, 256>(a, sh, it, tid);
+        }
+        u += t1 - t0;
+        if (u < sh.end) next_item<ROWS>(a, it);
+    }
+}
+
+template <class T, class C, int D> void few(const AttendArgs & a, const CUtensorMap & k, const CUtensorMap & v, int rows, int sms, cudaStream_t stream) {
+    const auto go = [&](auto kernel) {
+        NAVI_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, FewSmem<D>::BYTES));
+        kernel<<<sms, 288, FewSmem<D>::BYTES, stream>>>(a, k, v);
+    };
+    if (rows <= 16) go(k_attend_few<T, C, D, 1>);
+    else go(k_attend_few<T, C, D, 2>);
+    NAVI_CUDA(cudaGetLastError());
+}
+
+} // namespace
+
+void attend_few(const AttendArgs & a, const CUtensorMap & k, const CUtensorMap & v, int dtype, int cache, int rows, int sms, cudaStream_t stream) {
+    const bool wide = a.head_dim == 128;
+    if (dtype == NAVI_F32) wide ? few<float, __half, 128>(a, k, v, rows, sms, stream) : few<float, __half, 64>(a, k, v, rows, sms, stream);
+    else if (cache == NAVI_F16) wide ? few<__half, __half, 128>(a, k, v, rows, sms, stream) : few<__half, __half, 64>(a, k, v, rows, sms, stream);
+    else wide ? few<__nv_bfloat16, __nv_bfloat16, 128>(a, k, v, rows, sms, stream) : few<__nv_bfloat16, __nv_bfloat16, 64>(a, k, v, rows, sms, stream);
+}
+
+} // namespace navi::attn

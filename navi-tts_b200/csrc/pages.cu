@@ -4,6 +4,7 @@
 #include "pages.hpp"
 #include "device.cuh"
 
+#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -425,6 +426,27 @@ __global__ void __launch_bounds__(COMMIT_THREADS) k_pages_commit(const __grid_co
     }
 }
 
+// A pool as rows of head_dim values; a box is a page of one head, 64 dims wide, in 128-byte swizzled rows.
+CUtensorMap pool_map(void * pool, const navi_pages_desc & d) {
+    // the driver entry point is looked up at run time, so the library loads without libcuda
+    static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+    if (!encode) {
+        cudaDriverEntryPointQueryResult q{};
+        void * fn = nullptr;
+        NAVI_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
+        if (q != cudaDriverEntryPointSuccess || !fn) fail("pages: cuTensorMapEncodeTiled unavailable", NAVI_E_CUDA);
+        encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    }
+    CUtensorMap m{};
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(d.head_dim), static_cast<cuuint64_t>(d.n_pages) * d.n_kv_head * d.page_size};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(d.head_dim) * 2};
+    const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(d.page_size)}, one[2] = {1, 1};
+    const CUresult r = encode(&m, d.dtype == NAVI_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, pool, dims, strides, box, one,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) fail("pages: cuTensorMapEncodeTiled failed (" + std::to_string(static_cast<int>(r)) + ")", NAVI_E_CUDA);
+    return m;
+}
+
 bool aligned16(const void * p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 } // namespace
@@ -471,6 +493,8 @@ std::unique_ptr<Pages> Pages::create(const Device & dev, const navi_pages_desc &
     }
     p->d_.k = p->k_.data();
     p->d_.v = p->v_.data();
+    for (int l = 0; l < d.n_layer; ++l)
+        for (void * pool : {p->k_[static_cast<size_t>(l)], p->v_[static_cast<size_t>(l)]}) p->maps_.push_back(pool ? pool_map(pool, d) : CUtensorMap{});
     if (!given) {
         std::vector<int32_t> ids(static_cast<size_t>(d.n_pages));
         for (int i = 0; i < d.n_pages; ++i) ids[static_cast<size_t>(i)] = d.n_pages - 1 - i;
@@ -507,14 +531,15 @@ void Pages::plan(const navi_step & s, cudaStream_t stream) const {
     check_step(s, "pages plan");
     if (s.n_req == 0) return;
     NAVI_CUDA(cudaSetDevice(dev_->info().ordinal));
-    int * scratch = static_cast<int *>(dev_->scratch(stream, PagesScratch::BYTES));
-    PlanArgs a{s, d_.table, d_.held, d_.free_pages, d_.n_free, scratch, scratch + PagesScratch::TICKETS, d_.n_pages, shift_, d_.max_blocks, d_.max_requests};
+    const int sms = dev_->info().multiprocessors;
+    const PagesScratch sc(dev_->scratch(stream, PagesScratch::bytes(sms)), sms);
+    PlanArgs a{s, d_.table, d_.held, d_.free_pages, d_.n_free, sc.tickets, sc.broken, d_.n_pages, shift_, d_.max_blocks, d_.max_requests};
     const size_t smem = (4 * static_cast<size_t>(s.n_req) + 1) * sizeof(int);
     static_assert((4 * static_cast<size_t>(NAVI_PAGES_MAX_REQUESTS) + 1) * sizeof(int) < 200 * 1024);
     if (smem > 40 * 1024)
         NAVI_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(&k_pages_plan), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        static_cast<int>((4 * NAVI_PAGES_MAX_REQUESTS + 1) * sizeof(int))));
-    const int blocks = std::clamp((s.max_rows + PLAN_THREADS - 1) / PLAN_THREADS, 1, 2 * dev_->info().multiprocessors);
+    const int blocks = std::clamp((s.max_rows + PLAN_THREADS - 1) / PLAN_THREADS, 1, 2 * sms);
     k_pages_plan<<<blocks, PLAN_THREADS, smem, stream>>>(a);
     NAVI_CUDA(cudaGetLastError());
 }
@@ -574,6 +599,18 @@ void Pages::commit(const navi_step & s, const navi_commit_args & c, cudaStream_t
     const int z = std::clamp(4 * dev_->info().multiprocessors / s.n_req, 1, std::min(most, 65535));
     k_pages_commit<<<dim3(static_cast<unsigned>(s.n_req), static_cast<unsigned>(z)), COMMIT_THREADS, 0, stream>>>(a);
     NAVI_CUDA(cudaGetLastError());
+}
+
+void Pages::check(cudaStream_t stream) const {
+    NAVI_CUDA(cudaSetDevice(dev_->info().ordinal));
+    const int sms = dev_->info().multiprocessors;
+    const PagesScratch sc(dev_->scratch(stream, PagesScratch::bytes(sms)), sms);
+    int err = 0;
+    NAVI_CUDA(cudaMemcpyAsync(&err, sc.err, sizeof(int), cudaMemcpyDeviceToHost, stream));
+    NAVI_CUDA(cudaStreamSynchronize(stream));
+    if (!err) return;
+    NAVI_CUDA(cudaMemsetAsync(sc.tickets, 0, PagesScratch::ints(sms) * sizeof(int), stream));   // counters of blocks that gave up
+    fail("pages: a wait for a copy or a matrix product passed its deadline", NAVI_E_TIMEOUT);
 }
 
 } // namespace navi

@@ -6,6 +6,7 @@
 #include "../../include/navi_b200.h"
 #include "runtime.hpp"
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -25,6 +26,8 @@ public:
     void store(const navi_step & s, int layer, const navi_store_args & a, cudaStream_t stream) const;
     void attend(const navi_step & s, int layer, const navi_attend_args & a, cudaStream_t stream) const;
     void commit(const navi_step & s, const navi_commit_args & a, cudaStream_t stream) const;
+    // Waits for the stream; throws NAVI_E_TIMEOUT when a kernel on it gave up a wait since the last check.
+    void check(cudaStream_t stream) const;
 
 private:
     Pages() = default;
@@ -34,6 +37,7 @@ private:
     const Device * dev_ = nullptr;
     navi_pages_desc d_{};
     std::vector<void *> k_, v_;     // d_.k and d_.v point here
+    std::vector<CUtensorMap> maps_; // K, V of each layer: rows of head_dim, boxes of a page of one head x 64 dims
     std::vector<void *> owned_;
     int shift_ = 0;                 // log2(page_size)
 };
@@ -41,9 +45,17 @@ private:
 // The scratch of one stream (Device::scratch), laid out for every operator that hands work from
 // one block to another. All counters are zero between launches.
 struct PagesScratch {
-    static constexpr size_t TICKETS = 64;                                   // ints: launch-wide counters
-    static constexpr size_t BROKEN = NAVI_PAGES_MAX_REQUESTS;               // ints: plan, a request with a bad parent
-    static constexpr size_t BYTES = (TICKETS + BROKEN) * sizeof(int);
+    static constexpr size_t TICKETS = 64;                            // launch-wide counters
+    static constexpr size_t PIECE_FLOATS = 256 * (128 + 2);          // attend: one block's unfinished item
+    int * tickets, * broken, * arrived, * err;                       // broken: plan, a request with a bad parent
+    float * pieces;                                                  // two a block
+
+    // `blocks`: the most blocks of a launch that leave pieces (one a multiprocessor)
+    static size_t ints(int blocks) { return (TICKETS + NAVI_PAGES_MAX_REQUESTS + static_cast<size_t>(blocks) + 1 + 63) / 64 * 64; }
+    static size_t bytes(int blocks) { return ints(blocks) * sizeof(int) + 2 * static_cast<size_t>(blocks) * PIECE_FLOATS * sizeof(float); }
+    PagesScratch(void * p, int blocks)
+        : tickets(static_cast<int *>(p)), broken(tickets + TICKETS), arrived(broken + NAVI_PAGES_MAX_REQUESTS), err(arrived + blocks),
+          pieces(reinterpret_cast<float *>(tickets + ints(blocks))) {}
 };
 
 } // namespace navi

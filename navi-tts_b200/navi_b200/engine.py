@@ -304,6 +304,10 @@ class PagedKv:
         if st:
             check(st)
 
+    def check(self, stream: int | None = None) -> None:
+        """Waits for the stream; raises when a kernel of these calls on it gave up a wait."""
+        check(lib().navi_pages_check(self.h, self._stream if stream is None else stream))
+
     def close(self):
         if self.h:
             if _open(self.dev):
