@@ -10,6 +10,10 @@ namespace navi::attn {
 
 struct AttendArgs;
 
+// rows x heads of a KV head up to which the kernel for few rows is taken
+constexpr int FEW_ROWS = 32;
+
 void attend_few(const AttendArgs & a, const CUtensorMap & k, const CUtensorMap & v, int dtype, int cache, int rows, int sms, cudaStream_t stream);
+void attend_many(const AttendArgs & a, const CUtensorMap & k, const CUtensorMap & v, int dtype, int cache, int sms, cudaStream_t stream);
 
 } // namespace navi::attn

@@ -1,0 +1,438 @@
+// Attention over the paged KV cache for many rows of a request (paged_attn.cu): larger drafted
+// trees and chunks of prompts, on the tcgen05 tensor cores.
+#include "paged_attn.hpp"
+#include "paged_attn.cuh"
+#include "tmem.cuh"
+#include "umma.cuh"
+
+namespace navi::attn {
+
+namespace {
+
+using namespace navi::umma;
+
+// A block (one a multiprocessor) holds 128 or 256 rows x heads of an item. Two warpgroups do the
+// softmax, a thread a row; one thread feeds the ring of K and V tiles by TMA, one issues the MMAs.
+// Each warpgroup has its scores S (128 columns of tensor memory, its weights P written over them)
+// and its sums O (D columns), so that while one does its softmax the tensor cores work for the
+// other. With more than 128 rows the warpgroups take 128 rows each and share every K and V tile;
+// with fewer they take the key tiles in turn, each with a maximum and sums of its own, and join
+// them when the item ends.
+//
+// The MMA thread issues, for the pairs n = 0, 1, ... of (warpgroup n & 1, key tile):
+//   S(0) S(1) | P V(0) S(2) | P V(1) S(3) | ...     each P V after its warpgroup has written P
+// A commit covers all that was issued before it, so when S(n) is there P V(n - 2), the last to
+// touch this warpgroup's O, is done too, and the warpgroup may rescale O. It does so only where
+// a row's maximum grew by more than 2^8: weights up to 2^8 are as exact, and sums are f32.
+//
+// f32 rows: q and p as two f16 terms each against the exact cache values, as in the kernel for few
+// rows. Two tiles of q do not fit then, so their items have 128 rows.
+constexpr int LAZY = 8;
+
+template <class T, int D> struct ManySmem {
+    static constexpr bool SPLIT = std::is_same_v<T, float>;
+    static constexpr int QTILE = 128 * D * 2;                   // 128 rows, 16-bit: [D / 64][128][128 B], swizzled
+    static constexpr int STAGE = KT * D * 2;                    // K or V of a key tile
+    static constexpr int STAGES = D == 128 ? 5 : 8;
+    static constexpr int CONTROL = 3072;                        // ManyControl, and the tiles at 1024-byte boundaries
+    static constexpr int BYTES = CONTROL + 2 * QTILE + STAGES * STAGE;
+    static_assert(BYTES <= 227 * 1024);
+};
+
+struct ManyControl {
+    uint64_t full[8], empty[8], q_full, s_full[2], p_full[2], o_full[2], drained;
+    float stat[2][2][128];
+    long long red[12];
+    Share sh;
+    uint32_t tmem_at;
+    int abort_flag, is_last;
+};
+
+// K-major rows (Q, K): desc_kmajor_sw128 of umma.cuh. V is the B operand with its rows along the
+// summed dimension (MN-major): atoms of 64 dims x 8 keys, the next 8 keys 1024 bytes on, the next 64
+// dims `lbo` bytes on.
+__device__ __forceinline__ uint64_t desc_mnmajor_sw128(uint32_t addr, uint32_t lbo) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
+    d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16;
+    d |= static_cast<uint64_t>(1024 >> 4) << 32;
+    d |= static_cast<uint64_t>(1) << 46;
+    d |= static_cast<uint64_t>(2) << 61;
+    return d;
+}
+// kind::f16 with both operands f16 or both bf16, f32 sums; B along its rows when v_major
+template <class C> constexpr uint32_t idesc(int M, int N, bool v_major) {
+    constexpr uint32_t f = std::is_same_v<C, __nv_bfloat16> ? 1u : 0u;
+    return (1u << 4) | (f << 7) | (f << 10) | (v_major ? 1u << 16 : 0u) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+// D[tmem] (+)= A[tmem] B[smem]
+__device__ __forceinline__ void mma_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t id, bool accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(id), "r"(accumulate ? 1u : 0u)
+        : "memory");
+}
+
+// Bits 0..31: whether row j of the request sees the tokens ctx + a .. ctx + a + 31 (a may be negative:
+// those are cached tokens), of which `left` are the item's.
+__device__ __forceinline__ uint32_t seen_bits(const AttendArgs & a, const Item & it, int j, int at, int left) {
+    if (left <= 0) return 0u;
+    uint32_t b;
+    if (at + 31 < 0) b = ~0u;
+    else if (!a.mask) {
+        const int n = j - at + 1;            // tokens from `at` up to row j itself
+        b = n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
+    } else {
+        const uint64_t * m = a.mask + static_cast<size_t>(it.rq.row0 + j) * a.mask_words;
+        const int w = at >> 6;               // floor: -1 for the bits before row 0, all seen
+        const uint64_t lo = w < 0 ? ~0ull : w < a.mask_words ? __ldg(m + w) : 0ull;
+        const uint64_t hi = w + 1 < a.mask_words ? __ldg(m + w + 1) : 0ull;
+        const int s = at & 63;
+        b = static_cast<uint32_t>(s ? (lo >> s) | (hi << (64 - s)) : lo);
+    }
+    return left >= 32 ? b : b & ((1u << left) - 1u);
+}
+
+template <class T, class C, int D>
+__global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
+                                                        const __grid_constant__ CUtensorMap vmap) {
+    constexpr bool SPLIT = std::is_same_v<T, float>;
+    constexpr int ROWS = SPLIT ? 128 : 256;
+    using L = ManySmem<T, D>;
+    static_assert(sizeof(ManyControl) <= L::CONTROL && L::STAGES <= 8);
+    extern __shared__ __align__(1024) uint8_t raw[];   // all of the block's shared memory: at a 1024-byte boundary
+    ManyControl & S = *reinterpret_cast<ManyControl *>(raw);
+    uint8_t * qs = raw + L::CONTROL, * ring = qs + 2 * L::QTILE;
+    Share & sh = S.sh;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        S.abort_flag = 0;
+        for (int s = 0; s < L::STAGES; ++s) {
+            mbar_init(&S.full[s], 1);
+            mbar_init(&S.empty[s], 1);
+        }
+        mbar_init(&S.q_full, 256);
+        for (int g = 0; g < 2; ++g) {
+            mbar_init(&S.s_full[g], 1);
+            mbar_init(&S.p_full[g], 128);
+            mbar_init(&S.o_full[g], 1);
+        }
+        mbar_init(&S.drained, 1);
+        fence_mbar_init();
+    }
+    share_out<ROWS, 384>(a, &S.sh, S.red);
+    if (sh.u >= sh.end) return;
+    if (warp == 9) {
+        tmem_alloc(&S.tmem_at, 512);
+        tmem_relinquish();
+    }
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = S.tmem_at;
+    const Wait wait{&S.abort_flag, a.err};
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 8 && lane == 0) {
+            Item it = first_item<ROWS>(a, sh);
+            int n = 0;
+            bool ok = true;
+            for (long long u = sh.u; u < sh.end && ok;) {
+                const int t0 = static_cast<int>(u - it.u0), t1 = static_cast<int>(min(static_cast<long long>(it.tiles), sh.end - it.u0));
+                for (int t = t0; t < t1 && ok && it.n_keys > 0; ++t) {
+                    const int pages = tile_pages(a, it, t);
+                    for (int kv = 0; kv < 2 && ok; ++kv) {
+                        const int s = n % L::STAGES;
+                        ok = n < L::STAGES || wait(&S.empty[s], (n / L::STAGES - 1) & 1);
+                        if (!ok) break;
+                        mbar_arrive_expect_tx(&S.full[s], static_cast<uint32_t>((pages << a.shift) * D * 2));
+                        load_tile<D>(a, kv ? &vmap : &kmap, it, t, pages, ring + s * L::STAGE, &S.full[s]);
+                        ++n;
+                    }
+                }
+                u += t1 - t0;
+                if (u < sh.end) next_item<ROWS>(a, it);
+            }
+            // after an abort the copies still under way land before the block's shared memory goes
+            if (S.abort_flag)
+                for (int k = max(n - L::STAGES, 0); k < n; ++k) mbar_drain(&S.full[k % L::STAGES], (k / L::STAGES) & 1);
+        } else if (warp == 9 && lane == 0) {
+            Item it = first_item<ROWS>(a, sh);
+            constexpr uint32_t ID_S = idesc<C>(128, KT, false), ID_O = idesc<C>(128, D, true);
+            const uint32_t q_at = smem_addr(qs), ring_at = smem_addr(ring);
+            int base = 0, nq = 0, np[2] = {0, 0};
+            bool ok = true;
+            for (long long u = sh.u; u < sh.end && ok;) {
+                const int t0 = static_cast<int>(u - it.u0), t1 = static_cast<int>(min(static_cast<long long>(it.tiles), sh.end - it.u0));
+                const bool two = it.m > 128;
+                const int nt = it.n_keys > 0 ? t1 - t0 : 0, P = two ? 2 * nt : nt;
+                const auto tile = [&](int n) { return two ? n >> 1 : n; };
+                const auto scores = [&](int n) {
+                    const int g = n & 1, st = (base + 2 * tile(n)) % L::STAGES;
+                    if (!wait(&S.full[st], ((base + 2 * tile(n)) / L::STAGES) & 1)) return false;
+                    fence_after_sync();
+                    const uint32_t d = tmem + g * 128, q = q_at + (two ? g * L::QTILE : 0), k = ring_at + st * L::STAGE;
+#pragma unroll
+                    for (int term = 0; term < (SPLIT ? 2 : 1); ++term)
+#pragma unroll
+                        for (int ks = 0; ks < D / 16; ++ks) {
+                            const uint32_t o = (ks >> 2) * (128 * 128) + (ks & 3) * 32;
+                            mma_f16(d, desc_kmajor_sw128(q + (SPLIT ? (1 - term) * L::QTILE : 0) + o), desc_kmajor_sw128(k + o), ID_S, term > 0 || ks > 0);
+                        }
+                    commit(&S.s_full[g]);
+                    if (!two || g == 1) commit(&S.empty[st]);
+                    return true;
+                };
+                if (P > 0) {
+                    ok = wait(&S.q_full, nq & 1);
+                    fence_after_sync();
+                    ok = ok && scores(0) && (P < 2 || scores(1));
+                }
+                ++nq;
+                for (int n = 0; n < P && ok; ++n) {
+                    const int g = n & 1, idx = base + 2 * tile(n) + 1, st = idx % L::STAGES;
+                    ok = wait(&S.full[st], (idx / L::STAGES) & 1) && wait(&S.p_full[g], np[g] & 1);
+                    if (!ok) break;
+                    ++np[g];
+                    fence_after_sync();
+                    const uint32_t d = tmem + 256 + g * 128, p = tmem + g * 128, v = ring_at + st * L::STAGE;
+#pragma unroll
+                    for (int term = 0; term < (SPLIT ? 2 : 1); ++term)
+#pragma unroll
+                        for (int ks = 0; ks < KT / 16; ++ks)
+                            mma_ta(d, p + (SPLIT ? (1 - term) * 64 : 0) + ks * 8, desc_mnmajor_sw128(v + ks * 2048, KT * 128), ID_O, n > 1 || term > 0 || ks > 0);
+                    if (!two || g == 1) commit(&S.empty[st]);
+                    if (n + 2 >= P) commit(&S.o_full[g]);
+                    if (n + 2 < P) ok = scores(n + 2);
+                }
+                base += 2 * nt;
+                u += t1 - t0;
+                if (u < sh.end) next_item<ROWS>(a, it);
+            }
+            // nothing may still write the tensor memory when it is given back
+            commit(&S.drained);
+            mbar_drain(&S.drained, 0);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        Item it = first_item<ROWS>(a, sh);
+        const int wg = warp >> 2, r = tid & 127;
+        const uint32_t lane_at = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t s_at = tmem + lane_at + wg * 128, o_at = tmem + lane_at + 256 + wg * 128;
+        int base = 0, ns = 0, no = 0;
+        for (long long u = sh.u; u < sh.end;) {
+            const int t0 = static_cast<int>(u - it.u0), t1 = static_cast<int>(min(static_cast<long long>(it.tiles), sh.end - it.u0));
+            const bool two = it.m > 128;
+            const int nt = it.n_keys > 0 ? t1 - t0 : 0;
+            // q into shared memory: rows of 16-bit values (f32: the high terms, then the low ones)
+            if (nt > 0) {
+                for (int x = tid; x < (two ? 256 : 128) * (D / 8); x += 256) {
+                    const int m = x / (D / 8), c = x % (D / 8);
+                    uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+                    if (m < it.m) {
+                        const T * src = row_at<const T>(a, a.q, a.q_stride, it, m) + c * 8;
+                        if constexpr (SPLIT) {
+                            const float4 f = *reinterpret_cast<const float4 *>(src), g = *reinterpret_cast<const float4 *>(src + 4);
+                            const float w[8] = {f.x, f.y, f.z, f.w, g.x, g.y, g.z, g.w};
+                            uint32_t h[4], l[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                h[k] = pack<C>(w[2 * k], w[2 * k + 1]);
+                                const float2 b = unpack<C>(h[k]);
+                                l[k] = pack<C>(w[2 * k] - b.x, w[2 * k + 1] - b.y);
+                            }
+                            hi = make_uint4(h[0], h[1], h[2], h[3]);
+                            lo = make_uint4(l[0], l[1], l[2], l[3]);
+                        } else {
+                            hi = *reinterpret_cast<const uint4 *>(src);
+                        }
+                    }
+                    uint8_t * dst = qs + (m >> 7) * L::QTILE + (c >> 3) * (128 * 128) + (m & 127) * 128 + (((c & 7) ^ (m & 7)) << 4);
+                    *reinterpret_cast<uint4 *>(dst) = hi;
+                    if constexpr (SPLIT) *reinterpret_cast<uint4 *>(dst + L::QTILE) = lo;
+                }
+                fence_proxy_async_smem();
+            }
+            fence_before_sync();
+            if (nt > 0) mbar_arrive(&S.q_full);
+
+            const int m = (two ? wg * 128 : 0) + r, j = (it.m0 + min(m, it.m - 1)) / a.group;
+            float top = -INFINITY, sum = 0.f;
+            bool any = false;                             // this warpgroup has had a tile
+            for (int x = two ? 0 : wg; x < nt; x += two ? 1 : 2, ++ns) {
+                if (!wait(&S.s_full[wg], ns & 1)) break;
+                fence_after_sync();
+                uint32_t s[KT];
+                tmem_ld<64>(s_at, s);
+                tmem_ld<64>(s_at + 64, s + 64);
+                const int key0 = (t0 + x) * KT, left = it.n_keys - key0;
+                if (key0 + KT > it.rq.ctx) {              // some of these tokens are new rows, or past the last
+#pragma unroll
+                    for (int w = 0; w < KT / 32; ++w) {
+                        const uint32_t b = seen_bits(a, it, j, key0 + 32 * w - it.rq.ctx, left - 32 * w);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) s[32 * w + k] = b >> k & 1 ? s[32 * w + k] : __float_as_uint(-INFINITY);
+                    }
+                    if (left < KT) {                      // V rows past the last token: zeros, whatever the page holds there
+                        const int idx = base + 2 * x + 1, st = idx % L::STAGES;
+                        wait(&S.full[st], (idx / L::STAGES) & 1);
+                        for (int k = r; k < (KT - left) * (D / 8); k += 128) {
+                            const int key = left + k / (D / 8), c = k % (D / 8);
+                            *reinterpret_cast<uint4 *>(ring + st * L::STAGE + (c >> 3) * (KT * 128) + key * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_proxy_async_smem();
+                    }
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int k = 0; k < KT; ++k) mx[k & 3] = fmaxf(mx[k & 3], __uint_as_float(s[k]));
+                const float best = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale;
+                if (!any) {
+                    top = best;
+                } else if (__any_sync(0xffffffffu, best > top + LAZY)) {
+                    const float now = fmaxf(best, top), w = now == -INFINITY ? 1.f : exp2_fast(top - now);
+                    top = now;
+                    sum *= w;
+#pragma unroll
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld<32>(o_at + c, o);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * w);
+                        tmem_st<32>(o_at + c, o);
+                    }
+                }
+                any = true;
+                const float ref = top == -INFINITY ? 0.f : top;
+                float part[2] = {0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < KT; c += 32) {
+                    uint32_t hi[16], lo[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float p0 = exp2_fast(fmaf(__uint_as_float(s[c + 2 * k]), a.scale, -ref));
+                        const float p1 = exp2_fast(fmaf(__uint_as_float(s[c + 2 * k + 1]), a.scale, -ref));
+                        part[0] += p0;
+                        part[1] += p1;
+                        hi[k] = pack<C>(p0, p1);
+                        if constexpr (SPLIT) {
+                            const float2 b = unpack<C>(hi[k]);
+                            lo[k] = pack<C>(p0 - b.x, p1 - b.y);
+                        }
+                    }
+                    tmem_st<16>(s_at + c / 2, hi);
+                    if constexpr (SPLIT) tmem_st<16>(s_at + 64 + c / 2, lo);
+                }
+                sum += part[0] + part[1];
+                tmem_st_wait();
+                fence_before_sync();
+                mbar_arrive(&S.p_full[wg]);
+            }
+            base += 2 * nt;
+            if (any) {
+                wait(&S.o_full[wg], no & 1);
+                ++no;
+                fence_after_sync();
+            }
+
+            const bool whole = t0 == 0 && t1 == it.tiles;
+            float mine = 1.f;                             // what this warpgroup's O counts
+            if (!two) {
+                // the key tiles' two halves become one: the second warpgroup's sums go through the q tiles,
+                // which no MMA reads any more
+                S.stat[wg][0][r] = top;
+                S.stat[wg][1][r] = sum;
+                named_sync(1, 256);
+                const float t = fmaxf(S.stat[0][0][r], S.stat[1][0][r]), ref = t == -INFINITY ? 0.f : t;
+                mine = exp2_fast(top - ref);
+                sum = S.stat[0][1][r] * exp2_fast(S.stat[0][0][r] - ref) + S.stat[1][1][r] * exp2_fast(S.stat[1][0][r] - ref);
+                top = t;
+                if (wg == 1 && any) {
+                    float * dst = reinterpret_cast<float *>(qs) + r;
+#pragma unroll
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld<32>(o_at + c, o);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) dst[(c + k) * 128] = __uint_as_float(o[k]) * mine;
+                    }
+                }
+                named_sync(1, 256);
+            }
+            if (two || wg == 0) {
+                float * pc = piece(a, blockIdx.x, t0 == 0);
+                const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+                const bool other = !two && nt > 1, live = m < it.m;
+                const float * add = reinterpret_cast<const float *>(qs) + r;
+                T * dst = row_at<T>(a, a.out, a.out_stride, it, live ? m : 0);
+#pragma unroll
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    if (nt > 0) tmem_ld<32>(o_at + c, o);
+                    float v[32];
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) {
+                        v[k] = nt > 0 ? __uint_as_float(o[k]) * mine : 0.f;
+                        if (other) v[k] += add[(c + k) * 128];
+                        v[k] *= inv;
+                    }
+                    if (!live) continue;
+                    if (!whole) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4 *>(pc + static_cast<size_t>(m) * D + c + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                    } else if constexpr (SPLIT) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4 *>(dst + c + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 8)
+                            *reinterpret_cast<uint4 *>(dst + c + k) = make_uint4(pack<C>(v[k], v[k + 1]), pack<C>(v[k + 2], v[k + 3]), pack<C>(v[k + 4], v[k + 5]), pack<C>(v[k + 6], v[k + 7]));
+                    }
+                }
+                if (live && whole && a.lse) *lse_at(a, it, m) = lse_of(top, sum);
+                if (live && !whole) {
+                    pc[ROWS * D + m] = top;
+                    pc[ROWS * D + ROWS + m] = sum;
+                }
+            }
+            fence_before_sync();
+            if (!whole) __threadfence();
+            named_sync(1, 256);
+            if (!whole) {
+                if (tid == 0) S.is_last = arrive_piece(a, sh, it);
+                named_sync(1, 256);
+                if (S.is_last) join<T, C, ROWS, D, 256>(a, sh, it, tid);
+            }
+            u += t1 - t0;
+            if (u < sh.end) next_item<ROWS>(a, it);
+        }
+    }
+    __syncwarp();
+    fence_before_sync();
+    __syncthreads();
+    if (warp == 9) {
+        fence_after_sync();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <class T, class C, int D> void many(const AttendArgs & a, const CUtensorMap & k, const CUtensorMap & v, int sms, cudaStream_t stream) {
+    const auto kernel = k_attend_many<T, C, D>;
+    constexpr int smem = ManySmem<T, D>::BYTES;
+    NAVI_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    kernel<<<sms, 384, smem, stream>>>(a, k, v);
+    NAVI_CUDA(cudaGetLastError());
+}
+
+} // namespace
+
+void attend_many(const AttendArgs & a, const CUtensorMap & k, const CUtensorMap & v, int dtype, int cache, int sms, cudaStream_t stream) {
+    const bool wide = a.head_dim == 128;
+    if (dtype == NAVI_F32) wide ? many<float, __half, 128>(a, k, v, sms, stream) : many<float, __half, 64>(a, k, v, sms, stream);
+    else if (cache == NAVI_F16) wide ? many<__half, __half, 128>(a, k, v, sms, stream) : many<__half, __half, 64>(a, k, v, sms, stream);
+    else wide ? many<__nv_bfloat16, __nv_bfloat16, 128>(a, k, v, sms, stream) : many<__nv_bfloat16, __nv_bfloat16, 64>(a, k, v, sms, stream);
+}
+
+} // namespace navi::attn
