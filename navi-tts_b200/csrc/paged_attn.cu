@@ -30,8 +30,10 @@ void Pages::attend(const navi_step & s, int layer, const navi_attend_args & q, c
     const int sms = dev_->info().multiprocessors;
     const PagesScratch sc(dev_->scratch(stream, PagesScratch::bytes(sms)), sms);
     attn::AttendArgs a{q.q, q.out, q.lse, d_.table, s.req, s.ctx_len, s.cu_rows, s.status, s.parent ? s.mask : nullptr, sc.pieces, sc.arrived, sc.err,
-                 in, out, q.scale * 1.4426950408889634f, s.n_req, s.max_rows, s.mask_words, q.n_head, d_.n_kv_head, q.n_head / d_.n_kv_head, D, shift_,
+                 in, out, q.scale * 1.4426950408889634f, s.n_req, s.max_rows, s.mask_words, q.n_head, d_.n_kv_head, q.n_head / d_.n_kv_head, -1, D, shift_,
                  d_.n_pages, d_.max_blocks, d_.max_requests};
+    for (int b = 0; b < 12; ++b)
+        if (a.group == 1 << b) a.group_shift = b;
     const CUtensorMap & km = maps_[static_cast<size_t>(2 * layer)], & vm = maps_[static_cast<size_t>(2 * layer + 1)];
     const int64_t m = static_cast<int64_t>(std::min(s.max_new, s.max_rows)) * a.group;
     if (m <= attn::FEW_ROWS) return attn::attend_few(a, km, vm, q.dtype, d_.dtype, static_cast<int>(m), sms, stream);

@@ -26,26 +26,39 @@ struct AttendArgs {
     int * arrived, * err;
     int64_t q_stride, out_stride;
     float scale;                 // times log2(e)
-    int n_req, max_rows, mask_words, n_head, n_kv, group, head_dim, shift, n_pages, max_blocks, max_requests;
+    int n_req, max_rows, mask_words, n_head, n_kv, group, group_shift, head_dim, shift, n_pages, max_blocks, max_requests;
 };
 
 // What a block needs to know of one request.
 struct Request {
     int row0, n, ctx, keys;      // first row, rows, cached tokens, tokens in all
-    const int32_t * table;
+    int table;                   // its row of the block table
 };
 __device__ __forceinline__ Request request(const AttendArgs & a, int i) {
     Request r;
     r.row0 = a.cu_rows[i];
     r.n = max(min(a.cu_rows[i + 1], a.max_rows) - r.row0, 0);
     r.ctx = a.ctx_len[i];
-    const int tr = a.req ? a.req[i] : i;
-    const bool ok = a.status[i] == NAVI_OK && tr >= 0 && tr < a.max_requests && r.ctx >= 0 &&
+    r.table = a.req ? a.req[i] : i;
+    const bool ok = a.status[i] == NAVI_OK && r.table >= 0 && r.table < a.max_requests && r.ctx >= 0 &&
                     static_cast<long long>(r.ctx) + r.n <= (static_cast<long long>(a.max_blocks) << a.shift);
     r.keys = ok ? r.ctx + r.n : 0;
-    r.table = a.table + static_cast<size_t>(ok ? tr : 0) * a.max_blocks;
+    r.table = ok ? r.table : 0;
     return r;
 }
+// The requests from the block's first one on, in shared memory: a walk over items then costs no
+// trip to L2 for each.
+struct Window {
+    static constexpr int N = 32;
+    int first, count;
+    int row0[N], n[N], ctx[N], keys[N], table[N];
+};
+__device__ __forceinline__ Request request(const AttendArgs & a, const Window & w, int i) {
+    const int k = i - w.first;
+    if (k >= w.count) return request(a, i);
+    return {w.row0[k], w.n[k], w.ctx[k], w.keys[k], w.table[k]};
+}
+__device__ __forceinline__ int by_group(const AttendArgs & a, int x) { return a.group_shift >= 0 ? x >> a.group_shift : x / a.group; }
 
 template <class C> __device__ __forceinline__ uint32_t pack(float a, float b) {
     if constexpr (std::is_same_v<C, __half>) {
@@ -80,6 +93,19 @@ __device__ __forceinline__ float exp2_fast(float x) {
 
 constexpr int KT = 128;
 
+// x / y of values that are not negative: the 64-bit division is the slow one
+__device__ __forceinline__ long long cut(long long x, long long y) {
+    return (x | y) >> 32 ? x / y : static_cast<long long>(static_cast<uint32_t>(x) / static_cast<uint32_t>(y));
+}
+
+// This block's units [u, end) of total, and the item that holds the first.
+struct Share {
+    long long u, end, total;
+    int blocks, i;               // blocks that have work; the request of unit u
+    long long base;              // the request's first unit
+    Window window;
+};
+
 struct Item {
     int i, g, rt;                // request, KV head, row tile
     int tiles, n_keys;           // key tiles (1 at least) and keys that its rows may see
@@ -91,7 +117,7 @@ struct Item {
 template <int ROWS> __device__ __forceinline__ int row_tiles(const AttendArgs & a, const Request & r) { return (r.n * a.group + ROWS - 1) / ROWS; }
 template <int ROWS> __device__ __forceinline__ int keys_of(const AttendArgs & a, const Request & r, int rt) {
     if (a.mask || r.keys == 0) return r.keys;
-    return r.ctx + min(((rt + 1) * ROWS - 1) / a.group + 1, r.n);
+    return r.ctx + min(by_group(a, (rt + 1) * ROWS - 1) + 1, r.n);
 }
 __device__ __forceinline__ int tiles_of(int n_keys) { return max((n_keys + KT - 1) / KT, 1); }
 // the units of one KV head of a request
@@ -108,27 +134,20 @@ template <int ROWS> __device__ __forceinline__ void open_tile(const AttendArgs &
     it.m0 = it.rt * ROWS;
     it.m = min(it.rq.n * a.group - it.m0, ROWS);
 }
-template <int ROWS> __device__ __forceinline__ void next_item(const AttendArgs & a, Item & it) {
+template <int ROWS> __device__ __forceinline__ void next_item(const AttendArgs & a, const Share & sh, Item & it) {
     it.u0 += it.tiles;
     if (++it.rt >= row_tiles<ROWS>(a, it.rq)) {
         it.rt = 0;
         if (++it.g >= a.n_kv) {
             it.g = 0;
-            do it.rq = request(a, ++it.i);
+            do it.rq = request(a, sh.window, ++it.i);
             while (it.rq.n <= 0);   // more units follow, so a later request has rows
         }
     }
     open_tile<ROWS>(a, it);
 }
 
-// This block's units [u, end) of total, and the item that holds the first.
-struct Share {
-    long long u, end, total;
-    int blocks, i;               // blocks that have work; the request of unit u
-    long long base;              // the request's first unit
-};
-
-// Every thread of the block takes part (and passes two block barriers).
+// Every thread of the block takes part (and passes four block barriers).
 template <int ROWS, int THREADS> __device__ __forceinline__ void share_out(const AttendArgs & a, Share * sh, long long * red) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.n_req;
     const int per = (B + THREADS - 1) / THREADS, i0 = min(B, tid * per), i1 = min(B, i0 + per);
@@ -149,7 +168,7 @@ template <int ROWS, int THREADS> __device__ __forceinline__ void share_out(const
         total += red[w];
     }
     const long long G = min(static_cast<long long>(gridDim.x), total), c = blockIdx.x;
-    const long long u = G ? c * total / G : 0, end = G ? (c + 1) * total / G : 0;
+    const long long u = G ? cut(c * total, G) : 0, end = G ? cut((c + 1) * total, G) : 0;
     if (tid == 0) {
         sh->u = u;
         sh->end = c < G ? end : u;
@@ -159,24 +178,44 @@ template <int ROWS, int THREADS> __device__ __forceinline__ void share_out(const
     if (c < G && u >= base && u < base + mine) {
         int i = i0;
         long long b = base;
-        for (;; ++i) {
-            const long long n = units_of<ROWS>(a, request(a, i)) * a.n_kv;
-            if (u < b + n) break;
-            b += n;
-        }
+        if (per > 1)
+            for (;; ++i) {
+                const long long n = units_of<ROWS>(a, request(a, i)) * a.n_kv;
+                if (u < b + n) break;
+                b += n;
+            }
         sh->i = i;
         sh->base = b;
+    }
+    __syncthreads();
+    if (sh->u < sh->end && tid < Window::N) {
+        const int first = sh->i, count = min(Window::N, B - first);
+        if (tid < count) {
+            const Request r = request(a, first + tid);
+            sh->window.row0[tid] = r.row0;
+            sh->window.n[tid] = r.n;
+            sh->window.ctx[tid] = r.ctx;
+            sh->window.keys[tid] = r.keys;
+            sh->window.table[tid] = r.table;
+        }
+        if (tid == 0) {
+            sh->window.first = first;
+            sh->window.count = count;
+        }
     }
     __syncthreads();
 }
 template <int ROWS> __device__ __forceinline__ Item first_item(const AttendArgs & a, const Share & sh) {
     Item it{};
     it.i = sh.i;
-    it.rq = request(a, it.i);
+    it.rq = request(a, sh.window, it.i);
     const long long per_head = units_of<ROWS>(a, it.rq);
-    it.g = static_cast<int>((sh.u - sh.base) / per_head);
+    it.g = static_cast<int>(cut(sh.u - sh.base, per_head));
     it.u0 = sh.base + it.g * per_head;
-    it.rt = 0;
+    if (a.mask || it.rq.keys == 0) {   // every row tile has as many key tiles
+        it.rt = static_cast<int>(cut(sh.u - it.u0, tiles_of(it.rq.keys)));
+        it.u0 += static_cast<long long>(it.rt) * tiles_of(it.rq.keys);
+    }
     open_tile<ROWS>(a, it);
     while (it.u0 + it.tiles <= sh.u) {
         it.u0 += it.tiles;
@@ -185,21 +224,21 @@ template <int ROWS> __device__ __forceinline__ Item first_item(const AttendArgs 
     }
     return it;
 }
-__device__ __forceinline__ int block_of(const Share & sh, long long unit) { return static_cast<int>(((unit + 1) * sh.blocks - 1) / sh.total); }
+__device__ __forceinline__ int block_of(const Share & sh, long long unit) { return static_cast<int>(cut((unit + 1) * sh.blocks - 1, sh.total)); }
 
-// A piece in the scratch: [rows][D] sums, then [rows] maxima and [rows] sums of weights.
+// A piece in the scratch: the rows' sums as float4 [D / 4][ROWS], then [ROWS] maxima and [ROWS] sums of weights.
 __device__ __forceinline__ float * piece(const AttendArgs & a, int block, int slot) {
     return a.pieces + (static_cast<size_t>(block) * 2 + slot) * PagesScratch::PIECE_FLOATS;
 }
 
 // Row m of an item: where its q and its result are.
 template <class T> __device__ __forceinline__ T * row_at(const AttendArgs & a, const void * base, int64_t stride, const Item & it, int m) {
-    const int at = it.m0 + m;
-    return static_cast<T *>(const_cast<void *>(base)) + (it.rq.row0 + at / a.group) * stride + static_cast<int64_t>(it.g * a.group + at % a.group) * (a.head_dim);
+    const int at = it.m0 + m, j = by_group(a, at);
+    return static_cast<T *>(const_cast<void *>(base)) + (it.rq.row0 + j) * stride + static_cast<int64_t>(it.g * a.group + at - j * a.group) * a.head_dim;
 }
 __device__ __forceinline__ float * lse_at(const AttendArgs & a, const Item & it, int m) {
-    const int at = it.m0 + m;
-    return a.lse + static_cast<size_t>(it.rq.row0 + at / a.group) * a.n_head + it.g * a.group + at % a.group;
+    const int at = it.m0 + m, j = by_group(a, at);
+    return a.lse + static_cast<size_t>(it.rq.row0 + j) * a.n_head + it.g * a.group + at - j * a.group;
 }
 __device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f; }
 
@@ -212,31 +251,64 @@ __device__ __forceinline__ bool arrive_piece(const AttendArgs & a, const Share &
     return true;
 }
 
-// Joins the pieces of an item, in order; THREADS threads of the block, all of them.
-template <class T, class C, int ROWS, int D, int THREADS>
-__device__ __forceinline__ void join(const AttendArgs & a, const Share & sh, const Item & it, int tid) {
-    const int c0 = block_of(sh, it.u0), c1 = block_of(sh, it.u0 + it.tiles - 1);
-    constexpr int Q = D / 4;
-    for (int x = tid; x < it.m * Q; x += THREADS) {
-        const int m = x / Q, q = x % Q;
-        float top = -INFINITY;
-        for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(piece(a, c, c == c0) + ROWS * D + m));
-        const float ref = top == -INFINITY ? 0.f : top;
-        float l = 0.f;
-        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+// Joins the pieces of an item, in order: THREADS threads of the block, all of them. First what each
+// piece counts in each row goes to `weight` (CAP floats of shared memory), LANES lanes to a row,
+// then the sums are read, four rows a thread at a time.
+template <class T, class C, int ROWS, int D, int THREADS, int LANES, int CAP>
+__device__ __forceinline__ void join(const AttendArgs & a, const Share & sh, const Item & it, int tid, float * weight) {
+    const int c0 = block_of(sh, it.u0), np = block_of(sh, it.u0 + it.tiles - 1) - c0 + 1;
+    const auto part = [&](int p) { return piece(a, c0 + p, p == 0); };
+    const int most = CAP / np;                        // rows at a time: up to 256 blocks share an item
+    for (int m0 = 0; m0 < it.m; m0 += most) {
+        const int rows = min(most, it.m - m0), sub = tid % LANES;
+        for (int r = tid / LANES; r < (rows + THREADS / LANES - 1) / (THREADS / LANES) * (THREADS / LANES); r += THREADS / LANES) {
+            const bool live = r < rows;
+            const int m = m0 + (live ? r : 0);
+            float top = -INFINITY, l = 0.f;
 #pragma unroll 4
-        for (int c = c0; c <= c1; ++c) {
-            const float * p = piece(a, c, c == c0);
-            const float w = exp2_fast(__ldcg(p + ROWS * D + m) - ref);
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + m * D) + q);
-            l += w * __ldcg(p + ROWS * D + ROWS + m);
-            s.x += w * v.x; s.y += w * v.y; s.z += w * v.z; s.w += w * v.w;
+            for (int p = sub; p < np; p += LANES) top = fmaxf(top, __ldcg(part(p) + ROWS * D + m));
+#pragma unroll
+            for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll 4
+            for (int p = sub; p < np; p += LANES) {
+                const float w = exp2_fast(__ldcg(part(p) + ROWS * D + m) - ref);
+                l += w * __ldcg(part(p) + ROWS * D + ROWS + m);
+                if (live) weight[p * rows + r] = w;
+            }
+#pragma unroll
+            for (int o = 1; o < LANES; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            if (live)
+                for (int p = sub; p < np; p += LANES) weight[p * rows + r] *= inv;
+            if (live && sub == 0 && a.lse) *lse_at(a, it, m) = lse_of(top, l);
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        T * dst = row_at<T>(a, a.out, a.out_stride, it, m) + 4 * q;
-        if constexpr (std::is_same_v<T, float>) *reinterpret_cast<float4 *>(dst) = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
-        else *reinterpret_cast<uint2 *>(dst) = make_uint2(pack<C>(s.x * inv, s.y * inv), pack<C>(s.z * inv, s.w * inv));
-        if (a.lse && q == 0) *lse_at(a, it, m) = lse_of(top, l);
+        named_sync(1, THREADS);
+        for (int x0 = tid; x0 < rows * (D / 4); x0 += 4 * THREADS) {
+            float4 s[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+            for (int p = 0; p < np; ++p) {
+                const float4 * src = reinterpret_cast<const float4 *>(part(p)) + m0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int x = min(x0 + k * THREADS, rows * (D / 4) - 1), q = x / rows, r = x - q * rows;
+                    const float4 v = __ldcg(src + q * ROWS + r);
+                    const float w = weight[p * rows + r];
+                    s[k].x += w * v.x; s[k].y += w * v.y; s[k].z += w * v.z; s[k].w += w * v.w;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int x = x0 + k * THREADS, q = x / rows, r = x - q * rows;
+                if (x >= rows * (D / 4)) break;
+                T * dst = row_at<T>(a, a.out, a.out_stride, it, m0 + r) + 4 * q;
+                if constexpr (std::is_same_v<T, float>) *reinterpret_cast<float4 *>(dst) = s[k];
+                else *reinterpret_cast<uint2 *>(dst) = make_uint2(pack<C>(s[k].x, s[k].y), pack<C>(s[k].z, s[k].w));
+            }
+        }
+        named_sync(1, THREADS);
     }
 }
 
@@ -284,16 +356,18 @@ __device__ __forceinline__ bool sees(const AttendArgs & a, const Item & it, int 
 __device__ __forceinline__ int tile_pages(const AttendArgs & a, const Item & it, int t) {
     return (min(it.n_keys - t * KT, KT) + (1 << a.shift) - 1) >> a.shift;
 }
-// Those pages from one pool's map into dst: halves of 64 dims, each [KT][64] in 128-byte rows that
-// the copy swizzles; only pages with keys of the item, so rows past them keep what they held. One
-// thread; the bytes (tile_pages * page * D * 2) arrive on `bar`.
-template <int D>
-__device__ __forceinline__ void load_tile(const AttendArgs & a, const CUtensorMap * map, const Item & it, int t, int pages, uint8_t * dst, uint64_t * bar) {
-    for (int p = 0; p < pages; ++p) {
-        const int id = min(max(__ldg(it.rq.table + (t * KT >> a.shift) + p), 0), a.n_pages - 1), y = (id * a.n_kv + it.g) << a.shift;
-#pragma unroll
-        for (int h = 0; h < D / 64; ++h) tma_box_2d(dst + h * (KT * 128) + (p << a.shift) * 128, map, h * 64, y, bar);
-    }
+// A warp brings them from a pool's map to dst: halves of 64 dims, each [KT][64] in 128-byte rows that
+// the copy swizzles; only pages with keys of the item, so rows past them keep what they held.
+// The bytes (tile_pages * page * D * 2) arrive on `bar`. Lane x has the x-th box of the tile, at
+// most 16 of them (a page of 16 tokens, two halves), so the page ids, which it reads a tile ahead,
+// cost one latency together and not one each.
+template <int D> __device__ __forceinline__ int page_of_box(const AttendArgs & a, const Item & it, int t, int box) {
+    const int p = box / (D / 64);
+    return p < tile_pages(a, it, t) ? min(max(__ldg(a.table + static_cast<size_t>(it.rq.table) * a.max_blocks + (t * KT >> a.shift) + p), 0), a.n_pages - 1) : -1;
+}
+template <int D> __device__ __forceinline__ void load_box(const AttendArgs & a, const CUtensorMap * map, const Item & it, int page, int box, uint8_t * dst, uint64_t * bar) {
+    const int p = box / (D / 64), h = box % (D / 64);
+    if (page >= 0) tma_box_2d(dst + h * (KT * 128) + (p << a.shift) * 128, map, h * 64, (page * a.n_kv + it.g) << a.shift, bar);
 }
 
 } // namespace navi::attn

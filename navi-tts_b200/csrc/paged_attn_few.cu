@@ -69,23 +69,26 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
     Item it = first_item<ROWS>(a, sh);
 
     if (warp == 8) {
-        if (lane != 0) return;
         int n = 0;
-        for (long long u = sh.u; u < sh.end;) {
+        bool ok = true;
+        const int kv = lane >> 4, box = lane & 15;   // half a warp each for K and V
+        for (long long u = sh.u; u < sh.end && ok;) {
             const int t0 = static_cast<int>(u - it.u0), t1 = static_cast<int>(min(static_cast<long long>(it.tiles), sh.end - it.u0));
-            if (it.n_keys > 0)
+            if (it.n_keys > 0) {
+                int page = page_of_box<D>(a, it, t0, box);
                 for (int t = t0; t < t1; ++t, ++n) {
-                    const int s = n % L::STAGES, pages = tile_pages(a, it, t);
-                    if (n >= L::STAGES && !wait(&empty[s], (n / L::STAGES - 1) & 1)) goto drain;
-                    uint8_t * dst = ring + s * L::STAGE;
-                    mbar_arrive_expect_tx(&full[s], static_cast<uint32_t>(2 * (pages << a.shift) * D * 2));
-                    load_tile<D>(a, &kmap, it, t, pages, dst, &full[s]);
-                    load_tile<D>(a, &vmap, it, t, pages, dst + L::STAGE / 2, &full[s]);
+                    const int s = n % L::STAGES, next = t + 1 < t1 ? page_of_box<D>(a, it, t + 1, box) : -1;
+                    if (n >= L::STAGES) ok = __shfl_sync(0xffffffffu, lane == 0 ? wait(&empty[s], (n / L::STAGES - 1) & 1) : 0, 0);
+                    if (!ok) break;
+                    if (lane == 0) mbar_arrive_expect_tx(&full[s], static_cast<uint32_t>(2 * (tile_pages(a, it, t) << a.shift) * D * 2));
+                    __syncwarp();
+                    load_box<D>(a, kv ? &vmap : &kmap, it, page, box, ring + s * L::STAGE + kv * (L::STAGE / 2), &full[s]);
+                    page = next;
                 }
+            }
             u += t1 - t0;
-            if (u < sh.end) next_item<ROWS>(a, it);
+            if (u < sh.end) next_item<ROWS>(a, sh, it);
         }
-    drain:
         // after an abort the copies still under way land before the block's shared memory goes
         if (abort_flag)
             for (int k = max(n - L::STAGES, 0); k < n; ++k) mbar_drain(&full[k % L::STAGES], (k / L::STAGES) & 1);
@@ -105,7 +108,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
         for (int x = 0; x < 2; ++x) {
             const int m = rt * 16 + gq + 8 * x;
             const bool live = m < it.m;
-            row[x] = live ? (it.m0 + m) / a.group : 0;
+            row[x] = live ? by_group(a, it.m0 + m) : 0;
             const T * q = row_at<const T>(a, a.q, a.q_stride, it, live ? m : 0) + 2 * tq;
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks)
@@ -308,7 +311,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
                     if (a.lse && tq == 0) *lse_at(a, it, m) = lse_of(top[x], sum[x]);
                 } else {
 #pragma unroll
-                    for (int d = 0; d < D / 8; ++d) *reinterpret_cast<float2 *>(pc + m * D + d * 8 + 2 * tq) = make_float2(o[d][2 * x], o[d][2 * x + 1]);
+                    for (int d = 0; d < D / 8; ++d) *reinterpret_cast<float2 *>(pc + ((2 * d + (tq >> 1)) * ROWS + m) * 4 + 2 * (tq & 1)) = make_float2(o[d][2 * x], o[d][2 * x + 1]);
                     if (tq == 0) {
                         pc[ROWS * D + m] = top[x];
                         pc[ROWS * D + ROWS + m] = sum[x];
@@ -321,10 +324,10 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
             named_sync(1, 256);
             if (tid == 0) is_last = arrive_piece(a, sh, it);
             named_sync(1, 256);
-            if (is_last) join<T, C, ROWS, D, 256>(a, sh, it, tid);
+            if (is_last) join<T, C, ROWS, D, 256, 8, L::JOIN / 4>(a, sh, it, tid, sums);
         }
         u += t1 - t0;
-        if (u < sh.end) next_item<ROWS>(a, it);
+        if (u < sh.end) next_item<ROWS>(a, sh, it);
     }
 }
 

@@ -74,6 +74,12 @@ __device__ __forceinline__ void mma_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_
         : "memory");
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
 // Bits 0..31: whether row j of the request sees the tokens ctx + a .. ctx + a + 31 (a may be negative:
 // those are cached tokens), of which `left` are the item's.
 __device__ __forceinline__ uint32_t seen_bits(const AttendArgs & a, const Item & it, int j, int at, int left) {
@@ -135,25 +141,28 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (warp == 8 && lane == 0) {
+        if (warp == 8) {
             Item it = first_item<ROWS>(a, sh);
             int n = 0;
             bool ok = true;
             for (long long u = sh.u; u < sh.end && ok;) {
                 const int t0 = static_cast<int>(u - it.u0), t1 = static_cast<int>(min(static_cast<long long>(it.tiles), sh.end - it.u0));
+                int page = it.n_keys > 0 ? page_of_box<D>(a, it, t0, lane & 15) : -1;
                 for (int t = t0; t < t1 && ok && it.n_keys > 0; ++t) {
-                    const int pages = tile_pages(a, it, t);
+                    const int next = t + 1 < t1 ? page_of_box<D>(a, it, t + 1, lane & 15) : -1;
                     for (int kv = 0; kv < 2 && ok; ++kv) {
                         const int s = n % L::STAGES;
-                        ok = n < L::STAGES || wait(&S.empty[s], (n / L::STAGES - 1) & 1);
+                        if (n >= L::STAGES) ok = __shfl_sync(0xffffffffu, lane == 0 ? wait(&S.empty[s], (n / L::STAGES - 1) & 1) : 0, 0);
                         if (!ok) break;
-                        mbar_arrive_expect_tx(&S.full[s], static_cast<uint32_t>((pages << a.shift) * D * 2));
-                        load_tile<D>(a, kv ? &vmap : &kmap, it, t, pages, ring + s * L::STAGE, &S.full[s]);
+                        if (lane == 0) mbar_arrive_expect_tx(&S.full[s], static_cast<uint32_t>((tile_pages(a, it, t) << a.shift) * D * 2));
+                        __syncwarp();
+                        if (lane < 16) load_box<D>(a, kv ? &vmap : &kmap, it, page, lane, ring + s * L::STAGE, &S.full[s]);
                         ++n;
                     }
+                    page = next;
                 }
                 u += t1 - t0;
-                if (u < sh.end) next_item<ROWS>(a, it);
+                if (u < sh.end) next_item<ROWS>(a, sh, it);
             }
             // after an abort the copies still under way land before the block's shared memory goes
             if (S.abort_flag)
@@ -209,7 +218,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 }
                 base += 2 * nt;
                 u += t1 - t0;
-                if (u < sh.end) next_item<ROWS>(a, it);
+                if (u < sh.end) next_item<ROWS>(a, sh, it);
             }
             // nothing may still write the tensor memory when it is given back
             commit(&S.drained);
@@ -228,37 +237,50 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
             const int nt = it.n_keys > 0 ? t1 - t0 : 0;
             // q into shared memory: rows of 16-bit values (f32: the high terms, then the low ones)
             if (nt > 0) {
-                for (int x = tid; x < (two ? 256 : 128) * (D / 8); x += 256) {
-                    const int m = x / (D / 8), c = x % (D / 8);
-                    uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-                    if (m < it.m) {
-                        const T * src = row_at<const T>(a, a.q, a.q_stride, it, m) + c * 8;
-                        if constexpr (SPLIT) {
-                            const float4 f = *reinterpret_cast<const float4 *>(src), g = *reinterpret_cast<const float4 *>(src + 4);
-                            const float w[8] = {f.x, f.y, f.z, f.w, g.x, g.y, g.z, g.w};
-                            uint32_t h[4], l[4];
+                constexpr int CH = D / 8, STEP = 256 / CH, U = 128 / STEP;   // 16-byte pieces of a row; rows a pass; passes a tile
+                const int c = tid % CH;
+                for (int m1 = tid / CH; m1 < (two ? 256 : 128); m1 += 128) {
+                    uint4 v[U], w[SPLIT ? U : 1];
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                h[k] = pack<C>(w[2 * k], w[2 * k + 1]);
-                                const float2 b = unpack<C>(h[k]);
-                                l[k] = pack<C>(w[2 * k] - b.x, w[2 * k + 1] - b.y);
-                            }
-                            hi = make_uint4(h[0], h[1], h[2], h[3]);
-                            lo = make_uint4(l[0], l[1], l[2], l[3]);
-                        } else {
-                            hi = *reinterpret_cast<const uint4 *>(src);
+                    for (int k = 0; k < U; ++k) {
+                        const int m = m1 + k * STEP;
+                        v[k] = make_uint4(0, 0, 0, 0);
+                        if constexpr (SPLIT) w[k] = v[k];
+                        if (m < it.m) {
+                            const uint4 * src = reinterpret_cast<const uint4 *>(row_at<const T>(a, a.q, a.q_stride, it, m) + c * 8);
+                            v[k] = __ldg(src);
+                            if constexpr (SPLIT) w[k] = __ldg(src + 1);
                         }
                     }
-                    uint8_t * dst = qs + (m >> 7) * L::QTILE + (c >> 3) * (128 * 128) + (m & 127) * 128 + (((c & 7) ^ (m & 7)) << 4);
-                    *reinterpret_cast<uint4 *>(dst) = hi;
-                    if constexpr (SPLIT) *reinterpret_cast<uint4 *>(dst + L::QTILE) = lo;
+#pragma unroll
+                    for (int k = 0; k < U; ++k) {
+                        const int m = m1 + k * STEP;
+                        uint8_t * dst = qs + (m >> 7) * L::QTILE + (c >> 3) * (128 * 128) + (m & 127) * 128 + (((c & 7) ^ (m & 7)) << 4);
+                        if constexpr (SPLIT) {
+                            const uint32_t f[8] = {v[k].x, v[k].y, v[k].z, v[k].w, w[k].x, w[k].y, w[k].z, w[k].w};
+                            uint32_t h[4], l[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float f0 = __uint_as_float(f[2 * e]), f1 = __uint_as_float(f[2 * e + 1]);
+                                h[e] = pack<C>(f0, f1);
+                                const float2 b = unpack<C>(h[e]);
+                                l[e] = pack<C>(f0 - b.x, f1 - b.y);
+                            }
+                            *reinterpret_cast<uint4 *>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
+                            *reinterpret_cast<uint4 *>(dst + L::QTILE) = make_uint4(l[0], l[1], l[2], l[3]);
+                        } else {
+                            *reinterpret_cast<uint4 *>(dst) = v[k];
+                        }
+                    }
                 }
                 fence_proxy_async_smem();
             }
             fence_before_sync();
             if (nt > 0) mbar_arrive(&S.q_full);
 
-            const int m = (two ? wg * 128 : 0) + r, j = (it.m0 + min(m, it.m - 1)) / a.group;
+            const int m = (two ? wg * 128 : 0) + r, j = by_group(a, it.m0 + min(m, it.m - 1));
+            // every row of the warp sees the tokens before `open`
+            const int open = it.rq.ctx + (a.mask ? 0 : by_group(a, it.m0 + min((two ? wg * 128 : 0) + (warp & 3) * 32, it.m - 1)) + 1);
             float top = -INFINITY, sum = 0.f;
             bool any = false;                             // this warpgroup has had a tile
             for (int x = two ? 0 : wg; x < nt; x += two ? 1 : 2, ++ns) {
@@ -268,7 +290,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 tmem_ld<64>(s_at, s);
                 tmem_ld<64>(s_at + 64, s + 64);
                 const int key0 = (t0 + x) * KT, left = it.n_keys - key0;
-                if (key0 + KT > it.rq.ctx) {              // some of these tokens are new rows, or past the last
+                if (key0 + KT > open) {                   // some of these tokens are not seen by every row of the warp
 #pragma unroll
                     for (int w = 0; w < KT / 32; ++w) {
                         const uint32_t b = seen_bits(a, it, j, key0 + 32 * w - it.rq.ctx, left - 32 * w);
@@ -287,7 +309,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 }
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int k = 0; k < KT; ++k) mx[k & 3] = fmaxf(mx[k & 3], __uint_as_float(s[k]));
+                for (int k = 0; k < KT; k += 2) mx[k / 2 & 3] = max3(mx[k / 2 & 3], __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
                 const float best = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale;
                 if (!any) {
                     top = best;
@@ -306,26 +328,26 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 }
                 any = true;
                 const float ref = top == -INFINITY ? 0.f : top;
-                float part[2] = {0.f, 0.f};
+                const float2 scale2 = make_float2(a.scale, a.scale), ref2 = make_float2(-ref, -ref);
+                float2 part[2] = {};
 #pragma unroll
                 for (int c = 0; c < KT; c += 32) {
                     uint32_t hi[16], lo[16];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        const float p0 = exp2_fast(fmaf(__uint_as_float(s[c + 2 * k]), a.scale, -ref));
-                        const float p1 = exp2_fast(fmaf(__uint_as_float(s[c + 2 * k + 1]), a.scale, -ref));
-                        part[0] += p0;
-                        part[1] += p1;
-                        hi[k] = pack<C>(p0, p1);
+                        const float2 e = __ffma2_rn(make_float2(__uint_as_float(s[c + 2 * k]), __uint_as_float(s[c + 2 * k + 1])), scale2, ref2);
+                        const float2 w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                        part[k & 1] = __fadd2_rn(part[k & 1], w);
+                        hi[k] = pack<C>(w.x, w.y);
                         if constexpr (SPLIT) {
                             const float2 b = unpack<C>(hi[k]);
-                            lo[k] = pack<C>(p0 - b.x, p1 - b.y);
+                            lo[k] = pack<C>(w.x - b.x, w.y - b.y);
                         }
                     }
                     tmem_st<16>(s_at + c / 2, hi);
                     if constexpr (SPLIT) tmem_st<16>(s_at + 64 + c / 2, lo);
                 }
-                sum += part[0] + part[1];
+                sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
                 tmem_st_wait();
                 fence_before_sync();
                 mbar_arrive(&S.p_full[wg]);
@@ -339,9 +361,11 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
 
             const bool whole = t0 == 0 && t1 == it.tiles;
             float mine = 1.f;                             // what this warpgroup's O counts
+            float * const half = reinterpret_cast<float *>(qs);
+            int c_lo = 0, c_hi = D;                       // the columns that this warpgroup finishes
             if (!two) {
-                // the key tiles' two halves become one: the second warpgroup's sums go through the q tiles,
-                // which no MMA reads any more
+                // the key tiles' two halves become one: each warpgroup finishes half of the columns and hands
+                // the other half over through the q tiles, which no MMA reads any more
                 S.stat[wg][0][r] = top;
                 S.stat[wg][1][r] = sum;
                 named_sync(1, 256);
@@ -349,39 +373,49 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 mine = exp2_fast(top - ref);
                 sum = S.stat[0][1][r] * exp2_fast(S.stat[0][0][r] - ref) + S.stat[1][1][r] * exp2_fast(S.stat[1][0][r] - ref);
                 top = t;
-                if (wg == 1 && any) {
-                    float * dst = reinterpret_cast<float *>(qs) + r;
+                c_lo = wg * (D / 2);
+                c_hi = c_lo + D / 2;
+                if (any && nt > 1) {
+                    const int give = (1 - wg) * (D / 2);
 #pragma unroll
-                    for (int c = 0; c < D; c += 32) {
+                    for (int c = 0; c < D / 2; c += 32) {
                         uint32_t o[32];
-                        tmem_ld<32>(o_at + c, o);
+                        tmem_ld<32>(o_at + give + c, o);
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) dst[(c + k) * 128] = __uint_as_float(o[k]) * mine;
+                        for (int k = 0; k < 32; ++k) half[(give + c + k) * 128 + r] = __uint_as_float(o[k]) * mine;
+                    }
+                } else if (any) {                         // the only one with a tile: the other has nothing to add
+#pragma unroll
+                    for (int c = 0; c < D / 2; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld<32>(o_at + D / 2 + c, o);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) half[(D / 2 + c + k) * 128 + r] = __uint_as_float(o[k]) * mine;
                     }
                 }
                 named_sync(1, 256);
             }
-            if (two || wg == 0) {
-                float * pc = piece(a, blockIdx.x, t0 == 0);
+            {
+                float4 * pc = reinterpret_cast<float4 *>(piece(a, blockIdx.x, t0 == 0)) + m;
                 const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
-                const bool other = !two && nt > 1, live = m < it.m;
-                const float * add = reinterpret_cast<const float *>(qs) + r;
+                const bool other = !two && (wg == 1 ? nt > 0 : nt > 1), live = m < it.m;
                 T * dst = row_at<T>(a, a.out, a.out_stride, it, live ? m : 0);
-#pragma unroll
-                for (int c = 0; c < D; c += 32) {
+                for (int c = c_lo; c < c_hi; c += 32) {
                     uint32_t o[32];
-                    if (nt > 0) tmem_ld<32>(o_at + c, o);
+                    if (any) tmem_ld<32>(o_at + c, o);
                     float v[32];
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        v[k] = nt > 0 ? __uint_as_float(o[k]) * mine : 0.f;
-                        if (other) v[k] += add[(c + k) * 128];
-                        v[k] *= inv;
+                    for (int k = 0; k < 32; ++k) v[k] = any ? __uint_as_float(o[k]) * mine : 0.f;
+                    if (other) {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) v[k] += half[(c + k) * 128 + r];
                     }
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) v[k] *= inv;
                     if (!live) continue;
                     if (!whole) {
 #pragma unroll
-                        for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4 *>(pc + static_cast<size_t>(m) * D + c + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                        for (int k = 0; k < 32; k += 4) pc[(c + k) / 4 * ROWS] = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
                     } else if constexpr (SPLIT) {
 #pragma unroll
                         for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4 *>(dst + c + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
@@ -391,10 +425,14 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                             *reinterpret_cast<uint4 *>(dst + c + k) = make_uint4(pack<C>(v[k], v[k + 1]), pack<C>(v[k + 2], v[k + 3]), pack<C>(v[k + 4], v[k + 5]), pack<C>(v[k + 6], v[k + 7]));
                     }
                 }
-                if (live && whole && a.lse) *lse_at(a, it, m) = lse_of(top, sum);
-                if (live && !whole) {
-                    pc[ROWS * D + m] = top;
-                    pc[ROWS * D + ROWS + m] = sum;
+                if (live && (two || wg == 0)) {
+                    if (whole) {
+                        if (a.lse) *lse_at(a, it, m) = lse_of(top, sum);
+                    } else {
+                        float * st = piece(a, blockIdx.x, t0 == 0) + ROWS * D + m;
+                        st[0] = top;
+                        st[ROWS] = sum;
+                    }
                 }
             }
             fence_before_sync();
@@ -403,10 +441,10 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
             if (!whole) {
                 if (tid == 0) S.is_last = arrive_piece(a, sh, it);
                 named_sync(1, 256);
-                if (S.is_last) join<T, C, ROWS, D, 256>(a, sh, it, tid);
+                if (S.is_last) join<T, C, ROWS, D, 256, 1, 2 * L::QTILE / 4>(a, sh, it, tid, reinterpret_cast<float *>(qs));
             }
             u += t1 - t0;
-            if (u < sh.end) next_item<ROWS>(a, it);
+            if (u < sh.end) next_item<ROWS>(a, sh, it);
         }
     }
     __syncwarp();
