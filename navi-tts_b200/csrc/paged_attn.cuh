@@ -50,6 +50,7 @@ __device__ __forceinline__ Request request(const AttendArgs & a, int i) {
 // trip to L2 for each.
 struct Window {
     static constexpr int N = 32;
+    long long base;              // the first unit of request `first`
     int first, count;
     int row0[N], n[N], ctx[N], keys[N], table[N];
 };
@@ -103,7 +104,6 @@ struct Share {
     long long u, end, total;
     int blocks, i;               // blocks that have work; the request of unit u
     long long base;              // the request's first unit
-    Window window;
 };
 
 struct Item {
@@ -134,81 +134,107 @@ template <int ROWS> __device__ __forceinline__ void open_tile(const AttendArgs &
     it.m0 = it.rt * ROWS;
     it.m = min(it.rq.n * a.group - it.m0, ROWS);
 }
-template <int ROWS> __device__ __forceinline__ void next_item(const AttendArgs & a, const Share & sh, Item & it) {
+template <int ROWS> __device__ __forceinline__ void next_item(const AttendArgs & a, const Window & win, Item & it) {
     it.u0 += it.tiles;
     if (++it.rt >= row_tiles<ROWS>(a, it.rq)) {
         it.rt = 0;
         if (++it.g >= a.n_kv) {
             it.g = 0;
-            do it.rq = request(a, sh.window, ++it.i);
+            do it.rq = request(a, win, ++it.i);
             while (it.rq.n <= 0);   // more units follow, so a later request has rows
         }
     }
     open_tile<ROWS>(a, it);
 }
 
-// Every thread of the block takes part (and passes four block barriers).
-template <int ROWS, int THREADS> __device__ __forceinline__ void share_out(const AttendArgs & a, Share * sh, long long * red) {
+// Every thread of the block takes part. It holds the block's only barriers before the roles part, so
+// what the block's threads write to shared memory before the call is there for all after it.
+// Up to 32 requests every warp does the sums by itself, a lane a request: one trip to L2 and no
+// barrier between.
+template <int ROWS, int THREADS> __device__ __forceinline__ void share_out(const AttendArgs & a, Window & win, Share & out, long long * red) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.n_req;
-    const int per = (B + THREADS - 1) / THREADS, i0 = min(B, tid * per), i1 = min(B, i0 + per);
+    const bool one = B <= 32;
+    const int per = one ? 1 : (B + THREADS - 1) / THREADS, i0 = min(B, one ? lane : tid * per), i1 = min(B, i0 + per);
     long long mine = 0;
-    for (int i = i0; i < i1; ++i) mine += units_of<ROWS>(a, request(a, i)) * a.n_kv;
+    Request r{};
+    for (int i = i0; i < i1; ++i) {
+        r = request(a, i);
+        mine += units_of<ROWS>(a, r) * a.n_kv;
+    }
     long long x = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const long long y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
-    if (lane == 31) red[warp] = x;
-    __syncthreads();
-    long long base = x - mine, total = 0;
+    long long base = x - mine, total = __shfl_sync(0xffffffffu, x, 31);
+    if (!one) {
+        if (lane == 31) red[warp] = x;
+        __syncthreads();
+        total = 0;
 #pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) {
-        if (w < warp) base += red[w];
-        total += red[w];
+        for (int w = 0; w < THREADS / 32; ++w) {
+            if (w < warp) base += red[w];
+            total += red[w];
+        }
     }
+    Share sh;
     const long long G = min(static_cast<long long>(gridDim.x), total), c = blockIdx.x;
-    const long long u = G ? cut(c * total, G) : 0, end = G ? cut((c + 1) * total, G) : 0;
-    if (tid == 0) {
-        sh->u = u;
-        sh->end = c < G ? end : u;
-        sh->total = total;
-        sh->blocks = static_cast<int>(G);
-    }
-    if (c < G && u >= base && u < base + mine) {
-        int i = i0;
-        long long b = base;
-        if (per > 1)
-            for (;; ++i) {
-                const long long n = units_of<ROWS>(a, request(a, i)) * a.n_kv;
-                if (u < b + n) break;
-                b += n;
-            }
-        sh->i = i;
-        sh->base = b;
-    }
-    __syncthreads();
-    if (sh->u < sh->end && tid < Window::N) {
-        const int first = sh->i, count = min(Window::N, B - first);
-        if (tid < count) {
-            const Request r = request(a, first + tid);
-            sh->window.row0[tid] = r.row0;
-            sh->window.n[tid] = r.n;
-            sh->window.ctx[tid] = r.ctx;
-            sh->window.keys[tid] = r.keys;
-            sh->window.table[tid] = r.table;
+    sh.total = total;
+    sh.blocks = static_cast<int>(G);
+    sh.u = G ? cut(c * total, G) : 0;
+    sh.end = c < G ? cut((c + 1) * total, G) : sh.u;
+    const bool holds = c < G && sh.u >= base && sh.u < base + mine;
+    if (one) {
+        const int from = __ffs(__ballot_sync(0xffffffffu, holds)) - 1;
+        sh.i = max(from, 0);
+        sh.base = __shfl_sync(0xffffffffu, base, sh.i);
+        if (warp == 0 && lane < B) {
+            win.row0[lane] = r.row0;
+            win.n[lane] = r.n;
+            win.ctx[lane] = r.ctx;
+            win.keys[lane] = r.keys;
+            win.table[lane] = r.table;
         }
         if (tid == 0) {
-            sh->window.first = first;
-            sh->window.count = count;
+            win.first = 0;
+            win.count = B;
+        }
+    } else {
+        if (holds) {
+            int i = i0;
+            long long b = base;
+            for (;; ++i) {
+                const long long n = units_of<ROWS>(a, request(a, i)) * a.n_kv;
+                if (sh.u < b + n) break;
+                b += n;
+            }
+            win.first = i;
+            win.base = b;
+        }
+        __syncthreads();
+        sh.i = win.first;
+        sh.base = win.base;
+        if (sh.u < sh.end && tid < Window::N) {
+            const int count = min(Window::N, B - sh.i);
+            if (tid < count) {
+                const Request q = request(a, sh.i + tid);
+                win.row0[tid] = q.row0;
+                win.n[tid] = q.n;
+                win.ctx[tid] = q.ctx;
+                win.keys[tid] = q.keys;
+                win.table[tid] = q.table;
+            }
+            if (tid == 0) win.count = count;
         }
     }
+    if (tid == 0) out = sh;
     __syncthreads();
 }
-template <int ROWS> __device__ __forceinline__ Item first_item(const AttendArgs & a, const Share & sh) {
+template <int ROWS> __device__ __forceinline__ Item first_item(const AttendArgs & a, const Window & win, const Share & sh) {
     Item it{};
     it.i = sh.i;
-    it.rq = request(a, sh.window, it.i);
+    it.rq = request(a, win, it.i);
     const long long per_head = units_of<ROWS>(a, it.rq);
     it.g = static_cast<int>(cut(sh.u - sh.base, per_head));
     it.u0 = sh.base + it.g * per_head;
@@ -253,7 +279,7 @@ __device__ __forceinline__ bool arrive_piece(const AttendArgs & a, const Share &
 
 // Joins the pieces of an item, in order: THREADS threads of the block, all of them. First what each
 // piece counts in each row goes to `weight` (CAP floats of shared memory), LANES lanes to a row,
-// then the sums are read, four rows a thread at a time.
+// then the sums are read.
 template <class T, class C, int ROWS, int D, int THREADS, int LANES, int CAP>
 __device__ __forceinline__ void join(const AttendArgs & a, const Share & sh, const Item & it, int tid, float * weight) {
     const int c0 = block_of(sh, it.u0), np = block_of(sh, it.u0 + it.tiles - 1) - c0 + 1;
@@ -284,32 +310,44 @@ __device__ __forceinline__ void join(const AttendArgs & a, const Share & sh, con
             if (live && sub == 0 && a.lse) *lse_at(a, it, m) = lse_of(top, l);
         }
         named_sync(1, THREADS);
-        for (int x0 = tid; x0 < rows * (D / 4); x0 += 4 * THREADS) {
-            float4 s[4];
+        // a thread stays with its row: neighbours read neighbouring rows, the weights come without conflicts
+        constexpr int QS = THREADS / ROWS > 0 ? THREADS / ROWS : 1, N = D / 4 / QS, U = N < 8 ? N : 8;
+        static_assert(THREADS >= ROWS && N % U == 0);
+        const int r = tid % ROWS, q0 = tid / ROWS;
+        if (r < rows) {
+            T * dst = row_at<T>(a, a.out, a.out_stride, it, m0 + r);
+            for (int q = q0; q < D / 4; q += U * QS) {
+                float4 s[U];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int k = 0; k < U; ++k) s[k] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 2
-            for (int p = 0; p < np; ++p) {
-                const float4 * src = reinterpret_cast<const float4 *>(part(p)) + m0;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int x = min(x0 + k * THREADS, rows * (D / 4) - 1), q = x / rows, r = x - q * rows;
-                    const float4 v = __ldcg(src + q * ROWS + r);
+                for (int p = 0; p < np; ++p) {
+                    const float4 * src = reinterpret_cast<const float4 *>(part(p)) + m0 + r;
                     const float w = weight[p * rows + r];
-                    s[k].x += w * v.x; s[k].y += w * v.y; s[k].z += w * v.z; s[k].w += w * v.w;
-                }
-            }
+                    float4 v[U];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int x = x0 + k * THREADS, q = x / rows, r = x - q * rows;
-                if (x >= rows * (D / 4)) break;
-                T * dst = row_at<T>(a, a.out, a.out_stride, it, m0 + r) + 4 * q;
-                if constexpr (std::is_same_v<T, float>) *reinterpret_cast<float4 *>(dst) = s[k];
-                else *reinterpret_cast<uint2 *>(dst) = make_uint2(pack<C>(s[k].x, s[k].y), pack<C>(s[k].z, s[k].w));
+                    for (int k = 0; k < U; ++k) v[k] = __ldcg(src + (q + k * QS) * ROWS);
+#pragma unroll
+                    for (int k = 0; k < U; ++k) {
+                        s[k].x += w * v[k].x; s[k].y += w * v[k].y; s[k].z += w * v[k].z; s[k].w += w * v[k].w;
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < U; ++k) {
+                    if constexpr (std::is_same_v<T, float>) *reinterpret_cast<float4 *>(dst + 4 * (q + k * QS)) = s[k];
+                    else *reinterpret_cast<uint2 *>(dst + 4 * (q + k * QS)) = make_uint2(pack<C>(s[k].x, s[k].y), pack<C>(s[k].z, s[k].w));
+                }
             }
         }
         named_sync(1, THREADS);
     }
+}
+
+// 32 bytes to global memory in one store: a whole sector
+__device__ __forceinline__ void store32(void * p, const uint32_t * v) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+                 "r"(v[6]), "r"(v[7])
+                 : "memory");
 }
 
 // ---- waits --------------------------------------------------------------------------------------

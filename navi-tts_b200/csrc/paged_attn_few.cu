@@ -52,6 +52,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
     __shared__ __align__(8) uint64_t full[L::STAGES], empty[L::STAGES];
     __shared__ float stat[8][2][16];
     __shared__ long long red[9];
+    __shared__ Window win;
     __shared__ Share sh;
     __shared__ int abort_flag, is_last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, tq = lane & 3;
@@ -63,10 +64,12 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
         }
         fence_mbar_init();
     }
-    share_out<ROWS, 288>(a, &sh, red);
+    griddep_wait();
+    griddep_launch_dependents();
+    share_out<ROWS, 288>(a, win, sh, red);
     if (sh.u >= sh.end) return;
     const Wait wait{&abort_flag, a.err};
-    Item it = first_item<ROWS>(a, sh);
+    Item it = first_item<ROWS>(a, win, sh);
 
     if (warp == 8) {
         int n = 0;
@@ -87,7 +90,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
                 }
             }
             u += t1 - t0;
-            if (u < sh.end) next_item<ROWS>(a, sh, it);
+            if (u < sh.end) next_item<ROWS>(a, win, it);
         }
         // after an abort the copies still under way land before the block's shared memory goes
         if (abort_flag)
@@ -327,18 +330,17 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
             if (is_last) join<T, C, ROWS, D, 256, 8, L::JOIN / 4>(a, sh, it, tid, sums);
         }
         u += t1 - t0;
-        if (u < sh.end) next_item<ROWS>(a, sh, it);
+        if (u < sh.end) next_item<ROWS>(a, win, it);
     }
 }
 
 template <class T, class C, int D> void few(const AttendArgs & a, const CUtensorMap & k, const CUtensorMap & v, int rows, int sms, cudaStream_t stream) {
     const auto go = [&](auto kernel) {
         NAVI_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, FewSmem<D>::BYTES));
-        kernel<<<sms, 288, FewSmem<D>::BYTES, stream>>>(a, k, v);
+        NAVI_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(sms)), dim3(288), FewSmem<D>::BYTES, stream, a, k, v));
     };
     if (rows <= 16) go(k_attend_few<T, C, D, 1>);
     else go(k_attend_few<T, C, D, 2>);
-    NAVI_CUDA(cudaGetLastError());
 }
 
 } // namespace

@@ -43,6 +43,7 @@ struct ManyControl {
     uint64_t full[8], empty[8], q_full, s_full[2], p_full[2], o_full[2], drained;
     float stat[2][2][128];
     long long red[12];
+    Window win;
     Share sh;
     uint32_t tmem_at;
     int abort_flag, is_last;
@@ -110,7 +111,6 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
     extern __shared__ __align__(1024) uint8_t raw[];   // all of the block's shared memory: at a 1024-byte boundary
     ManyControl & S = *reinterpret_cast<ManyControl *>(raw);
     uint8_t * qs = raw + L::CONTROL, * ring = qs + 2 * L::QTILE;
-    Share & sh = S.sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         S.abort_flag = 0;
@@ -127,22 +127,27 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
         mbar_init(&S.drained, 1);
         fence_mbar_init();
     }
-    share_out<ROWS, 384>(a, &S.sh, S.red);
-    if (sh.u >= sh.end) return;
     if (warp == 9) {
         tmem_alloc(&S.tmem_at, 512);
         tmem_relinquish();
     }
     fence_before_sync();
-    __syncthreads();
+    griddep_wait();
+    griddep_launch_dependents();
+    share_out<ROWS, 384>(a, S.win, S.sh, S.red);
+    const Share & sh = S.sh;
     fence_after_sync();
     const uint32_t tmem = S.tmem_at;
     const Wait wait{&S.abort_flag, a.err};
+    if (sh.u >= sh.end) {
+        if (warp == 9) tmem_dealloc(tmem, 512);
+        return;
+    }
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 8) {
-            Item it = first_item<ROWS>(a, sh);
+            Item it = first_item<ROWS>(a, S.win, sh);
             int n = 0;
             bool ok = true;
             for (long long u = sh.u; u < sh.end && ok;) {
@@ -162,13 +167,13 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                     page = next;
                 }
                 u += t1 - t0;
-                if (u < sh.end) next_item<ROWS>(a, sh, it);
+                if (u < sh.end) next_item<ROWS>(a, S.win, it);
             }
             // after an abort the copies still under way land before the block's shared memory goes
             if (S.abort_flag)
                 for (int k = max(n - L::STAGES, 0); k < n; ++k) mbar_drain(&S.full[k % L::STAGES], (k / L::STAGES) & 1);
         } else if (warp == 9 && lane == 0) {
-            Item it = first_item<ROWS>(a, sh);
+            Item it = first_item<ROWS>(a, S.win, sh);
             constexpr uint32_t ID_S = idesc<C>(128, KT, false), ID_O = idesc<C>(128, D, true);
             const uint32_t q_at = smem_addr(qs), ring_at = smem_addr(ring);
             int base = 0, nq = 0, np[2] = {0, 0};
@@ -218,7 +223,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 }
                 base += 2 * nt;
                 u += t1 - t0;
-                if (u < sh.end) next_item<ROWS>(a, sh, it);
+                if (u < sh.end) next_item<ROWS>(a, S.win, it);
             }
             // nothing may still write the tensor memory when it is given back
             commit(&S.drained);
@@ -226,7 +231,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        Item it = first_item<ROWS>(a, sh);
+        Item it = first_item<ROWS>(a, S.win, sh);
         const int wg = warp >> 2, r = tid & 127;
         const uint32_t lane_at = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + lane_at + wg * 128, o_at = tmem + lane_at + 256 + wg * 128;
@@ -400,6 +405,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
                 const bool other = !two && (wg == 1 ? nt > 0 : nt > 1), live = m < it.m;
                 T * dst = row_at<T>(a, a.out, a.out_stride, it, live ? m : 0);
+                const bool wide = (reinterpret_cast<uintptr_t>(dst) & 31) == 0;   // rows are at least 16-byte aligned
                 for (int c = c_lo; c < c_hi; c += 32) {
                     uint32_t o[32];
                     if (any) tmem_ld<32>(o_at + c, o);
@@ -416,13 +422,24 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                     if (!whole) {
 #pragma unroll
                         for (int k = 0; k < 32; k += 4) pc[(c + k) / 4 * ROWS] = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
-                    } else if constexpr (SPLIT) {
+                    } else if (wide) {
+                        constexpr int W = SPLIT ? 8 : 16;
 #pragma unroll
-                        for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4 *>(dst + c + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                        for (int k = 0; k < 32; k += W) {
+                            uint32_t y[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                if constexpr (SPLIT) y[e] = __float_as_uint(v[k + e]);
+                                else y[e] = pack<C>(v[k + 2 * e], v[k + 2 * e + 1]);
+                            }
+                            store32(dst + c + k, y);
+                        }
                     } else {
 #pragma unroll
-                        for (int k = 0; k < 32; k += 8)
-                            *reinterpret_cast<uint4 *>(dst + c + k) = make_uint4(pack<C>(v[k], v[k + 1]), pack<C>(v[k + 2], v[k + 3]), pack<C>(v[k + 4], v[k + 5]), pack<C>(v[k + 6], v[k + 7]));
+                        for (int k = 0; k < 32; k += 4) {
+                            if constexpr (SPLIT) *reinterpret_cast<float4 *>(dst + c + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                            else *reinterpret_cast<uint2 *>(dst + c + k) = make_uint2(pack<C>(v[k], v[k + 1]), pack<C>(v[k + 2], v[k + 3]));
+                        }
                     }
                 }
                 if (live && (two || wg == 0)) {
@@ -444,7 +461,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 if (S.is_last) join<T, C, ROWS, D, 256, 1, 2 * L::QTILE / 4>(a, sh, it, tid, reinterpret_cast<float *>(qs));
             }
             u += t1 - t0;
-            if (u < sh.end) next_item<ROWS>(a, sh, it);
+            if (u < sh.end) next_item<ROWS>(a, S.win, it);
         }
     }
     __syncwarp();
@@ -460,8 +477,7 @@ template <class T, class C, int D> void many(const AttendArgs & a, const CUtenso
     const auto kernel = k_attend_many<T, C, D>;
     constexpr int smem = ManySmem<T, D>::BYTES;
     NAVI_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    kernel<<<sms, 384, smem, stream>>>(a, k, v);
-    NAVI_CUDA(cudaGetLastError());
+    NAVI_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(sms)), dim3(384), smem, stream, a, k, v));
 }
 
 } // namespace

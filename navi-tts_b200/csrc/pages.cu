@@ -77,6 +77,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_pages_plan(const __grid_consta
     __shared__ int red[PLAN_THREADS / 32];
     __shared__ int par[2 * PLAN_THREADS];
     __shared__ int last_block, taken_s;
+    griddep_wait();
+    griddep_launch_dependents();
     const int B = a.s.n_req, tid = threadIdx.x, MB = a.max_blocks;
     int * cu = plan_smem, * cg = cu + B + 1, * cs = cg + B, * st = cs + B;
 
@@ -287,6 +289,8 @@ template <class T, int E> __device__ __forceinline__ void store_vec(T * p, const
 // element i is i + D / 2, half a head's lanes away.
 template <class T, class C, int D> __global__ void __launch_bounds__(128) k_pages_store(const __grid_constant__ StoreArgs a) {
     constexpr int E = 16 / sizeof(T), LANES = D / E, HPW = 32 / LANES;   // elements a lane, lanes a head, heads a warp
+    griddep_wait();
+    griddep_launch_dependents();
     const int w = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
     const int r = w / a.parts, part = w % a.parts;
     if (r >= a.max_rows || r >= a.cu_rows[a.n_req]) return;
@@ -369,6 +373,8 @@ __global__ void __launch_bounds__(COMMIT_THREADS) k_pages_commit(const __grid_co
     __shared__ int path[NAVI_STEP_MAX_TREE];
     __shared__ int64_t from[NAVI_STEP_MAX_TREE], to[NAVI_STEP_MAX_TREE];
     __shared__ int count, moved;
+    griddep_wait();
+    griddep_launch_dependents();
     const int i = blockIdx.x, tid = threadIdx.x, W = a.c.width;
     const int r0 = a.s.cu_rows[i], n = min(a.s.cu_rows[i + 1] - r0, NAVI_STEP_MAX_TREE);
     const bool served = a.s.status[i] == NAVI_OK;
@@ -540,8 +546,7 @@ void Pages::plan(const navi_step & s, cudaStream_t stream) const {
         NAVI_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(&k_pages_plan), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        static_cast<int>((4 * NAVI_PAGES_MAX_REQUESTS + 1) * sizeof(int))));
     const int blocks = std::clamp((s.max_rows + PLAN_THREADS - 1) / PLAN_THREADS, 1, 2 * sms);
-    k_pages_plan<<<blocks, PLAN_THREADS, smem, stream>>>(a);
-    NAVI_CUDA(cudaGetLastError());
+    NAVI_CUDA(launch_pdl(k_pages_plan, dim3(static_cast<unsigned>(blocks)), dim3(PLAN_THREADS), smem, stream, a));
 }
 
 void Pages::store(const navi_step & s, int layer, const navi_store_args & q, cudaStream_t stream) const {
@@ -566,11 +571,10 @@ void Pages::store(const navi_step & s, int layer, const navi_store_args & q, cud
     const int64_t warps = static_cast<int64_t>(s.max_rows) * a.parts;
     if (warps > INT32_MAX / 32) fail("pages store: too many rows", NAVI_E_SHAPE);
     const unsigned blocks = static_cast<unsigned>((warps + 3) / 4);
-    const auto go = [&](auto kernel) { kernel<<<blocks, 128, 0, stream>>>(a); };
+    const auto go = [&](auto kernel) { NAVI_CUDA(launch_pdl(kernel, dim3(blocks), dim3(128), 0, stream, a)); };
     if (q.dtype == NAVI_F32) D == 128 ? go(k_pages_store<float, __half, 128>) : go(k_pages_store<float, __half, 64>);
     else if (q.dtype == NAVI_F16) D == 128 ? go(k_pages_store<__half, __half, 128>) : go(k_pages_store<__half, __half, 64>);
     else D == 128 ? go(k_pages_store<__nv_bfloat16, __nv_bfloat16, 128>) : go(k_pages_store<__nv_bfloat16, __nv_bfloat16, 64>);
-    NAVI_CUDA(cudaGetLastError());
 }
 
 void Pages::commit(const navi_step & s, const navi_commit_args & c, cudaStream_t stream) const {
@@ -597,8 +601,7 @@ void Pages::commit(const navi_step & s, const navi_commit_args & c, cudaStream_t
     if (items > INT32_MAX / 2) fail("pages commit: too many heads", NAVI_E_SHAPE);
     const int most = static_cast<int>((items + COMMIT_THREADS - 1) / COMMIT_THREADS);
     const int z = std::clamp(4 * dev_->info().multiprocessors / s.n_req, 1, std::min(most, 65535));
-    k_pages_commit<<<dim3(static_cast<unsigned>(s.n_req), static_cast<unsigned>(z)), COMMIT_THREADS, 0, stream>>>(a);
-    NAVI_CUDA(cudaGetLastError());
+    NAVI_CUDA(launch_pdl(k_pages_commit, dim3(static_cast<unsigned>(s.n_req), static_cast<unsigned>(z)), dim3(COMMIT_THREADS), 0, stream, a));
 }
 
 void Pages::check(cudaStream_t stream) const {
