@@ -30,12 +30,16 @@ void Pages::attend(const navi_step & s, int layer, const navi_attend_args & q, c
     const int sms = dev_->info().multiprocessors;
     const PagesScratch sc(dev_->scratch(stream, PagesScratch::bytes(sms)), sms);
     attn::AttendArgs a{q.q, q.out, q.lse, d_.table, s.req, s.ctx_len, s.cu_rows, s.status, s.parent ? s.mask : nullptr, sc.pieces, sc.arrived, sc.err,
-                 in, out, q.scale * 1.4426950408889634f, s.n_req, s.max_rows, s.mask_words, q.n_head, d_.n_kv_head, q.n_head / d_.n_kv_head, -1, D, shift_,
+                 in, out, q.scale * 1.4426950408889634f, 0, s.n_req, s.max_rows, s.mask_words, q.n_head, d_.n_kv_head, q.n_head / d_.n_kv_head, D, shift_,
                  d_.n_pages, d_.max_blocks, d_.max_requests};
-    for (int b = 0; b < 12; ++b)
-        if (a.group == 1 << b) a.group_shift = b;
+    const int64_t most = std::min(s.max_new, s.max_rows);
+    if (a.group > 1) a.group_mul = static_cast<uint32_t>(((1ull << 32) + static_cast<uint64_t>(a.group) - 1) / static_cast<uint64_t>(a.group));
+    if ((a.group & (a.group - 1)) != 0 && (most + 512) * a.group * a.group >= 1ll << 32) fail("pages attend: too many rows for this many heads to a KV head", NAVI_E_SHAPE);
+    // the list of key tiles that the blocks divide
+    const int64_t rows = most * a.group <= attn::FEW_ROWS ? 16 : 128, items = (most * a.group + rows - 1) / rows * d_.n_kv_head * s.n_req, tiles = (static_cast<int64_t>(d_.max_blocks) * d_.page_size + attn::KT - 1) / attn::KT;
+    if (items * tiles >= 1ll << 31) fail("pages attend: requests x heads x tokens pass 31 bits of key tiles", NAVI_E_SHAPE);
     const CUtensorMap & km = maps_[static_cast<size_t>(2 * layer)], & vm = maps_[static_cast<size_t>(2 * layer + 1)];
-    const int64_t m = static_cast<int64_t>(std::min(s.max_new, s.max_rows)) * a.group;
+    const int64_t m = most * a.group;
     if (m <= attn::FEW_ROWS) return attn::attend_few(a, km, vm, q.dtype, d_.dtype, static_cast<int>(m), sms, stream);
     attn::attend_many(a, km, vm, q.dtype, d_.dtype, sms, stream);
 }

@@ -12,6 +12,12 @@
 
 #include <type_traits>
 
+// What runs seldom: out of line, to keep the code short. A kernel that moves registers between its warps
+// (setmaxnreg) can make no calls and defines this as __forceinline__ before it includes the file.
+#ifndef NAVI_ATTN_SELDOM
+#define NAVI_ATTN_SELDOM __noinline__
+#endif
+
 namespace navi::attn {
 
 using namespace navi::dev;
@@ -26,7 +32,8 @@ struct AttendArgs {
     int * arrived, * err;
     int64_t q_stride, out_stride;
     float scale;                 // times log2(e)
-    int n_req, max_rows, mask_words, n_head, n_kv, group, group_shift, head_dim, shift, n_pages, max_blocks, max_requests;
+    uint32_t group_mul;          // 2^32 / group rounded up, 0 for 1
+    int n_req, max_rows, mask_words, n_head, n_kv, group, head_dim, shift, n_pages, max_blocks, max_requests;
 };
 
 // What a block needs to know of one request.
@@ -34,7 +41,7 @@ struct Request {
     int row0, n, ctx, keys;      // first row, rows, cached tokens, tokens in all
     int table;                   // its row of the block table
 };
-__device__ __forceinline__ Request request(const AttendArgs & a, int i) {
+static __device__ NAVI_ATTN_SELDOM Request request(const AttendArgs & a, int i) {
     Request r;
     r.row0 = a.cu_rows[i];
     r.n = max(min(a.cu_rows[i + 1], a.max_rows) - r.row0, 0);
@@ -46,20 +53,10 @@ __device__ __forceinline__ Request request(const AttendArgs & a, int i) {
     r.table = ok ? r.table : 0;
     return r;
 }
-// The requests from the block's first one on, in shared memory: a walk over items then costs no
-// trip to L2 for each.
-struct Window {
-    static constexpr int N = 32;
-    long long base;              // the first unit of request `first`
-    int first, count;
-    int row0[N], n[N], ctx[N], keys[N], table[N];
-};
-__device__ __forceinline__ Request request(const AttendArgs & a, const Window & w, int i) {
-    const int k = i - w.first;
-    if (k >= w.count) return request(a, i);
-    return {w.row0[k], w.n[k], w.ctx[k], w.keys[k], w.table[k]};
+// A row x head of a request -> its row: x / group as a product, exact below 2^32 / group (the host checks).
+__device__ __forceinline__ int by_group(const AttendArgs & a, int x) {
+    return a.group_mul ? static_cast<int>(__umulhi(static_cast<uint32_t>(x), a.group_mul)) : x;
 }
-__device__ __forceinline__ int by_group(const AttendArgs & a, int x) { return a.group_shift >= 0 ? x >> a.group_shift : x / a.group; }
 
 template <class C> __device__ __forceinline__ uint32_t pack(float a, float b) {
     if constexpr (std::is_same_v<C, __half>) {
@@ -74,6 +71,12 @@ template <class C> __device__ __forceinline__ float2 unpack(uint32_t v) {
     if constexpr (std::is_same_v<C, __half>) return __half22float2(*reinterpret_cast<const __half2 *>(&v));
     else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v));
 }
+// two f32 values as pairs of 16-bit terms, v = hi + lo to about twice the bits
+template <class C> __device__ __forceinline__ void split_pair(float x, float y, uint32_t & hi, uint32_t & lo) {
+    hi = pack<C>(x, y);
+    const float2 b = unpack<C>(hi);
+    lo = pack<C>(x - b.x, y - b.y);
+}
 // 2^x by the hardware's approximation (two units of the last place); 2^-inf = 0
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -85,33 +88,26 @@ __device__ __forceinline__ float exp2_fast(float x) {
 //
 // The work of a launch is a list of units: for each request, each KV head and each tile of ROWS
 // rows (rows x heads of the KV head, an item), the item's key tiles of KT keys, at least one.
-// Lengths are on the device and ragged, so the blocks divide the list evenly themselves: block c
-// of G takes the units [c W / G, (c + 1) W / G), whatever request they belong to. An item that
-// falls to several blocks leaves its pieces (the sums and each row's maximum and sum, f32) in
-// the stream's scratch, and the block that arrives last joins them in the blocks' order, so
-// the result does not depend on who was last. A block has at most two such pieces: slot 0 for
-// one that begins inside an item, slot 1 for one that only ends inside it.
+// Lengths are on the device and ragged, so the blocks divide the list evenly themselves,
+// whatever request the units belong to. An item that falls to several blocks leaves its pieces
+// (the sums and each row's maximum and sum, f32) in the stream's scratch, and the block that
+// arrives last joins them in the blocks' order, so the result does not depend on who was last. A
+// block has at most two such pieces: slot 0 for one that begins inside an item, slot 1 for one
+// that only ends inside it.
+//
+// One warp of the block walks the list and hands each part of it (a segment: the block's key tiles
+// of one item) to the others through a small ring in shared memory. The walk is long code that
+// runs seldom; the roles that run often stay short, which for a step of a few microseconds
+// matters more than anything else: its instructions are read once, from L2.
 
 constexpr int KT = 128;
 
-// x / y of values that are not negative: the 64-bit division is the slow one
-__device__ __forceinline__ long long cut(long long x, long long y) {
-    return (x | y) >> 32 ? x / y : static_cast<long long>(static_cast<uint32_t>(x) / static_cast<uint32_t>(y));
-}
-
-// This block's units [u, end) of total, and the item that holds the first.
-struct Share {
-    long long u, end, total;
-    int blocks, i;               // blocks that have work; the request of unit u
-    long long base;              // the request's first unit
-};
-
-struct Item {
-    int i, g, rt;                // request, KV head, row tile
-    int tiles, n_keys;           // key tiles (1 at least) and keys that its rows may see
-    int m0, m;                   // its first row x head, and how many
-    long long u0;                // its first unit
-    Request rq;
+struct Segment {
+    int row0, ctx, table, g;     // the request, the KV head
+    int m0, m, n_keys;           // its first row x head, how many, the keys that they may see
+    int t0, nt;                  // key tiles t0 .. t0 + nt - 1; nt -1: no more segments
+    int whole, slot;             // all of the item's tiles; else the piece's slot,
+    int c0, np;                  // and the blocks c0 .. c0 + np - 1 that have pieces of it
 };
 
 template <int ROWS> __device__ __forceinline__ int row_tiles(const AttendArgs & a, const Request & r) { return (r.n * a.group + ROWS - 1) / ROWS; }
@@ -121,182 +117,195 @@ template <int ROWS> __device__ __forceinline__ int keys_of(const AttendArgs & a,
 }
 __device__ __forceinline__ int tiles_of(int n_keys) { return max((n_keys + KT - 1) / KT, 1); }
 // the units of one KV head of a request
-template <int ROWS> __device__ __forceinline__ long long units_of(const AttendArgs & a, const Request & r) {
+template <int ROWS> __device__ NAVI_ATTN_SELDOM int units_of(const AttendArgs & a, const Request & r) {
     const int rts = row_tiles<ROWS>(a, r);
-    if (a.mask || r.keys == 0) return static_cast<long long>(rts) * tiles_of(r.keys);
-    long long n = 0;
+    if (a.mask || r.keys == 0) return rts * tiles_of(r.keys);
+    int n = 0;
+#pragma unroll 1
     for (int rt = 0; rt < rts; ++rt) n += tiles_of(keys_of<ROWS>(a, r, rt));
     return n;
 }
-template <int ROWS> __device__ __forceinline__ void open_tile(const AttendArgs & a, Item & it) {
-    it.n_keys = keys_of<ROWS>(a, it.rq, it.rt);
-    it.tiles = tiles_of(it.n_keys);
-    it.m0 = it.rt * ROWS;
-    it.m = min(it.rq.n * a.group - it.m0, ROWS);
-}
-template <int ROWS> __device__ __forceinline__ void next_item(const AttendArgs & a, const Window & win, Item & it) {
-    it.u0 += it.tiles;
-    if (++it.rt >= row_tiles<ROWS>(a, it.rq)) {
-        it.rt = 0;
-        if (++it.g >= a.n_kv) {
-            it.g = 0;
-            do it.rq = request(a, win, ++it.i);
-            while (it.rq.n <= 0);   // more units follow, so a later request has rows
-        }
-    }
-    open_tile<ROWS>(a, it);
-}
 
-// Every thread of the block takes part. It holds the block's only barriers before the roles part, so
-// what the block's threads write to shared memory before the call is there for all after it.
-// Up to 32 requests every warp does the sums by itself, a lane a request: one trip to L2 and no
-// barrier between.
-template <int ROWS, int THREADS> __device__ __forceinline__ void share_out(const AttendArgs & a, Window & win, Share & out, long long * red) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.n_req;
-    const bool one = B <= 32;
-    const int per = one ? 1 : (B + THREADS - 1) / THREADS, i0 = min(B, one ? lane : tid * per), i1 = min(B, i0 + per);
-    long long mine = 0;
-    Request r{};
-    for (int i = i0; i < i1; ++i) {
-        r = request(a, i);
-        mine += units_of<ROWS>(a, r) * a.n_kv;
+// How the units divide: `more` blocks of `per` + 1 units, then blocks of `per`.
+struct Division {
+    int per, more;
+    __device__ __forceinline__ int first(int block) const { return block * per + min(block, more); }
+    __device__ __forceinline__ int block(int unit) const {
+        const int x = unit - more * (per + 1);
+        return x < 0 ? unit / (per + 1) : more + x / per;
     }
-    long long x = mine;
+};
+// What the block's threads find out together: the division, and the request that holds the block's first unit.
+struct Share {
+    Division d;
+    int u, end;                  // this block's units
+    int i, base;                 // the request of unit u, and its first unit
+};
+
+// Every thread of the block takes part. What the threads wrote to shared memory before is there for
+// all of them after it. (The host has checked that the units fit 31 bits.)
+template <int ROWS, int THREADS> __device__ __forceinline__ void share_out(const AttendArgs & a, Share & sh, int * red) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.n_req;
+    const bool one = B <= 32;    // every warp does the sums by itself, a lane a request: one trip to L2 and no barrier between
+    const int per = one ? 1 : (B + THREADS - 1) / THREADS, i0 = min(B, one ? lane : tid * per), i1 = min(B, i0 + per);
+    int mine = 0;
+#pragma unroll 1
+    for (int i = i0; i < i1; ++i) mine += units_of<ROWS>(a, request(a, i)) * a.n_kv;
+    int x = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
-    long long base = x - mine, total = __shfl_sync(0xffffffffu, x, 31);
+    int base = x - mine, total = __shfl_sync(0xffffffffu, x, 31);
     if (!one) {
         if (lane == 31) red[warp] = x;
         __syncthreads();
         total = 0;
-#pragma unroll
+#pragma unroll 1
         for (int w = 0; w < THREADS / 32; ++w) {
             if (w < warp) base += red[w];
             total += red[w];
         }
     }
-    Share sh;
-    const long long G = min(static_cast<long long>(gridDim.x), total), c = blockIdx.x;
-    sh.total = total;
-    sh.blocks = static_cast<int>(G);
-    sh.u = G ? cut(c * total, G) : 0;
-    sh.end = c < G ? cut((c + 1) * total, G) : sh.u;
-    const bool holds = c < G && sh.u >= base && sh.u < base + mine;
-    if (one) {
-        const int from = __ffs(__ballot_sync(0xffffffffu, holds)) - 1;
-        sh.i = max(from, 0);
-        sh.base = __shfl_sync(0xffffffffu, base, sh.i);
-        if (warp == 0 && lane < B) {
-            win.row0[lane] = r.row0;
-            win.n[lane] = r.n;
-            win.ctx[lane] = r.ctx;
-            win.keys[lane] = r.keys;
-            win.table[lane] = r.table;
-        }
-        if (tid == 0) {
-            win.first = 0;
-            win.count = B;
-        }
-    } else {
-        if (holds) {
-            int i = i0;
-            long long b = base;
-            for (;; ++i) {
-                const long long n = units_of<ROWS>(a, request(a, i)) * a.n_kv;
-                if (sh.u < b + n) break;
-                b += n;
-            }
-            win.first = i;
-            win.base = b;
-        }
-        __syncthreads();
-        sh.i = win.first;
-        sh.base = win.base;
-        if (sh.u < sh.end && tid < Window::N) {
-            const int count = min(Window::N, B - sh.i);
-            if (tid < count) {
-                const Request q = request(a, sh.i + tid);
-                win.row0[tid] = q.row0;
-                win.n[tid] = q.n;
-                win.ctx[tid] = q.ctx;
-                win.keys[tid] = q.keys;
-                win.table[tid] = q.table;
-            }
-            if (tid == 0) win.count = count;
-        }
+    const int G = min(static_cast<int>(gridDim.x), total), c = blockIdx.x;
+    Division d{0, 0};
+    if (G > 0) {
+        d.per = total / G;
+        d.more = total - d.per * G;
     }
-    if (tid == 0) out = sh;
+    const int u = d.first(c), end = c < G ? d.first(c + 1) : u;
+    if (tid == 0) {
+        sh.d = d;
+        sh.u = u;
+        sh.end = end;
+    }
+    if ((!one || warp == 0) && u < end && u >= base && u < base + mine) {
+        int i = i0, b = base;
+#pragma unroll 1
+        for (; per > 1; ++i) {
+            const int n = units_of<ROWS>(a, request(a, i)) * a.n_kv;
+            if (u < b + n) break;
+            b += n;
+        }
+        sh.i = i;
+        sh.base = b;
+    }
     __syncthreads();
 }
-template <int ROWS> __device__ __forceinline__ Item first_item(const AttendArgs & a, const Window & win, const Share & sh) {
-    Item it{};
-    it.i = sh.i;
-    it.rq = request(a, win, it.i);
-    const long long per_head = units_of<ROWS>(a, it.rq);
-    it.g = static_cast<int>(cut(sh.u - sh.base, per_head));
-    it.u0 = sh.base + it.g * per_head;
-    if (a.mask || it.rq.keys == 0) {   // every row tile has as many key tiles
-        it.rt = static_cast<int>(cut(sh.u - it.u0, tiles_of(it.rq.keys)));
-        it.u0 += static_cast<long long>(it.rt) * tiles_of(it.rq.keys);
+
+// The walk over the block's segments: next() fills in the next one; false when there is none.
+template <int ROWS> struct Walk {
+    const AttendArgs & a;
+    const Share & sh;
+    Request r;
+    int i, g, rt, u0, u, tiles, n_keys;
+
+    __device__ __forceinline__ Walk(const AttendArgs & args, const Share & share) : a(args), sh(share) {
+        i = sh.i;
+        u = sh.u;
+        r = request(a, i);
+        const int per_head = units_of<ROWS>(a, r);
+        g = (u - sh.base) / per_head;
+        u0 = sh.base + g * per_head;
+        rt = 0;
+        if (a.mask || r.keys == 0) {   // every row tile has as many key tiles
+            rt = (u - u0) / tiles_of(r.keys);
+            u0 += rt * tiles_of(r.keys);
+        }
+        open();
+        while (u0 + tiles <= u) {
+            u0 += tiles;
+            ++rt;
+            open();
+        }
     }
-    open_tile<ROWS>(a, it);
-    while (it.u0 + it.tiles <= sh.u) {
-        it.u0 += it.tiles;
-        ++it.rt;
-        open_tile<ROWS>(a, it);
+    __device__ __forceinline__ void open() {
+        n_keys = keys_of<ROWS>(a, r, rt);
+        tiles = tiles_of(n_keys);
     }
-    return it;
-}
-__device__ __forceinline__ int block_of(const Share & sh, long long unit) { return static_cast<int>(cut((unit + 1) * sh.blocks - 1, sh.total)); }
+    __device__ __forceinline__ bool next(Segment & s) {
+        if (u >= sh.end) {
+            s.nt = -1;
+            return false;
+        }
+        if (u >= u0 + tiles) {
+            u0 += tiles;
+            if (++rt >= row_tiles<ROWS>(a, r)) {
+                rt = 0;
+                if (++g >= a.n_kv) {
+                    g = 0;
+                    do r = request(a, ++i);
+                    while (r.n <= 0);   // more units follow, so a later request has rows
+                }
+            }
+            open();
+        }
+        const int t1 = min(tiles, sh.end - u0);
+        s.row0 = r.row0;
+        s.ctx = r.ctx;
+        s.table = r.table;
+        s.g = g;
+        s.m0 = rt * ROWS;
+        s.m = min(r.n * a.group - s.m0, ROWS);
+        s.n_keys = n_keys;
+        s.t0 = u - u0;
+        s.nt = t1 - s.t0;
+        s.whole = s.nt == tiles;
+        s.slot = s.t0 == 0;
+        s.c0 = sh.d.block(u0);
+        s.np = sh.d.block(u0 + tiles - 1) - s.c0 + 1;
+        u += s.nt;
+        return true;
+    }
+};
 
 // A piece in the scratch: the rows' sums as float4 [D / 4][ROWS], then [ROWS] maxima and [ROWS] sums of weights.
 __device__ __forceinline__ float * piece(const AttendArgs & a, int block, int slot) {
     return a.pieces + (static_cast<size_t>(block) * 2 + slot) * PagesScratch::PIECE_FLOATS;
 }
 
-// Row m of an item: where its q and its result are.
-template <class T> __device__ __forceinline__ T * row_at(const AttendArgs & a, const void * base, int64_t stride, const Item & it, int m) {
-    const int at = it.m0 + m, j = by_group(a, at);
-    return static_cast<T *>(const_cast<void *>(base)) + (it.rq.row0 + j) * stride + static_cast<int64_t>(it.g * a.group + at - j * a.group) * a.head_dim;
+// Row m of a segment: where its q and its result are.
+template <class T> __device__ __forceinline__ T * row_at(const AttendArgs & a, const void * base, int64_t stride, const Segment & s, int m) {
+    const int at = s.m0 + m, j = by_group(a, at);
+    return static_cast<T *>(const_cast<void *>(base)) + (s.row0 + j) * stride + static_cast<int64_t>(s.g * a.group + at - j * a.group) * a.head_dim;
 }
-__device__ __forceinline__ float * lse_at(const AttendArgs & a, const Item & it, int m) {
-    const int at = it.m0 + m, j = by_group(a, at);
-    return a.lse + static_cast<size_t>(it.rq.row0 + j) * a.n_head + it.g * a.group + at - j * a.group;
+__device__ __forceinline__ void put_lse(const AttendArgs & a, const Segment & s, int m, float top, float l) {
+    const int at = s.m0 + m, j = by_group(a, at);
+    a.lse[static_cast<size_t>(s.row0 + j) * a.n_head + s.g * a.group + at - j * a.group] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
 }
-__device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f; }
 
 // One thread of a block whose piece is written: whether it is the item's last.
-__device__ __forceinline__ bool arrive_piece(const AttendArgs & a, const Share & sh, const Item & it) {
-    const int c0 = block_of(sh, it.u0), c1 = block_of(sh, it.u0 + it.tiles - 1);
-    if (atomicAdd(a.arrived + c0, 1) != c1 - c0) return false;
-    a.arrived[c0] = 0;
+__device__ __forceinline__ bool arrive_piece(const AttendArgs & a, const Segment & s) {
+    if (atomicAdd(a.arrived + s.c0, 1) != s.np - 1) return false;
+    a.arrived[s.c0] = 0;
     __threadfence();
     return true;
 }
 
 // Joins the pieces of an item, in order: THREADS threads of the block, all of them. First what each
 // piece counts in each row goes to `weight` (CAP floats of shared memory), LANES lanes to a row,
-// then the sums are read.
+// then the sums are read, by a thread that stays with its row: neighbours read neighbouring rows.
 template <class T, class C, int ROWS, int D, int THREADS, int LANES, int CAP>
-__device__ __forceinline__ void join(const AttendArgs & a, const Share & sh, const Item & it, int tid, float * weight) {
-    const int c0 = block_of(sh, it.u0), np = block_of(sh, it.u0 + it.tiles - 1) - c0 + 1;
+__device__ __forceinline__ void join(const AttendArgs & a, const Segment & s, int tid, float * weight) {
+    const int c0 = s.c0, np = s.np;
     const auto part = [&](int p) { return piece(a, c0 + p, p == 0); };
-    const int most = CAP / np;                        // rows at a time: up to 256 blocks share an item
-    for (int m0 = 0; m0 < it.m; m0 += most) {
-        const int rows = min(most, it.m - m0), sub = tid % LANES;
-        for (int r = tid / LANES; r < (rows + THREADS / LANES - 1) / (THREADS / LANES) * (THREADS / LANES); r += THREADS / LANES) {
+    const int most = min(CAP / np, ROWS);             // rows at a time: up to a block a multiprocessor shares an item
+#pragma unroll 1
+    for (int m0 = 0; m0 < s.m; m0 += most) {
+        const int rows = min(most, s.m - m0), sub = tid % LANES;
+        constexpr int RP = THREADS / LANES;           // rows a pass
+#pragma unroll 1
+        for (int r = tid / LANES; r < (rows + RP - 1) / RP * RP; r += RP) {
             const bool live = r < rows;
             const int m = m0 + (live ? r : 0);
             float top = -INFINITY, l = 0.f;
-#pragma unroll 4
+#pragma unroll 2
             for (int p = sub; p < np; p += LANES) top = fmaxf(top, __ldcg(part(p) + ROWS * D + m));
 #pragma unroll
             for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll 4
+#pragma unroll 2
             for (int p = sub; p < np; p += LANES) {
                 const float w = exp2_fast(__ldcg(part(p) + ROWS * D + m) - ref);
                 l += w * __ldcg(part(p) + ROWS * D + ROWS + m);
@@ -305,21 +314,21 @@ __device__ __forceinline__ void join(const AttendArgs & a, const Share & sh, con
 #pragma unroll
             for (int o = 1; o < LANES; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            if (live)
-                for (int p = sub; p < np; p += LANES) weight[p * rows + r] *= inv;
-            if (live && sub == 0 && a.lse) *lse_at(a, it, m) = lse_of(top, l);
+#pragma unroll 1
+            for (int p = sub; p < np && live; p += LANES) weight[p * rows + r] *= inv;
+            if (live && sub == 0 && a.lse) put_lse(a, s, m, top, l);
         }
         named_sync(1, THREADS);
-        // a thread stays with its row: neighbours read neighbouring rows, the weights come without conflicts
-        constexpr int QS = THREADS / ROWS > 0 ? THREADS / ROWS : 1, N = D / 4 / QS, U = N < 8 ? N : 8;
-        static_assert(THREADS >= ROWS && N % U == 0);
-        const int r = tid % ROWS, q0 = tid / ROWS;
+        constexpr int QS = THREADS / ROWS, N = D / 4 / QS, U = N < 8 ? N : 8;
+        static_assert(THREADS % ROWS == 0 && N % U == 0);
+        const int r = tid % ROWS;
         if (r < rows) {
-            T * dst = row_at<T>(a, a.out, a.out_stride, it, m0 + r);
-            for (int q = q0; q < D / 4; q += U * QS) {
-                float4 s[U];
+            T * dst = row_at<T>(a, a.out, a.out_stride, s, m0 + r);
+#pragma unroll 1
+            for (int q = tid / ROWS; q < D / 4; q += U * QS) {
+                float4 y[U];
 #pragma unroll
-                for (int k = 0; k < U; ++k) s[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int k = 0; k < U; ++k) y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 2
                 for (int p = 0; p < np; ++p) {
                     const float4 * src = reinterpret_cast<const float4 *>(part(p)) + m0 + r;
@@ -329,13 +338,13 @@ __device__ __forceinline__ void join(const AttendArgs & a, const Share & sh, con
                     for (int k = 0; k < U; ++k) v[k] = __ldcg(src + (q + k * QS) * ROWS);
 #pragma unroll
                     for (int k = 0; k < U; ++k) {
-                        s[k].x += w * v[k].x; s[k].y += w * v[k].y; s[k].z += w * v[k].z; s[k].w += w * v[k].w;
+                        y[k].x += w * v[k].x; y[k].y += w * v[k].y; y[k].z += w * v[k].z; y[k].w += w * v[k].w;
                     }
                 }
 #pragma unroll
                 for (int k = 0; k < U; ++k) {
-                    if constexpr (std::is_same_v<T, float>) *reinterpret_cast<float4 *>(dst + 4 * (q + k * QS)) = s[k];
-                    else *reinterpret_cast<uint2 *>(dst + 4 * (q + k * QS)) = make_uint2(pack<C>(s[k].x, s[k].y), pack<C>(s[k].z, s[k].w));
+                    if constexpr (std::is_same_v<T, float>) *reinterpret_cast<float4 *>(dst + 4 * (q + k * QS)) = y[k];
+                    else *reinterpret_cast<uint2 *>(dst + 4 * (q + k * QS)) = make_uint2(pack<C>(y[k].x, y[k].y), pack<C>(y[k].z, y[k].w));
                 }
             }
         }
@@ -360,6 +369,10 @@ struct Wait {
     volatile int * abort;
     int * err;
     __device__ __forceinline__ bool operator()(uint64_t * bar, uint32_t parity) const {
+        return mbar_try_wait(bar, parity) || slow(bar, parity);
+    }
+    __device__ NAVI_ATTN_SELDOM bool slow(uint64_t * bar, uint32_t parity) const {
+#pragma unroll 1
         for (int k = 0; k < 64; ++k)
             if (mbar_try_wait(bar, parity)) return true;
         const unsigned long long t0 = globaltimer();
@@ -381,31 +394,44 @@ __device__ __forceinline__ void mbar_drain(uint64_t * bar, uint32_t parity) {
     while (!mbar_try_wait(bar, parity) && globaltimer() - t0 < 2 * DEADLINE_NS) {}
 }
 
-// Whether row j of the item's request sees token `key`.
-__device__ __forceinline__ bool sees(const AttendArgs & a, const Item & it, int key, int j) {
-    if (key >= it.n_keys) return false;
-    const int at = key - it.rq.ctx;
+// Whether row j of the segment's request sees token `key`.
+__device__ __forceinline__ bool sees(const AttendArgs & a, const Segment & s, int key, int j) {
+    if (key >= s.n_keys) return false;
+    const int at = key - s.ctx;
     if (at < 0) return true;
     if (!a.mask) return at <= j;
-    return at < 64 * a.mask_words && (__ldg(a.mask + static_cast<size_t>(it.rq.row0 + j) * a.mask_words + (at >> 6)) >> (at & 63) & 1);
+    return at < 64 * a.mask_words && (__ldg(a.mask + static_cast<size_t>(s.row0 + j) * a.mask_words + (at >> 6)) >> (at & 63) & 1);
 }
 
-// The pages that hold key tile t of an item, and the bytes of them that one pool contributes.
-__device__ __forceinline__ int tile_pages(const AttendArgs & a, const Item & it, int t) {
-    return (min(it.n_keys - t * KT, KT) + (1 << a.shift) - 1) >> a.shift;
+// The pages that hold key tile t, and the bytes of them that one pool contributes.
+__device__ __forceinline__ int tile_pages(const AttendArgs & a, const Segment & s, int t) {
+    return (min(s.n_keys - t * KT, KT) + (1 << a.shift) - 1) >> a.shift;
 }
 // A warp brings them from a pool's map to dst: halves of 64 dims, each [KT][64] in 128-byte rows that
 // the copy swizzles; only pages with keys of the item, so rows past them keep what they held.
 // The bytes (tile_pages * page * D * 2) arrive on `bar`. Lane x has the x-th box of the tile, at
 // most 16 of them (a page of 16 tokens, two halves), so the page ids, which it reads a tile ahead,
 // cost one latency together and not one each.
-template <int D> __device__ __forceinline__ int page_of_box(const AttendArgs & a, const Item & it, int t, int box) {
+template <int D> __device__ __forceinline__ int page_of_box(const AttendArgs & a, const Segment & s, int t, int box) {
     const int p = box / (D / 64);
-    return p < tile_pages(a, it, t) ? min(max(__ldg(a.table + static_cast<size_t>(it.rq.table) * a.max_blocks + (t * KT >> a.shift) + p), 0), a.n_pages - 1) : -1;
+    return p < tile_pages(a, s, t) ? min(max(__ldg(a.table + static_cast<size_t>(s.table) * a.max_blocks + (t * KT >> a.shift) + p), 0), a.n_pages - 1) : -1;
 }
-template <int D> __device__ __forceinline__ void load_box(const AttendArgs & a, const CUtensorMap * map, const Item & it, int page, int box, uint8_t * dst, uint64_t * bar) {
+template <int D> __device__ __forceinline__ void load_box(const AttendArgs & a, const CUtensorMap * map, const Segment & s, int page, int box, uint8_t * dst, uint64_t * bar) {
     const int p = box / (D / 64), h = box % (D / 64);
-    if (page >= 0) tma_box_2d(dst + h * (KT * 128) + (p << a.shift) * 128, map, h * 64, (page * a.n_kv + it.g) << a.shift, bar);
+    if (page >= 0) tma_box_2d(dst + h * (KT * 128) + (p << a.shift) * 128, map, h * 64, (page * a.n_kv + s.g) << a.shift, bar);
 }
+
+// The ring of segments: one warp fills it, every other role reads it.
+struct SegmentRing {
+    static constexpr int N = 4;
+    Segment s[N];
+    uint64_t full[N], empty[N];
+    __device__ __forceinline__ void init(int readers) {
+        for (int k = 0; k < N; ++k) {
+            mbar_init(&full[k], 1);
+            mbar_init(&empty[k], readers);
+        }
+    }
+};
 
 } // namespace navi::attn

@@ -1,5 +1,6 @@
 // Attention over the paged KV cache for many rows of a request (paged_attn.cu): larger drafted
 // trees and chunks of prompts, on the tcgen05 tensor cores.
+#define NAVI_ATTN_SELDOM __forceinline__
 #include "paged_attn.hpp"
 #include "paged_attn.cuh"
 #include "tmem.cuh"
@@ -42,8 +43,8 @@ template <class T, int D> struct ManySmem {
 struct ManyControl {
     uint64_t full[8], empty[8], q_full, s_full[2], p_full[2], o_full[2], drained;
     float stat[2][2][128];
-    long long red[12];
-    Window win;
+    SegmentRing segs;
+    int red[12];
     Share sh;
     uint32_t tmem_at;
     int abort_flag, is_last;
@@ -83,7 +84,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 // Bits 0..31: whether row j of the request sees the tokens ctx + a .. ctx + a + 31 (a may be negative:
 // those are cached tokens), of which `left` are the item's.
-__device__ __forceinline__ uint32_t seen_bits(const AttendArgs & a, const Item & it, int j, int at, int left) {
+__device__ __forceinline__ uint32_t seen_bits(const AttendArgs & a, const Segment & it, int j, int at, int left) {
     if (left <= 0) return 0u;
     uint32_t b;
     if (at + 31 < 0) b = ~0u;
@@ -91,7 +92,7 @@ __device__ __forceinline__ uint32_t seen_bits(const AttendArgs & a, const Item &
         const int n = j - at + 1;            // tokens from `at` up to row j itself
         b = n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
     } else {
-        const uint64_t * m = a.mask + static_cast<size_t>(it.rq.row0 + j) * a.mask_words;
+        const uint64_t * m = a.mask + static_cast<size_t>(it.row0 + j) * a.mask_words;
         const int w = at >> 6;               // floor: -1 for the bits before row 0, all seen
         const uint64_t lo = w < 0 ? ~0ull : w < a.mask_words ? __ldg(m + w) : 0ull;
         const uint64_t hi = w + 1 < a.mask_words ? __ldg(m + w + 1) : 0ull;
@@ -125,6 +126,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
             mbar_init(&S.o_full[g], 1);
         }
         mbar_init(&S.drained, 1);
+        S.segs.init(9);
         fence_mbar_init();
     }
     if (warp == 9) {
@@ -134,54 +136,67 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
     fence_before_sync();
     griddep_wait();
     griddep_launch_dependents();
-    share_out<ROWS, 384>(a, S.win, S.sh, S.red);
-    const Share & sh = S.sh;
+    share_out<ROWS, 384>(a, S.sh, S.red);
     fence_after_sync();
     const uint32_t tmem = S.tmem_at;
     const Wait wait{&S.abort_flag, a.err};
-    if (sh.u >= sh.end) {
+    if (S.sh.u >= S.sh.end) {
         if (warp == 9) tmem_dealloc(tmem, 512);
         return;
     }
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 8) {
-            Item it = first_item<ROWS>(a, S.win, sh);
+            Walk<ROWS> walk(a, S.sh);
             int n = 0;
             bool ok = true;
-            for (long long u = sh.u; u < sh.end && ok;) {
-                const int t0 = static_cast<int>(u - it.u0), t1 = static_cast<int>(min(static_cast<long long>(it.tiles), sh.end - it.u0));
-                int page = it.n_keys > 0 ? page_of_box<D>(a, it, t0, lane & 15) : -1;
-                for (int t = t0; t < t1 && ok && it.n_keys > 0; ++t) {
-                    const int next = t + 1 < t1 ? page_of_box<D>(a, it, t + 1, lane & 15) : -1;
+#pragma unroll 1
+            for (int k = 0; ok; ++k) {
+                Segment s;
+                const bool more = walk.next(s);
+                if (k >= SegmentRing::N) ok = __shfl_sync(0xffffffffu, lane == 0 ? wait(&S.segs.empty[k % SegmentRing::N], (k / SegmentRing::N - 1) & 1) : 0, 0);
+                if (!ok) break;
+                if (lane == 0) {
+                    S.segs.s[k % SegmentRing::N] = s;
+                    mbar_arrive(&S.segs.full[k % SegmentRing::N]);
+                }
+                if (!more) break;
+                if (s.n_keys <= 0) continue;
+                int page = page_of_box<D>(a, s, s.t0, lane & 15);
+#pragma unroll 1
+                for (int t = s.t0; t < s.t0 + s.nt && ok; ++t) {
+                    const int next = t + 1 < s.t0 + s.nt ? page_of_box<D>(a, s, t + 1, lane & 15) : -1;
+#pragma unroll 1
                     for (int kv = 0; kv < 2 && ok; ++kv) {
-                        const int s = n % L::STAGES;
-                        if (n >= L::STAGES) ok = __shfl_sync(0xffffffffu, lane == 0 ? wait(&S.empty[s], (n / L::STAGES - 1) & 1) : 0, 0);
+                        const int st = n % L::STAGES;
+                        if (n >= L::STAGES) ok = __shfl_sync(0xffffffffu, lane == 0 ? wait(&S.empty[st], (n / L::STAGES - 1) & 1) : 0, 0);
                         if (!ok) break;
-                        if (lane == 0) mbar_arrive_expect_tx(&S.full[s], static_cast<uint32_t>((tile_pages(a, it, t) << a.shift) * D * 2));
+                        if (lane == 0) mbar_arrive_expect_tx(&S.full[st], static_cast<uint32_t>((tile_pages(a, s, t) << a.shift) * D * 2));
                         __syncwarp();
-                        if (lane < 16) load_box<D>(a, kv ? &vmap : &kmap, it, page, lane, ring + s * L::STAGE, &S.full[s]);
+                        if (lane < 16) load_box<D>(a, kv ? &vmap : &kmap, s, page, lane, ring + st * L::STAGE, &S.full[st]);
                         ++n;
                     }
                     page = next;
                 }
-                u += t1 - t0;
-                if (u < sh.end) next_item<ROWS>(a, S.win, it);
             }
             // after an abort the copies still under way land before the block's shared memory goes
             if (S.abort_flag)
                 for (int k = max(n - L::STAGES, 0); k < n; ++k) mbar_drain(&S.full[k % L::STAGES], (k / L::STAGES) & 1);
         } else if (warp == 9 && lane == 0) {
-            Item it = first_item<ROWS>(a, S.win, sh);
             constexpr uint32_t ID_S = idesc<C>(128, KT, false), ID_O = idesc<C>(128, D, true);
             const uint32_t q_at = smem_addr(qs), ring_at = smem_addr(ring);
             int base = 0, nq = 0, np[2] = {0, 0};
             bool ok = true;
-            for (long long u = sh.u; u < sh.end && ok;) {
-                const int t0 = static_cast<int>(u - it.u0), t1 = static_cast<int>(min(static_cast<long long>(it.tiles), sh.end - it.u0));
-                const bool two = it.m > 128;
-                const int nt = it.n_keys > 0 ? t1 - t0 : 0, P = two ? 2 * nt : nt;
+#pragma unroll 1
+            for (int sn = 0; ok; ++sn) {
+                if (!wait(&S.segs.full[sn % SegmentRing::N], (sn / SegmentRing::N) & 1)) break;
+                const Segment & s = S.segs.s[sn % SegmentRing::N];
+                if (s.nt < 0) break;
+                const bool two = s.m > 128;
+                const int nt = s.n_keys > 0 ? s.nt : 0, P = two ? 2 * nt : nt;
+                mbar_arrive(&S.segs.empty[sn % SegmentRing::N]);
+                if (P == 0) continue;
                 const auto tile = [&](int n) { return two ? n >> 1 : n; };
                 const auto scores = [&](int n) {
                     const int g = n & 1, st = (base + 2 * tile(n)) % L::STAGES;
@@ -199,13 +214,16 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                     if (!two || g == 1) commit(&S.empty[st]);
                     return true;
                 };
-                if (P > 0) {
-                    ok = wait(&S.q_full, nq & 1);
-                    fence_after_sync();
-                    ok = ok && scores(0) && (P < 2 || scores(1));
-                }
+                // the first of the loop's steps only ask for scores
+                ok = wait(&S.q_full, nq & 1);
                 ++nq;
-                for (int n = 0; n < P && ok; ++n) {
+                fence_after_sync();
+#pragma unroll 1
+                for (int n = -2; n < P && ok; ++n) {
+                    if (n < 0) {
+                        if (n + 2 < P) ok = scores(n + 2);
+                        continue;
+                    }
                     const int g = n & 1, idx = base + 2 * tile(n) + 1, st = idx % L::STAGES;
                     ok = wait(&S.full[st], (idx / L::STAGES) & 1) && wait(&S.p_full[g], np[g] & 1);
                     if (!ok) break;
@@ -222,24 +240,26 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                     if (n + 2 < P) ok = scores(n + 2);
                 }
                 base += 2 * nt;
-                u += t1 - t0;
-                if (u < sh.end) next_item<ROWS>(a, S.win, it);
             }
             // nothing may still write the tensor memory when it is given back
             commit(&S.drained);
             mbar_drain(&S.drained, 0);
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        Item it = first_item<ROWS>(a, S.win, sh);
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int wg = warp >> 2, r = tid & 127;
         const uint32_t lane_at = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + lane_at + wg * 128, o_at = tmem + lane_at + 256 + wg * 128;
         int base = 0, ns = 0, no = 0;
-        for (long long u = sh.u; u < sh.end;) {
-            const int t0 = static_cast<int>(u - it.u0), t1 = static_cast<int>(min(static_cast<long long>(it.tiles), sh.end - it.u0));
+#pragma unroll 1
+        for (int sn = 0;; ++sn) {
+            const bool got = wait(&S.segs.full[sn % SegmentRing::N], (sn / SegmentRing::N) & 1);
+            // after an abort all warps leave together
+            if (named_sync_or(1, 256, !got)) break;
+            const Segment & it = S.segs.s[sn % SegmentRing::N];
+            if (it.nt < 0) break;
             const bool two = it.m > 128;
-            const int nt = it.n_keys > 0 ? t1 - t0 : 0;
+            const int nt = it.n_keys > 0 ? it.nt : 0, n_keys = it.n_keys, ctx = it.ctx, t0 = it.t0;
             // q into shared memory: rows of 16-bit values (f32: the high terms, then the low ones)
             if (nt > 0) {
                 constexpr int CH = D / 8, STEP = 256 / CH, U = 128 / STEP;   // 16-byte pieces of a row; rows a pass; passes a tile
@@ -285,31 +305,31 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
 
             const int m = (two ? wg * 128 : 0) + r, j = by_group(a, it.m0 + min(m, it.m - 1));
             // every row of the warp sees the tokens before `open`
-            const int open = it.rq.ctx + (a.mask ? 0 : by_group(a, it.m0 + min((two ? wg * 128 : 0) + (warp & 3) * 32, it.m - 1)) + 1);
+            const int open = ctx + (a.mask ? 0 : by_group(a, it.m0 + min((two ? wg * 128 : 0) + (warp & 3) * 32, it.m - 1)) + 1);
             float top = -INFINITY, sum = 0.f;
             bool any = false;                             // this warpgroup has had a tile
             for (int x = two ? 0 : wg; x < nt; x += two ? 1 : 2, ++ns) {
                 if (!wait(&S.s_full[wg], ns & 1)) break;
                 fence_after_sync();
+                const int key0 = (t0 + x) * KT, left = n_keys - key0;
+                if (left < KT) {                      // V rows past the last token: zeros, whatever the page holds there
+                    const int idx = base + 2 * x + 1, st = idx % L::STAGES;
+                    wait(&S.full[st], (idx / L::STAGES) & 1);
+                    for (int k = r; k < (KT - left) * (D / 8); k += 128) {
+                        const int key = left + k / (D / 8), c = k % (D / 8);
+                        *reinterpret_cast<uint4 *>(ring + st * L::STAGE + (c >> 3) * (KT * 128) + key * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_smem();
+                }
                 uint32_t s[KT];
                 tmem_ld<64>(s_at, s);
                 tmem_ld<64>(s_at + 64, s + 64);
-                const int key0 = (t0 + x) * KT, left = it.n_keys - key0;
                 if (key0 + KT > open) {                   // some of these tokens are not seen by every row of the warp
 #pragma unroll
                     for (int w = 0; w < KT / 32; ++w) {
-                        const uint32_t b = seen_bits(a, it, j, key0 + 32 * w - it.rq.ctx, left - 32 * w);
+                        const uint32_t b = seen_bits(a, it, j, key0 + 32 * w - ctx, left - 32 * w);
 #pragma unroll
                         for (int k = 0; k < 32; ++k) s[32 * w + k] = b >> k & 1 ? s[32 * w + k] : __float_as_uint(-INFINITY);
-                    }
-                    if (left < KT) {                      // V rows past the last token: zeros, whatever the page holds there
-                        const int idx = base + 2 * x + 1, st = idx % L::STAGES;
-                        wait(&S.full[st], (idx / L::STAGES) & 1);
-                        for (int k = r; k < (KT - left) * (D / 8); k += 128) {
-                            const int key = left + k / (D / 8), c = k % (D / 8);
-                            *reinterpret_cast<uint4 *>(ring + st * L::STAGE + (c >> 3) * (KT * 128) + key * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
-                        }
-                        fence_proxy_async_smem();
                     }
                 }
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -322,7 +342,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                     const float now = fmaxf(best, top), w = now == -INFINITY ? 1.f : exp2_fast(top - now);
                     top = now;
                     sum *= w;
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
                         uint32_t o[32];
                         tmem_ld<32>(o_at + c, o);
@@ -364,7 +384,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 fence_after_sync();
             }
 
-            const bool whole = t0 == 0 && t1 == it.tiles;
+            const bool whole = it.whole;
             float mine = 1.f;                             // what this warpgroup's O counts
             float * const half = reinterpret_cast<float *>(qs);
             int c_lo = 0, c_hi = D;                       // the columns that this warpgroup finishes
@@ -380,32 +400,25 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 top = t;
                 c_lo = wg * (D / 2);
                 c_hi = c_lo + D / 2;
-                if (any && nt > 1) {
+                if (any) {
                     const int give = (1 - wg) * (D / 2);
-#pragma unroll
-                    for (int c = 0; c < D / 2; c += 32) {
+#pragma unroll 1
+                    for (int c = give; c < give + D / 2; c += 32) {
                         uint32_t o[32];
-                        tmem_ld<32>(o_at + give + c, o);
+                        tmem_ld<32>(o_at + c, o);
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) half[(give + c + k) * 128 + r] = __uint_as_float(o[k]) * mine;
-                    }
-                } else if (any) {                         // the only one with a tile: the other has nothing to add
-#pragma unroll
-                    for (int c = 0; c < D / 2; c += 32) {
-                        uint32_t o[32];
-                        tmem_ld<32>(o_at + D / 2 + c, o);
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) half[(D / 2 + c + k) * 128 + r] = __uint_as_float(o[k]) * mine;
+                        for (int k = 0; k < 32; ++k) half[(c + k) * 128 + r] = __uint_as_float(o[k]) * mine;
                     }
                 }
                 named_sync(1, 256);
             }
             {
-                float4 * pc = reinterpret_cast<float4 *>(piece(a, blockIdx.x, t0 == 0)) + m;
+                float4 * pc = reinterpret_cast<float4 *>(piece(a, blockIdx.x, it.slot)) + m;
                 const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
                 const bool other = !two && (wg == 1 ? nt > 0 : nt > 1), live = m < it.m;
                 T * dst = row_at<T>(a, a.out, a.out_stride, it, live ? m : 0);
                 const bool wide = (reinterpret_cast<uintptr_t>(dst) & 31) == 0;   // rows are at least 16-byte aligned
+#pragma unroll 1
                 for (int c = c_lo; c < c_hi; c += 32) {
                     uint32_t o[32];
                     if (any) tmem_ld<32>(o_at + c, o);
@@ -444,9 +457,9 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 }
                 if (live && (two || wg == 0)) {
                     if (whole) {
-                        if (a.lse) *lse_at(a, it, m) = lse_of(top, sum);
+                        if (a.lse) put_lse(a, it, m, top, sum);
                     } else {
-                        float * st = piece(a, blockIdx.x, t0 == 0) + ROWS * D + m;
+                        float * st = piece(a, blockIdx.x, it.slot) + ROWS * D + m;
                         st[0] = top;
                         st[ROWS] = sum;
                     }
@@ -456,12 +469,12 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
             if (!whole) __threadfence();
             named_sync(1, 256);
             if (!whole) {
-                if (tid == 0) S.is_last = arrive_piece(a, sh, it);
+                if (tid == 0) S.is_last = arrive_piece(a, it);
                 named_sync(1, 256);
-                if (S.is_last) join<T, C, ROWS, D, 256, 1, 2 * L::QTILE / 4>(a, sh, it, tid, reinterpret_cast<float *>(qs));
+                if (S.is_last) join<T, C, ROWS, D, 256, 1, 2 * L::QTILE / 4>(a, it, tid, reinterpret_cast<float *>(qs));
             }
-            u += t1 - t0;
-            if (u < sh.end) next_item<ROWS>(a, S.win, it);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&S.segs.empty[sn % SegmentRing::N]);
         }
     }
     __syncwarp();
