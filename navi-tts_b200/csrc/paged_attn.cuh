@@ -12,12 +12,6 @@
 
 #include <type_traits>
 
-// What runs seldom: out of line, to keep the code short. A kernel that moves registers between its warps
-// (setmaxnreg) can make no calls and defines this as __forceinline__ before it includes the file.
-#ifndef NAVI_ATTN_SELDOM
-#define NAVI_ATTN_SELDOM __noinline__
-#endif
-
 namespace navi::attn {
 
 using namespace navi::dev;
@@ -41,7 +35,7 @@ struct Request {
     int row0, n, ctx, keys;      // first row, rows, cached tokens, tokens in all
     int table;                   // its row of the block table
 };
-static __device__ NAVI_ATTN_SELDOM Request request(const AttendArgs & a, int i) {
+__device__ __forceinline__ Request request(const AttendArgs & a, int i) {
     Request r;
     r.row0 = a.cu_rows[i];
     r.n = max(min(a.cu_rows[i + 1], a.max_rows) - r.row0, 0);
@@ -93,7 +87,8 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // (the sums and each row's maximum and sum, f32) in the stream's scratch, and the block that
 // arrives last joins them in the blocks' order, so the result does not depend on who was last. A
 // block has at most two such pieces: slot 0 for one that begins inside an item, slot 1 for one
-// that only ends inside it.
+// that begins with the item and ends inside it. Arrivals are counted in key tiles at the item's
+// first block.
 //
 // One warp of the block walks the list and hands each part of it (a segment: the block's key tiles
 // of one item) to the others through a small ring in shared memory. The walk is long code that
@@ -106,9 +101,9 @@ struct Segment {
     int row0, ctx, table, g;     // the request, the KV head
     int m0, m, n_keys;           // its first row x head, how many, the keys that they may see
     int t0, nt;                  // key tiles t0 .. t0 + nt - 1; nt -1: no more segments
-    int whole, slot;             // all of the item's tiles; else the piece's slot,
-    int c0, np;                  // and the blocks c0 .. c0 + np - 1 that have pieces of it
+    int u0, tiles;               // the item's units
 };
+__device__ __forceinline__ bool is_whole(const Segment & s) { return s.nt == s.tiles; }
 
 template <int ROWS> __device__ __forceinline__ int row_tiles(const AttendArgs & a, const Request & r) { return (r.n * a.group + ROWS - 1) / ROWS; }
 template <int ROWS> __device__ __forceinline__ int keys_of(const AttendArgs & a, const Request & r, int rt) {
@@ -117,7 +112,7 @@ template <int ROWS> __device__ __forceinline__ int keys_of(const AttendArgs & a,
 }
 __device__ __forceinline__ int tiles_of(int n_keys) { return max((n_keys + KT - 1) / KT, 1); }
 // the units of one KV head of a request
-template <int ROWS> __device__ NAVI_ATTN_SELDOM int units_of(const AttendArgs & a, const Request & r) {
+template <int ROWS> __device__ __forceinline__ int units_of(const AttendArgs & a, const Request & r) {
     const int rts = row_tiles<ROWS>(a, r);
     if (a.mask || r.keys == 0) return rts * tiles_of(r.keys);
     int n = 0;
@@ -126,70 +121,100 @@ template <int ROWS> __device__ NAVI_ATTN_SELDOM int units_of(const AttendArgs & 
     return n;
 }
 
+// x / y of x >= 0, y > 0. (x + 1/2) / y is 1 / 2y away from an integer at least, the approximate quotient
+// off by 2^-21 of itself at most: exact below 2^20.
+__device__ __forceinline__ int quick_div(int x, int y) {
+    return x < 1 << 20 ? static_cast<int>(__fdividef(static_cast<float>(x) + 0.5f, static_cast<float>(y))) : x / y;
+}
+
 // How the units divide: `more` blocks of `per` + 1 units, then blocks of `per`.
 struct Division {
     int per, more;
     __device__ __forceinline__ int first(int block) const { return block * per + min(block, more); }
     __device__ __forceinline__ int block(int unit) const {
         const int x = unit - more * (per + 1);
-        return x < 0 ? unit / (per + 1) : more + x / per;
+        return x < 0 ? quick_div(unit, per + 1) : more + quick_div(x, per);
     }
 };
-// What the block's threads find out together: the division, and the request that holds the block's first unit.
+// The division, this block's units [u, end), and the request i that holds the first of them and begins
+// at unit `base`.
 struct Share {
     Division d;
-    int u, end;                  // this block's units
-    int i, base;                 // the request of unit u, and its first unit
+    int u, end, i, base;
 };
 
-// Every thread of the block takes part. What the threads wrote to shared memory before is there for
-// all of them after it. (The host has checked that the units fit 31 bits.)
-template <int ROWS, int THREADS> __device__ __forceinline__ void share_out(const AttendArgs & a, Share & sh, int * red) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.n_req;
-    const bool one = B <= 32;    // every warp does the sums by itself, a lane a request: one trip to L2 and no barrier between
-    const int per = one ? 1 : (B + THREADS - 1) / THREADS, i0 = min(B, one ? lane : tid * per), i1 = min(B, i0 + per);
-    int mine = 0;
-#pragma unroll 1
-    for (int i = i0; i < i1; ++i) mine += units_of<ROWS>(a, request(a, i)) * a.n_kv;
-    int x = mine;
+__device__ __forceinline__ int warp_scan(int x) {   // inclusive
+    const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
-    int base = x - mine, total = __shfl_sync(0xffffffffu, x, 31);
-    if (!one) {
-        if (lane == 31) red[warp] = x;
-        __syncthreads();
-        total = 0;
-#pragma unroll 1
-        for (int w = 0; w < THREADS / 32; ++w) {
-            if (w < warp) base += red[w];
-            total += red[w];
-        }
-    }
+    return x;
+}
+__device__ __forceinline__ void take(Share & sh, int total) {
     const int G = min(static_cast<int>(gridDim.x), total), c = blockIdx.x;
-    Division d{0, 0};
+    sh.d = {0, 0};
     if (G > 0) {
-        d.per = total / G;
-        d.more = total - d.per * G;
+        sh.d.per = quick_div(total, G);
+        sh.d.more = total - sh.d.per * G;
     }
-    const int u = d.first(c), end = c < G ? d.first(c + 1) : u;
-    if (tid == 0) {
-        sh.d = d;
-        sh.u = u;
-        sh.end = end;
-    }
-    if ((!one || warp == 0) && u < end && u >= base && u < base + mine) {
-        int i = i0, b = base;
+    sh.u = sh.d.first(c);
+    sh.end = c < G ? sh.d.first(c + 1) : sh.u;
+}
+// Up to 32 requests a warp finds its block's share by itself, a lane a request. (The host has checked
+// that the units fit 31 bits.)
+template <int ROWS> __device__ __forceinline__ Share share_of_warp(const AttendArgs & a, Request & first) {
+    const int lane = threadIdx.x & 31;
+    Request r{};
+    if (lane < a.n_req) r = request(a, lane);
+    const int mine = units_of<ROWS>(a, r) * a.n_kv, x = warp_scan(mine);
+    Share sh;
+    take(sh, __shfl_sync(0xffffffffu, x, 31));
+    sh.i = max(__ffs(__ballot_sync(0xffffffffu, sh.u < x)) - 1, 0);   // the first request that ends after unit u
+    sh.base = __shfl_sync(0xffffffffu, x - mine, sh.i);
+    first.row0 = __shfl_sync(0xffffffffu, r.row0, sh.i);
+    first.n = __shfl_sync(0xffffffffu, r.n, sh.i);
+    first.ctx = __shfl_sync(0xffffffffu, r.ctx, sh.i);
+    first.keys = __shfl_sync(0xffffffffu, r.keys, sh.i);
+    first.table = __shfl_sync(0xffffffffu, r.table, sh.i);
+    return sh;
+}
+// More: all THREADS threads of the block, each some requests in a row. What they wrote to shared memory
+// before is there for all of them after it.
+template <int ROWS, int THREADS> __device__ __forceinline__ void share_of_block(const AttendArgs & a, Share & out, int * red) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.n_req;
+    const int per = (B + THREADS - 1) / THREADS, i0 = min(B, tid * per), i1 = min(B, i0 + per);
+    int mine = 0;
 #pragma unroll 1
-        for (; per > 1; ++i) {
+    for (int i = i0; i < i1; ++i) mine += units_of<ROWS>(a, request(a, i)) * a.n_kv;
+    const int x = warp_scan(mine);
+    if (lane == 31) red[warp] = x;
+    __syncthreads();
+    int base = x - mine, total = 0;
+#pragma unroll 1
+    for (int w = 0; w < THREADS / 32; ++w) {
+        if (w < warp) base += red[w];
+        total += red[w];
+    }
+    Share sh{};
+    take(sh, total);
+    const int u = sh.u;
+    if (tid == 0) {
+        out.d = sh.d;
+        out.u = u;
+        out.end = sh.end;
+    }
+    if (u < sh.end && u >= base && u < base + mine) {
+        int i = i0;
+#pragma unroll 1
+        for (;; ++i) {
             const int n = units_of<ROWS>(a, request(a, i)) * a.n_kv;
-            if (u < b + n) break;
-            b += n;
+            if (u < base + n) break;
+            base += n;
         }
-        sh.i = i;
-        sh.base = b;
+        out.i = i;
+        out.base = base;
     }
     __syncthreads();
 }
@@ -197,20 +222,20 @@ template <int ROWS, int THREADS> __device__ __forceinline__ void share_out(const
 // The walk over the block's segments: next() fills in the next one; false when there is none.
 template <int ROWS> struct Walk {
     const AttendArgs & a;
-    const Share & sh;
+    Share sh;
     Request r;
     int i, g, rt, u0, u, tiles, n_keys;
 
-    __device__ __forceinline__ Walk(const AttendArgs & args, const Share & share) : a(args), sh(share) {
+    __device__ __forceinline__ Walk(const AttendArgs & args, const Share & share, const Request & first) : a(args), sh(share), r(first) {
         i = sh.i;
         u = sh.u;
-        r = request(a, i);
+        if (u >= sh.end) return;
         const int per_head = units_of<ROWS>(a, r);
-        g = (u - sh.base) / per_head;
+        g = quick_div(u - sh.base, per_head);
         u0 = sh.base + g * per_head;
         rt = 0;
         if (a.mask || r.keys == 0) {   // every row tile has as many key tiles
-            rt = (u - u0) / tiles_of(r.keys);
+            rt = quick_div(u - u0, tiles_of(r.keys));
             u0 += rt * tiles_of(r.keys);
         }
         open();
@@ -251,10 +276,8 @@ template <int ROWS> struct Walk {
         s.n_keys = n_keys;
         s.t0 = u - u0;
         s.nt = t1 - s.t0;
-        s.whole = s.nt == tiles;
-        s.slot = s.t0 == 0;
-        s.c0 = sh.d.block(u0);
-        s.np = sh.d.block(u0 + tiles - 1) - s.c0 + 1;
+        s.u0 = u0;
+        s.tiles = tiles;
         u += s.nt;
         return true;
     }
@@ -275,10 +298,12 @@ __device__ __forceinline__ void put_lse(const AttendArgs & a, const Segment & s,
     a.lse[static_cast<size_t>(s.row0 + j) * a.n_head + s.g * a.group + at - j * a.group] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
 }
 
-// One thread of a block whose piece is written: whether it is the item's last.
-__device__ __forceinline__ bool arrive_piece(const AttendArgs & a, const Segment & s) {
-    if (atomicAdd(a.arrived + s.c0, 1) != s.np - 1) return false;
-    a.arrived[s.c0] = 0;
+// One thread of a block whose piece is written (and a barrier passed since): whether it is the item's last.
+__device__ __forceinline__ bool arrive_piece(const AttendArgs & a, const Division & d, const Segment & s) {
+    const int c0 = s.t0 == 0 ? static_cast<int>(blockIdx.x) : d.block(s.u0);
+    __threadfence();
+    if (atomicAdd(a.arrived + c0, s.nt) + s.nt != s.tiles) return false;
+    a.arrived[c0] = 0;
     __threadfence();
     return true;
 }
@@ -287,8 +312,8 @@ __device__ __forceinline__ bool arrive_piece(const AttendArgs & a, const Segment
 // piece counts in each row goes to `weight` (CAP floats of shared memory), LANES lanes to a row,
 // then the sums are read, by a thread that stays with its row: neighbours read neighbouring rows.
 template <class T, class C, int ROWS, int D, int THREADS, int LANES, int CAP>
-__device__ __forceinline__ void join(const AttendArgs & a, const Segment & s, int tid, float * weight) {
-    const int c0 = s.c0, np = s.np;
+__device__ __forceinline__ void join(const AttendArgs & a, const Division & d, const Segment & s, int tid, float * weight) {
+    const int c0 = d.block(s.u0), np = d.block(s.u0 + s.tiles - 1) - c0 + 1;
     const auto part = [&](int p) { return piece(a, c0 + p, p == 0); };
     const int most = min(CAP / np, ROWS);             // rows at a time: up to a block a multiprocessor shares an item
 #pragma unroll 1
@@ -319,7 +344,7 @@ __device__ __forceinline__ void join(const AttendArgs & a, const Segment & s, in
             if (live && sub == 0 && a.lse) put_lse(a, s, m, top, l);
         }
         named_sync(1, THREADS);
-        constexpr int QS = THREADS / ROWS, N = D / 4 / QS, U = N < 8 ? N : 8;
+        constexpr int QS = THREADS / ROWS < D / 4 ? THREADS / ROWS : D / 4, N = D / 4 / QS, U = N < 8 ? N : 8;
         static_assert(THREADS % ROWS == 0 && N % U == 0);
         const int r = tid % ROWS;
         if (r < rows) {
@@ -371,7 +396,7 @@ struct Wait {
     __device__ __forceinline__ bool operator()(uint64_t * bar, uint32_t parity) const {
         return mbar_try_wait(bar, parity) || slow(bar, parity);
     }
-    __device__ NAVI_ATTN_SELDOM bool slow(uint64_t * bar, uint32_t parity) const {
+    __device__ __forceinline__ bool slow(uint64_t * bar, uint32_t parity) const {
 #pragma unroll 1
         for (int k = 0; k < 64; ++k)
             if (mbar_try_wait(bar, parity)) return true;
@@ -394,13 +419,24 @@ __device__ __forceinline__ void mbar_drain(uint64_t * bar, uint32_t parity) {
     while (!mbar_try_wait(bar, parity) && globaltimer() - t0 < 2 * DEADLINE_NS) {}
 }
 
-// Whether row j of the segment's request sees token `key`.
-__device__ __forceinline__ bool sees(const AttendArgs & a, const Segment & s, int key, int j) {
-    if (key >= s.n_keys) return false;
-    const int at = key - s.ctx;
-    if (at < 0) return true;
-    if (!a.mask) return at <= j;
-    return at < 64 * a.mask_words && (__ldg(a.mask + static_cast<size_t>(s.row0 + j) * a.mask_words + (at >> 6)) >> (at & 63) & 1);
+// Bits 0..31: whether row j of the request sees the tokens ctx + a .. ctx + a + 31 (a may be negative:
+// those are cached tokens), of which `left` are the item's.
+__device__ __forceinline__ uint32_t seen_bits(const AttendArgs & a, const Segment & it, int j, int at, int left) {
+    if (left <= 0) return 0u;
+    uint32_t b;
+    if (at + 31 < 0) b = ~0u;
+    else if (!a.mask) {
+        const int n = j - at + 1;            // tokens from `at` up to row j itself
+        b = n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
+    } else {
+        const uint64_t * m = a.mask + static_cast<size_t>(it.row0 + j) * a.mask_words;
+        const int w = at >> 6;               // floor: -1 for the bits before row 0, all seen
+        const uint64_t lo = w < 0 ? ~0ull : w < a.mask_words ? __ldg(m + w) : 0ull;
+        const uint64_t hi = w + 1 < a.mask_words ? __ldg(m + w + 1) : 0ull;
+        const int s = at & 63;
+        b = static_cast<uint32_t>(s ? (lo >> s) | (hi << (64 - s)) : lo);
+    }
+    return left >= 32 ? b : b & ((1u << left) - 1u);
 }
 
 // The pages that hold key tile t, and the bytes of them that one pool contributes.

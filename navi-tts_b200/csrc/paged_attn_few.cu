@@ -24,37 +24,43 @@ template <class C> __device__ __forceinline__ void mma(float (&c)[4], const uint
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// RT tiles of 16 rows, 8 / RT warps to each, which divide a key tile of 128 between them, each with
-// a running maximum and sums of its own until the item ends; a ninth warp keeps a ring of tiles
-// full by TMA. K and V are read once however many rows there are, so up to 32 rows the bound is
-// HBM. f32 rows enter the products as two f16 terms, q = hi + lo and p = hi + lo, against the
-// exact cache values, about 22 bits; the tensor cores' sums truncate, so the low terms and each
-// step's contribution are summed apart and added in f32. 16-bit rows are exact, and p is
-// rounded once to the type that the result has.
+// A tile of 16 rows (8, where a block has no more) belongs to KQ warps, which divide a key tile of
+// 128 between them, each with a running maximum and sums of its own until the segment ends; a
+// ninth warp keeps a ring of tiles full by TMA. K and V are read once however many rows there are,
+// so up to 32 rows the bound is HBM.
+//
+// f32 rows enter the products as two f16 terms, q = hi + lo and p = hi + lo, against the exact cache
+// values, about 22 bits. With 8 rows the high terms are rows 0..7 of the 16 that a product has
+// and the low ones rows 8..15, so that they cost nothing. The tensor cores' sums truncate: the low
+// terms and each step's contribution are summed apart and added in f32. 16-bit rows are exact, and
+// p is rounded once to the type that the result has.
 template <int D> struct FewSmem {
     static constexpr int STAGE = KT * D * 4;                    // K and V of a tile
     static constexpr int STAGES = D == 128 ? 3 : 6;
-    static constexpr int JOIN = 4 * 16 * D * 4;                 // four warps' sums
+    static constexpr int JOIN = 8 * 16 * 64 * 4;                // eight warps' sums over 64 dims
     static constexpr int BYTES = 1024 + STAGES * STAGE + JOIN;  // 1024: to align the ring to the swizzle's 1024 bytes
 };
 
-template <class T, class C, int D, int RT>
+template <class T, class C, int D, int ROWS>   // ROWS: 8, 16 or 32 rows of an item
 __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
                                                        const __grid_constant__ CUtensorMap vmap) {
-    constexpr bool SPLIT = std::is_same_v<T, float>;
-    constexpr int ROWS = 16 * RT, KQ = 8 / RT, WK = KT / KQ;    // WK: keys of a tile that a warp takes
+    constexpr bool SPLIT = std::is_same_v<T, float>, EIGHT = ROWS == 8;
+    constexpr int RT = EIGHT ? 1 : ROWS / 16, KQ = 8 / RT, WK = KT / KQ;    // row tiles; warps and keys of a tile a warp takes
+    constexpr int XR = EIGHT ? 1 : 2, MR = 8 * XR;                          // rows a thread and a warp have
+    constexpr bool TERMS = SPLIT && !EIGHT;                                 // the low terms are products of their own
     using L = FewSmem<D>;
     extern __shared__ uint8_t raw[];
     uint8_t * ring = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
     float4 * sums = reinterpret_cast<float4 *>(ring + L::STAGES * L::STAGE);
-    // q lies in the upper half of the warps' sums, which are idle while it is read: [ROWS][D], f32 rows twice
-    uint8_t * qs = reinterpret_cast<uint8_t *>(sums) + L::JOIN / 2;
-    static_assert(2 * 32 * D * 2 <= L::JOIN / 2);
+    // q lies where the warps' sums come when it is no longer read: [16 RT][D], the low terms of f32 rows in rows
+    // 8..15 or, with more than 8 rows, in as many rows again
+    uint8_t * qs = reinterpret_cast<uint8_t *>(sums);
+    static_assert(2 * 32 * D * 2 <= L::JOIN);
     __shared__ __align__(8) uint64_t full[L::STAGES], empty[L::STAGES];
     __shared__ __align__(8) SegmentRing segs;
-    __shared__ float stat[8][2][16];
+    __shared__ float stat[8][2][MR];
     __shared__ int red[9];
-    __shared__ Share sh;
+    __shared__ Share share;
     __shared__ int abort_flag, is_last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, tq = lane & 3;
     if (tid == 0) {
@@ -66,14 +72,24 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
         segs.init(8);
         fence_mbar_init();
     }
+    __syncthreads();
     griddep_wait();
     griddep_launch_dependents();
-    share_out<ROWS, 288>(a, sh, red);
-    if (sh.u >= sh.end) return;
+    const bool one = a.n_req <= 32;
+    if (!one) share_of_block<ROWS, 288>(a, share, red);
     const Wait wait{&abort_flag, a.err};
 
     if (warp == 8) {
-        Walk<ROWS> walk(a, sh);
+        Request first{};
+        Share sh;
+        if (one) {
+            sh = share_of_warp<ROWS>(a, first);
+            if (lane == 0) share.d = sh.d;           // the other warps read it after a segment
+        } else {
+            sh = share;
+            if (sh.u < sh.end) first = request(a, sh.i);
+        }
+        Walk<ROWS> walk(a, sh, first);
         int n = 0;
         bool ok = true;
         const int kv = lane >> 4, box = lane & 15;   // half a warp each for K and V
@@ -81,6 +97,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
         for (int k = 0; ok; ++k) {
             Segment s;
             const bool more = walk.next(s);
+            int page = more && s.n_keys > 0 ? page_of_box<D>(a, s, s.t0, box) : -1;
             if (k >= SegmentRing::N) ok = __shfl_sync(0xffffffffu, lane == 0 ? wait(&segs.empty[k % SegmentRing::N], (k / SegmentRing::N - 1) & 1) : 0, 0);
             if (!ok) break;
             if (lane == 0) {
@@ -89,7 +106,6 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
             }
             if (!more) break;
             if (s.n_keys <= 0) continue;
-            int page = page_of_box<D>(a, s, s.t0, box);
 #pragma unroll 1
             for (int t = s.t0; t < s.t0 + s.nt; ++t, ++n) {
                 const int st = n % L::STAGES, next = t + 1 < s.t0 + s.nt ? page_of_box<D>(a, s, t + 1, box) : -1;
@@ -108,9 +124,17 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
     }
 
     const int rt = warp / KQ, kq = warp % KQ, k0 = kq * WK;
-    const uint32_t ring_at = smem_addr(ring), q_at = smem_addr(qs);
-    const auto at = [](uint32_t base, int key, int piece) { return base + (piece >> 3) * (KT * 128) + key * 128 + (((piece & 7) ^ (key & 7)) << 4); };
-    const auto q_swz = [](int row, int piece) { return static_cast<uint32_t>(row * (D * 2) + ((piece ^ (row & 7)) << 4)); };
+    // Shared-memory rows are 128 bytes of a half of 64 dims, their eight 16-byte pieces swizzled by the row. The lanes of
+    // an ldmatrix read eight rows in a row from a multiple of 8 on, so the swizzle is the lane's own, and piece
+    // 2 j + b of a row lies at one of four offsets.
+    uint32_t off_k[4], off_v[4];                      // b = (lane >> 3) & 1 for K, lane >> 4 for V and q
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        off_k[j] = ((2 * j + ((lane >> 3) & 1)) ^ (lane & 7)) << 4;
+        off_v[j] = ((2 * j + (lane >> 4)) ^ (lane & 7)) << 4;
+    }
+    const uint32_t k_at = smem_addr(ring) + (k0 + (lane & 7) + (lane >> 4) * 8) * 128, v_at = smem_addr(ring) + L::STAGE / 2 + (k0 + (lane & 15)) * 128;
+    const uint32_t q_at = smem_addr(qs) + (rt * 16 + (lane & 15)) * (D * 2);
     int n = 0;
 #pragma unroll 1
     for (int sn = 0;; ++sn) {
@@ -136,25 +160,34 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
                     hi = *reinterpret_cast<const uint4 *>(src);
                 }
             }
-            *reinterpret_cast<uint4 *>(qs + q_swz(m, c)) = hi;
-            if constexpr (SPLIT) *reinterpret_cast<uint4 *>(qs + ROWS * D * 2 + q_swz(m, c)) = lo;
+            uint8_t * dst = qs + m * (D * 2) + ((c ^ (m & 7)) << 4);
+            *reinterpret_cast<uint4 *>(dst) = hi;
+            if constexpr (SPLIT || EIGHT) *reinterpret_cast<uint4 *>(dst + (EIGHT ? 8 : ROWS) * D * 2) = lo;
         }
         named_sync(1, 256);
-        float o[D / 8][4], mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        float o[D / 8][2 * XR], mx[XR], l[XR];
+        int row[XR];
 #pragma unroll
-        for (int x = 0; x < D / 8; ++x) o[x][0] = o[x][1] = o[x][2] = o[x][3] = 0.f;
+        for (int x = 0; x < XR; ++x) {
+            mx[x] = -INFINITY;
+            l[x] = 0.f;
+            row[x] = by_group(a, s.m0 + min(rt * 16 + gq + 8 * x, s.m - 1));
+        }
+#pragma unroll
+        for (int d = 0; d < D / 8; ++d)
+#pragma unroll
+            for (int e = 0; e < 2 * XR; ++e) o[d][e] = 0.f;
         const int n_keys = s.n_keys, ctx = s.ctx, tiles = n_keys > 0 ? s.nt : 0;
 #pragma unroll 1
         for (int t = 0; t < tiles; ++t, ++n) {
             const int st = n % L::STAGES;
-            if (!wait(&full[st], (n / L::STAGES) & 1)) break;
-            const uint32_t sk = ring_at + st * L::STAGE, sv = sk + L::STAGE / 2;
             const int first = (s.t0 + t) * KT + k0, valid = n_keys - first;   // this warp's keys of the tile
+            if (!wait(&full[st], (n / L::STAGES) & 1)) break;
             if (valid > 0 && valid < WK) {   // V rows past the item's keys: zeros, whatever the page holds there
 #pragma unroll 1
                 for (int x = lane; x < (WK - valid) * (D / 8); x += 32) {
-                    const int key = k0 + valid + x / (D / 8);
-                    *reinterpret_cast<uint4 *>(ring + (at(sv, key, x % (D / 8)) - ring_at)) = make_uint4(0, 0, 0, 0);
+                    const int key = k0 + valid + x / (D / 8), c = x % (D / 8);
+                    *reinterpret_cast<uint4 *>(ring + st * L::STAGE + L::STAGE / 2 + (c >> 3) * (KT * 128) + key * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -162,40 +195,44 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
             // 16 keys at a time
 #pragma unroll 1
             for (int k = 0; k < WK && k < valid; k += 16) {
+                const bool masked = first + k + 16 > ctx;   // some of these keys are new rows, or past the last
+                uint32_t seen[XR];
+                if (masked) {
+#pragma unroll
+                    for (int x = 0; x < XR; ++x) seen[x] = seen_bits(a, s, row[x], first + k - ctx, valid - k);
+                }
                 float sc[2][4] = {}, low[2][4] = {};
-#pragma unroll 4
+                const uint32_t kk = k_at + st * L::STAGE + k * 128, vv = v_at + st * L::STAGE + k * 128;
+#pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks) {
-                    uint32_t b[4], qh[4];
-                    ldsm4(qh, q_at + q_swz(rt * 16 + (lane & 15), ks * 2 + (lane >> 4)));
-                    ldsm4(b, at(sk, k0 + k + (lane & 7) + (lane >> 4) * 8, ks * 2 + ((lane >> 3) & 1)));
-                    mma<C>(sc[0], qh, b[0], b[1]);
-                    mma<C>(sc[1], qh, b[2], b[3]);
-                    if constexpr (SPLIT) {
-                        ldsm4(qh, q_at + ROWS * D * 2 + q_swz(rt * 16 + (lane & 15), ks * 2 + (lane >> 4)));
-                        mma<C>(low[0], qh, b[0], b[1]);
-                        mma<C>(low[1], qh, b[2], b[3]);
+                    uint32_t b[4], q[4];
+                    ldsm4(q, q_at + (ks >> 2) * 128 + off_v[ks & 3]);
+                    ldsm4(b, kk + (ks >> 2) * (KT * 128) + off_k[ks & 3]);
+                    mma<C>(sc[0], q, b[0], b[1]);
+                    mma<C>(sc[1], q, b[2], b[3]);
+                    if constexpr (TERMS) {
+                        ldsm4(q, q_at + ROWS * D * 2 + (ks >> 2) * 128 + off_v[ks & 3]);
+                        mma<C>(low[0], q, b[0], b[1]);
+                        mma<C>(low[1], q, b[2], b[3]);
                     }
                 }
                 if constexpr (SPLIT) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        sc[0][e] += low[0][e];
-                        sc[1][e] += low[1][e];
-                    }
-                }
-                if (first + k + 16 > ctx) {   // some of these keys are new rows, or past the last
+                    for (int y = 0; y < 2; ++y)
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const int j = by_group(a, s.m0 + min(rt * 16 + gq + 8 * x, s.m - 1));
+                        for (int e = 0; e < 2 * XR; ++e) sc[y][e] += EIGHT ? sc[y][2 + e] : low[y][e];
+                }
+                if (masked) {
+#pragma unroll
+                    for (int x = 0; x < XR; ++x)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            if (!sees(a, s, first + k + (e >> 1) * 8 + 2 * tq + (e & 1), j)) sc[e >> 1][2 * x + (e & 1)] = -INFINITY;
-                    }
+                            if (!(seen[x] >> ((e >> 1) * 8 + 2 * tq + (e & 1)) & 1)) sc[e >> 1][2 * x + (e & 1)] = -INFINITY;
                 }
-                float m[2];
+                float m[XR];
                 bool more = false;
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
+                for (int x = 0; x < XR; ++x) {
                     m[x] = fmaxf(fmaxf(sc[0][2 * x], sc[0][2 * x + 1]), fmaxf(sc[1][2 * x], sc[1][2 * x + 1]));
                     m[x] = fmaxf(m[x], __shfl_xor_sync(0xffffffffu, m[x], 1));
                     m[x] = fmaxf(m[x], __shfl_xor_sync(0xffffffffu, m[x], 2)) * a.scale;
@@ -203,7 +240,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
                 }
                 if (__any_sync(0xffffffffu, more)) {
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
+                    for (int x = 0; x < XR; ++x) {
                         m[x] = fmaxf(m[x], mx[x]);
                         const float w = m[x] == -INFINITY ? 1.f : exp2_fast(mx[x] - m[x]);
                         mx[x] = m[x];
@@ -215,33 +252,35 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
                         }
                     }
                 }
-                uint32_t ph[4], pl[4];
+                uint32_t ph[4] = {0, 0, 0, 0}, pl[4];
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
+                for (int x = 0; x < XR; ++x) {
                     const float ref = mx[x] == -INFINITY ? 0.f : mx[x];
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
                         const float p0 = exp2_fast(fmaf(sc[y][2 * x], a.scale, -ref)), p1 = exp2_fast(fmaf(sc[y][2 * x + 1], a.scale, -ref));
                         l[x] += p0 + p1;
-                        if constexpr (SPLIT) split_pair<C>(p0, p1, ph[2 * y + x], pl[2 * y + x]);
+                        if constexpr (TERMS) split_pair<C>(p0, p1, ph[2 * y + x], pl[2 * y + x]);
+                        else if constexpr (SPLIT) split_pair<C>(p0, p1, ph[2 * y], ph[2 * y + 1]);
                         else ph[2 * y + x] = pack<C>(p0, p1);
                     }
                 }
 #pragma unroll
                 for (int dp = 0; dp < D / 16; ++dp) {
                     uint32_t b[4];
-                    ldsm4t(b, at(sv, k0 + k + (lane & 15), dp * 2 + (lane >> 4)));
-                    if constexpr (SPLIT) {
+                    ldsm4t(b, vv + (dp >> 2) * (KT * 128) + off_v[dp & 3]);
+                    if constexpr (SPLIT || EIGHT) {
                         float c[2][4] = {};
-                        mma<C>(c[0], pl, b[0], b[1]);
-                        mma<C>(c[1], pl, b[2], b[3]);
+                        if constexpr (TERMS) {
+                            mma<C>(c[0], pl, b[0], b[1]);
+                            mma<C>(c[1], pl, b[2], b[3]);
+                        }
                         mma<C>(c[0], ph, b[0], b[1]);
                         mma<C>(c[1], ph, b[2], b[3]);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            o[2 * dp][e] += c[0][e];
-                            o[2 * dp + 1][e] += c[1][e];
-                        }
+                        for (int y = 0; y < 2; ++y)
+#pragma unroll
+                            for (int e = 0; e < 2 * XR; ++e) o[2 * dp + y][e] += SPLIT && EIGHT ? c[y][e] + c[y][2 + e] : c[y][e];
                     } else {
                         mma<C>(o[2 * dp], ph, b[0], b[1]);
                         mma<C>(o[2 * dp + 1], ph, b[2], b[3]);
@@ -252,9 +291,12 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
             if (lane == 0) mbar_arrive(&empty[st]);
         }
 
-        // the warps' sums of a row become one
+        // the warps' sums of a row become one: W dims at a time through shared memory, [warp][MR][W / 4 x 4], the pieces of
+        // 4 swizzled by row; then a thread has 4 dims of a row
+        constexpr int W = EIGHT ? D : 64, Q = W / 4;
+        static_assert(8 * MR * W * 4 <= L::JOIN);
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
+        for (int x = 0; x < XR; ++x) {
             l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
             l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
             if (tq == 0) {
@@ -262,75 +304,56 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
                 stat[warp][1][gq + 8 * x] = l[x];
             }
         }
-        named_sync(1, 256);
-        float top[2], sum[2];
+        const bool whole = is_whole(s);
+        float4 * pc = reinterpret_cast<float4 *>(piece(a, blockIdx.x, s.t0 == 0));
+        named_sync(1, 256);                                      // q is read
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            top[x] = -INFINITY;
-            sum[x] = 0.f;
-#pragma unroll 4
-            for (int k = 0; k < KQ; ++k) top[x] = fmaxf(top[x], stat[rt * KQ + k][0][gq + 8 * x]);
-            const float ref = top[x] == -INFINITY ? 0.f : top[x];
-#pragma unroll 4
-            for (int k = 0; k < KQ; ++k) sum[x] += stat[rt * KQ + k][1][gq + 8 * x] * exp2_fast(stat[rt * KQ + k][0][gq + 8 * x] - ref);
-            const float w = exp2_fast(mx[x] - ref);
+        for (int h = 0; h < D / W; ++h) {
 #pragma unroll
-            for (int d = 0; d < D / 8; ++d) {
-                o[d][2 * x] *= w;
-                o[d][2 * x + 1] *= w;
-            }
-        }
+            for (int d = 0; d < W / 8; ++d)
+#pragma unroll
+                for (int x = 0; x < XR; ++x) {
+                    float2 * p = reinterpret_cast<float2 *>(sums + (warp * MR + gq + 8 * x) * Q + ((2 * d + (tq >> 1)) ^ gq)) + (tq & 1);
+                    *p = make_float2(o[W / 8 * h + d][2 * x], o[W / 8 * h + d][2 * x + 1]);
+                }
+            named_sync(1, 256);
 #pragma unroll 1
-        for (int half = KQ / 2; half >= 1; half /= 2) {
-            float4 * slot = sums + (kq % half * RT + rt) * (4 * D) + lane;
-            if (kq >= half && kq < 2 * half) {
+            for (int x = tid; x < ROWS * Q; x += 256) {
+                const int m = x / Q, q = x % Q, r = m % MR, w0 = m / MR * KQ;
+                if (m >= s.m) break;
+                float top = -INFINITY, sum = 0.f;
 #pragma unroll
-                for (int d = 0; d < D / 8; ++d) slot[d * 32] = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
+                for (int k = 0; k < KQ; ++k) top = fmaxf(top, stat[w0 + k][0][r]);
+                const float ref = top == -INFINITY ? 0.f : top;
+                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int k = 0; k < KQ; ++k) {
+                    const float w = exp2_fast(stat[w0 + k][0][r] - ref);
+                    const float4 v = sums[((w0 + k) * MR + r) * Q + (q ^ (r & 7))];
+                    sum += w * stat[w0 + k][1][r];
+                    y.x += w * v.x; y.y += w * v.y; y.z += w * v.z; y.w += w * v.w;
+                }
+                if (whole) {
+                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                    T * dst = row_at<T>(a, a.out, a.out_stride, s, m) + W * h + 4 * q;
+                    if constexpr (SPLIT) *reinterpret_cast<float4 *>(dst) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+                    else *reinterpret_cast<uint2 *>(dst) = make_uint2(pack<C>(y.x * inv, y.y * inv), pack<C>(y.z * inv, y.w * inv));
+                    if (a.lse && h == 0 && q == 0) put_lse(a, s, m, top, sum);
+                } else {
+                    pc[(Q * h + q) * ROWS + m] = y;
+                    if (h == 0 && q == 0) {
+                        float * st = reinterpret_cast<float *>(pc) + ROWS * D + m;
+                        st[0] = top;
+                        st[ROWS] = sum;
+                    }
+                }
             }
             named_sync(1, 256);
-            if (kq < half) {
-#pragma unroll
-                for (int d = 0; d < D / 8; ++d) {
-                    const float4 v = slot[d * 32];
-                    o[d][0] += v.x; o[d][1] += v.y; o[d][2] += v.z; o[d][3] += v.w;
-                }
-            }
-            if (half > 1) named_sync(1, 256);
-        }
-        const int whole = s.whole;
-        if (kq == 0) {
-            float * pc = piece(a, blockIdx.x, s.slot);
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int m = rt * 16 + gq + 8 * x;
-                if (m >= s.m) continue;
-                if (whole) {
-                    const float inv = sum[x] == 0.f ? 0.f : 1.f / sum[x];
-                    T * dst = row_at<T>(a, a.out, a.out_stride, s, m) + 2 * tq;
-#pragma unroll
-                    for (int d = 0; d < D / 8; ++d) {
-                        const float v = o[d][2 * x] * inv, w = o[d][2 * x + 1] * inv;
-                        if constexpr (SPLIT) *reinterpret_cast<float2 *>(dst + d * 8) = make_float2(v, w);
-                        else *reinterpret_cast<uint32_t *>(dst + d * 8) = pack<C>(v, w);
-                    }
-                    if (a.lse && tq == 0) put_lse(a, s, m, top[x], sum[x]);
-                } else {
-#pragma unroll
-                    for (int d = 0; d < D / 8; ++d)
-                        *reinterpret_cast<float2 *>(pc + ((2 * d + (tq >> 1)) * ROWS + m) * 4 + 2 * (tq & 1)) = make_float2(o[d][2 * x], o[d][2 * x + 1]);
-                    if (tq == 0) {
-                        pc[ROWS * D + m] = top[x];
-                        pc[ROWS * D + ROWS + m] = sum[x];
-                    }
-                }
-            }
         }
         if (!whole) {
-            __threadfence();
+            if (tid == 0) is_last = arrive_piece(a, share.d, s);
             named_sync(1, 256);
-            if (tid == 0) is_last = arrive_piece(a, s);
-            named_sync(1, 256);
-            if (is_last) join<T, C, ROWS, D, 256, 8, L::JOIN / 4>(a, s, tid, reinterpret_cast<float *>(sums));
+            if (is_last) join<T, C, ROWS, D, 256, 8, L::JOIN / 4>(a, share.d, s, tid, reinterpret_cast<float *>(sums));
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&segs.empty[sn % SegmentRing::N]);
@@ -342,8 +365,9 @@ template <class T, class C, int D> void few(const AttendArgs & a, const CUtensor
         NAVI_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, FewSmem<D>::BYTES));
         NAVI_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(sms)), dim3(288), FewSmem<D>::BYTES, stream, a, k, v));
     };
-    if (rows <= 16) go(k_attend_few<T, C, D, 1>);
-    else go(k_attend_few<T, C, D, 2>);
+    if (rows <= 8) go(k_attend_few<T, C, D, 8>);
+    else if (rows <= 16) go(k_attend_few<T, C, D, 16>);
+    else go(k_attend_few<T, C, D, 32>);
 }
 
 } // namespace

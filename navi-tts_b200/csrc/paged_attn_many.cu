@@ -1,6 +1,5 @@
 // Attention over the paged KV cache for many rows of a request (paged_attn.cu): larger drafted
 // trees and chunks of prompts, on the tcgen05 tensor cores.
-#define NAVI_ATTN_SELDOM __forceinline__
 #include "paged_attn.hpp"
 #include "paged_attn.cuh"
 #include "tmem.cuh"
@@ -82,26 +81,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return y;
 }
 
-// Bits 0..31: whether row j of the request sees the tokens ctx + a .. ctx + a + 31 (a may be negative:
-// those are cached tokens), of which `left` are the item's.
-__device__ __forceinline__ uint32_t seen_bits(const AttendArgs & a, const Segment & it, int j, int at, int left) {
-    if (left <= 0) return 0u;
-    uint32_t b;
-    if (at + 31 < 0) b = ~0u;
-    else if (!a.mask) {
-        const int n = j - at + 1;            // tokens from `at` up to row j itself
-        b = n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
-    } else {
-        const uint64_t * m = a.mask + static_cast<size_t>(it.row0 + j) * a.mask_words;
-        const int w = at >> 6;               // floor: -1 for the bits before row 0, all seen
-        const uint64_t lo = w < 0 ? ~0ull : w < a.mask_words ? __ldg(m + w) : 0ull;
-        const uint64_t hi = w + 1 < a.mask_words ? __ldg(m + w + 1) : 0ull;
-        const int s = at & 63;
-        b = static_cast<uint32_t>(s ? (lo >> s) | (hi << (64 - s)) : lo);
-    }
-    return left >= 32 ? b : b & ((1u << left) - 1u);
-}
-
 template <class T, class C, int D>
 __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
                                                         const __grid_constant__ CUtensorMap vmap) {
@@ -134,21 +113,28 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
         tmem_relinquish();
     }
     fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
     griddep_wait();
     griddep_launch_dependents();
-    share_out<ROWS, 384>(a, S.sh, S.red);
-    fence_after_sync();
+    const bool one = a.n_req <= 32;
+    if (!one) share_of_block<ROWS, 384>(a, S.sh, S.red);
     const uint32_t tmem = S.tmem_at;
     const Wait wait{&S.abort_flag, a.err};
-    if (S.sh.u >= S.sh.end) {
-        if (warp == 9) tmem_dealloc(tmem, 512);
-        return;
-    }
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 8) {
-            Walk<ROWS> walk(a, S.sh);
+            Request first{};
+            Share sh;
+            if (one) {
+                sh = share_of_warp<ROWS>(a, first);
+                if (lane == 0) S.sh.d = sh.d;                   // the other roles read it after a segment
+            } else {
+                sh = S.sh;
+                if (sh.u < sh.end) first = request(a, sh.i);
+            }
+            Walk<ROWS> walk(a, sh, first);
             int n = 0;
             bool ok = true;
 #pragma unroll 1
@@ -157,13 +143,13 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 const bool more = walk.next(s);
                 if (k >= SegmentRing::N) ok = __shfl_sync(0xffffffffu, lane == 0 ? wait(&S.segs.empty[k % SegmentRing::N], (k / SegmentRing::N - 1) & 1) : 0, 0);
                 if (!ok) break;
+                int page = more && s.n_keys > 0 ? page_of_box<D>(a, s, s.t0, lane & 15) : -1;
                 if (lane == 0) {
                     S.segs.s[k % SegmentRing::N] = s;
                     mbar_arrive(&S.segs.full[k % SegmentRing::N]);
                 }
                 if (!more) break;
                 if (s.n_keys <= 0) continue;
-                int page = page_of_box<D>(a, s, s.t0, lane & 15);
 #pragma unroll 1
                 for (int t = s.t0; t < s.t0 + s.nt && ok; ++t) {
                     const int next = t + 1 < s.t0 + s.nt ? page_of_box<D>(a, s, t + 1, lane & 15) : -1;
@@ -384,7 +370,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 fence_after_sync();
             }
 
-            const bool whole = it.whole;
+            const bool whole = is_whole(it);
             float mine = 1.f;                             // what this warpgroup's O counts
             float * const half = reinterpret_cast<float *>(qs);
             int c_lo = 0, c_hi = D;                       // the columns that this warpgroup finishes
@@ -413,7 +399,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 named_sync(1, 256);
             }
             {
-                float4 * pc = reinterpret_cast<float4 *>(piece(a, blockIdx.x, it.slot)) + m;
+                float4 * pc = reinterpret_cast<float4 *>(piece(a, blockIdx.x, it.t0 == 0)) + m;
                 const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
                 const bool other = !two && (wg == 1 ? nt > 0 : nt > 1), live = m < it.m;
                 T * dst = row_at<T>(a, a.out, a.out_stride, it, live ? m : 0);
@@ -459,19 +445,18 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                     if (whole) {
                         if (a.lse) put_lse(a, it, m, top, sum);
                     } else {
-                        float * st = piece(a, blockIdx.x, it.slot) + ROWS * D + m;
+                        float * st = piece(a, blockIdx.x, it.t0 == 0) + ROWS * D + m;
                         st[0] = top;
                         st[ROWS] = sum;
                     }
                 }
             }
             fence_before_sync();
-            if (!whole) __threadfence();
             named_sync(1, 256);
             if (!whole) {
-                if (tid == 0) S.is_last = arrive_piece(a, it);
+                if (tid == 0) S.is_last = arrive_piece(a, S.sh.d, it);
                 named_sync(1, 256);
-                if (S.is_last) join<T, C, ROWS, D, 256, 1, 2 * L::QTILE / 4>(a, it, tid, reinterpret_cast<float *>(qs));
+                if (S.is_last) join<T, C, ROWS, D, 256, 1, 2 * L::QTILE / 4>(a, S.sh.d, it, tid, reinterpret_cast<float *>(qs));
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&S.segs.empty[sn % SegmentRing::N]);
