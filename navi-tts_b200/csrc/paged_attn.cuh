@@ -308,72 +308,59 @@ __device__ __forceinline__ bool arrive_piece(const AttendArgs & a, const Divisio
     return true;
 }
 
-// Joins the pieces of an item, in order: THREADS threads of the block, all of them. First what each
-// piece counts in each row goes to `weight` (CAP floats of shared memory), LANES lanes to a row,
-// then the sums are read, by a thread that stays with its row: neighbours read neighbouring rows.
-template <class T, class C, int ROWS, int D, int THREADS, int LANES, int CAP>
-__device__ __forceinline__ void join(const AttendArgs & a, const Division & d, const Segment & s, int tid, float * weight) {
+// Joins the pieces of an item, in order: THREADS threads of the block. A thread has U pieces of 4 dims of
+// a row (neighbours have neighbouring rows) and reads P blocks' pieces at once, their maxima and sums
+// with them: one trip to L2 for each P blocks.
+template <class T, class C, int ROWS, int D, int THREADS, int U, int P>
+__device__ __forceinline__ void join(const AttendArgs & a, const Division & d, const Segment & s, int tid) {
     const int c0 = d.block(s.u0), np = d.block(s.u0 + s.tiles - 1) - c0 + 1;
-    const auto part = [&](int p) { return piece(a, c0 + p, p == 0); };
-    const int most = min(CAP / np, ROWS);             // rows at a time: up to a block a multiprocessor shares an item
+    constexpr int N = D / 4 / U;                      // threads of a row
 #pragma unroll 1
-    for (int m0 = 0; m0 < s.m; m0 += most) {
-        const int rows = min(most, s.m - m0), sub = tid % LANES;
-        constexpr int RP = THREADS / LANES;           // rows a pass
-#pragma unroll 1
-        for (int r = tid / LANES; r < (rows + RP - 1) / RP * RP; r += RP) {
-            const bool live = r < rows;
-            const int m = m0 + (live ? r : 0);
-            float top = -INFINITY, l = 0.f;
-#pragma unroll 2
-            for (int p = sub; p < np; p += LANES) top = fmaxf(top, __ldcg(part(p) + ROWS * D + m));
+    for (int x = tid; x < ROWS * N; x += THREADS) {
+        const int r = x % ROWS, q = x / ROWS;
+        if (r >= s.m) continue;
+        float top = -INFINITY, l = 0.f;
+        float4 y[U];
 #pragma unroll
-            for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll 2
-            for (int p = sub; p < np; p += LANES) {
-                const float w = exp2_fast(__ldcg(part(p) + ROWS * D + m) - ref);
-                l += w * __ldcg(part(p) + ROWS * D + ROWS + m);
-                if (live) weight[p * rows + r] = w;
+        for (int k = 0; k < U; ++k) y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int p0 = 0; p0 < np; p0 += P) {
+            float m[P], w[P];
+            float4 v[P][U];
+            float best = top;
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                const float * at = piece(a, c0 + min(p0 + p, np - 1), p0 + p == 0);
+                m[p] = __ldcg(at + ROWS * D + r);
+                w[p] = __ldcg(at + ROWS * D + ROWS + r);
+#pragma unroll
+                for (int k = 0; k < U; ++k) v[p][k] = __ldcg(reinterpret_cast<const float4 *>(at) + (q + k * N) * ROWS + r);
             }
 #pragma unroll
-            for (int o = 1; o < LANES; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll 1
-            for (int p = sub; p < np && live; p += LANES) weight[p * rows + r] *= inv;
-            if (live && sub == 0 && a.lse) put_lse(a, s, m, top, l);
-        }
-        named_sync(1, THREADS);
-        constexpr int QS = THREADS / ROWS < D / 4 ? THREADS / ROWS : D / 4, N = D / 4 / QS, U = N < 8 ? N : 8;
-        static_assert(THREADS % ROWS == 0 && N % U == 0);
-        const int r = tid % ROWS;
-        if (r < rows) {
-            T * dst = row_at<T>(a, a.out, a.out_stride, s, m0 + r);
-#pragma unroll 1
-            for (int q = tid / ROWS; q < D / 4; q += U * QS) {
-                float4 y[U];
+            for (int p = 0; p < P; ++p) best = p0 + p < np ? fmaxf(best, m[p]) : best;
+            const float ref = best == -INFINITY ? 0.f : best, old = exp2_fast(top - ref);
+            top = best;
+            l *= old;
 #pragma unroll
-                for (int k = 0; k < U; ++k) y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-                for (int p = 0; p < np; ++p) {
-                    const float4 * src = reinterpret_cast<const float4 *>(part(p)) + m0 + r;
-                    const float w = weight[p * rows + r];
-                    float4 v[U];
+            for (int k = 0; k < U; ++k) { y[k].x *= old; y[k].y *= old; y[k].z *= old; y[k].w *= old; }
 #pragma unroll
-                    for (int k = 0; k < U; ++k) v[k] = __ldcg(src + (q + k * QS) * ROWS);
-#pragma unroll
-                    for (int k = 0; k < U; ++k) {
-                        y[k].x += w * v[k].x; y[k].y += w * v[k].y; y[k].z += w * v[k].z; y[k].w += w * v[k].w;
-                    }
-                }
+            for (int p = 0; p < P; ++p) {
+                const float c = p0 + p < np ? exp2_fast(m[p] - ref) : 0.f;
+                l += c * w[p];
 #pragma unroll
                 for (int k = 0; k < U; ++k) {
-                    if constexpr (std::is_same_v<T, float>) *reinterpret_cast<float4 *>(dst + 4 * (q + k * QS)) = y[k];
-                    else *reinterpret_cast<uint2 *>(dst + 4 * (q + k * QS)) = make_uint2(pack<C>(y[k].x, y[k].y), pack<C>(y[k].z, y[k].w));
+                    y[k].x += c * v[p][k].x; y[k].y += c * v[p][k].y; y[k].z += c * v[p][k].z; y[k].w += c * v[p][k].w;
                 }
             }
         }
-        named_sync(1, THREADS);
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        T * dst = row_at<T>(a, a.out, a.out_stride, s, r);
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            if constexpr (std::is_same_v<T, float>) *reinterpret_cast<float4 *>(dst + 4 * (q + k * N)) = make_float4(y[k].x * inv, y[k].y * inv, y[k].z * inv, y[k].w * inv);
+            else *reinterpret_cast<uint2 *>(dst + 4 * (q + k * N)) = make_uint2(pack<C>(y[k].x * inv, y[k].y * inv), pack<C>(y[k].z * inv, y[k].w * inv));
+        }
+        if (q == 0 && a.lse) put_lse(a, s, r, top, l);
     }
 }
 

@@ -47,6 +47,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
     constexpr bool SPLIT = std::is_same_v<T, float>, EIGHT = ROWS == 8;
     constexpr int RT = EIGHT ? 1 : ROWS / 16, KQ = 8 / RT, WK = KT / KQ;    // row tiles; warps and keys of a tile a warp takes
     constexpr int XR = EIGHT ? 1 : 2, MR = 8 * XR;                          // rows a thread and a warp have
+    constexpr int KS = WK / 16;                                             // 16-key products a warp does at a time
     constexpr bool TERMS = SPLIT && !EIGHT;                                 // the low terms are products of their own
     using L = FewSmem<D>;
     extern __shared__ uint8_t raw[];
@@ -192,33 +193,35 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
                 fence_proxy_async_smem();
                 __syncwarp();
             }
-            // 16 keys at a time
-#pragma unroll 1
-            for (int k = 0; k < WK && k < valid; k += 16) {
-                const bool masked = first + k + 16 > ctx;   // some of these keys are new rows, or past the last
+            if (valid > 0) {
+                const bool masked = first + WK > ctx;       // some of these keys are new rows, or past the last
                 uint32_t seen[XR];
                 if (masked) {
 #pragma unroll
-                    for (int x = 0; x < XR; ++x) seen[x] = seen_bits(a, s, row[x], first + k - ctx, valid - k);
+                    for (int x = 0; x < XR; ++x) seen[x] = seen_bits(a, s, row[x], first - ctx, valid);
                 }
-                float sc[2][4] = {}, low[2][4] = {};
-                const uint32_t kk = k_at + st * L::STAGE + k * 128, vv = v_at + st * L::STAGE + k * 128;
+                float sc[2 * KS][4] = {}, low[2 * KS][4] = {};
+                const uint32_t kk = k_at + st * L::STAGE, vv = v_at + st * L::STAGE;
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks) {
-                    uint32_t b[4], q[4];
+                    uint32_t q[4], p[4], b[KS][4];
                     ldsm4(q, q_at + (ks >> 2) * 128 + off_v[ks & 3]);
-                    ldsm4(b, kk + (ks >> 2) * (KT * 128) + off_k[ks & 3]);
-                    mma<C>(sc[0], q, b[0], b[1]);
-                    mma<C>(sc[1], q, b[2], b[3]);
-                    if constexpr (TERMS) {
-                        ldsm4(q, q_at + ROWS * D * 2 + (ks >> 2) * 128 + off_v[ks & 3]);
-                        mma<C>(low[0], q, b[0], b[1]);
-                        mma<C>(low[1], q, b[2], b[3]);
+                    if constexpr (TERMS) ldsm4(p, q_at + ROWS * D * 2 + (ks >> 2) * 128 + off_v[ks & 3]);
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) ldsm4(b[k], kk + k * (16 * 128) + (ks >> 2) * (KT * 128) + off_k[ks & 3]);
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        mma<C>(sc[2 * k], q, b[k][0], b[k][1]);
+                        mma<C>(sc[2 * k + 1], q, b[k][2], b[k][3]);
+                        if constexpr (TERMS) {
+                            mma<C>(low[2 * k], p, b[k][0], b[k][1]);
+                            mma<C>(low[2 * k + 1], p, b[k][2], b[k][3]);
+                        }
                     }
                 }
                 if constexpr (SPLIT) {
 #pragma unroll
-                    for (int y = 0; y < 2; ++y)
+                    for (int y = 0; y < 2 * KS; ++y)
 #pragma unroll
                         for (int e = 0; e < 2 * XR; ++e) sc[y][e] += EIGHT ? sc[y][2 + e] : low[y][e];
                 }
@@ -226,14 +229,18 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
 #pragma unroll
                     for (int x = 0; x < XR; ++x)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (!(seen[x] >> ((e >> 1) * 8 + 2 * tq + (e & 1)) & 1)) sc[e >> 1][2 * x + (e & 1)] = -INFINITY;
+                        for (int y = 0; y < 2 * KS; ++y)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                if (!(seen[x] >> (y * 8 + 2 * tq + e) & 1)) sc[y][2 * x + e] = -INFINITY;
                 }
                 float m[XR];
                 bool more = false;
 #pragma unroll
                 for (int x = 0; x < XR; ++x) {
-                    m[x] = fmaxf(fmaxf(sc[0][2 * x], sc[0][2 * x + 1]), fmaxf(sc[1][2 * x], sc[1][2 * x + 1]));
+                    m[x] = -INFINITY;
+#pragma unroll
+                    for (int y = 0; y < 2 * KS; ++y) m[x] = fmaxf(m[x], fmaxf(sc[y][2 * x], sc[y][2 * x + 1]));
                     m[x] = fmaxf(m[x], __shfl_xor_sync(0xffffffffu, m[x], 1));
                     m[x] = fmaxf(m[x], __shfl_xor_sync(0xffffffffu, m[x], 2)) * a.scale;
                     more = more || m[x] > mx[x];
@@ -252,38 +259,51 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
                         }
                     }
                 }
-                uint32_t ph[4] = {0, 0, 0, 0}, pl[4];
+                uint32_t ph[KS][4] = {}, pl[KS][4];
 #pragma unroll
                 for (int x = 0; x < XR; ++x) {
                     const float ref = mx[x] == -INFINITY ? 0.f : mx[x];
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        const float p0 = exp2_fast(fmaf(sc[y][2 * x], a.scale, -ref)), p1 = exp2_fast(fmaf(sc[y][2 * x + 1], a.scale, -ref));
-                        l[x] += p0 + p1;
-                        if constexpr (TERMS) split_pair<C>(p0, p1, ph[2 * y + x], pl[2 * y + x]);
-                        else if constexpr (SPLIT) split_pair<C>(p0, p1, ph[2 * y], ph[2 * y + 1]);
-                        else ph[2 * y + x] = pack<C>(p0, p1);
-                    }
+                    for (int k = 0; k < KS; ++k)
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            const float * v = sc[2 * k + y] + 2 * x;
+                            const float p0 = exp2_fast(fmaf(v[0], a.scale, -ref)), p1 = exp2_fast(fmaf(v[1], a.scale, -ref));
+                            l[x] += p0 + p1;
+                            if constexpr (TERMS) split_pair<C>(p0, p1, ph[k][2 * y + x], pl[k][2 * y + x]);
+                            else if constexpr (SPLIT) split_pair<C>(p0, p1, ph[k][2 * y], ph[k][2 * y + 1]);
+                            else ph[k][2 * y + x] = pack<C>(p0, p1);
+                        }
                 }
 #pragma unroll
                 for (int dp = 0; dp < D / 16; ++dp) {
-                    uint32_t b[4];
-                    ldsm4t(b, vv + (dp >> 2) * (KT * 128) + off_v[dp & 3]);
+                    uint32_t b[KS][4];
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) ldsm4t(b[k], vv + k * (16 * 128) + (dp >> 2) * (KT * 128) + off_v[dp & 3]);
                     if constexpr (SPLIT || EIGHT) {
                         float c[2][4] = {};
                         if constexpr (TERMS) {
-                            mma<C>(c[0], pl, b[0], b[1]);
-                            mma<C>(c[1], pl, b[2], b[3]);
+#pragma unroll
+                            for (int k = 0; k < KS; ++k) {
+                                mma<C>(c[0], pl[k], b[k][0], b[k][1]);
+                                mma<C>(c[1], pl[k], b[k][2], b[k][3]);
+                            }
                         }
-                        mma<C>(c[0], ph, b[0], b[1]);
-                        mma<C>(c[1], ph, b[2], b[3]);
+#pragma unroll
+                        for (int k = 0; k < KS; ++k) {
+                            mma<C>(c[0], ph[k], b[k][0], b[k][1]);
+                            mma<C>(c[1], ph[k], b[k][2], b[k][3]);
+                        }
 #pragma unroll
                         for (int y = 0; y < 2; ++y)
 #pragma unroll
                             for (int e = 0; e < 2 * XR; ++e) o[2 * dp + y][e] += SPLIT && EIGHT ? c[y][e] + c[y][2 + e] : c[y][e];
                     } else {
-                        mma<C>(o[2 * dp], ph, b[0], b[1]);
-                        mma<C>(o[2 * dp + 1], ph, b[2], b[3]);
+#pragma unroll
+                        for (int k = 0; k < KS; ++k) {
+                            mma<C>(o[2 * dp], ph[k], b[k][0], b[k][1]);
+                            mma<C>(o[2 * dp + 1], ph[k], b[k][2], b[k][3]);
+                        }
                     }
                 }
             }
@@ -353,7 +373,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
         if (!whole) {
             if (tid == 0) is_last = arrive_piece(a, share.d, s);
             named_sync(1, 256);
-            if (is_last) join<T, C, ROWS, D, 256, 8, L::JOIN / 4>(a, share.d, s, tid, reinterpret_cast<float *>(sums));
+            if (is_last) join<T, C, ROWS, D, 256, ROWS / 8, ROWS == 8 ? 8 : 4>(a, share.d, s, tid);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&segs.empty[sn % SegmentRing::N]);

@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
             if (!whole) {
                 if (tid == 0) S.is_last = arrive_piece(a, S.sh.d, it);
                 named_sync(1, 256);
-                if (S.is_last) join<T, C, ROWS, D, 256, 1, 2 * L::QTILE / 4>(a, S.sh.d, it, tid, reinterpret_cast<float *>(qs));
+                if (S.is_last) join<T, C, ROWS, D, 256, 8, 2>(a, S.sh.d, it, tid);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&S.segs.empty[sn % SegmentRing::N]);
