@@ -36,7 +36,7 @@ void Pages::attend(const navi_step & s, int layer, const navi_attend_args & q, c
     if (a.group > 1) a.group_mul = static_cast<uint32_t>(((1ull << 32) + static_cast<uint64_t>(a.group) - 1) / static_cast<uint64_t>(a.group));
     if ((a.group & (a.group - 1)) != 0 && (most + 512) * a.group * a.group >= 1ll << 32) fail("pages attend: too many rows for this many heads to a KV head", NAVI_E_SHAPE);
     // the list of key tiles that the blocks divide
-    const int64_t rows = most * a.group <= attn::FEW_ROWS ? 16 : 128, items = (most * a.group + rows - 1) / rows * d_.n_kv_head * s.n_req, tiles = (static_cast<int64_t>(d_.max_blocks) * d_.page_size + attn::KT - 1) / attn::KT;
+    const int64_t rows = most * a.group <= attn::FEW_ROWS ? 16 : 128, items = (most * a.group + rows - 1) / rows * d_.n_kv_head * s.n_req, tiles = (static_cast<int64_t>(d_.max_blocks) * d_.page_size + attn::KT - 1) / attn::KT + 2;
     if (items * tiles >= 1ll << 31) fail("pages attend: requests x heads x tokens pass 31 bits of key tiles", NAVI_E_SHAPE);
     const CUtensorMap & km = maps_[static_cast<size_t>(2 * layer)], & vm = maps_[static_cast<size_t>(2 * layer + 1)];
     const int64_t m = most * a.group;

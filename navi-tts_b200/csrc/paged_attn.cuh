@@ -81,7 +81,8 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // ---- who does what ----------------------------------------------------------------------------
 //
 // The work of a launch is a list of units: for each request, each KV head and each tile of ROWS
-// rows (rows x heads of the KV head, an item), the item's key tiles of KT keys, at least one.
+// rows (rows x heads of the KV head, an item), the item's key tiles of KT keys, at least one,
+// after EXTRA units that stand for what an item costs beside its tiles.
 // Lengths are on the device and ragged, so the blocks divide the list evenly themselves,
 // whatever request the units belong to. An item that falls to several blocks leaves its pieces
 // (the sums and each row's maximum and sum, f32) in the stream's scratch, and the block that
@@ -101,7 +102,7 @@ struct Segment {
     int row0, ctx, table, g;     // the request, the KV head
     int m0, m, n_keys;           // its first row x head, how many, the keys that they may see
     int t0, nt;                  // key tiles t0 .. t0 + nt - 1; nt -1: no more segments
-    int u0, tiles;               // the item's units
+    int u0, tiles;               // the item's key tiles among the units
 };
 __device__ __forceinline__ bool is_whole(const Segment & s) { return s.nt == s.tiles; }
 
@@ -112,10 +113,10 @@ template <int ROWS> __device__ __forceinline__ int keys_of(const AttendArgs & a,
 }
 __device__ __forceinline__ int tiles_of(int n_keys) { return max((n_keys + KT - 1) / KT, 1); }
 // the units of one KV head of a request
-template <int ROWS> __device__ __forceinline__ int units_of(const AttendArgs & a, const Request & r) {
+template <int ROWS, int EXTRA> __device__ __forceinline__ int units_of(const AttendArgs & a, const Request & r) {
     const int rts = row_tiles<ROWS>(a, r);
-    if (a.mask || r.keys == 0) return rts * tiles_of(r.keys);
-    int n = 0;
+    if (a.mask || r.keys == 0) return rts * (EXTRA + tiles_of(r.keys));
+    int n = rts * EXTRA;
 #pragma unroll 1
     for (int rt = 0; rt < rts; ++rt) n += tiles_of(keys_of<ROWS>(a, r, rt));
     return n;
@@ -164,11 +165,11 @@ __device__ __forceinline__ void take(Share & sh, int total) {
 }
 // Up to 32 requests a warp finds its block's share by itself, a lane a request. (The host has checked
 // that the units fit 31 bits.)
-template <int ROWS> __device__ __forceinline__ Share share_of_warp(const AttendArgs & a, Request & first) {
+template <int ROWS, int EXTRA> __device__ __forceinline__ Share share_of_warp(const AttendArgs & a, Request & first) {
     const int lane = threadIdx.x & 31;
     Request r{};
     if (lane < a.n_req) r = request(a, lane);
-    const int mine = units_of<ROWS>(a, r) * a.n_kv, x = warp_scan(mine);
+    const int mine = units_of<ROWS, EXTRA>(a, r) * a.n_kv, x = warp_scan(mine);
     Share sh;
     take(sh, __shfl_sync(0xffffffffu, x, 31));
     sh.i = max(__ffs(__ballot_sync(0xffffffffu, sh.u < x)) - 1, 0);   // the first request that ends after unit u
@@ -182,12 +183,12 @@ template <int ROWS> __device__ __forceinline__ Share share_of_warp(const AttendA
 }
 // More: all THREADS threads of the block, each some requests in a row. What they wrote to shared memory
 // before is there for all of them after it.
-template <int ROWS, int THREADS> __device__ __forceinline__ void share_of_block(const AttendArgs & a, Share & out, int * red) {
+template <int ROWS, int EXTRA, int THREADS> __device__ __forceinline__ void share_of_block(const AttendArgs & a, Share & out, int * red) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.n_req;
     const int per = (B + THREADS - 1) / THREADS, i0 = min(B, tid * per), i1 = min(B, i0 + per);
     int mine = 0;
 #pragma unroll 1
-    for (int i = i0; i < i1; ++i) mine += units_of<ROWS>(a, request(a, i)) * a.n_kv;
+    for (int i = i0; i < i1; ++i) mine += units_of<ROWS, EXTRA>(a, request(a, i)) * a.n_kv;
     const int x = warp_scan(mine);
     if (lane == 31) red[warp] = x;
     __syncthreads();
@@ -209,7 +210,7 @@ template <int ROWS, int THREADS> __device__ __forceinline__ void share_of_block(
         int i = i0;
 #pragma unroll 1
         for (;; ++i) {
-            const int n = units_of<ROWS>(a, request(a, i)) * a.n_kv;
+            const int n = units_of<ROWS, EXTRA>(a, request(a, i)) * a.n_kv;
             if (u < base + n) break;
             base += n;
         }
@@ -220,27 +221,28 @@ template <int ROWS, int THREADS> __device__ __forceinline__ void share_of_block(
 }
 
 // The walk over the block's segments: next() fills in the next one; false when there is none.
-template <int ROWS> struct Walk {
+template <int ROWS, int EXTRA> struct Walk {
     const AttendArgs & a;
     Share sh;
     Request r;
-    int i, g, rt, u0, u, tiles, n_keys;
+    int i, g, rt, u0, u, tiles, n_keys;   // u0: the item's first key tile
 
     __device__ __forceinline__ Walk(const AttendArgs & args, const Share & share, const Request & first) : a(args), sh(share), r(first) {
         i = sh.i;
         u = sh.u;
         if (u >= sh.end) return;
-        const int per_head = units_of<ROWS>(a, r);
+        const int per_head = units_of<ROWS, EXTRA>(a, r);
         g = quick_div(u - sh.base, per_head);
-        u0 = sh.base + g * per_head;
+        u0 = sh.base + g * per_head + EXTRA;
         rt = 0;
         if (a.mask || r.keys == 0) {   // every row tile has as many key tiles
-            rt = quick_div(u - u0, tiles_of(r.keys));
-            u0 += rt * tiles_of(r.keys);
+            const int each = EXTRA + tiles_of(r.keys);
+            rt = quick_div(u - u0 + EXTRA, each);
+            u0 += rt * each;
         }
         open();
         while (u0 + tiles <= u) {
-            u0 += tiles;
+            u0 += tiles + EXTRA;
             ++rt;
             open();
         }
@@ -250,12 +252,8 @@ template <int ROWS> struct Walk {
         tiles = tiles_of(n_keys);
     }
     __device__ __forceinline__ bool next(Segment & s) {
-        if (u >= sh.end) {
-            s.nt = -1;
-            return false;
-        }
-        if (u >= u0 + tiles) {
-            u0 += tiles;
+        if (u < sh.end && u >= u0 + tiles) {
+            u0 += tiles + EXTRA;
             if (++rt >= row_tiles<ROWS>(a, r)) {
                 rt = 0;
                 if (++g >= a.n_kv) {
@@ -266,6 +264,11 @@ template <int ROWS> struct Walk {
             }
             open();
         }
+        if (u >= sh.end || u0 >= sh.end) {   // no more, or nothing but what an item costs beside its tiles
+            s.nt = -1;
+            return false;
+        }
+        u = max(u, u0);
         const int t1 = min(tiles, sh.end - u0);
         s.row0 = r.row0;
         s.ctx = r.ctx;

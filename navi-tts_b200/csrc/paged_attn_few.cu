@@ -77,20 +77,20 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
     griddep_wait();
     griddep_launch_dependents();
     const bool one = a.n_req <= 32;
-    if (!one) share_of_block<ROWS, 288>(a, share, red);
+    if (!one) share_of_block<ROWS, 0, 288>(a, share, red);
     const Wait wait{&abort_flag, a.err};
 
     if (warp == 8) {
         Request first{};
         Share sh;
         if (one) {
-            sh = share_of_warp<ROWS>(a, first);
+            sh = share_of_warp<ROWS, 0>(a, first);
             if (lane == 0) share.d = sh.d;           // the other warps read it after a segment
         } else {
             sh = share;
             if (sh.u < sh.end) first = request(a, sh.i);
         }
-        Walk<ROWS> walk(a, sh, first);
+        Walk<ROWS, 0> walk(a, sh, first);
         int n = 0;
         bool ok = true;
         const int kv = lane >> 4, box = lane & 15;   // half a warp each for K and V

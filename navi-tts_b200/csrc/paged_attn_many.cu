@@ -28,6 +28,7 @@ using namespace navi::umma;
 // f32 rows: q and p as two f16 terms each against the exact cache values, as in the kernel for few
 // rows. Two tiles of q do not fit then, so their items have 128 rows.
 constexpr int LAZY = 8;
+constexpr int EXTRA = 2;                                        // what an item costs beside its key tiles, in key tiles
 
 template <class T, int D> struct ManySmem {
     static constexpr bool SPLIT = std::is_same_v<T, float>;
@@ -40,7 +41,7 @@ template <class T, int D> struct ManySmem {
 };
 
 struct ManyControl {
-    uint64_t full[8], empty[8], q_full, s_full[2], p_full[2], o_full[2], drained;
+    uint64_t full[8], empty[8], q_full, q_empty, s_full[2], p_full[2], o_full[2], drained;
     float stat[2][2][128];
     SegmentRing segs;
     int red[12];
@@ -98,14 +99,15 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
             mbar_init(&S.full[s], 1);
             mbar_init(&S.empty[s], 1);
         }
-        mbar_init(&S.q_full, 256);
+        mbar_init(&S.q_full, 64);
+        mbar_init(&S.q_empty, 1);
         for (int g = 0; g < 2; ++g) {
             mbar_init(&S.s_full[g], 1);
             mbar_init(&S.p_full[g], 128);
             mbar_init(&S.o_full[g], 1);
         }
         mbar_init(&S.drained, 1);
-        S.segs.init(9);
+        S.segs.init(11);
         fence_mbar_init();
     }
     if (warp == 9) {
@@ -118,7 +120,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
     griddep_wait();
     griddep_launch_dependents();
     const bool one = a.n_req <= 32;
-    if (!one) share_of_block<ROWS, 384>(a, S.sh, S.red);
+    if (!one) share_of_block<ROWS, EXTRA, 384>(a, S.sh, S.red);
     const uint32_t tmem = S.tmem_at;
     const Wait wait{&S.abort_flag, a.err};
 
@@ -128,13 +130,13 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
             Request first{};
             Share sh;
             if (one) {
-                sh = share_of_warp<ROWS>(a, first);
+                sh = share_of_warp<ROWS, EXTRA>(a, first);
                 if (lane == 0) S.sh.d = sh.d;                   // the other roles read it after a segment
             } else {
                 sh = S.sh;
                 if (sh.u < sh.end) first = request(a, sh.i);
             }
-            Walk<ROWS> walk(a, sh, first);
+            Walk<ROWS, EXTRA> walk(a, sh, first);
             int n = 0;
             bool ok = true;
 #pragma unroll 1
@@ -197,6 +199,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                             mma_f16(d, desc_kmajor_sw128(q + (SPLIT ? (1 - term) * L::QTILE : 0) + o), desc_kmajor_sw128(k + o), ID_S, term > 0 || ks > 0);
                         }
                     commit(&S.s_full[g]);
+                    if (n + 1 == P) commit(&S.q_empty);
                     if (!two || g == 1) commit(&S.empty[st]);
                     return true;
                 };
@@ -230,13 +233,65 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
             // nothing may still write the tensor memory when it is given back
             commit(&S.drained);
             mbar_drain(&S.drained, 0);
+        } else if (warp >= 10) {
+            // q of a segment into shared memory, as soon as no MMA reads the last one's: 64 threads, 16-byte
+            // pieces of 16-bit values, U of them at a time (f32 rows: the high terms, then the low ones)
+            int nq = 0;
+#pragma unroll 1
+            for (int sn = 0;; ++sn) {
+                bool ok = wait(&S.segs.full[sn % SegmentRing::N], (sn / SegmentRing::N) & 1);
+                const Segment & it = S.segs.s[sn % SegmentRing::N];
+                const bool has = ok && it.nt > 0 && it.n_keys > 0;
+                if (has && nq > 0) ok = wait(&S.q_empty, (nq - 1) & 1);
+                if (named_sync_or(2, 64, !ok) || it.nt < 0) break;   // after an abort both warps leave together
+                if (has) {
+                    ++nq;
+                    constexpr int CH = D / 8, STEP = 64 / CH, U = SPLIT ? 4 : 8;   // pieces of a row; rows a pass
+                    const int c = tid % CH, rows = it.m > 128 ? 256 : 128;
+#pragma unroll 1
+                    for (int m1 = (tid & 63) / CH; m1 < rows; m1 += U * STEP) {
+                        uint4 v[U], w[SPLIT ? U : 1];
+#pragma unroll
+                        for (int k = 0; k < U; ++k) {
+                            const int m = m1 + k * STEP;
+                            v[k] = make_uint4(0, 0, 0, 0);
+                            if constexpr (SPLIT) w[k] = v[k];
+                            if (m < it.m) {
+                                const uint4 * src = reinterpret_cast<const uint4 *>(row_at<const T>(a, a.q, a.q_stride, it, m) + c * 8);
+                                v[k] = __ldg(src);
+                                if constexpr (SPLIT) w[k] = __ldg(src + 1);
+                            }
+                        }
+#pragma unroll
+                        for (int k = 0; k < U; ++k) {
+                            const int m = m1 + k * STEP;
+                            uint8_t * dst = qs + (m >> 7) * L::QTILE + (c >> 3) * (128 * 128) + (m & 127) * 128 + (((c & 7) ^ (m & 7)) << 4);
+                            if constexpr (SPLIT) {
+                                uint4 hi, lo;
+                                split_pair<C>(__uint_as_float(v[k].x), __uint_as_float(v[k].y), hi.x, lo.x);
+                                split_pair<C>(__uint_as_float(v[k].z), __uint_as_float(v[k].w), hi.y, lo.y);
+                                split_pair<C>(__uint_as_float(w[k].x), __uint_as_float(w[k].y), hi.z, lo.z);
+                                split_pair<C>(__uint_as_float(w[k].z), __uint_as_float(w[k].w), hi.w, lo.w);
+                                *reinterpret_cast<uint4 *>(dst) = hi;
+                                *reinterpret_cast<uint4 *>(dst + L::QTILE) = lo;
+                            } else {
+                                *reinterpret_cast<uint4 *>(dst) = v[k];
+                            }
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    mbar_arrive(&S.q_full);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&S.segs.empty[sn % SegmentRing::N]);
+            }
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int wg = warp >> 2, r = tid & 127;
         const uint32_t lane_at = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + lane_at + wg * 128, o_at = tmem + lane_at + 256 + wg * 128;
-        int base = 0, ns = 0, no = 0;
+        int base = 0, ns = 0, no0 = 0, no1 = 0;
 #pragma unroll 1
         for (int sn = 0;; ++sn) {
             const bool got = wait(&S.segs.full[sn % SegmentRing::N], (sn / SegmentRing::N) & 1);
@@ -246,49 +301,6 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
             if (it.nt < 0) break;
             const bool two = it.m > 128;
             const int nt = it.n_keys > 0 ? it.nt : 0, n_keys = it.n_keys, ctx = it.ctx, t0 = it.t0;
-            // q into shared memory: rows of 16-bit values (f32: the high terms, then the low ones)
-            if (nt > 0) {
-                constexpr int CH = D / 8, STEP = 256 / CH, U = 128 / STEP;   // 16-byte pieces of a row; rows a pass; passes a tile
-                const int c = tid % CH;
-                for (int m1 = tid / CH; m1 < (two ? 256 : 128); m1 += 128) {
-                    uint4 v[U], w[SPLIT ? U : 1];
-#pragma unroll
-                    for (int k = 0; k < U; ++k) {
-                        const int m = m1 + k * STEP;
-                        v[k] = make_uint4(0, 0, 0, 0);
-                        if constexpr (SPLIT) w[k] = v[k];
-                        if (m < it.m) {
-                            const uint4 * src = reinterpret_cast<const uint4 *>(row_at<const T>(a, a.q, a.q_stride, it, m) + c * 8);
-                            v[k] = __ldg(src);
-                            if constexpr (SPLIT) w[k] = __ldg(src + 1);
-                        }
-                    }
-#pragma unroll
-                    for (int k = 0; k < U; ++k) {
-                        const int m = m1 + k * STEP;
-                        uint8_t * dst = qs + (m >> 7) * L::QTILE + (c >> 3) * (128 * 128) + (m & 127) * 128 + (((c & 7) ^ (m & 7)) << 4);
-                        if constexpr (SPLIT) {
-                            const uint32_t f[8] = {v[k].x, v[k].y, v[k].z, v[k].w, w[k].x, w[k].y, w[k].z, w[k].w};
-                            uint32_t h[4], l[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float f0 = __uint_as_float(f[2 * e]), f1 = __uint_as_float(f[2 * e + 1]);
-                                h[e] = pack<C>(f0, f1);
-                                const float2 b = unpack<C>(h[e]);
-                                l[e] = pack<C>(f0 - b.x, f1 - b.y);
-                            }
-                            *reinterpret_cast<uint4 *>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
-                            *reinterpret_cast<uint4 *>(dst + L::QTILE) = make_uint4(l[0], l[1], l[2], l[3]);
-                        } else {
-                            *reinterpret_cast<uint4 *>(dst) = v[k];
-                        }
-                    }
-                }
-                fence_proxy_async_smem();
-            }
-            fence_before_sync();
-            if (nt > 0) mbar_arrive(&S.q_full);
-
             const int m = (two ? wg * 128 : 0) + r, j = by_group(a, it.m0 + min(m, it.m - 1));
             // every row of the warp sees the tokens before `open`
             const int open = ctx + (a.mask ? 0 : by_group(a, it.m0 + min((two ? wg * 128 : 0) + (warp & 3) * 32, it.m - 1)) + 1);
@@ -364,59 +376,51 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 mbar_arrive(&S.p_full[wg]);
             }
             base += 2 * nt;
-            if (any) {
-                wait(&S.o_full[wg], no & 1);
-                ++no;
-                fence_after_sync();
-            }
-
+            // which warpgroup's sums there are; both read both where they took the key tiles in turn
+            const bool use0 = two ? wg == 0 : nt > 0, use1 = two ? wg == 1 : nt > 1;
+            if (use0) wait(&S.o_full[0], no0 & 1);
+            if (use1) wait(&S.o_full[1], no1 & 1);
+            no0 += nt > 0;
+            no1 += two ? nt > 0 : nt > 1;
+            fence_after_sync();
             const bool whole = is_whole(it);
-            float mine = 1.f;                             // what this warpgroup's O counts
-            float * const half = reinterpret_cast<float *>(qs);
+            float w0 = 1.f, w1 = 1.f;                     // what their O count
             int c_lo = 0, c_hi = D;                       // the columns that this warpgroup finishes
             if (!two) {
-                // the key tiles' two halves become one: each warpgroup finishes half of the columns and hands
-                // the other half over through the q tiles, which no MMA reads any more
                 S.stat[wg][0][r] = top;
                 S.stat[wg][1][r] = sum;
                 named_sync(1, 256);
-                const float t = fmaxf(S.stat[0][0][r], S.stat[1][0][r]), ref = t == -INFINITY ? 0.f : t;
-                mine = exp2_fast(top - ref);
-                sum = S.stat[0][1][r] * exp2_fast(S.stat[0][0][r] - ref) + S.stat[1][1][r] * exp2_fast(S.stat[1][0][r] - ref);
-                top = t;
+                const float t0 = S.stat[0][0][r], t1 = S.stat[1][0][r];
+                top = fmaxf(t0, t1);
+                const float ref = top == -INFINITY ? 0.f : top;
+                w0 = exp2_fast(t0 - ref);
+                w1 = exp2_fast(t1 - ref);
+                sum = S.stat[0][1][r] * w0 + S.stat[1][1][r] * w1;
                 c_lo = wg * (D / 2);
                 c_hi = c_lo + D / 2;
-                if (any) {
-                    const int give = (1 - wg) * (D / 2);
-#pragma unroll 1
-                    for (int c = give; c < give + D / 2; c += 32) {
-                        uint32_t o[32];
-                        tmem_ld<32>(o_at + c, o);
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) half[(c + k) * 128 + r] = __uint_as_float(o[k]) * mine;
-                    }
-                }
-                named_sync(1, 256);
             }
             {
                 float4 * pc = reinterpret_cast<float4 *>(piece(a, blockIdx.x, it.t0 == 0)) + m;
                 const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
-                const bool other = !two && (wg == 1 ? nt > 0 : nt > 1), live = m < it.m;
+                const bool live = m < it.m;
                 T * dst = row_at<T>(a, a.out, a.out_stride, it, live ? m : 0);
                 const bool wide = (reinterpret_cast<uintptr_t>(dst) & 31) == 0;   // rows are at least 16-byte aligned
+                w0 *= inv;
+                w1 *= inv;
 #pragma unroll 1
                 for (int c = c_lo; c < c_hi; c += 32) {
                     uint32_t o[32];
-                    if (any) tmem_ld<32>(o_at + c, o);
-                    float v[32];
+                    float v[32] = {};
+                    if (use0) {
+                        tmem_ld<32>(tmem + lane_at + 256 + c, o);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) v[k] = any ? __uint_as_float(o[k]) * mine : 0.f;
-                    if (other) {
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) v[k] += half[(c + k) * 128 + r];
+                        for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(o[k]) * w0;
                     }
+                    if (use1) {
+                        tmem_ld<32>(tmem + lane_at + 384 + c, o);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) v[k] *= inv;
+                        for (int k = 0; k < 32; ++k) v[k] += __uint_as_float(o[k]) * w1;
+                    }
                     if (!live) continue;
                     if (!whole) {
 #pragma unroll
