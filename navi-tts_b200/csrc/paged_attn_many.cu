@@ -28,7 +28,7 @@ using namespace navi::umma;
 // f32 rows: q and p as two f16 terms each against the exact cache values, as in the kernel for few
 // rows. Two tiles of q do not fit then, so their items have 128 rows.
 constexpr int LAZY = 8;
-constexpr int EXTRA = 2;                                        // what an item costs beside its key tiles, in key tiles
+constexpr int EXTRA = 1;                                        // what an item costs beside its key tiles, in key tiles
 
 template <class T, int D> struct ManySmem {
     static constexpr bool SPLIT = std::is_same_v<T, float>;
@@ -67,20 +67,36 @@ template <class C> constexpr uint32_t idesc(int M, int N, bool v_major) {
     constexpr uint32_t f = std::is_same_v<C, __nv_bfloat16> ? 1u : 0u;
     return (1u << 4) | (f << 7) | (f << 10) | (v_major ? 1u << 16 : 0u) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
-// D[tmem] (+)= A[tmem] B[smem]
-__device__ __forceinline__ void mma_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t id, bool accumulate) {
+// The warp that issues the MMAs runs as one, so that descriptors stay in uniform registers (moving
+// them there for every MMA cost more than the MMA); `leader` is set in one of its lanes.
+// D[tmem] (+)= A[smem] B[smem]
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t id, bool accumulate, uint32_t leader) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b_desc), "r"(id), "r"(accumulate ? 1u : 0u)
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(id), "r"(accumulate ? 1u : 0u), "r"(leader)
         : "memory");
 }
-
+// D[tmem] (+)= A[tmem] B[smem]
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t id, bool accumulate, uint32_t leader) {
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(id), "r"(accumulate ? 1u : 0u), "r"(leader)
+        : "memory");
+}
+__device__ __forceinline__ void commit_by(uint64_t * bar, uint32_t leader) {
+    asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(
+                     smem_addr(bar)),
+                 "r"(leader)
+                 : "memory");
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
 }
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 
 template <class T, class C, int D>
 __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
@@ -171,67 +187,73 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
             // after an abort the copies still under way land before the block's shared memory goes
             if (S.abort_flag)
                 for (int k = max(n - L::STAGES, 0); k < n; ++k) mbar_drain(&S.full[k % L::STAGES], (k / L::STAGES) & 1);
-        } else if (warp == 9 && lane == 0) {
+        } else if (warp == 9) {
             constexpr uint32_t ID_S = idesc<C>(128, KT, false), ID_O = idesc<C>(128, D, true);
-            const uint32_t q_at = smem_addr(qs), ring_at = smem_addr(ring);
-            int base = 0, nq = 0, np[2] = {0, 0};
+            const uint32_t leader = lane == 0, tm = static_cast<uint32_t>(uniform(static_cast<int>(tmem)));
+            const uint64_t q_desc = desc_kmajor_sw128(smem_addr(qs)), k_desc = desc_kmajor_sw128(smem_addr(ring)), v_desc = desc_mnmajor_sw128(smem_addr(ring), KT * 128);
+            const auto wait_all = [&](uint64_t * bar, int parity) { return __all_sync(0xffffffffu, wait(bar, static_cast<uint32_t>(parity))) != 0; };
+            int base = 0, nq = 0, np0 = 0, np1 = 0;
             bool ok = true;
 #pragma unroll 1
             for (int sn = 0; ok; ++sn) {
-                if (!wait(&S.segs.full[sn % SegmentRing::N], (sn / SegmentRing::N) & 1)) break;
+                if (!wait_all(&S.segs.full[sn % SegmentRing::N], (sn / SegmentRing::N) & 1)) break;
                 const Segment & s = S.segs.s[sn % SegmentRing::N];
-                if (s.nt < 0) break;
-                const bool two = s.m > 128;
-                const int nt = s.n_keys > 0 ? s.nt : 0, P = two ? 2 * nt : nt;
-                mbar_arrive(&S.segs.empty[sn % SegmentRing::N]);
+                const int s_nt = uniform(s.nt), s_m = uniform(s.m), s_keys = uniform(s.n_keys);
+                if (s_nt < 0) break;
+                const bool two = s_m > 128;
+                const int nt = s_keys > 0 ? s_nt : 0, P = two ? 2 * nt : nt;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&S.segs.empty[sn % SegmentRing::N]);
                 if (P == 0) continue;
-                const auto tile = [&](int n) { return two ? n >> 1 : n; };
-                const auto scores = [&](int n) {
-                    const int g = n & 1, st = (base + 2 * tile(n)) % L::STAGES;
-                    if (!wait(&S.full[st], ((base + 2 * tile(n)) / L::STAGES) & 1)) return false;
-                    fence_after_sync();
-                    const uint32_t d = tmem + g * 128, q = q_at + (two ? g * L::QTILE : 0), k = ring_at + st * L::STAGE;
-#pragma unroll
-                    for (int term = 0; term < (SPLIT ? 2 : 1); ++term)
-#pragma unroll
-                        for (int ks = 0; ks < D / 16; ++ks) {
-                            const uint32_t o = (ks >> 2) * (128 * 128) + (ks & 3) * 32;
-                            mma_f16(d, desc_kmajor_sw128(q + (SPLIT ? (1 - term) * L::QTILE : 0) + o), desc_kmajor_sw128(k + o), ID_S, term > 0 || ks > 0);
-                        }
-                    commit(&S.s_full[g]);
-                    if (n + 1 == P) commit(&S.q_empty);
-                    if (!two || g == 1) commit(&S.empty[st]);
-                    return true;
-                };
-                // the first of the loop's steps only ask for scores
-                ok = wait(&S.q_full, nq & 1);
+                ok = wait_all(&S.q_full, nq & 1);
                 ++nq;
                 fence_after_sync();
+                // step n asks for the scores of pair n + 2 once P V of pair n is under way; the first two only ask
 #pragma unroll 1
                 for (int n = -2; n < P && ok; ++n) {
-                    if (n < 0) {
-                        if (n + 2 < P) ok = scores(n + 2);
-                        continue;
+                    const int g = n & 1;
+                    if (n >= 0) {
+                        const int idx = base + 2 * (two ? n >> 1 : n) + 1, st = idx % L::STAGES, turn = g ? np1 : np0;
+                        ok = wait_all(&S.full[st], (idx / L::STAGES) & 1) && wait_all(&S.p_full[g], turn & 1);
+                        if (!ok) break;
+                        if (g) ++np1;
+                        else ++np0;
+                        fence_after_sync();
+                        const uint32_t d = tm + 256 + g * 128, p = tm + g * 128;
+                        const uint64_t v = v_desc + static_cast<uint32_t>(st * (L::STAGE >> 4));
+#pragma unroll
+                        for (int term = 0; term < (SPLIT ? 2 : 1); ++term)
+#pragma unroll
+                            for (int ks = 0; ks < KT / 16; ++ks)
+                                mma_ts(d, p + (SPLIT ? (1 - term) * 64 : 0) + ks * 8, v + ks * (2048 >> 4), ID_O, n > 1 || term > 0 || ks > 0, leader);
+                        if (!two || g == 1) commit_by(&S.empty[st], leader);
+                        if (n + 2 >= P) commit_by(&S.o_full[g], leader);
                     }
-                    const int g = n & 1, idx = base + 2 * tile(n) + 1, st = idx % L::STAGES;
-                    ok = wait(&S.full[st], (idx / L::STAGES) & 1) && wait(&S.p_full[g], np[g] & 1);
-                    if (!ok) break;
-                    ++np[g];
-                    fence_after_sync();
-                    const uint32_t d = tmem + 256 + g * 128, p = tmem + g * 128, v = ring_at + st * L::STAGE;
+                    if (n + 2 < P) {
+                        const int idx = base + 2 * (two ? (n + 2) >> 1 : n + 2), st = idx % L::STAGES;
+                        ok = wait_all(&S.full[st], (idx / L::STAGES) & 1);
+                        if (!ok) break;
+                        fence_after_sync();
+                        const uint32_t d = tm + g * 128;
+                        const uint64_t q = q_desc + static_cast<uint32_t>(two ? g * (L::QTILE >> 4) : 0), k = k_desc + static_cast<uint32_t>(st * (L::STAGE >> 4));
 #pragma unroll
-                    for (int term = 0; term < (SPLIT ? 2 : 1); ++term)
+                        for (int term = 0; term < (SPLIT ? 2 : 1); ++term)
 #pragma unroll
-                        for (int ks = 0; ks < KT / 16; ++ks)
-                            mma_ta(d, p + (SPLIT ? (1 - term) * 64 : 0) + ks * 8, desc_mnmajor_sw128(v + ks * 2048, KT * 128), ID_O, n > 1 || term > 0 || ks > 0);
-                    if (!two || g == 1) commit(&S.empty[st]);
-                    if (n + 2 >= P) commit(&S.o_full[g]);
-                    if (n + 2 < P) ok = scores(n + 2);
+                            for (int ks = 0; ks < D / 16; ++ks) {
+                                constexpr int HALF = 128 * 128 >> 4;
+                                const int o = (ks >> 2) * HALF + (ks & 3) * 2;
+                                mma_ss(d, q + (SPLIT ? (1 - term) * (L::QTILE >> 4) : 0) + o, k + o, ID_S, term > 0 || ks > 0, leader);
+                            }
+                        commit_by(&S.s_full[g], leader);
+                        if (n + 3 == P) commit_by(&S.q_empty, leader);
+                        if (!two || g == 1) commit_by(&S.empty[st], leader);
+                    }
                 }
                 base += 2 * nt;
             }
             // nothing may still write the tensor memory when it is given back
-            commit(&S.drained);
+            commit_by(&S.drained, leader);
+            __syncwarp();
             mbar_drain(&S.drained, 0);
         } else if (warp >= 10) {
             // q of a segment into shared memory, as soon as no MMA reads the last one's: 64 threads, 16-byte
