@@ -158,6 +158,13 @@ __device__ __forceinline__ void tma_box_2d(void * dst, const void * tmap, int x,
                  "l"(tmap), "r"(x), "r"(y), "r"(smem_addr(bar))
                  : "memory");
 }
+// The same of a 3-D map (x innermost).
+__device__ __forceinline__ void tma_box_3d(void * dst, const void * tmap, int x, int y, int z, uint64_t * bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                     smem_addr(dst)),
+                 "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+                 : "memory");
+}
 // Orders this thread's later tensor-map reads after generic-proxy writes of the map (the host's
 // copy before the launch), so a map rewritten at the same address is not read stale.
 __device__ __forceinline__ void tensormap_acquire(const void * tmap) {

@@ -30,7 +30,7 @@ void Pages::attend(const navi_step & s, int layer, const navi_attend_args & q, c
     const int sms = dev_->info().multiprocessors;
     const PagesScratch sc(dev_->scratch(stream, PagesScratch::bytes(sms)), sms);
     attn::AttendArgs a{q.q, q.out, q.lse, d_.table, s.req, s.ctx_len, s.cu_rows, s.status, s.parent ? s.mask : nullptr, sc.pieces, sc.arrived, sc.err,
-                 in, out, q.scale * 1.4426950408889634f, 0, s.n_req, s.max_rows, s.mask_words, q.n_head, d_.n_kv_head, q.n_head / d_.n_kv_head, D, shift_,
+                 in, out, q.scale * 1.4426950408889634f, 0, s.n_req, s.max_rows, s.mask_words, q.n_head, d_.n_kv_head, q.n_head / d_.n_kv_head, 0, D, shift_,
                  d_.n_pages, d_.max_blocks, d_.max_requests};
     const int64_t most = std::min(s.max_new, s.max_rows);
     if (a.group > 1) a.group_mul = static_cast<uint32_t>(((1ull << 32) + static_cast<uint64_t>(a.group) - 1) / static_cast<uint64_t>(a.group));
@@ -41,7 +41,15 @@ void Pages::attend(const navi_step & s, int layer, const navi_attend_args & q, c
     const CUtensorMap & km = maps_[static_cast<size_t>(2 * layer)], & vm = maps_[static_cast<size_t>(2 * layer + 1)];
     const int64_t m = most * a.group;
     if (m <= attn::FEW_ROWS) return attn::attend_few(a, km, vm, q.dtype, d_.dtype, static_cast<int>(m), sms, stream);
-    attn::attend_many(a, km, vm, q.dtype, d_.dtype, sms, stream);
+    CUtensorMap qm{};
+    if (q.dtype != NAVI_F32 && m > 128 && a.group <= 128 && (a.group & (a.group - 1)) == 0) {
+        a.q_boxes = 1;
+        const cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(q.n_head), static_cast<cuuint64_t>(s.max_rows)};
+        const cuuint64_t strides[2] = {static_cast<cuuint64_t>(D) * 2, static_cast<cuuint64_t>(in) * 2};
+        const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(a.group), static_cast<cuuint32_t>(128 / a.group)};
+        qm = swizzled_map(q.q, q.dtype, 3, dims, strides, box);
+    }
+    attn::attend_many(a, km, vm, qm, q.dtype, d_.dtype, sms, stream);
 }
 
 } // namespace navi

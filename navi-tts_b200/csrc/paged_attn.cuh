@@ -27,7 +27,8 @@ struct AttendArgs {
     int64_t q_stride, out_stride;
     float scale;                 // times log2(e)
     uint32_t group_mul;          // 2^32 / group rounded up, 0 for 1
-    int n_req, max_rows, mask_words, n_head, n_kv, group, head_dim, shift, n_pages, max_blocks, max_requests;
+    // q_boxes: q comes as boxes of a tensor map (16-bit rows, group a power of two up to 128)
+    int n_req, max_rows, mask_words, n_head, n_kv, group, q_boxes, head_dim, shift, n_pages, max_blocks, max_requests;
 };
 
 // What a block needs to know of one request.

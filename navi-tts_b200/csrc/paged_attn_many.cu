@@ -100,7 +100,7 @@ __device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, 
 
 template <class T, class C, int D>
 __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
-                                                        const __grid_constant__ CUtensorMap vmap) {
+                                                        const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap qmap) {
     constexpr bool SPLIT = std::is_same_v<T, float>;
     constexpr int ROWS = SPLIT ? 128 : 256;
     using L = ManySmem<T, D>;
@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
             mbar_init(&S.full[s], 1);
             mbar_init(&S.empty[s], 1);
         }
-        mbar_init(&S.q_full, 64);
+        mbar_init(&S.q_full, a.q_boxes ? 1 : 64);
         mbar_init(&S.q_empty, 1);
         for (int g = 0; g < 2; ++g) {
             mbar_init(&S.s_full[g], 1);
@@ -211,31 +211,39 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 // step n asks for the scores of pair n + 2 once P V of pair n is under way; the first two only ask
 #pragma unroll 1
                 for (int n = -2; n < P && ok; ++n) {
-                    const int g = n & 1;
+                    const int g = n & 1, tn = two ? n >> 1 : n, tk = two ? (n + 2) >> 1 : n + 2;   // the pair's tile, and that of pair n + 2
+                    const int iv = base + 2 * tn + 1, ik = base + 2 * tk, sv = iv % L::STAGES, sk = ik % L::STAGES;
+                    // where the warpgroups share the tiles, arithmetic is the bound: all that is waited for comes before the
+                    // two products, which then follow one another. Otherwise HBM is, and P V, which frees a stage, does
+                    // not wait for the next K.
+                    if (n >= 0 && (!two || g == 0)) ok = wait_all(&S.full[sv], (iv / L::STAGES) & 1);
+                    if (n + 2 < P && two && g == 0) ok = ok && wait_all(&S.full[sk], (ik / L::STAGES) & 1);
                     if (n >= 0) {
-                        const int idx = base + 2 * (two ? n >> 1 : n) + 1, st = idx % L::STAGES, turn = g ? np1 : np0;
-                        ok = wait_all(&S.full[st], (idx / L::STAGES) & 1) && wait_all(&S.p_full[g], turn & 1);
-                        if (!ok) break;
+                        ok = ok && wait_all(&S.p_full[g], (g ? np1 : np0) & 1);
                         if (g) ++np1;
                         else ++np0;
-                        fence_after_sync();
+                    }
+                    if (!ok) break;
+                    fence_after_sync();
+                    if (n >= 0) {
                         const uint32_t d = tm + 256 + g * 128, p = tm + g * 128;
-                        const uint64_t v = v_desc + static_cast<uint32_t>(st * (L::STAGE >> 4));
+                        const uint64_t v = v_desc + static_cast<uint32_t>(sv * (L::STAGE >> 4));
 #pragma unroll
                         for (int term = 0; term < (SPLIT ? 2 : 1); ++term)
 #pragma unroll
                             for (int ks = 0; ks < KT / 16; ++ks)
                                 mma_ts(d, p + (SPLIT ? (1 - term) * 64 : 0) + ks * 8, v + ks * (2048 >> 4), ID_O, n > 1 || term > 0 || ks > 0, leader);
-                        if (!two || g == 1) commit_by(&S.empty[st], leader);
                         if (n + 2 >= P) commit_by(&S.o_full[g], leader);
+                        if (!two || g == 1) commit_by(&S.empty[sv], leader);
                     }
                     if (n + 2 < P) {
-                        const int idx = base + 2 * (two ? (n + 2) >> 1 : n + 2), st = idx % L::STAGES;
-                        ok = wait_all(&S.full[st], (idx / L::STAGES) & 1);
-                        if (!ok) break;
-                        fence_after_sync();
+                        if (!two) {
+                            ok = wait_all(&S.full[sk], (ik / L::STAGES) & 1);
+                            if (!ok) break;
+                            fence_after_sync();
+                        }
                         const uint32_t d = tm + g * 128;
-                        const uint64_t q = q_desc + static_cast<uint32_t>(two ? g * (L::QTILE >> 4) : 0), k = k_desc + static_cast<uint32_t>(st * (L::STAGE >> 4));
+                        const uint64_t q = q_desc + static_cast<uint32_t>(two ? g * (L::QTILE >> 4) : 0), k = k_desc + static_cast<uint32_t>(sk * (L::STAGE >> 4));
 #pragma unroll
                         for (int term = 0; term < (SPLIT ? 2 : 1); ++term)
 #pragma unroll
@@ -246,7 +254,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                             }
                         commit_by(&S.s_full[g], leader);
                         if (n + 3 == P) commit_by(&S.q_empty, leader);
-                        if (!two || g == 1) commit_by(&S.empty[st], leader);
+                        if (!two || g == 1) commit_by(&S.empty[sk], leader);
                     }
                 }
                 base += 2 * nt;
@@ -256,8 +264,9 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
             __syncwarp();
             mbar_drain(&S.drained, 0);
         } else if (warp >= 10) {
-            // q of a segment into shared memory, as soon as no MMA reads the last one's: 64 threads, 16-byte
-            // pieces of 16-bit values, U of them at a time (f32 rows: the high terms, then the low ones)
+            // q of a segment into shared memory, as soon as no MMA reads the last one's: by TMA, the heads of a
+            // row next to one another, or 64 threads, 16-byte pieces of 16-bit values, U of them at a time (f32
+            // rows: the high terms, then the low ones)
             int nq = 0;
 #pragma unroll 1
             for (int sn = 0;; ++sn) {
@@ -266,7 +275,18 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 const bool has = ok && it.nt > 0 && it.n_keys > 0;
                 if (has && nq > 0) ok = wait(&S.q_empty, (nq - 1) & 1);
                 if (named_sync_or(2, 64, !ok) || it.nt < 0) break;   // after an abort both warps leave together
-                if (has) {
+                if (has && a.q_boxes) {
+                    ++nq;
+                    if (tid == 320) {
+                        const int tiles = it.m > 128 ? 2 : 1;
+                        mbar_arrive_expect_tx(&S.q_full, static_cast<uint32_t>(tiles * L::QTILE));
+#pragma unroll 1
+                        for (int x = 0; x < tiles * (D / 64); ++x) {
+                            const int tile = x / (D / 64), h = x % (D / 64);
+                            tma_box_3d(qs + tile * L::QTILE + h * (128 * 128), &qmap, h * 64, it.g * a.group, it.row0 + by_group(a, it.m0 + tile * 128), &S.q_full);
+                        }
+                    }
+                } else if (has) {
                     ++nq;
                     constexpr int CH = D / 8, STEP = 64 / CH, U = SPLIT ? 4 : 8;   // pieces of a row; rows a pass
                     const int c = tid % CH, rows = it.m > 128 ? 256 : 128;
@@ -497,20 +517,21 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
     }
 }
 
-template <class T, class C, int D> void many(const AttendArgs & a, const CUtensorMap & k, const CUtensorMap & v, int sms, cudaStream_t stream) {
+template <class T, class C, int D>
+void many(const AttendArgs & a, const CUtensorMap & k, const CUtensorMap & v, const CUtensorMap & q, int sms, cudaStream_t stream) {
     const auto kernel = k_attend_many<T, C, D>;
     constexpr int smem = ManySmem<T, D>::BYTES;
     NAVI_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    NAVI_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(sms)), dim3(384), smem, stream, a, k, v));
+    NAVI_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(sms)), dim3(384), smem, stream, a, k, v, q));
 }
 
 } // namespace
 
-void attend_many(const AttendArgs & a, const CUtensorMap & k, const CUtensorMap & v, int dtype, int cache, int sms, cudaStream_t stream) {
+void attend_many(const AttendArgs & a, const CUtensorMap & k, const CUtensorMap & v, const CUtensorMap & q, int dtype, int cache, int sms, cudaStream_t stream) {
     const bool wide = a.head_dim == 128;
-    if (dtype == NAVI_F32) wide ? many<float, __half, 128>(a, k, v, sms, stream) : many<float, __half, 64>(a, k, v, sms, stream);
-    else if (cache == NAVI_F16) wide ? many<__half, __half, 128>(a, k, v, sms, stream) : many<__half, __half, 64>(a, k, v, sms, stream);
-    else wide ? many<__nv_bfloat16, __nv_bfloat16, 128>(a, k, v, sms, stream) : many<__nv_bfloat16, __nv_bfloat16, 64>(a, k, v, sms, stream);
+    if (dtype == NAVI_F32) wide ? many<float, __half, 128>(a, k, v, q, sms, stream) : many<float, __half, 64>(a, k, v, q, sms, stream);
+    else if (cache == NAVI_F16) wide ? many<__half, __half, 128>(a, k, v, q, sms, stream) : many<__half, __half, 64>(a, k, v, q, sms, stream);
+    else wide ? many<__nv_bfloat16, __nv_bfloat16, 128>(a, k, v, q, sms, stream) : many<__nv_bfloat16, __nv_bfloat16, 64>(a, k, v, q, sms, stream);
 }
 
 } // namespace navi::attn

@@ -15,6 +15,25 @@
 
 namespace navi {
 
+CUtensorMap swizzled_map(const void * base, int dtype, int rank, const cuuint64_t * dims, const cuuint64_t * strides, const cuuint32_t * box) {
+    // the driver entry point is looked up at run time, so the library loads without libcuda
+    static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+    if (!encode) {
+        cudaDriverEntryPointQueryResult q{};
+        void * fn = nullptr;
+        NAVI_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
+        if (q != cudaDriverEntryPointSuccess || !fn) fail("pages: cuTensorMapEncodeTiled unavailable", NAVI_E_CUDA);
+        encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    }
+    CUtensorMap m{};
+    const cuuint32_t one[3] = {1, 1, 1};
+    const CUresult r = encode(&m, dtype == NAVI_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank),
+                              const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) fail("pages: cuTensorMapEncodeTiled failed (" + std::to_string(static_cast<int>(r)) + ")", NAVI_E_CUDA);
+    return m;
+}
+
 namespace {
 
 using namespace navi::dev;
@@ -432,25 +451,12 @@ __global__ void __launch_bounds__(COMMIT_THREADS) k_pages_commit(const __grid_co
     }
 }
 
-// A pool as rows of head_dim values; a box is a page of one head, 64 dims wide, in 128-byte swizzled rows.
+// A pool as rows of head_dim values; a box is a page of one head, 64 dims wide.
 CUtensorMap pool_map(void * pool, const navi_pages_desc & d) {
-    // the driver entry point is looked up at run time, so the library loads without libcuda
-    static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
-    if (!encode) {
-        cudaDriverEntryPointQueryResult q{};
-        void * fn = nullptr;
-        NAVI_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
-        if (q != cudaDriverEntryPointSuccess || !fn) fail("pages: cuTensorMapEncodeTiled unavailable", NAVI_E_CUDA);
-        encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-    }
-    CUtensorMap m{};
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(d.head_dim), static_cast<cuuint64_t>(d.n_pages) * d.n_kv_head * d.page_size};
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(d.head_dim) * 2};
-    const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(d.page_size)}, one[2] = {1, 1};
-    const CUresult r = encode(&m, d.dtype == NAVI_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, pool, dims, strides, box, one,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) fail("pages: cuTensorMapEncodeTiled failed (" + std::to_string(static_cast<int>(r)) + ")", NAVI_E_CUDA);
-    return m;
+    const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(d.page_size)};
+    return swizzled_map(pool, d.dtype, 2, dims, strides, box);
 }
 
 bool aligned16(const void * p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

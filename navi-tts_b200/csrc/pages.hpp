@@ -15,6 +15,10 @@
 
 namespace navi {
 
+// A tensor map of 16-bit values (dtype NAVI_F16 or NAVI_BF16) whose boxes land in 128-byte swizzled
+// rows of shared memory; values outside the tensor read as zero.
+CUtensorMap swizzled_map(const void * base, int dtype, int rank, const cuuint64_t * dims, const cuuint64_t * strides, const cuuint32_t * box);
+
 class Pages {
 public:
     static std::unique_ptr<Pages> create(const Device & dev, const navi_pages_desc & d);
