@@ -49,7 +49,7 @@ void Pages::attend(const navi_step & s, int layer, const navi_attend_args & q, c
         const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(a.group), static_cast<cuuint32_t>(128 / a.group)};
         qm = swizzled_map(q.q, q.dtype, 3, dims, strides, box);
     }
-    attn::attend_many(a, km, vm, qm, q.dtype, d_.dtype, sms, stream);
+    attn::attend_many(a, km, vm, qm, q.dtype, d_.dtype, m, sms, stream);
 }
 
 } // namespace navi

@@ -15,6 +15,6 @@ constexpr int FEW_ROWS = 32;
 
 void attend_few(const AttendArgs & a, const CUtensorMap & k, const CUtensorMap & v, int dtype, int cache, int rows, int sms, cudaStream_t stream);
 // q: rows x heads in boxes of 128 rows of one KV head, where a.q_boxes is set
-void attend_many(const AttendArgs & a, const CUtensorMap & k, const CUtensorMap & v, const CUtensorMap & q, int dtype, int cache, int sms, cudaStream_t stream);
+void attend_many(const AttendArgs & a, const CUtensorMap & k, const CUtensorMap & v, const CUtensorMap & q, int dtype, int cache, int64_t rows, int sms, cudaStream_t stream);
 
 } // namespace navi::attn

@@ -30,13 +30,14 @@ using namespace navi::umma;
 constexpr int LAZY = 8;
 constexpr int EXTRA = 1;                                        // what an item costs beside its key tiles, in key tiles
 
-template <class T, int D> struct ManySmem {
+template <class T, int D, int ROWS> struct ManySmem {
     static constexpr bool SPLIT = std::is_same_v<T, float>;
     static constexpr int QTILE = 128 * D * 2;                   // 128 rows, 16-bit: [D / 64][128][128 B], swizzled
     static constexpr int STAGE = KT * D * 2;                    // K or V of a key tile
-    static constexpr int STAGES = D == 128 ? 5 : 8;
+    static constexpr int QTILES = SPLIT || ROWS > 128 ? 2 : 1;
+    static constexpr int STAGES = D == 128 ? 7 - QTILES : 8;
     static constexpr int CONTROL = 3072;                        // ManyControl, and the tiles at 1024-byte boundaries
-    static constexpr int BYTES = CONTROL + 2 * QTILE + STAGES * STAGE;
+    static constexpr int BYTES = CONTROL + QTILES * QTILE + STAGES * STAGE;
     static_assert(BYTES <= 227 * 1024);
 };
 
@@ -98,16 +99,15 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 __device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 
-template <class T, class C, int D>
+template <class T, class C, int D, int ROWS>   // ROWS: 128 or 256 rows of an item
 __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
                                                         const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap qmap) {
     constexpr bool SPLIT = std::is_same_v<T, float>;
-    constexpr int ROWS = SPLIT ? 128 : 256;
-    using L = ManySmem<T, D>;
+    using L = ManySmem<T, D, ROWS>;
     static_assert(sizeof(ManyControl) <= L::CONTROL && L::STAGES <= 8);
     extern __shared__ __align__(1024) uint8_t raw[];   // all of the block's shared memory: at a 1024-byte boundary
     ManyControl & S = *reinterpret_cast<ManyControl *>(raw);
-    uint8_t * qs = raw + L::CONTROL, * ring = qs + 2 * L::QTILE;
+    uint8_t * qs = raw + L::CONTROL, * ring = qs + L::QTILES * L::QTILE;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         S.abort_flag = 0;
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 const Segment & s = S.segs.s[sn % SegmentRing::N];
                 const int s_nt = uniform(s.nt), s_m = uniform(s.m), s_keys = uniform(s.n_keys);
                 if (s_nt < 0) break;
-                const bool two = s_m > 128;
+                const bool two = ROWS > 128 && s_m > 128;
                 const int nt = s_keys > 0 ? s_nt : 0, P = two ? 2 * nt : nt;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&S.segs.empty[sn % SegmentRing::N]);
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
             if (named_sync_or(1, 256, !got)) break;
             const Segment & it = S.segs.s[sn % SegmentRing::N];
             if (it.nt < 0) break;
-            const bool two = it.m > 128;
+            const bool two = ROWS > 128 && it.m > 128;
             const int nt = it.n_keys > 0 ? it.nt : 0, n_keys = it.n_keys, ctx = it.ctx, t0 = it.t0;
             const int m = (two ? wg * 128 : 0) + r, j = by_group(a, it.m0 + min(m, it.m - 1));
             // every row of the warp sees the tokens before `open`
@@ -518,20 +518,23 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
 }
 
 template <class T, class C, int D>
-void many(const AttendArgs & a, const CUtensorMap & k, const CUtensorMap & v, const CUtensorMap & q, int sms, cudaStream_t stream) {
-    const auto kernel = k_attend_many<T, C, D>;
-    constexpr int smem = ManySmem<T, D>::BYTES;
-    NAVI_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    NAVI_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(sms)), dim3(384), smem, stream, a, k, v, q));
+void many(const AttendArgs & a, const CUtensorMap & k, const CUtensorMap & v, const CUtensorMap & q, int64_t rows, int sms, cudaStream_t stream) {
+    const auto go = [&](auto kernel, int smem) {
+        NAVI_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        NAVI_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(sms)), dim3(384), static_cast<size_t>(smem), stream, a, k, v, q));
+    };
+    if constexpr (!std::is_same_v<T, float>)
+        if (rows > 128) return go(k_attend_many<T, C, D, 256>, ManySmem<T, D, 256>::BYTES);
+    go(k_attend_many<T, C, D, 128>, ManySmem<T, D, 128>::BYTES);
 }
 
 } // namespace
 
-void attend_many(const AttendArgs & a, const CUtensorMap & k, const CUtensorMap & v, const CUtensorMap & q, int dtype, int cache, int sms, cudaStream_t stream) {
+void attend_many(const AttendArgs & a, const CUtensorMap & k, const CUtensorMap & v, const CUtensorMap & q, int dtype, int cache, int64_t rows, int sms, cudaStream_t stream) {
     const bool wide = a.head_dim == 128;
-    if (dtype == NAVI_F32) wide ? many<float, __half, 128>(a, k, v, q, sms, stream) : many<float, __half, 64>(a, k, v, q, sms, stream);
-    else if (cache == NAVI_F16) wide ? many<__half, __half, 128>(a, k, v, q, sms, stream) : many<__half, __half, 64>(a, k, v, q, sms, stream);
-    else wide ? many<__nv_bfloat16, __nv_bfloat16, 128>(a, k, v, q, sms, stream) : many<__nv_bfloat16, __nv_bfloat16, 64>(a, k, v, q, sms, stream);
+    if (dtype == NAVI_F32) wide ? many<float, __half, 128>(a, k, v, q, rows, sms, stream) : many<float, __half, 64>(a, k, v, q, rows, sms, stream);
+    else if (cache == NAVI_F16) wide ? many<__half, __half, 128>(a, k, v, q, rows, sms, stream) : many<__half, __half, 64>(a, k, v, q, rows, sms, stream);
+    else wide ? many<__nv_bfloat16, __nv_bfloat16, 128>(a, k, v, q, rows, sms, stream) : many<__nv_bfloat16, __nv_bfloat16, 64>(a, k, v, q, rows, sms, stream);
 }
 
 } // namespace navi::attn
