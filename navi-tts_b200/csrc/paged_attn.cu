@@ -38,9 +38,9 @@ void Pages::attend(const navi_step & s, int layer, const navi_attend_args & q, c
     // the list of key tiles that the blocks divide
     const int64_t rows = most * a.group <= attn::FEW_ROWS ? 16 : 128, items = (most * a.group + rows - 1) / rows * d_.n_kv_head * s.n_req, tiles = (static_cast<int64_t>(d_.max_blocks) * d_.page_size + attn::KT - 1) / attn::KT + 2;
     if (items * tiles >= 1ll << 31) fail("pages attend: requests x heads x tokens pass 31 bits of key tiles", NAVI_E_SHAPE);
-    const CUtensorMap & km = maps_[static_cast<size_t>(2 * layer)], & vm = maps_[static_cast<size_t>(2 * layer + 1)];
     const int64_t m = most * a.group;
-    if (m <= attn::FEW_ROWS) return attn::attend_few(a, km, vm, q.dtype, d_.dtype, static_cast<int>(m), sms, stream);
+    const size_t at = static_cast<size_t>(2 * layer);
+    if (m <= attn::FEW_ROWS) return attn::attend_few(a, page_maps_[at], page_maps_[at + 1], q.dtype, d_.dtype, static_cast<int>(m), sms, stream);
     CUtensorMap qm{};
     if (q.dtype != NAVI_F32 && m > 128 && a.group <= 128 && (a.group & (a.group - 1)) == 0) {
         a.q_boxes = 1;
@@ -49,7 +49,7 @@ void Pages::attend(const navi_step & s, int layer, const navi_attend_args & q, c
         const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(a.group), static_cast<cuuint32_t>(128 / a.group)};
         qm = swizzled_map(q.q, q.dtype, 3, dims, strides, box);
     }
-    attn::attend_many(a, km, vm, qm, q.dtype, d_.dtype, m, sms, stream);
+    attn::attend_many(a, maps_[at], maps_[at + 1], qm, q.dtype, d_.dtype, m, sms, stream);
 }
 
 } // namespace navi

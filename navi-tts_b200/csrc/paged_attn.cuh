@@ -434,18 +434,11 @@ __device__ __forceinline__ uint32_t seen_bits(const AttendArgs & a, const Segmen
 __device__ __forceinline__ int tile_pages(const AttendArgs & a, const Segment & s, int t) {
     return (min(s.n_keys - t * KT, KT) + (1 << a.shift) - 1) >> a.shift;
 }
-// A warp brings them from a pool's map to dst: halves of 64 dims, each [KT][64] in 128-byte rows that
-// the copy swizzles; only pages with keys of the item, so rows past them keep what they held.
-// The bytes (tile_pages * page * D * 2) arrive on `bar`. Lane x has the x-th box of the tile, at
-// most 16 of them (a page of 16 tokens, two halves), so the page ids, which it reads a tile ahead,
-// cost one latency together and not one each.
-template <int D> __device__ __forceinline__ int page_of_box(const AttendArgs & a, const Segment & s, int t, int box) {
-    const int p = box / (D / 64);
+// A warp brings them from a pool's map by TMA, a box a lane; only pages with keys of the item, so rows
+// past them keep what they held. The bytes (tile_pages * page * D * 2) arrive on a barrier. Every lane
+// reads its page's id a tile ahead, so the ids cost one latency together and not one each.
+__device__ __forceinline__ int page_at(const AttendArgs & a, const Segment & s, int t, int p) {
     return p < tile_pages(a, s, t) ? min(max(__ldg(a.table + static_cast<size_t>(s.table) * a.max_blocks + (t * KT >> a.shift) + p), 0), a.n_pages - 1) : -1;
-}
-template <int D> __device__ __forceinline__ void load_box(const AttendArgs & a, const CUtensorMap * map, const Segment & s, int page, int box, uint8_t * dst, uint64_t * bar) {
-    const int p = box / (D / 64), h = box % (D / 64);
-    if (page >= 0) tma_box_2d(dst + h * (KT * 128) + (p << a.shift) * 128, map, h * 64, (page * a.n_kv + s.g) << a.shift, bar);
 }
 
 // The ring of segments: one warp fills it, every other role reads it.

@@ -93,12 +93,12 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
         Walk<ROWS, 0> walk(a, sh, first);
         int n = 0;
         bool ok = true;
-        const int kv = lane >> 4, box = lane & 15;   // half a warp each for K and V
+        const int kv = lane >> 4, nth = lane & 15;   // half a warp each for K and V; a box is a page: [D / 64][page][64]
 #pragma unroll 1
         for (int k = 0; ok; ++k) {
             Segment s;
             const bool more = walk.next(s);
-            int page = more && s.n_keys > 0 ? page_of_box<D>(a, s, s.t0, box) : -1;
+            int page = more && s.n_keys > 0 ? page_at(a, s, s.t0, nth) : -1;
             if (k >= SegmentRing::N) ok = __shfl_sync(0xffffffffu, lane == 0 ? wait(&segs.empty[k % SegmentRing::N], (k / SegmentRing::N - 1) & 1) : 0, 0);
             if (!ok) break;
             if (lane == 0) {
@@ -109,12 +109,14 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
             if (s.n_keys <= 0) continue;
 #pragma unroll 1
             for (int t = s.t0; t < s.t0 + s.nt; ++t, ++n) {
-                const int st = n % L::STAGES, next = t + 1 < s.t0 + s.nt ? page_of_box<D>(a, s, t + 1, box) : -1;
+                const int st = n % L::STAGES, next = t + 1 < s.t0 + s.nt ? page_at(a, s, t + 1, nth) : -1;
                 if (n >= L::STAGES) ok = __shfl_sync(0xffffffffu, lane == 0 ? wait(&empty[st], (n / L::STAGES - 1) & 1) : 0, 0);
                 if (!ok) break;
                 if (lane == 0) mbar_arrive_expect_tx(&full[st], static_cast<uint32_t>(2 * (tile_pages(a, s, t) << a.shift) * D * 2));
                 __syncwarp();
-                load_box<D>(a, kv ? &vmap : &kmap, s, page, box, ring + st * L::STAGE + kv * (L::STAGE / 2), &full[st]);
+                if (page >= 0)
+                    tma_box_3d(ring + st * L::STAGE + kv * (L::STAGE / 2) + (nth << a.shift) * (D * 2), kv ? &vmap : &kmap, 0, (page * a.n_kv + s.g) << a.shift, 0,
+                               &full[st]);
                 page = next;
             }
         }
@@ -125,16 +127,23 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
     }
 
     const int rt = warp / KQ, kq = warp % KQ, k0 = kq * WK;
-    // Shared-memory rows are 128 bytes of a half of 64 dims, their eight 16-byte pieces swizzled by the row. The lanes of
-    // an ldmatrix read eight rows in a row from a multiple of 8 on, so the swizzle is the lane's own, and piece
-    // 2 j + b of a row lies at one of four offsets.
+    // A tile lies page after page, [D / 64][page][64]: rows of 128 bytes, their eight 16-byte pieces swizzled by the row.
+    // The lanes of an ldmatrix read eight rows in a row from a multiple of 8 on, so the swizzle is the lane's own,
+    // and piece 2 j + b of a row lies at one of four offsets. 16 keys never leave a page.
     uint32_t off_k[4], off_v[4];                      // b = (lane >> 3) & 1 for K, lane >> 4 for V and q
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         off_k[j] = ((2 * j + ((lane >> 3) & 1)) ^ (lane & 7)) << 4;
         off_v[j] = ((2 * j + (lane >> 4)) ^ (lane & 7)) << 4;
     }
-    const uint32_t k_at = smem_addr(ring) + (k0 + (lane & 7) + (lane >> 4) * 8) * 128, v_at = smem_addr(ring) + L::STAGE / 2 + (k0 + (lane & 15)) * 128;
+    const uint32_t half = 128u << a.shift;            // from a page's first 64 dims to the next
+    const auto place = [&](int key) { return static_cast<uint32_t>((key >> a.shift << a.shift) * (D * 2) + (key & ((1 << a.shift) - 1)) * 128); };
+    uint32_t k_at[KS], v_at[KS];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+        k_at[k] = smem_addr(ring) + place(k0 + 16 * k) + ((lane & 7) + (lane >> 4) * 8) * 128;
+        v_at[k] = smem_addr(ring) + L::STAGE / 2 + place(k0 + 16 * k) + (lane & 15) * 128;
+    }
     const uint32_t q_at = smem_addr(qs) + (rt * 16 + (lane & 15)) * (D * 2);
     int n = 0;
 #pragma unroll 1
@@ -188,7 +197,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
 #pragma unroll 1
                 for (int x = lane; x < (WK - valid) * (D / 8); x += 32) {
                     const int key = k0 + valid + x / (D / 8), c = x % (D / 8);
-                    *reinterpret_cast<uint4 *>(ring + st * L::STAGE + L::STAGE / 2 + (c >> 3) * (KT * 128) + key * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4 *>(ring + st * L::STAGE + L::STAGE / 2 + place(key) + (c >> 3) * half + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -201,14 +210,14 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
                     for (int x = 0; x < XR; ++x) seen[x] = seen_bits(a, s, row[x], first - ctx, valid);
                 }
                 float sc[2 * KS][4] = {}, low[2 * KS][4] = {};
-                const uint32_t kk = k_at + st * L::STAGE, vv = v_at + st * L::STAGE;
+                const uint32_t stage = st * L::STAGE;
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks) {
                     uint32_t q[4], p[4], b[KS][4];
                     ldsm4(q, q_at + (ks >> 2) * 128 + off_v[ks & 3]);
                     if constexpr (TERMS) ldsm4(p, q_at + ROWS * D * 2 + (ks >> 2) * 128 + off_v[ks & 3]);
 #pragma unroll
-                    for (int k = 0; k < KS; ++k) ldsm4(b[k], kk + k * (16 * 128) + (ks >> 2) * (KT * 128) + off_k[ks & 3]);
+                    for (int k = 0; k < KS; ++k) ldsm4(b[k], stage + k_at[k] + (ks >> 2) * half + off_k[ks & 3]);
 #pragma unroll
                     for (int k = 0; k < KS; ++k) {
                         mma<C>(sc[2 * k], q, b[k][0], b[k][1]);
@@ -279,7 +288,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
                 for (int dp = 0; dp < D / 16; ++dp) {
                     uint32_t b[KS][4];
 #pragma unroll
-                    for (int k = 0; k < KS; ++k) ldsm4t(b[k], vv + k * (16 * 128) + (dp >> 2) * (KT * 128) + off_v[dp & 3]);
+                    for (int k = 0; k < KS; ++k) ldsm4t(b[k], stage + v_at[k] + (dp >> 2) * half + off_v[dp & 3]);
                     if constexpr (SPLIT || EIGHT) {
                         float c[2][4] = {};
                         if constexpr (TERMS) {

@@ -161,7 +161,9 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 const bool more = walk.next(s);
                 if (k >= SegmentRing::N) ok = __shfl_sync(0xffffffffu, lane == 0 ? wait(&S.segs.empty[k % SegmentRing::N], (k / SegmentRing::N - 1) & 1) : 0, 0);
                 if (!ok) break;
-                int page = more && s.n_keys > 0 ? page_of_box<D>(a, s, s.t0, lane & 15) : -1;
+                // a box is half of a page's dims (D = 128), so that a tile is halves of [KT][64] in 128-byte swizzled rows
+                const int half = lane % (D / 64), nth = (lane & 15) / (D / 64);
+                int page = more && s.n_keys > 0 ? page_at(a, s, s.t0, nth) : -1;
                 if (lane == 0) {
                     S.segs.s[k % SegmentRing::N] = s;
                     mbar_arrive(&S.segs.full[k % SegmentRing::N]);
@@ -170,7 +172,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 if (s.n_keys <= 0) continue;
 #pragma unroll 1
                 for (int t = s.t0; t < s.t0 + s.nt && ok; ++t) {
-                    const int next = t + 1 < s.t0 + s.nt ? page_of_box<D>(a, s, t + 1, lane & 15) : -1;
+                    const int next = t + 1 < s.t0 + s.nt ? page_at(a, s, t + 1, nth) : -1;
 #pragma unroll 1
                     for (int kv = 0; kv < 2 && ok; ++kv) {
                         const int st = n % L::STAGES;
@@ -178,7 +180,9 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                         if (!ok) break;
                         if (lane == 0) mbar_arrive_expect_tx(&S.full[st], static_cast<uint32_t>((tile_pages(a, s, t) << a.shift) * D * 2));
                         __syncwarp();
-                        if (lane < 16) load_box<D>(a, kv ? &vmap : &kmap, s, page, lane, ring + st * L::STAGE, &S.full[st]);
+                        if (lane < 16 && page >= 0)
+                            tma_box_2d(ring + st * L::STAGE + half * (KT * 128) + (nth << a.shift) * 128, kv ? &vmap : &kmap, half * 64,
+                                       (page * a.n_kv + s.g) << a.shift, &S.full[st]);
                         ++n;
                     }
                     page = next;

@@ -451,10 +451,16 @@ __global__ void __launch_bounds__(COMMIT_THREADS) k_pages_commit(const __grid_co
     }
 }
 
-// A pool as rows of head_dim values; a box is a page of one head, 64 dims wide.
-CUtensorMap pool_map(void * pool, const navi_pages_desc & d) {
-    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(d.head_dim), static_cast<cuuint64_t>(d.n_pages) * d.n_kv_head * d.page_size};
-    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(d.head_dim) * 2};
+// A pool as rows of head_dim values; a box is a page of one head: 64 dims of it, or all, half after half.
+CUtensorMap pool_map(void * pool, const navi_pages_desc & d, bool whole) {
+    const cuuint64_t rows = static_cast<cuuint64_t>(d.n_pages) * d.n_kv_head * d.page_size, halves = static_cast<cuuint64_t>(d.head_dim) / 64;
+    const cuuint64_t row = static_cast<cuuint64_t>(d.head_dim) * 2;
+    if (whole) {
+        const cuuint64_t dims[3] = {64, rows, halves}, strides[2] = {row, 128};
+        const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(d.page_size), static_cast<cuuint32_t>(halves)};
+        return swizzled_map(pool, d.dtype, 3, dims, strides, box);
+    }
+    const cuuint64_t dims[2] = {64 * halves, rows}, strides[1] = {row};
     const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(d.page_size)};
     return swizzled_map(pool, d.dtype, 2, dims, strides, box);
 }
@@ -506,7 +512,10 @@ std::unique_ptr<Pages> Pages::create(const Device & dev, const navi_pages_desc &
     p->d_.k = p->k_.data();
     p->d_.v = p->v_.data();
     for (int l = 0; l < d.n_layer; ++l)
-        for (void * pool : {p->k_[static_cast<size_t>(l)], p->v_[static_cast<size_t>(l)]}) p->maps_.push_back(pool ? pool_map(pool, d) : CUtensorMap{});
+        for (void * pool : {p->k_[static_cast<size_t>(l)], p->v_[static_cast<size_t>(l)]}) {
+            p->maps_.push_back(pool ? pool_map(pool, d, false) : CUtensorMap{});
+            p->page_maps_.push_back(pool ? pool_map(pool, d, true) : CUtensorMap{});
+        }
     if (!given) {
         std::vector<int32_t> ids(static_cast<size_t>(d.n_pages));
         for (int i = 0; i < d.n_pages; ++i) ids[static_cast<size_t>(i)] = d.n_pages - 1 - i;

@@ -41,7 +41,7 @@ private:
     const Device * dev_ = nullptr;
     navi_pages_desc d_{};
     std::vector<void *> k_, v_;     // d_.k and d_.v point here
-    std::vector<CUtensorMap> maps_; // K, V of each layer: rows of head_dim, boxes of a page of one head x 64 dims
+    std::vector<CUtensorMap> maps_, page_maps_;   // K, V of each layer: boxes of a page of one head, 64 dims or all
     std::vector<void *> owned_;
     int shift_ = 0;                 // log2(page_size)
 };
