@@ -71,6 +71,18 @@ template <class T> __device__ __forceinline__ T block_scan(T v, T * red, T & tot
     return base + x - v;
 }
 
+template <class T> __device__ __forceinline__ T warp_scan(T v, T & total) {
+    const int lane = threadIdx.x & 31;
+    T x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const T y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    total = __shfl_sync(0xffffffffu, x, 31);
+    return x - v;
+}
+
 // The last i with a[i] <= e, for a[0] = 0 <= e and a[] not decreasing.
 __device__ __forceinline__ int owner(const int * a, int n, int e) {
     int lo = 0, hi = n;   // a[lo] <= e < a[hi]
@@ -93,67 +105,67 @@ __device__ __forceinline__ int owner(const int * a, int n, int e) {
 __global__ void __launch_bounds__(PLAN_THREADS) k_pages_plan(const __grid_constant__ PlanArgs a) {
     extern __shared__ int plan_smem[];
     __shared__ long long red64[PLAN_THREADS / 32];
-    __shared__ int red[PLAN_THREADS / 32];
     __shared__ int par[2 * PLAN_THREADS];
-    __shared__ int last_block, taken_s;
+    __shared__ int last_block, taken_s, top_s;
     griddep_wait();
     griddep_launch_dependents();
     const int B = a.s.n_req, tid = threadIdx.x, MB = a.max_blocks;
     int * cu = plan_smem, * cg = cu + B + 1, * cs = cg + B, * st = cs + B;
 
-    const int per = (B + PLAN_THREADS - 1) / PLAN_THREADS, i0 = min(B, tid * per), i1 = min(B, i0 + per);
+    // up to 256 requests the first warp does the sums alone, with no barrier until it is done
+    const bool one = B <= 256;
+    const int lanes = one ? 32 : PLAN_THREADS, per = (B + lanes - 1) / lanes, i0 = min(B, tid * per), i1 = min(B, i0 + per);
     const long long cap = a.s.max_rows;
-    long long rows = 0;
-    for (int i = i0; i < i1; ++i) rows += max(a.s.n_new[i], 0);
-    long long total_rows;
-    long long row = block_scan(rows, red64, total_rows);
-    int grow = 0, surplus = 0;
-    for (int i = i0; i < i1; ++i) {
-        const int n = a.s.n_new[i], ctx = a.s.ctx_len[i], tr = a.s.req ? a.s.req[i] : i;
-        cu[i] = static_cast<int>(min(row, cap));
-        row += max(n, 0);
-        int status = NAVI_OK, g = 0, u = 0;
-        if (n < 0 || ctx < 0 || tr < 0 || tr >= a.max_requests) status = NAVI_E_ARG;
-        else {
-            const int held = a.held[tr];
-            const long long need = (static_cast<long long>(ctx) + n + (1 << a.shift) - 1) >> a.shift;
-            if (held < 0 || held > MB) status = NAVI_E_ARG;
-            else if (n > a.s.max_new || need > MB || row > cap) status = NAVI_E_SHAPE;
+    const int F = min(max(*a.n_free, 0), a.n_pages);
+    if (tid == 0) taken_s = top_s = 0;
+    if (!one || tid < 32) {
+        const auto scan = [&](long long x, long long & total) { return one ? warp_scan(x, total) : block_scan(x, red64, total); };
+        long long rows = 0, total;
+        for (int i = i0; i < i1; ++i) rows += max(a.s.n_new[i], 0);
+        long long row = scan(rows, total);
+        if (tid == 0) cu[B] = static_cast<int>(min(total, cap));
+        long long grow = 0, surplus = 0;
+        for (int i = i0; i < i1; ++i) {
+            const int n = a.s.n_new[i], ctx = a.s.ctx_len[i], tr = a.s.req ? a.s.req[i] : i;
+            cu[i] = static_cast<int>(min(row, cap));
+            row += max(n, 0);
+            int status = NAVI_OK, g = 0, u = 0;
+            if (n < 0 || ctx < 0 || tr < 0 || tr >= a.max_requests) status = NAVI_E_ARG;
             else {
-                g = max(static_cast<int>(need) - held, 0);
-                u = max(held - static_cast<int>(need), 0);
+                const int held = a.held[tr];
+                const long long need = (static_cast<long long>(ctx) + n + (1 << a.shift) - 1) >> a.shift;
+                if (held < 0 || held > MB) status = NAVI_E_ARG;
+                else if (n > a.s.max_new || need > MB || row > cap) status = NAVI_E_SHAPE;
+                else {
+                    g = max(static_cast<int>(need) - held, 0);
+                    u = max(held - static_cast<int>(need), 0);
+                }
+            }
+            cg[i] = g;
+            cs[i] = u;
+            st[i] = status;
+            grow += g;
+            surplus += u;
+        }
+        long long all_grow, all_surplus, g = scan(grow, all_grow), u = scan(surplus, all_surplus);
+        const int top = static_cast<int>(min(F + all_surplus, static_cast<long long>(a.n_pages)));
+        int taken = 0;
+        for (int i = i0; i < i1; ++i) {
+            const int gi = cg[i], ui = cs[i];
+            cg[i] = static_cast<int>(min(g, static_cast<long long>(INT_MAX)));
+            cs[i] = static_cast<int>(min(u, static_cast<long long>(INT_MAX)));
+            g += gi;
+            u += ui;
+            if (gi > 0) {
+                if (g <= top) taken = static_cast<int>(g);
+                else st[i] = NAVI_E_KV_FULL;
             }
         }
-        cg[i] = g;
-        cs[i] = u;
-        st[i] = status;
-        grow += g;
-        surplus += u;
+        if (taken > 0) atomicMax(&taken_s, taken);
+        if (tid == 0) top_s = top;
     }
-    if (tid == 0) {
-        cu[B] = static_cast<int>(min(total_rows, cap));
-        taken_s = 0;
-    }
-    int all_grow, all_surplus;
-    int g = block_scan(grow, red, all_grow);
-    int u = block_scan(surplus, red, all_surplus);
-    const int F = min(max(*a.n_free, 0), a.n_pages);
-    const int top = min(F + all_surplus, a.n_pages);
-    int taken = 0;
-    for (int i = i0; i < i1; ++i) {
-        const int gi = cg[i], ui = cs[i];
-        cg[i] = g;
-        cs[i] = u;
-        g += gi;
-        u += ui;
-        if (gi > 0) {
-            if (g <= top) taken = g;
-            else st[i] = NAVI_E_KV_FULL;
-        }
-    }
-    if (taken > 0) atomicMax(&taken_s, taken);
     __syncthreads();
-    taken = taken_s;
+    const int taken = taken_s, top = top_s, all_surplus = top - F;
 
     const auto need_of = [&](int i) { return (a.s.ctx_len[i] + max(a.s.n_new[i], 0) + (1 << a.shift) - 1) >> a.shift; };
     const auto table_row = [&](int i) { return a.table + static_cast<size_t>(a.s.req ? a.s.req[i] : i) * MB; };
@@ -335,37 +347,45 @@ template <class T, class C, int D> __global__ void __launch_bounds__(128) k_page
             sn[x] = e0 < D / 2 ? -row[D / 2 + e0 + x] : row[e0 + x];
         }
     }
-    for (int h0 = part * HPW; h0 < total; h0 += a.parts * HPW) {
-        const int h = h0 + lane / LANES;
-        const bool here = h < total;
-        float x[E];
-        load16<T>(in + static_cast<size_t>(here ? h : 0) * D, x);
-        const bool is_q = h < H, is_v = h >= H + a.n_kv;
-        const float * nw = is_q ? a.q_norm : a.k_norm;
-        float ss = 0.f;
+    constexpr int U = 4;   // heads of a lane whose loads are under way together
+    const int stride = a.parts * HPW;
+    for (int h0 = part * HPW + lane / LANES; h0 - lane / LANES < total; h0 += U * stride) {
+        float x[U][E];
 #pragma unroll
-        for (int c = 0; c < E; ++c) ss += x[c] * x[c];
-#pragma unroll
-        for (int o = 1; o < LANES; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float scale = nw ? rsqrtf(ss / static_cast<float>(D) + a.eps) : 1.f;
-        float y[E];
-#pragma unroll
-        for (int c = 0; c < E; ++c) y[c] = x[c] * scale * (is_q ? qw[c] : kw[c]);
-#pragma unroll
-        for (int c = 0; c < E; ++c) {
-            const float z = __shfl_xor_sync(0xffffffffu, y[c], LANES / 2);
-            y[c] = y[c] * cs[c] + z * sn[c];
+        for (int u = 0; u < U; ++u) {
+            const int h = h0 + u * stride;
+            load16<T>(in + static_cast<size_t>(h < total ? h : 0) * D, x[u]);
         }
-        if (!here) continue;
-        if (is_q) {
-            if (!known) {
 #pragma unroll
-                for (int c = 0; c < E; ++c) y[c] = 0.f;
+        for (int u = 0; u < U; ++u) {
+            const int h = h0 + u * stride;
+            if (h - lane / LANES >= total) break;   // the same for the whole warp
+            const bool is_q = h < H, is_v = h >= H + a.n_kv;
+            float ss = 0.f;
+#pragma unroll
+            for (int c = 0; c < E; ++c) ss += x[u][c] * x[u][c];
+#pragma unroll
+            for (int o = 1; o < LANES; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const float scale = (is_q ? a.q_norm : a.k_norm) ? rsqrtf(ss / static_cast<float>(D) + a.eps) : 1.f;
+            float y[E];
+#pragma unroll
+            for (int c = 0; c < E; ++c) y[c] = x[u][c] * scale * (is_q ? qw[c] : kw[c]);
+#pragma unroll
+            for (int c = 0; c < E; ++c) {
+                const float z = __shfl_xor_sync(0xffffffffu, y[c], LANES / 2);
+                y[c] = y[c] * cs[c] + z * sn[c];
             }
-            store_vec<T, E>(qo + static_cast<size_t>(h) * D, y);
-        } else if (slot >= 0 && page < a.n_pages && known) {
-            C * dst = (is_v ? v : k) + (static_cast<size_t>(h - H - (is_v ? a.n_kv : 0)) << a.shift) * D;
-            store_vec<C, E>(dst, is_v ? x : y);
+            if (h >= total) continue;
+            if (is_q) {
+                if (!known) {
+#pragma unroll
+                    for (int c = 0; c < E; ++c) y[c] = 0.f;
+                }
+                store_vec<T, E>(qo + static_cast<size_t>(h) * D, y);
+            } else if (slot >= 0 && page < a.n_pages && known) {
+                C * dst = (is_v ? v : k) + (static_cast<size_t>(h - H - (is_v ? a.n_kv : 0)) << a.shift) * D;
+                store_vec<C, E>(dst, is_v ? x[u] : y);
+            }
         }
     }
 }
@@ -399,14 +419,26 @@ __global__ void __launch_bounds__(COMMIT_THREADS) k_pages_commit(const __grid_co
     const bool served = a.s.status[i] == NAVI_OK;
     for (int j = tid; j <= n; j += COMMIT_THREADS) child[j] = INT_MAX;
     __syncthreads();
-    for (int j = tid; j < n; j += COMMIT_THREADS) {
-        const int up = a.s.parent[r0 + j];
-        if (!served || up < -1 || up >= j) continue;
-        const int32_t * want = up >= 0 ? a.c.targets + static_cast<size_t>(r0 + up) * W : a.c.root_target + static_cast<size_t>(i) * W;
-        const int32_t * have = a.c.tokens + static_cast<size_t>(r0 + j) * W;
-        bool same = true;
-        for (int x = 0; x < W; ++x) same = same && want[x] == have[x];
-        if (same) atomicMin(&child[up + 1], j);
+    // 4 lanes compare a row's ids, 16 bytes at a time where they are that
+    const bool vec = W % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.c.tokens) | reinterpret_cast<uintptr_t>(a.c.targets) | reinterpret_cast<uintptr_t>(a.c.root_target)) & 15) == 0;
+    for (int x = tid; x < (n + COMMIT_THREADS / 4 - 1) / (COMMIT_THREADS / 4) * COMMIT_THREADS; x += COMMIT_THREADS) {
+        const int j = x >> 2, part = x & 3;
+        const int up = served && j < n ? a.s.parent[r0 + j] : -2;
+        bool same = up >= -1 && up < j;
+        if (same) {
+            const int32_t * want = up >= 0 ? a.c.targets + static_cast<size_t>(r0 + up) * W : a.c.root_target + static_cast<size_t>(i) * W;
+            const int32_t * have = a.c.tokens + static_cast<size_t>(r0 + j) * W;
+            if (vec) {
+                for (int y = part * 4; y < W; y += 16) {
+                    const int4 p = *reinterpret_cast<const int4 *>(want + y), q = *reinterpret_cast<const int4 *>(have + y);
+                    same = same && p.x == q.x && p.y == q.y && p.z == q.z && p.w == q.w;
+                }
+            } else {
+                for (int y = part; y < W; y += 4) same = same && want[y] == have[y];
+            }
+        }
+        const unsigned all = __ballot_sync(0xffffffffu, same);
+        if (part == 0 && (all >> (tid & 31) & 15) == 15) atomicMin(&child[up + 1], j);
     }
     __syncthreads();
     if (tid == 0) {
@@ -446,8 +478,16 @@ __global__ void __launch_bounds__(COMMIT_THREADS) k_pages_commit(const __grid_co
     for (int x = blockIdx.y * COMMIT_THREADS + tid; x < items; x += gridDim.y * COMMIT_THREADS) {
         const int l = x / (2 * per), y = x % (2 * per), kv = y / per, z = y % per, h = z / a.chunks, c = z % a.chunks;
         uint4 * pool = reinterpret_cast<uint4 *>(kv ? a.v[l] : a.k[l]) + (static_cast<size_t>(h) << a.shift) * a.chunks + c;
-        for (int k = k0; k < k1; ++k)
-            if (from[k] >= 0 && to[k] >= 0) pool[to[k]] = pool[from[k]];
+        // places are written behind the ones that are read, so four reads go ahead of their writes
+        for (int k = k0; k < k1; k += 4) {
+            uint4 v[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+                if (k + y < k1 && from[k + y] >= 0) v[y] = pool[from[k + y]];
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+                if (k + y < k1 && from[k + y] >= 0 && to[k + y] >= 0) pool[to[k + y]] = v[y];
+        }
     }
 }
 
