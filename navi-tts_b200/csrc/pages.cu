@@ -71,18 +71,6 @@ template <class T> __device__ __forceinline__ T block_scan(T v, T * red, T & tot
     return base + x - v;
 }
 
-template <class T> __device__ __forceinline__ T warp_scan(T v, T & total) {
-    const int lane = threadIdx.x & 31;
-    T x = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const T y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-    }
-    total = __shfl_sync(0xffffffffu, x, 31);
-    return x - v;
-}
-
 // The last i with a[i] <= e, for a[0] = 0 <= e and a[] not decreasing.
 __device__ __forceinline__ int owner(const int * a, int n, int e) {
     int lo = 0, hi = n;   // a[lo] <= e < a[hi]
@@ -106,49 +94,70 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_pages_plan(const __grid_consta
     extern __shared__ int plan_smem[];
     __shared__ long long red64[PLAN_THREADS / 32];
     __shared__ int par[2 * PLAN_THREADS];
-    __shared__ int last_block, taken_s, top_s;
+    __shared__ int last_block, taken_s;
     griddep_wait();
     griddep_launch_dependents();
     const int B = a.s.n_req, tid = threadIdx.x, MB = a.max_blocks;
     int * cu = plan_smem, * cg = cu + B + 1, * cs = cg + B, * st = cs + B;
 
-    // up to 256 requests the first warp does the sums alone, with no barrier until it is done
-    const bool one = B <= 256;
-    const int lanes = one ? 32 : PLAN_THREADS, per = (B + lanes - 1) / lanes, i0 = min(B, tid * per), i1 = min(B, i0 + per);
+    const int per = (B + PLAN_THREADS - 1) / PLAN_THREADS, i0 = min(B, tid * per), i1 = min(B, i0 + per);
     const long long cap = a.s.max_rows;
+    // what is read of the thread's first four requests (all of them, up to 1024), and the parents of the block's first
+    // rows and of as many before them, is asked for at once
+    constexpr int R = 4;
+    int n_r[R], ctx_r[R], tr_r[R], held_r[R], par1[2] = {-1, -1};
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        const int i = i0 + k;
+        n_r[k] = i < i1 ? a.s.n_new[i] : 0;
+        ctx_r[k] = i < i1 ? a.s.ctx_len[i] : 0;
+        tr_r[k] = i < i1 ? a.s.req ? a.s.req[i] : i : -1;
+    }
+    const int block_row = blockIdx.x * PLAN_THREADS;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int r = block_row - PLAN_THREADS + k * PLAN_THREADS + tid;
+        if (a.s.parent && r >= 0 && r < a.s.max_rows) par1[k] = a.s.parent[r];
+    }
     const int F = min(max(*a.n_free, 0), a.n_pages);
-    if (tid == 0) taken_s = top_s = 0;
-    if (!one || tid < 32) {
-        const auto scan = [&](long long x, long long & total) { return one ? warp_scan(x, total) : block_scan(x, red64, total); };
+#pragma unroll
+    for (int k = 0; k < R; ++k) held_r[k] = tr_r[k] >= 0 && tr_r[k] < a.max_requests ? a.held[tr_r[k]] : -1;
+    if (tid == 0) taken_s = 0;
+    int top;
+    {
         long long rows = 0, total;
-        for (int i = i0; i < i1; ++i) rows += max(a.s.n_new[i], 0);
-        long long row = scan(rows, total);
+#pragma unroll
+        for (int k = 0; k < R; ++k) rows += max(n_r[k], 0);
+        for (int i = i0 + R; i < i1; ++i) rows += max(a.s.n_new[i], 0);
+        long long row = block_scan(rows, red64, total);
         if (tid == 0) cu[B] = static_cast<int>(min(total, cap));
         long long grow = 0, surplus = 0;
-        for (int i = i0; i < i1; ++i) {
-            const int n = a.s.n_new[i], ctx = a.s.ctx_len[i], tr = a.s.req ? a.s.req[i] : i;
+        const auto sort = [&](int i, int n, int ctx, int tr, int held) {
             cu[i] = static_cast<int>(min(row, cap));
             row += max(n, 0);
             int status = NAVI_OK, g = 0, u = 0;
-            if (n < 0 || ctx < 0 || tr < 0 || tr >= a.max_requests) status = NAVI_E_ARG;
+            const long long need = (static_cast<long long>(max(ctx, 0)) + max(n, 0) + (1 << a.shift) - 1) >> a.shift;
+            if (n < 0 || ctx < 0 || tr < 0 || tr >= a.max_requests || held < 0 || held > MB) status = NAVI_E_ARG;
+            else if (n > a.s.max_new || need > MB || row > cap) status = NAVI_E_SHAPE;
             else {
-                const int held = a.held[tr];
-                const long long need = (static_cast<long long>(ctx) + n + (1 << a.shift) - 1) >> a.shift;
-                if (held < 0 || held > MB) status = NAVI_E_ARG;
-                else if (n > a.s.max_new || need > MB || row > cap) status = NAVI_E_SHAPE;
-                else {
-                    g = max(static_cast<int>(need) - held, 0);
-                    u = max(held - static_cast<int>(need), 0);
-                }
+                g = max(static_cast<int>(need) - held, 0);
+                u = max(held - static_cast<int>(need), 0);
             }
             cg[i] = g;
             cs[i] = u;
             st[i] = status;
             grow += g;
             surplus += u;
+        };
+#pragma unroll
+        for (int k = 0; k < R; ++k)
+            if (i0 + k < i1) sort(i0 + k, n_r[k], ctx_r[k], tr_r[k], held_r[k]);
+        for (int i = i0 + R; i < i1; ++i) {
+            const int tr = a.s.req ? a.s.req[i] : i;
+            sort(i, a.s.n_new[i], a.s.ctx_len[i], tr, tr >= 0 && tr < a.max_requests ? a.held[tr] : -1);
         }
-        long long all_grow, all_surplus, g = scan(grow, all_grow), u = scan(surplus, all_surplus);
-        const int top = static_cast<int>(min(F + all_surplus, static_cast<long long>(a.n_pages)));
+        long long all_grow, all_surplus, g = block_scan(grow, red64, all_grow), u = block_scan(surplus, red64, all_surplus);
+        top = static_cast<int>(min(F + all_surplus, static_cast<long long>(a.n_pages)));
         int taken = 0;
         for (int i = i0; i < i1; ++i) {
             const int gi = cg[i], ui = cs[i];
@@ -162,10 +171,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_pages_plan(const __grid_consta
             }
         }
         if (taken > 0) atomicMax(&taken_s, taken);
-        if (tid == 0) top_s = top;
     }
     __syncthreads();
-    const int taken = taken_s, top = top_s, all_surplus = top - F;
+    const int taken = taken_s, all_surplus = top - F;
 
     const auto need_of = [&](int i) { return (a.s.ctx_len[i] + max(a.s.n_new[i], 0) + (1 << a.shift) - 1) >> a.shift; };
     const auto table_row = [&](int i) { return a.table + static_cast<size_t>(a.s.req ? a.s.req[i] : i) * MB; };
@@ -194,11 +202,14 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_pages_plan(const __grid_consta
     const int n_rows = cu[B];
     for (int r0 = blockIdx.x * PLAN_THREADS; r0 < n_rows; r0 += step) {
         const int r = r0 + tid;
-        int base = 0;
-        if (a.s.parent) {   // the parents of these rows and of the rows before them in the first one's request
-            base = max(cu[owner(cu, B, r0)], r0 - PLAN_THREADS);
+        const int base = r0 - PLAN_THREADS;
+        if (a.s.parent) {   // the parents of these rows, and of the 256 before them: a tree's first row is among those
             __syncthreads();
-            for (int k = base + tid; k < min(r0 + PLAN_THREADS, n_rows); k += PLAN_THREADS) par[k - base] = a.s.parent[k];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int at = base + k * PLAN_THREADS + tid;
+                par[k * PLAN_THREADS + tid] = r0 == block_row ? par1[k] : at >= 0 && at < n_rows ? a.s.parent[at] : -1;
+            }
             __syncthreads();
         }
         if (r >= n_rows) continue;
@@ -206,25 +217,38 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_pages_plan(const __grid_consta
         int depth = j;
         bool whole = true;
         if (a.s.parent) {
-            uint64_t m[NAVI_STEP_MAX_TREE / 64] = {};
+            const int at0 = cu[i] - base;              // the request's first row among the staged ones; below 0: too many rows, refused
+            whole = at0 >= 0;
+            int at = whole ? j : -1;
             depth = -1;
-            int at = j;
-            while (at >= 0) {
-                ++depth;
+            if (a.s.mask_words == 1) {                 // the usual tree: one word
+                uint64_t m = 0;
+                while (at >= 0) {
+                    ++depth;
+                    m |= 1ull << (at & 63);
+                    const int up = par[at0 + at];
+                    whole = up >= -1 && up < at;
+                    at = whole ? up : -1;
+                }
+                a.s.mask[r] = whole ? m : 0;
+            } else {
+                uint64_t m[NAVI_STEP_MAX_TREE / 64] = {};
+                while (at >= 0) {
+                    ++depth;
 #pragma unroll
-                for (int w = 0; w < NAVI_STEP_MAX_TREE / 64; ++w)
-                    if ((at >> 6) == w) m[w] |= 1ull << (at & 63);
-                const int k = cu[i] + at - base;
-                const int up = k >= 0 ? par[k] : at;   // a request refused for its length may begin before the staged rows
-                whole = up >= -1 && up < at;
-                at = whole ? up : -1;
-            }
-            for (int w = 0; w < a.s.mask_words; ++w) {
-                uint64_t v = 0;
+                    for (int w = 0; w < NAVI_STEP_MAX_TREE / 64; ++w)
+                        if ((at >> 6) == w) m[w] |= 1ull << (at & 63);
+                    const int up = par[at0 + at];
+                    whole = up >= -1 && up < at;
+                    at = whole ? up : -1;
+                }
+                for (int w = 0; w < a.s.mask_words; ++w) {
+                    uint64_t v = 0;
 #pragma unroll
-                for (int x = 0; x < NAVI_STEP_MAX_TREE / 64; ++x)
-                    if (x == w) v = m[x];
-                a.s.mask[static_cast<size_t>(r) * a.s.mask_words + w] = whole ? v : 0;
+                    for (int x = 0; x < NAVI_STEP_MAX_TREE / 64; ++x)
+                        if (x == w) v = m[x];
+                    a.s.mask[static_cast<size_t>(r) * a.s.mask_words + w] = whole ? v : 0;
+                }
             }
         }
         int64_t slot = -1;
@@ -240,12 +264,14 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_pages_plan(const __grid_consta
     }
 
     if (nb > 1) {
-        __threadfence();
         __syncthreads();
-        if (tid == 0) last_block = atomicAdd(a.ticket, 1) == nb - 1;
+        if (tid == 0) {
+            __threadfence();
+            last_block = atomicAdd(a.ticket, 1) == nb - 1;
+            __threadfence();
+        }
         __syncthreads();
         if (!last_block) return;
-        __threadfence();
     } else {
         __syncthreads();
     }
@@ -655,7 +681,7 @@ void Pages::commit(const navi_step & s, const navi_commit_args & c, cudaStream_t
     const int64_t items = static_cast<int64_t>(d_.n_layer) * 2 * d_.n_kv_head * a.chunks;
     if (items > INT32_MAX / 2) fail("pages commit: too many heads", NAVI_E_SHAPE);
     const int most = static_cast<int>((items + COMMIT_THREADS - 1) / COMMIT_THREADS);
-    const int z = std::clamp(4 * dev_->info().multiprocessors / s.n_req, 1, std::min(most, 65535));
+    const int z = std::clamp(8 * dev_->info().multiprocessors / s.n_req, 1, std::min(most, 65535));
     NAVI_CUDA(launch_pdl(k_pages_commit, dim3(static_cast<unsigned>(s.n_req), static_cast<unsigned>(z)), dim3(COMMIT_THREADS), 0, stream, a));
 }
 
