@@ -12,6 +12,7 @@
 #include <climits>
 #include <cstring>
 #include <string>
+#include <type_traits>
 
 namespace navi {
 
@@ -304,113 +305,138 @@ struct StoreArgs {
     int n_req, max_rows, n_head, n_kv, shift, n_pages, rope_positions, parts;
 };
 
-template <class T> __device__ __forceinline__ void load16(const T * p, float * v);
-template <> __device__ __forceinline__ void load16<float>(const float * p, float * v) {
-    const float4 x = *reinterpret_cast<const float4 *>(p);
-    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-}
-template <> __device__ __forceinline__ void load16<__half>(const __half * p, float * v) {
-    const uint4 x = *reinterpret_cast<const uint4 *>(p);
-    const __half2 * h = reinterpret_cast<const __half2 *>(&x);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) { const float2 f = __half22float2(h[k]); v[2 * k] = f.x; v[2 * k + 1] = f.y; }
-}
-template <> __device__ __forceinline__ void load16<__nv_bfloat16>(const __nv_bfloat16 * p, float * v) {
-    const uint4 x = *reinterpret_cast<const uint4 *>(p);
-    const __nv_bfloat162 * h = reinterpret_cast<const __nv_bfloat162 *>(&x);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) { const float2 f = __bfloat1622float2(h[k]); v[2 * k] = f.x; v[2 * k + 1] = f.y; }
-}
-template <class T> __device__ __forceinline__ uint32_t pack2(float a, float b);
-template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-// E values (4 or 8) rounded to T and written with one store
-template <class T, int E> __device__ __forceinline__ void store_vec(T * p, const float * v) {
-    if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    } else if constexpr (E == 4) {
-        *reinterpret_cast<uint2 *>(p) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+// 8 bytes of T as pairs of floats (one pair of f32, two of 16-bit values), and back
+template <class T> __device__ __forceinline__ void load8(const T * p, float2 * v) {
+    const uint2 x = *reinterpret_cast<const uint2 *>(p);
+    if constexpr (std::is_same_v<T, float>) {
+        v[0] = make_float2(__uint_as_float(x.x), __uint_as_float(x.y));
+    } else if constexpr (std::is_same_v<T, __half>) {
+        v[0] = __half22float2(*reinterpret_cast<const __half2 *>(&x.x));
+        v[1] = __half22float2(*reinterpret_cast<const __half2 *>(&x.y));
     } else {
-        *reinterpret_cast<uint4 *>(p) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+        v[0] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&x.x));
+        v[1] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&x.y));
     }
 }
+template <class T> __device__ __forceinline__ uint32_t pack2(float2 v) {
+    if constexpr (std::is_same_v<T, __half>) {
+        const __half2 h = __float22half2_rn(v);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __float22bfloat162_rn(v);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+template <class T, int N> __device__ __forceinline__ void store_pairs(T * p, const float2 * v) {
+    if constexpr (std::is_same_v<T, float>) *reinterpret_cast<float2 *>(p) = v[0];
+    else if constexpr (N == 1) *reinterpret_cast<uint32_t *>(p) = pack2<T>(v[0]);
+    else *reinterpret_cast<uint2 *>(p) = make_uint2(pack2<T>(v[0]), pack2<T>(v[1]));
+}
 
-// A warp takes a share (1 / parts) of one row's heads. A lane holds 16 bytes of the input, so a
-// head is D * sizeof(T) / 16 lanes and a warp reads 512 bytes at a time; the RoPE partner of
-// element i is i + D / 2, half a head's lanes away.
+// A warp takes a share (1 / parts) of one row's heads. A lane holds 8 bytes of a head's first half and the
+// 8 bytes that RoPE pairs them with in the second, so a head is D * sizeof(T) / 16 lanes, a warp reads 512
+// bytes at a time and the rotation needs no exchange between lanes; only the sum of squares does. With the
+// norm's weights in the coefficients, fixed for the row,
+//   y0 = s (x0 (w0 c) - x1 (w1 sin)),  y1 = s (x0 (w0 sin) + x1 (w1 c)),  s = rsqrt(mean x^2 + eps).
+// What bounds it is instructions, then HBM.
 template <class T, class C, int D> __global__ void __launch_bounds__(128) k_pages_store(const __grid_constant__ StoreArgs a) {
-    constexpr int E = 16 / sizeof(T), LANES = D / E, HPW = 32 / LANES;   // elements a lane, lanes a head, heads a warp
     griddep_wait();
     griddep_launch_dependents();
+    constexpr int N = 4 / sizeof(T), LANES = D / (4 * N), HPW = 32 / LANES;   // pairs of floats in 8 bytes, lanes a head, heads a warp
     const int w = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
     const int r = w / a.parts, part = w % a.parts;
     if (r >= a.max_rows || r >= a.cu_rows[a.n_req]) return;
-    const int sub = lane % LANES, e0 = sub * E, H = a.n_head, total = H + 2 * a.n_kv;
-    const int64_t slot = a.slot[r];
-    const int pos = a.pos[r];
-    const bool known = !a.rope || (pos >= 0 && pos < a.rope_positions);
-    const T * in = static_cast<const T *>(a.qkv) + r * a.in_stride + e0;
-    T * qo = static_cast<T *>(a.q_out) + r * a.out_stride + e0;
-    const int64_t page = slot >> a.shift, off = slot & ((1 << a.shift) - 1);
-    const size_t at = ((static_cast<size_t>(page) * a.n_kv << a.shift) + off) * D + e0;   // head 0 of the token
-    C * k = reinterpret_cast<C *>(a.k) + at, * v = reinterpret_cast<C *>(a.v) + at;
-    float qw[E], kw[E], cs[E], sn[E];
-#pragma unroll
-    for (int x = 0; x < E; ++x) { qw[x] = kw[x] = cs[x] = 1.f; sn[x] = 0.f; }
-#pragma unroll
-    for (int x = 0; x < E; ++x) {
-        if (a.q_norm) qw[x] = a.q_norm[e0 + x];
-        if (a.k_norm) kw[x] = a.k_norm[e0 + x];
-        if (a.rope && known) {
-            const float * row = a.rope + static_cast<size_t>(pos) * D;
-            cs[x] = row[(e0 + x) % (D / 2)];
-            sn[x] = e0 < D / 2 ? -row[D / 2 + e0 + x] : row[e0 + x];
-        }
-    }
+    const int e0 = lane % LANES * (2 * N), H = a.n_head, total = H + 2 * a.n_kv;
+    // the first heads are asked for before what the row's place and position lead to
     constexpr int U = 4;   // heads of a lane whose loads are under way together
-    const int stride = a.parts * HPW;
-    for (int h0 = part * HPW + lane / LANES; h0 - lane / LANES < total; h0 += U * stride) {
-        float x[U][E];
+    const int stride = a.parts * HPW, first = part * HPW + lane / LANES;
+    const T * in = static_cast<const T *>(a.qkv) + r * a.in_stride + e0;
+    float2 x0[U][N], x1[U][N];
+    const auto load = [&](int h0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int h = h0 + u * stride;
-            load16<T>(in + static_cast<size_t>(h < total ? h : 0) * D, x[u]);
+            const T * src = in + static_cast<size_t>(h < total ? h : 0) * D;
+            load8<T>(src, x0[u]);
+            load8<T>(src + D / 2, x1[u]);
         }
+    };
+    load(first);
+    const int64_t slot = a.slot[r];
+    const int pos = a.pos[r];
+    const bool known = !a.rope || (pos >= 0 && pos < a.rope_positions);
+    T * qo = static_cast<T *>(a.q_out) + r * a.out_stride + e0;
+    const int64_t page = slot >> a.shift, off = slot & ((1 << a.shift) - 1);
+    const bool stored = slot >= 0 && page < a.n_pages && known;
+    const size_t at = ((static_cast<size_t>(page) * a.n_kv << a.shift) + off) * D + e0;   // head 0 of the token
+    C * k = reinterpret_cast<C *>(a.k) + at, * v = reinterpret_cast<C *>(a.v) + at;
+    // [q or k][x0 -> y0, x1 -> y0, x0 -> y1, x1 -> y1]
+    float2 co[2][4][N];
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+        float2 c = make_float2(1.f, 1.f), s = make_float2(0.f, 0.f);
+        if (a.rope && known) {
+            const float * row = a.rope + static_cast<size_t>(pos) * D + e0 + 2 * x;
+            c = make_float2(row[0], row[1]);
+            s = make_float2(row[D / 2], row[D / 2 + 1]);
+        }
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const float * nw = g ? a.k_norm : a.q_norm;
+            float2 w0 = make_float2(1.f, 1.f), w1 = w0;
+            if (nw) {
+                nw += e0 + 2 * x;
+                w0 = make_float2(nw[0], nw[1]);
+                w1 = make_float2(nw[D / 2], nw[D / 2 + 1]);
+            }
+            co[g][0][x] = __fmul2_rn(w0, c);
+            co[g][1][x] = __fmul2_rn(w1, make_float2(-s.x, -s.y));
+            co[g][2][x] = __fmul2_rn(w0, s);
+            co[g][3][x] = __fmul2_rn(w1, c);
+        }
+    }
+    for (int h0 = first; h0 - lane / LANES < total; h0 += U * stride) {
+        if (h0 != first) load(h0);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int h = h0 + u * stride;
             if (h - lane / LANES >= total) break;   // the same for the whole warp
             const bool is_q = h < H, is_v = h >= H + a.n_kv;
-            float ss = 0.f;
+            float2 y0[N], y1[N];
+            if (!__all_sync(0xffffffffu, is_v)) {
+                float scale = 1.f;
+                if (a.q_norm || a.k_norm) {
+                    float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int c = 0; c < E; ++c) ss += x[u][c] * x[u][c];
+                    for (int x = 0; x < N; ++x) ss = __ffma2_rn(x0[u][x], x0[u][x], __ffma2_rn(x1[u][x], x1[u][x], ss));
+                    float sum = ss.x + ss.y;
 #pragma unroll
-            for (int o = 1; o < LANES; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const float scale = (is_q ? a.q_norm : a.k_norm) ? rsqrtf(ss / static_cast<float>(D) + a.eps) : 1.f;
-            float y[E];
+                    for (int o = 1; o < LANES; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    if (is_q ? a.q_norm : a.k_norm) scale = rsqrtf(sum * (1.f / D) + a.eps);
+                }
+                const float2 s2 = make_float2(scale, scale);
 #pragma unroll
-            for (int c = 0; c < E; ++c) y[c] = x[u][c] * scale * (is_q ? qw[c] : kw[c]);
+                for (int x = 0; x < N; ++x) {
+                    float2 m[4];
 #pragma unroll
-            for (int c = 0; c < E; ++c) {
-                const float z = __shfl_xor_sync(0xffffffffu, y[c], LANES / 2);
-                y[c] = y[c] * cs[c] + z * sn[c];
+                    for (int y = 0; y < 4; ++y) m[y] = is_q ? co[0][y][x] : co[1][y][x];
+                    y0[x] = __fmul2_rn(s2, __ffma2_rn(x0[u][x], m[0], __fmul2_rn(x1[u][x], m[1])));
+                    y1[x] = __fmul2_rn(s2, __ffma2_rn(x0[u][x], m[2], __fmul2_rn(x1[u][x], m[3])));
+                }
             }
             if (h >= total) continue;
             if (is_q) {
                 if (!known) {
 #pragma unroll
-                    for (int c = 0; c < E; ++c) y[c] = 0.f;
+                    for (int x = 0; x < N; ++x) y0[x] = y1[x] = make_float2(0.f, 0.f);
                 }
-                store_vec<T, E>(qo + static_cast<size_t>(h) * D, y);
-            } else if (slot >= 0 && page < a.n_pages && known) {
+                T * dst = qo + static_cast<size_t>(h) * D;
+                store_pairs<T, N>(dst, y0);
+                store_pairs<T, N>(dst + D / 2, y1);
+            } else if (stored) {
                 C * dst = (is_v ? v : k) + (static_cast<size_t>(h - H - (is_v ? a.n_kv : 0)) << a.shift) * D;
-                store_vec<C, E>(dst, is_v ? x[u] : y);
+                store_pairs<C, N>(dst, is_v ? x0[u] : y0);
+                store_pairs<C, N>(dst + D / 2, is_v ? x1[u] : y1);
             }
         }
     }
