@@ -490,6 +490,17 @@ int navi_pages_commit(navi_pages * p, const navi_step * s, const navi_commit_arg
  * no call hangs the device. */
 int navi_pages_check(navi_pages * p, void * stream);
 
+/* One step of many requests through the talker over a paged cache: navi_pages_plan of s, then
+ * the rows d_rows (device [s->max_rows][hidden], the input embeddings of each request's drafted
+ * frames, single frame or prompt rows) through every layer at their positions, each attending its
+ * request's tokens and its ancestors; d_hidden [s->max_rows][hidden] gets the post-norm hidden
+ * rows and d_logits [s->max_rows][vocab] (or NULL) their codec logits. The rows of the batch share one pass over
+ * the weights, which is what a drafted step saves. navi_pages_commit then keeps the branch that
+ * agrees. The cache is f16 with the talker's layers, KV heads and head_dim; s->max_rows <=
+ * max_prompt_tokens; a row past the talker's max_positions is not stored. Runs on the engine's
+ * stream and waits for it. navi_talker_last_ms gives the device time. */
+int navi_talker_step(navi_talker * t, navi_pages * p, const navi_step * s, const float * d_rows, float * d_hidden, float * d_logits);
+
 /* Inspection of the last frame (host copies): the talker's post-norm hidden [hidden],
  * its codec logits [talker vocab], and the 15 code-predictor logit rows [15][cp vocab].
  * Any pointer may be NULL. The reference keeps these in its Work buffers (frame.hip:51-70). */

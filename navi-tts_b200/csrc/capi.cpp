@@ -800,6 +800,14 @@ int navi_pages_check(navi_pages * p, void * stream) {
     });
 }
 
+int navi_talker_step(navi_talker * t, navi_pages * p, const navi_step * s, const float * d_rows, float * d_hidden, float * d_logits) {
+    return guard([&]() -> int {
+        if (!t || !p || !s) return set_err(NAVI_E_ARG, "NULL argument");
+        t->t->step(*p->p, *s, d_rows, d_hidden, d_logits);
+        return NAVI_OK;
+    });
+}
+
 int navi_conv1d(navi_device * dev, const navi_conv_args * a) {
     return guard([&]() -> int {
         if (!dev || !a || !a->w || !a->x || !a->y) return set_err(NAVI_E_ARG, "NULL argument");

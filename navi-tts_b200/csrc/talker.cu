@@ -393,6 +393,8 @@ struct Talker::Impl {
     std::vector<std::pair<int, cudaGraphExec_t>> graphs;
     std::vector<int> uncapturable;
     void enqueue_prefill(int T);
+    void finish_layer(int l, int T);
+    void check_waits();
     void capture_prefill(int T);
 
     static conv::Conv gemm_desc(const __half * W, const float * bias, int xs, int M, int K, int N, int ys, int epi, bool gate) {
@@ -614,15 +616,109 @@ void Talker::prefill(const Prompt & pr) {
     float ms = 0.f;
     NAVI_CUDA(cudaEventElapsedTime(&ms, I.ev0, I.ev1));
     I.last_ms = ms;
-    int err = 0;
-    NAVI_CUDA(cudaMemcpy(&err, I.ws.err, sizeof(int), cudaMemcpyDeviceToHost));
-    if (err) {
-        NAVI_CUDA(cudaMemset(I.ws.err, 0, sizeof(int)));
-        if (err == conv::ERR_ALIGN) fail("talker: a tensor-core GEMM's weight ring is misaligned for swizzled tiles", NAVI_E_SHAPE);
-        fail("talker: a tensor-core GEMM wait passed its deadline", NAVI_E_TIMEOUT);
-    }
+    I.check_waits();
     I.kv.n_used = T;
     if (!ge) I.capture_prefill(T);
+}
+
+// Throws when a GEMM of this talker gave up a wait (the stream is idle).
+void Talker::Impl::check_waits() {
+    int err = 0;
+    NAVI_CUDA(cudaMemcpy(&err, ws.err, sizeof(int), cudaMemcpyDeviceToHost));
+    if (!err) return;
+    NAVI_CUDA(cudaMemset(ws.err, 0, sizeof(int)));
+    if (err == conv::ERR_ALIGN) fail("talker: a tensor-core GEMM's weight ring is misaligned for swizzled tiles", NAVI_E_SHAPE);
+    fail("talker: a tensor-core GEMM wait passed its deadline", NAVI_E_TIMEOUT);
+}
+
+void Talker::step(const Pages & pages, const navi_step & s, const float * rows, float * hidden, float * logits) {
+    Impl & I = *impl_;
+    NAVI_CUDA(cudaSetDevice(I.ordinal));
+    const auto & tp = I.p.talker;
+    const navi_pages_desc & d = pages.desc();
+    if (d.n_layer != tp.n_layer || d.n_kv_head != I.NKV || d.head_dim != tp.head_dim || d.dtype != NAVI_F16)
+        fail("talker: the paged cache's layers, KV heads, head_dim or type are not the talker's", NAVI_E_SHAPE);
+    const int T = s.max_rows, H = I.H;
+    if (T > I.max_prompt) fail("talker: more rows than max_prompt_tokens", NAVI_E_ARG);
+    if (s.n_req > 0 && T > 0 && (!rows || !hidden)) fail("talker: NULL rows", NAVI_E_ARG);
+    pages.plan(s, I.stream);
+    if (s.n_req == 0 || T == 0) return;
+    NAVI_CUDA(cudaEventRecord(I.ev0, I.stream));
+    NAVI_CUDA(cudaMemcpyAsync(I.x, rows, static_cast<size_t>(T) * H * sizeof(float), cudaMemcpyDeviceToDevice, I.stream));
+    navi_store_args st{};
+    st.qkv = I.qkv;
+    st.q_out = I.qkv;
+    st.q_out_stride = I.QKV;
+    st.dtype = NAVI_F32;
+    st.n_head = I.NH;
+    st.eps = tp.rms_eps;
+    st.rope = I.rope;
+    st.rope_positions = I.kv.max_pos;
+    navi_attend_args at{};
+    at.q = I.qkv;
+    at.q_stride = I.QKV;
+    at.out = I.att;
+    at.dtype = NAVI_F32;
+    at.n_head = I.NH;
+    at.scale = 1.f / std::sqrt(static_cast<float>(tp.head_dim));
+    NAVI_CUDA(navi::dev::launch_pdl(k_rmsnorm, dim3(T), dim3(256), 0, I.stream, I.x, I.layers[0].ln1, H, tp.rms_eps, I.n));
+    for (int l = 0; l < tp.n_layer; ++l) {
+        const Layer & ly = I.layers[static_cast<size_t>(l)];
+        I.gemm(ly.wqkv, nullptr, I.n, H, T, H, I.QKV, I.qkv, I.QKV, EPI_NONE);
+        st.q_norm = ly.qn;
+        st.k_norm = ly.kn;
+        pages.store(s, l, st, I.stream);
+        pages.attend(s, l, at, I.stream);
+        I.finish_layer(l, T);
+    }
+    NAVI_CUDA(navi::dev::launch_pdl(k_rmsnorm, dim3(T), dim3(256), 0, I.stream, I.x, I.final_norm, H, tp.rms_eps, hidden));
+    if (logits) I.gemm(I.head, nullptr, hidden, H, T, H, I.TV, logits, I.TV, EPI_NONE);
+    NAVI_CUDA(cudaEventRecord(I.ev1, I.stream));
+    NAVI_CUDA(cudaEventSynchronize(I.ev1));
+    float ms = 0.f;
+    NAVI_CUDA(cudaEventElapsedTime(&ms, I.ev0, I.ev1));
+    I.last_ms = ms;
+    I.check_waits();
+    pages.check(I.stream);
+}
+
+// What follows attention in layer l, over the T rows in x and att: O, the norms, the MLP, and the next
+// layer's input norm.
+void Talker::Impl::finish_layer(int l, int T) {
+    Impl & I = *this;
+    const auto & tp = I.p.talker;
+    const int H = I.H;
+    const Layer & ly = I.layers[static_cast<size_t>(l)];
+    // the RMSNorms after the O projection and (but for the last layer) after the down
+    // projection are written by those GEMMs' launches
+    I.gemm(ly.wo, nullptr, I.att, I.Q, T, I.Q, H, I.x, H, EPI_RESIDUAL, false, I.x, ly.ln2, I.n);
+    // gate/up: a launch that splits K in two leaves both partial slices, and the down
+    // projection's staging adds them (one reduction launch fewer per layer)
+    const bool fold = T <= GU_FOLD_ROWS && conv::plan(gemm_desc(ly.wgu, nullptr, H, T, H, 2 * I.F, 2 * I.F, EPI_NONE, false), sms).splits == 2;
+    if (fold) {
+        conv::Conv c = gemm_desc(ly.wgu, nullptr, H, T, H, 2 * I.F, 2 * I.F, EPI_NONE, false);
+        c.x = I.n;
+        c.y = I.gu;
+        c.defer_reduce = true;
+        if (conv::launch(c, ws_gu, sms, stream) != 2) fail("talker: the gate/up projection did not split in two", NAVI_E_SHAPE);
+    } else {
+        I.gemm(ly.wgu, nullptr, I.n, H, T, H, 2 * I.F, I.gu, 2 * I.F, EPI_NONE);
+    }
+    const bool last = l + 1 == tp.n_layer;
+    {
+        conv::Conv c = gemm_desc(ly.wd, nullptr, 2 * I.F, T, I.F, H, H, EPI_RESIDUAL, true);
+        c.x = fold ? ws_gu.partial : I.gu;
+        if (fold) {
+            c.x_slices = 2;
+            c.x_slice_stride = static_cast<std::size_t>(T) * 2 * I.F;
+        }
+        c.y = I.x;
+        c.resid = I.x;
+        c.norm_w = last ? nullptr : I.layers[static_cast<size_t>(l + 1)].ln1;
+        c.norm_out = last ? nullptr : I.n;
+        c.norm_eps = tp.rms_eps;
+        conv::launch(c, ws, sms, stream);
+    }
 }
 
 // The 28 layers and the codec head over the T rows in x (the layer loop of prefill).
@@ -642,36 +738,7 @@ void Talker::Impl::enqueue_prefill(int T) {
                                         I.QKV, ly.qn, ly.kn, I.NH, I.NKV, tp.rms_eps, I.rope, 0, kc, vc));
         NAVI_CUDA(navi::dev::launch_pdl(k_prefill_attn_mma, dim3((T + PA_QT - 1) / PA_QT, I.NH), dim3(PA_THREADS), PA_SMEM, I.stream, I.qkv,
                                         I.QKV, kc, vc, T, I.NH, I.NKV, 0, I.att));
-        // the RMSNorms after the O projection and (but for the last layer) after the down
-        // projection are written by those GEMMs' launches
-        I.gemm(ly.wo, nullptr, I.att, I.Q, T, I.Q, H, I.x, H, EPI_RESIDUAL, false, I.x, ly.ln2, I.n);
-        // gate/up: a launch that splits K in two leaves both partial slices, and the down
-        // projection's staging adds them (one reduction launch fewer per layer)
-        const bool fold = T <= GU_FOLD_ROWS && conv::plan(gemm_desc(ly.wgu, nullptr, H, T, H, 2 * I.F, 2 * I.F, EPI_NONE, false), sms).splits == 2;
-        if (fold) {
-            conv::Conv c = gemm_desc(ly.wgu, nullptr, H, T, H, 2 * I.F, 2 * I.F, EPI_NONE, false);
-            c.x = I.n;
-            c.y = I.gu;
-            c.defer_reduce = true;
-            if (conv::launch(c, ws_gu, sms, stream) != 2) fail("talker: the gate/up projection did not split in two", NAVI_E_SHAPE);
-        } else {
-            I.gemm(ly.wgu, nullptr, I.n, H, T, H, 2 * I.F, I.gu, 2 * I.F, EPI_NONE);
-        }
-        const bool last = l + 1 == tp.n_layer;
-        {
-            conv::Conv c = gemm_desc(ly.wd, nullptr, 2 * I.F, T, I.F, H, H, EPI_RESIDUAL, true);
-            c.x = fold ? ws_gu.partial : I.gu;
-            if (fold) {
-                c.x_slices = 2;
-                c.x_slice_stride = static_cast<std::size_t>(T) * 2 * I.F;
-            }
-            c.y = I.x;
-            c.resid = I.x;
-            c.norm_w = last ? nullptr : I.layers[static_cast<size_t>(l + 1)].ln1;
-            c.norm_out = last ? nullptr : I.n;
-            c.norm_eps = tp.rms_eps;
-            conv::launch(c, ws, sms, stream);
-        }
+        finish_layer(l, T);
     }
     // the last row: final norm and the codec head
     NAVI_CUDA(navi::dev::launch_pdl(k_rmsnorm, dim3(1), dim3(256), 0, I.stream, I.x + static_cast<size_t>(T - 1) * H, I.final_norm, H,

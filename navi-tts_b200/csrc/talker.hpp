@@ -4,6 +4,7 @@
 #pragma once
 
 #include "frame.hpp"
+#include "pages.hpp"
 #include "runtime.hpp"
 
 #include <cstdint>
@@ -31,6 +32,11 @@ public:
     const Prompt & build_prompt(std::span<const std::int32_t> ids, const std::string & language, std::span<const float> speaker);
     // Runs the prompt's prefill rows through every layer at positions 0..n-1 and fills kv().
     void prefill(const Prompt & p);
+
+    // The rows of one step of many requests over a paged cache (include/navi_b200.h,
+    // navi_talker_step): plan, then every layer with store and attend in place of this talker's own cache.
+    // rows, hidden: device [s.max_rows][hidden]; logits: device [s.max_rows][vocab] or nullptr.
+    void step(const Pages & pages, const navi_step & s, const float * rows, float * hidden, float * logits);
 
     KvCache & kv();
     const float * d_hidden() const;   // post-norm hidden of the last prefill row [hidden]

@@ -196,6 +196,7 @@ SIGNATURES = [
     ("navi_pages_attend", c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
     ("navi_pages_commit", c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),
     ("navi_pages_check", c_int, [c_void_p, c_void_p]),
+    ("navi_talker_step", c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     ("navi_conv1d", c_int, [c_void_p, POINTER(ConvArgs)]),
     ("navi_frame_inspect", c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),
     ("navi_frame_set_profile", c_int, [c_void_p, c_int, c_int]),

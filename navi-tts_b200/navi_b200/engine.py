@@ -189,6 +189,11 @@ class Talker:
     def prefill(self, pr: capi.Prompt = None) -> None:
         check(lib().navi_talker_prefill(self.h, byref(pr or self.prompt)))
 
+    def step(self, pages: "PagedKv", step: "TreeStep", d_rows: int, d_hidden: int, d_logits: int = 0) -> None:
+        """The rows of one step of many requests over a paged cache (navi_talker_step): plan, every
+        layer, the post-norm hidden rows and, with d_logits, their codec logits."""
+        check(lib().navi_talker_step(self.h, pages.h, step.ptr, d_rows, d_hidden, d_logits or None))
+
     def kv(self) -> "KvCache":
         kv = KvCache()
         kv.s = capi.KV()
