@@ -10,7 +10,10 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <mutex>
+#include <set>
 #include <type_traits>
+#include <utility>
 
 namespace navi::attn {
 
@@ -77,6 +80,19 @@ __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Lets a kernel have `bytes` of dynamic shared memory, asking the runtime once a kernel and device.
+template <class... A> void allow_smem(void (*kernel)(A...), int bytes) {
+    static std::mutex lock;
+    static std::set<std::pair<int, const void *>> done;
+    int dev = 0;
+    NAVI_CUDA(cudaGetDevice(&dev));
+    const std::lock_guard<std::mutex> hold(lock);
+    const void * k = reinterpret_cast<const void *>(kernel);
+    if (done.count({dev, k})) return;
+    NAVI_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.insert({dev, k});
 }
 
 // ---- who does what ----------------------------------------------------------------------------

@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
 
 template <class T, class C, int D> void few(const AttendArgs & a, const CUtensorMap & k, const CUtensorMap & v, int rows, int sms, cudaStream_t stream) {
     const auto go = [&](auto kernel) {
-        NAVI_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, FewSmem<D>::BYTES));
+        allow_smem(kernel, FewSmem<D>::BYTES);
         NAVI_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(sms)), dim3(288), FewSmem<D>::BYTES, stream, a, k, v));
     };
     if (rows <= 8) go(k_attend_few<T, C, D, 8>);

@@ -524,7 +524,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
 template <class T, class C, int D>
 void many(const AttendArgs & a, const CUtensorMap & k, const CUtensorMap & v, const CUtensorMap & q, int64_t rows, int sms, cudaStream_t stream) {
     const auto go = [&](auto kernel, int smem) {
-        NAVI_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        allow_smem(kernel, smem);
         NAVI_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(sms)), dim3(384), static_cast<size_t>(smem), stream, a, k, v, q));
     };
     if constexpr (!std::is_same_v<T, float>)

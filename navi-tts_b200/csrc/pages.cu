@@ -345,7 +345,7 @@ template <class T, class C, int D> __global__ void __launch_bounds__(128) k_page
     constexpr int N = 4 / sizeof(T), LANES = D / (4 * N), HPW = 32 / LANES;   // pairs of floats in 8 bytes, lanes a head, heads a warp
     const int w = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
     const int r = w / a.parts, part = w % a.parts;
-    if (r >= a.max_rows || r >= a.cu_rows[a.n_req]) return;
+    if (r >= a.max_rows) return;
     const int e0 = lane % LANES * (2 * N), H = a.n_head, total = H + 2 * a.n_kv;
     // the first heads are asked for before what the row's place and position lead to
     constexpr int U = 4;   // heads of a lane whose loads are under way together
@@ -364,6 +364,7 @@ template <class T, class C, int D> __global__ void __launch_bounds__(128) k_page
     load(first);
     const int64_t slot = a.slot[r];
     const int pos = a.pos[r];
+    if (r >= a.cu_rows[a.n_req]) return;
     const bool known = !a.rope || (pos >= 0 && pos < a.rope_positions);
     T * qo = static_cast<T *>(a.q_out) + r * a.out_stride + e0;
     const int64_t page = slot >> a.shift, off = slot & ((1 << a.shift) - 1);
@@ -627,16 +628,16 @@ Pages::~Pages() {
 }
 
 void Pages::check_step(const navi_step & s, const char * who) const {
-    const std::string w(who);
-    if (s.n_req < 0 || s.n_req > d_.max_requests) fail(w + ": n_req outside 0..max_requests", NAVI_E_ARG);
-    if (s.max_rows < 0 || s.max_new < 0) fail(w + ": max_rows and max_new must not be negative", NAVI_E_ARG);
+    const auto refuse = [&](const char * why, int status) { fail(std::string(who) + why, status); };
+    if (s.n_req < 0 || s.n_req > d_.max_requests) refuse(": n_req outside 0..max_requests", NAVI_E_ARG);
+    if (s.max_rows < 0 || s.max_new < 0) refuse(": max_rows and max_new must not be negative", NAVI_E_ARG);
     if (s.n_req == 0) return;
-    if (!s.ctx_len || !s.n_new || !s.cu_rows || !s.status) fail(w + ": ctx_len, n_new, cu_rows and status are needed", NAVI_E_ARG);
-    if (s.max_rows > 0 && (!s.row_req || !s.pos || !s.slot)) fail(w + ": row_req, pos and slot are needed", NAVI_E_ARG);
+    if (!s.ctx_len || !s.n_new || !s.cu_rows || !s.status) refuse(": ctx_len, n_new, cu_rows and status are needed", NAVI_E_ARG);
+    if (s.max_rows > 0 && (!s.row_req || !s.pos || !s.slot)) refuse(": row_req, pos and slot are needed", NAVI_E_ARG);
     if (s.parent) {
-        if (s.max_new > NAVI_STEP_MAX_TREE) fail(w + ": a tree has at most NAVI_STEP_MAX_TREE rows", NAVI_E_SHAPE);
+        if (s.max_new > NAVI_STEP_MAX_TREE) refuse(": a tree has at most NAVI_STEP_MAX_TREE rows", NAVI_E_SHAPE);
         if (s.mask_words < 0 || s.mask_words > NAVI_STEP_MAX_TREE / 64 || 64 * s.mask_words < s.max_new || (s.max_new > 0 && !s.mask))
-            fail(w + ": mask of 64 * mask_words >= max_new bits is needed with parent", NAVI_E_ARG);
+            refuse(": mask of 64 * mask_words >= max_new bits is needed with parent", NAVI_E_ARG);
     }
 }
 
