@@ -42,7 +42,7 @@ template <class T, int D, int ROWS> struct ManySmem {
 };
 
 struct ManyControl {
-    uint64_t full[8], empty[8], q_full, q_empty, s_full[2], p_full[2], o_full[2], drained;
+    uint64_t full[8], empty[8], q_full, q_empty, s_full[2], p_full[2][2], o_full[2], drained;
     float stat[2][2][128];
     SegmentRing segs;
     int red[12];
@@ -119,7 +119,8 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
         mbar_init(&S.q_empty, 1);
         for (int g = 0; g < 2; ++g) {
             mbar_init(&S.s_full[g], 1);
-            mbar_init(&S.p_full[g], 128);
+            mbar_init(&S.p_full[g][0], 128);
+            mbar_init(&S.p_full[g][1], 128);
             mbar_init(&S.o_full[g], 1);
         }
         mbar_init(&S.drained, 1);
@@ -222,21 +223,26 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                     // not wait for the next K.
                     if (n >= 0 && (!two || g == 0)) ok = wait_all(&S.full[sv], (iv / L::STAGES) & 1);
                     if (n + 2 < P && two && g == 0) ok = ok && wait_all(&S.full[sk], (ik / L::STAGES) & 1);
+                    if (!ok) break;
                     if (n >= 0) {
-                        ok = ok && wait_all(&S.p_full[g], (g ? np1 : np0) & 1);
+                        const int turn = g ? np1 : np0;
                         if (g) ++np1;
                         else ++np0;
-                    }
-                    if (!ok) break;
-                    fence_after_sync();
-                    if (n >= 0) {
                         const uint32_t d = tm + 256 + g * 128, p = tm + g * 128;
                         const uint64_t v = v_desc + static_cast<uint32_t>(sv * (L::STAGE >> 4));
+                        // the weights come in two halves: P V of the first runs while the second is still made
 #pragma unroll
-                        for (int term = 0; term < (SPLIT ? 2 : 1); ++term)
+                        for (int h = 0; h < 2; ++h) {
+                            ok = ok && wait_all(&S.p_full[g][h], turn & 1);
+                            if (!ok) break;
+                            fence_after_sync();
 #pragma unroll
-                            for (int ks = 0; ks < KT / 16; ++ks)
-                                mma_ts(d, p + (SPLIT ? (1 - term) * 64 : 0) + ks * 8, v + ks * (2048 >> 4), ID_O, n > 1 || term > 0 || ks > 0, leader);
+                            for (int term = 0; term < (SPLIT ? 2 : 1); ++term)
+#pragma unroll
+                                for (int ks = 4 * h; ks < 4 * h + 4; ++ks)
+                                    mma_ts(d, p + (SPLIT ? (1 - term) * 64 : 0) + ks * 8, v + ks * (2048 >> 4), ID_O, n > 1 || term > 0 || ks > 0, leader);
+                        }
+                        if (!ok) break;
                         if (n + 2 >= P) commit_by(&S.o_full[g], leader);
                         if (!two || g == 1) commit_by(&S.empty[sv], leader);
                     }
@@ -400,26 +406,24 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 const float2 scale2 = make_float2(a.scale, a.scale), ref2 = make_float2(-ref, -ref);
                 float2 part[2] = {};
 #pragma unroll
-                for (int c = 0; c < KT; c += 32) {
-                    uint32_t hi[16], lo[16];
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t hi[32], lo[SPLIT ? 32 : 1];
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const float2 e = __ffma2_rn(make_float2(__uint_as_float(s[c + 2 * k]), __uint_as_float(s[c + 2 * k + 1])), scale2, ref2);
+                    for (int k = 0; k < 32; ++k) {
+                        const int c = 64 * h + 2 * k;
+                        const float2 e = __ffma2_rn(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), scale2, ref2);
                         const float2 w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
                         part[k & 1] = __fadd2_rn(part[k & 1], w);
-                        hi[k] = pack<C>(w.x, w.y);
-                        if constexpr (SPLIT) {
-                            const float2 b = unpack<C>(hi[k]);
-                            lo[k] = pack<C>(w.x - b.x, w.y - b.y);
-                        }
+                        if constexpr (SPLIT) split_pair<C>(w.x, w.y, hi[k], lo[k]);
+                        else hi[k] = pack<C>(w.x, w.y);
                     }
-                    tmem_st<16>(s_at + c / 2, hi);
-                    if constexpr (SPLIT) tmem_st<16>(s_at + 64 + c / 2, lo);
+                    tmem_st<32>(s_at + 32 * h, hi);
+                    if constexpr (SPLIT) tmem_st<32>(s_at + 64 + 32 * h, lo);
+                    tmem_st_wait();
+                    fence_before_sync();
+                    mbar_arrive(&S.p_full[wg][h]);
                 }
                 sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
-                tmem_st_wait();
-                fence_before_sync();
-                mbar_arrive(&S.p_full[wg]);
             }
             base += 2 * nt;
             // which warpgroup's sums there are; both read both where they took the key tiles in turn
