@@ -197,63 +197,71 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
             const uint32_t leader = lane == 0, tm = static_cast<uint32_t>(uniform(static_cast<int>(tmem)));
             const uint64_t q_desc = desc_kmajor_sw128(smem_addr(qs)), k_desc = desc_kmajor_sw128(smem_addr(ring)), v_desc = desc_mnmajor_sw128(smem_addr(ring), KT * 128);
             const auto wait_all = [&](uint64_t * bar, int parity) { return __all_sync(0xffffffffu, wait(bar, static_cast<uint32_t>(parity))) != 0; };
-            int base = 0, nq = 0, np0 = 0, np1 = 0;
-            bool ok = true;
-#pragma unroll 1
-            for (int sn = 0; ok; ++sn) {
-                if (!wait_all(&S.segs.full[sn % SegmentRing::N], (sn / SegmentRing::N) & 1)) break;
-                const Segment & s = S.segs.s[sn % SegmentRing::N];
-                const int s_nt = uniform(s.nt), s_m = uniform(s.m), s_keys = uniform(s.n_keys);
-                if (s_nt < 0) break;
-                const bool two = ROWS > 128 && s_m > 128;
-                const int nt = s_keys > 0 ? s_nt : 0, P = two ? 2 * nt : nt;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&S.segs.empty[sn % SegmentRing::N]);
-                if (P == 0) continue;
-                ok = wait_all(&S.q_full, nq & 1);
-                ++nq;
-                fence_after_sync();
+            const auto all = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
+            // places in the ring: stage and the parity of its turn
+            struct Place {
+                int st = 0, turn = 0;
+                __device__ __forceinline__ void go(int by) {
+                    st += by;
+                    if (st >= L::STAGES) {
+                        st -= L::STAGES;
+                        turn ^= 1;
+                    }
+                }
+            };
+            Place kp, vp;                                  // the next K and V tile
+            vp.go(1);
+            int nq = 0, np0 = 0, np1 = 0;
+            // The pairs of a segment. A barrier's answer takes a while, so those that a step needs are asked together, and
+            // waited for one by one only if one of them says no. TWO: the warpgroups share the tiles, arithmetic is the bound,
+            // and everything is there before the two products, which then follow one another. Otherwise HBM is the bound,
+            // and P V, which frees a stage, does not wait for the next K.
+            const auto run = [&](auto two_c, int P) {
+                constexpr bool TWO = decltype(two_c)::value;
                 // step n asks for the scores of pair n + 2 once P V of pair n is under way; the first two only ask
 #pragma unroll 1
-                for (int n = -2; n < P && ok; ++n) {
-                    const int g = n & 1, tn = two ? n >> 1 : n, tk = two ? (n + 2) >> 1 : n + 2;   // the pair's tile, and that of pair n + 2
-                    const int iv = base + 2 * tn + 1, ik = base + 2 * tk, sv = iv % L::STAGES, sk = ik % L::STAGES;
-                    // where the warpgroups share the tiles, arithmetic is the bound: all that is waited for comes before the
-                    // two products, which then follow one another. Otherwise HBM is, and P V, which frees a stage, does
-                    // not wait for the next K.
-                    if (n >= 0 && (!two || g == 0)) ok = wait_all(&S.full[sv], (iv / L::STAGES) & 1);
-                    if (n + 2 < P && two && g == 0) ok = ok && wait_all(&S.full[sk], (ik / L::STAGES) & 1);
-                    if (!ok) break;
-                    if (n >= 0) {
-                        const int turn = g ? np1 : np0;
+                for (int n = -2; n < P; ++n) {
+                    const int g = n & 1, turn = (g ? np1 : np0) & 1;
+                    const bool pv = n >= 0, next = n + 2 < P, opens = !TWO || g == 0, closes = !TWO || g == 1;   // a tile's first and last pair
+                    const bool r_v = !pv || !opens || mbar_try_wait(&S.full[vp.st], vp.turn), r_k = !TWO || !next || !opens || mbar_try_wait(&S.full[kp.st], kp.turn);
+                    const bool r_0 = !pv || mbar_try_wait(&S.p_full[g][0], turn), r_1 = !pv || mbar_try_wait(&S.p_full[g][1], turn);
+                    if (!all(r_v && r_k && r_0)) {
+                        if (pv && opens && !wait_all(&S.full[vp.st], vp.turn)) return false;
+                        if (TWO && next && opens && !wait_all(&S.full[kp.st], kp.turn)) return false;
+                        if (pv && !wait_all(&S.p_full[g][0], turn)) return false;
+                    }
+                    fence_after_sync();
+                    if (pv) {
                         if (g) ++np1;
                         else ++np0;
                         const uint32_t d = tm + 256 + g * 128, p = tm + g * 128;
-                        const uint64_t v = v_desc + static_cast<uint32_t>(sv * (L::STAGE >> 4));
-                        // the weights come in two halves: P V of the first runs while the second is still made
+                        const uint64_t v = v_desc + static_cast<uint32_t>(vp.st * (L::STAGE >> 4));
+                        // the weights come in two halves: P V of the first may run while the second is still made
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            ok = ok && wait_all(&S.p_full[g][h], turn & 1);
-                            if (!ok) break;
-                            fence_after_sync();
+                            if (h == 1 && !all(r_1)) {
+                                if (!wait_all(&S.p_full[g][1], turn)) return false;
+                                fence_after_sync();
+                            }
 #pragma unroll
                             for (int term = 0; term < (SPLIT ? 2 : 1); ++term)
 #pragma unroll
                                 for (int ks = 4 * h; ks < 4 * h + 4; ++ks)
                                     mma_ts(d, p + (SPLIT ? (1 - term) * 64 : 0) + ks * 8, v + ks * (2048 >> 4), ID_O, n > 1 || term > 0 || ks > 0, leader);
                         }
-                        if (!ok) break;
                         if (n + 2 >= P) commit_by(&S.o_full[g], leader);
-                        if (!two || g == 1) commit_by(&S.empty[sv], leader);
+                        if (closes) {
+                            commit_by(&S.empty[vp.st], leader);
+                            vp.go(2);
+                        }
                     }
-                    if (n + 2 < P) {
-                        if (!two) {
-                            ok = wait_all(&S.full[sk], (ik / L::STAGES) & 1);
-                            if (!ok) break;
+                    if (next) {
+                        if (!TWO) {
+                            if (!wait_all(&S.full[kp.st], kp.turn)) return false;
                             fence_after_sync();
                         }
                         const uint32_t d = tm + g * 128;
-                        const uint64_t q = q_desc + static_cast<uint32_t>(two ? g * (L::QTILE >> 4) : 0), k = k_desc + static_cast<uint32_t>(sk * (L::STAGE >> 4));
+                        const uint64_t q = q_desc + static_cast<uint32_t>(TWO ? g * (L::QTILE >> 4) : 0), k = k_desc + static_cast<uint32_t>(kp.st * (L::STAGE >> 4));
 #pragma unroll
                         for (int term = 0; term < (SPLIT ? 2 : 1); ++term)
 #pragma unroll
@@ -264,10 +272,30 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                             }
                         commit_by(&S.s_full[g], leader);
                         if (n + 3 == P) commit_by(&S.q_empty, leader);
-                        if (!two || g == 1) commit_by(&S.empty[sk], leader);
+                        if (closes) {
+                            commit_by(&S.empty[kp.st], leader);
+                            kp.go(2);
+                        }
                     }
                 }
-                base += 2 * nt;
+                return true;
+            };
+#pragma unroll 1
+            for (int sn = 0;; ++sn) {
+                if (!wait_all(&S.segs.full[sn % SegmentRing::N], (sn / SegmentRing::N) & 1)) break;
+                const Segment & s = S.segs.s[sn % SegmentRing::N];
+                const int s_nt = uniform(s.nt), s_m = uniform(s.m), nt = uniform(s.n_keys) > 0 ? s_nt : 0;
+                if (s_nt < 0) break;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&S.segs.empty[sn % SegmentRing::N]);
+                if (nt == 0) continue;
+                if (!wait_all(&S.q_full, nq & 1)) break;
+                ++nq;
+                fence_after_sync();
+                bool ok;
+                if (ROWS > 128 && s_m > 128) ok = run(std::bool_constant<(ROWS > 128)>{}, 2 * nt);
+                else ok = run(std::false_type{}, nt);
+                if (!ok) break;
             }
             // nothing may still write the tensor memory when it is given back
             commit_by(&S.drained, leader);
