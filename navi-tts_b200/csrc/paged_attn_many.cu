@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 // step n asks for the scores of pair n + 2 once P V of pair n is under way; the first two only ask
 #pragma unroll 1
                 for (int n = -2; n < P; ++n) {
-                    const int g = n & 1, turn = (g ? np1 : np0) & 1;
+                    const int g = n & 1, turn = (g ? np1 : np0) & 1, v_st = uniform(vp.st), k_st = uniform(kp.st);
                     const bool pv = n >= 0, next = n + 2 < P, opens = !TWO || g == 0, closes = !TWO || g == 1;   // a tile's first and last pair
                     const bool r_v = !pv || !opens || mbar_try_wait(&S.full[vp.st], vp.turn), r_k = !TWO || !next || !opens || mbar_try_wait(&S.full[kp.st], kp.turn);
                     const bool r_0 = !pv || mbar_try_wait(&S.p_full[g][0], turn), r_1 = !pv || mbar_try_wait(&S.p_full[g][1], turn);
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                         if (g) ++np1;
                         else ++np0;
                         const uint32_t d = tm + 256 + g * 128, p = tm + g * 128;
-                        const uint64_t v = v_desc + static_cast<uint32_t>(vp.st * (L::STAGE >> 4));
+                        const uint64_t v = v_desc + static_cast<uint32_t>(v_st * (L::STAGE >> 4));
                         // the weights come in two halves: P V of the first may run while the second is still made
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                             fence_after_sync();
                         }
                         const uint32_t d = tm + g * 128;
-                        const uint64_t q = q_desc + static_cast<uint32_t>(TWO ? g * (L::QTILE >> 4) : 0), k = k_desc + static_cast<uint32_t>(kp.st * (L::STAGE >> 4));
+                        const uint64_t q = q_desc + static_cast<uint32_t>(TWO ? g * (L::QTILE >> 4) : 0), k = k_desc + static_cast<uint32_t>(k_st * (L::STAGE >> 4));
 #pragma unroll
                         for (int term = 0; term < (SPLIT ? 2 : 1); ++term)
 #pragma unroll
