@@ -29,7 +29,8 @@ void Pages::attend(const navi_step & s, int layer, const navi_attend_args & q, c
     NAVI_CUDA(cudaSetDevice(dev_->info().ordinal));
     const int sms = dev_->info().multiprocessors;
     const PagesScratch sc(dev_->scratch(stream, PagesScratch::bytes(sms)), sms);
-    attn::AttendArgs a{q.q, q.out, q.lse, d_.table, s.req, s.ctx_len, s.cu_rows, s.status, s.parent ? s.mask : nullptr, sc.pieces, sc.arrived, sc.err,
+    attn::AttendArgs a{q.q, q.out, q.lse, static_cast<const uint8_t *>(k_[static_cast<size_t>(layer)]),
+                       static_cast<const uint8_t *>(v_[static_cast<size_t>(layer)]), d_.table, s.req, s.ctx_len, s.cu_rows, s.status, s.parent ? s.mask : nullptr, sc.pieces, sc.arrived, sc.err,
                  in, out, q.scale * 1.4426950408889634f, 0, s.n_req, s.max_rows, s.mask_words, q.n_head, d_.n_kv_head, q.n_head / d_.n_kv_head, 0, D, shift_,
                  d_.n_pages, d_.max_blocks, d_.max_requests};
     const int64_t most = std::min(s.max_new, s.max_rows);

@@ -23,6 +23,7 @@ struct AttendArgs {
     const void * q;
     void * out;
     float * lse;
+    const uint8_t * k, * v;      // the layer's pools, for what does not come by TMA
     const int32_t * table, * req, * ctx_len, * cu_rows, * status;
     const uint64_t * mask;       // nullptr: a chain
     float * pieces;              // the stream's scratch: unfinished sums, arrival counters, error word
@@ -365,11 +366,13 @@ __device__ __forceinline__ void join(const AttendArgs & a, const Division & d, c
             for (int k = 0; k < U; ++k) { y[k].x *= old; y[k].y *= old; y[k].z *= old; y[k].w *= old; }
 #pragma unroll
             for (int p = 0; p < P; ++p) {
-                const float c = p0 + p < np ? exp2_fast(m[p] - ref) : 0.f;
+                const bool there = p0 + p < np;       // no branch: the loads above stay together
+                const float c = there ? exp2_fast(m[p] - ref) : 0.f;
                 l += c * w[p];
 #pragma unroll
                 for (int k = 0; k < U; ++k) {
-                    y[k].x += c * v[p][k].x; y[k].y += c * v[p][k].y; y[k].z += c * v[p][k].z; y[k].w += c * v[p][k].w;
+                    const float4 z = there ? v[p][k] : make_float4(0.f, 0.f, 0.f, 0.f);
+                    y[k].x += c * z.x; y[k].y += c * z.y; y[k].z += c * z.z; y[k].w += c * z.w;
                 }
             }
         }
@@ -455,6 +458,46 @@ __device__ __forceinline__ int tile_pages(const AttendArgs & a, const Segment & 
 // reads its page's id a tile ahead, so the ids cost one latency together and not one each.
 __device__ __forceinline__ int page_at(const AttendArgs & a, const Segment & s, int t, int p) {
     return p < tile_pages(a, s, t) ? min(max(__ldg(a.table + static_cast<size_t>(s.table) * a.max_blocks + (t * KT >> a.shift) + p), 0), a.n_pages - 1) : -1;
+}
+
+// ---- values that are not finite where a row does not look --------------------------------------
+//
+// A weight of zero times a V value that is infinite or NaN is NaN, so tokens that some rows do not see
+// must not enter their product. Past the last token shared memory is cleared. Among the new rows
+// (a sibling in the tree, a later row of the chain) every token is some row's own: in the tiles that
+// have such tokens, those whose V is not finite are looked for and cleared too, and the rows that do
+// see them add them from the pool, one by one. That is seldom; the looking costs the last tiles of an item
+// 16 loads a thread.
+
+// The larger of the magnitudes so far and those of 16 bytes, as pairs of 16-bit patterns.
+__device__ __forceinline__ uint32_t magnitude(uint32_t m, uint4 v) {
+    m = __vmaxu2(m, v.x & 0x7fff7fffu);
+    m = __vmaxu2(m, v.y & 0x7fff7fffu);
+    m = __vmaxu2(m, v.z & 0x7fff7fffu);
+    return __vmaxu2(m, v.w & 0x7fff7fffu);
+}
+template <class C> __device__ __forceinline__ bool not_finite(uint32_t m) {
+    constexpr uint32_t inf = std::is_same_v<C, __half> ? 0x7c00u : 0x7f80u;
+    return (m & 0xffffu) >= inf || (m >> 16) >= inf;
+}
+// Token `key` of the segment's request and KV head in a pool.
+template <class C, int D> __device__ __forceinline__ const C * token_at(const AttendArgs & a, const Segment & s, const uint8_t * pool, int key) {
+    const int page = min(max(__ldg(a.table + static_cast<size_t>(s.table) * a.max_blocks + (key >> a.shift)), 0), a.n_pages - 1);
+    return reinterpret_cast<const C *>(pool) + (((static_cast<size_t>(page) * a.n_kv + s.g) << a.shift) + (key & ((1 << a.shift) - 1))) * D;
+}
+
+// y += 2^(scale q k - ref) v[dim .. dim + 3] of row m of the segment and token `key`.
+template <class T, class C, int D> __device__ __forceinline__ void add_token(const AttendArgs & a, const Segment & s, int m, int key, float ref, int dim, float4 & y) {
+    const T * q = row_at<const T>(a, a.q, a.q_stride, s, m);
+    const C * k = token_at<C, D>(a, s, a.k, key), * v = token_at<C, D>(a, s, a.v, key) + dim;
+    float z = 0.f;
+#pragma unroll 1
+    for (int d = 0; d < D; ++d) z += static_cast<float>(q[d]) * static_cast<float>(k[d]);
+    const float w = exp2_fast(fmaf(z, a.scale, -ref));
+    y.x += w * static_cast<float>(v[0]);
+    y.y += w * static_cast<float>(v[1]);
+    y.z += w * static_cast<float>(v[2]);
+    y.w += w * static_cast<float>(v[3]);
 }
 
 // The ring of segments: one warp fills it, every other role reads it.

@@ -41,6 +41,20 @@ template <int D> struct FewSmem {
     static constexpr int BYTES = 1024 + STAGES * STAGE + JOIN;  // 1024: to align the ring to the swizzle's 1024 bytes
 };
 
+// y and what the tokens that were cleared add to row m of a segment, if it sees them. Out of line: it seldom runs.
+template <class T, class C, int D>
+__device__ __noinline__ float4 with_bad(const AttendArgs & a, const Segment & s, const uint32_t * bad, int m, float ref, int dim, float4 y) {
+    const int bad0 = s.ctx / KT * KT, j = by_group(a, s.m0 + m);
+#pragma unroll 1
+    for (int w = 0; w < 16; ++w)
+#pragma unroll 1
+        for (uint32_t left = bad[w]; left; left &= left - 1) {
+            const int key = bad0 + 32 * w + __ffs(left) - 1;
+            if (seen_bits(a, s, j, key - s.ctx, s.n_keys - key) & 1) add_token<T, C, D>(a, s, m, key, ref, dim, y);
+        }
+    return y;
+}
+
 template <class T, class C, int D, int ROWS>   // ROWS: 8, 16 or 32 rows of an item
 __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
                                                        const __grid_constant__ CUtensorMap vmap) {
@@ -60,6 +74,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
     __shared__ __align__(8) uint64_t full[L::STAGES], empty[L::STAGES];
     __shared__ __align__(8) SegmentRing segs;
     __shared__ float stat[8][2][MR];
+    __shared__ uint32_t bad[16];   // tokens from the item's first masked tile on whose V is not finite
     __shared__ int red[9];
     __shared__ Share share;
     __shared__ int abort_flag, is_last;
@@ -149,6 +164,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
 #pragma unroll 1
     for (int sn = 0;; ++sn) {
         const bool got = wait(&segs.full[sn % SegmentRing::N], (sn / SegmentRing::N) & 1);
+        if (tid < 16) bad[tid] = 0;
         // after an abort all warps leave together
         if (named_sync_or(1, 256, !got)) break;
         const Segment & s = segs.s[sn % SegmentRing::N];
@@ -235,6 +251,25 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
                         for (int e = 0; e < 2 * XR; ++e) sc[y][e] += EIGHT ? sc[y][2 + e] : low[y][e];
                 }
                 if (masked) {
+                    // tokens that not every row sees: those whose V is not finite are cleared, and come in by themselves at the end
+                    const int key = k0 + lane % WK, bit = first + lane % WK - s.ctx / KT * KT;   // a lane a token, or half of one
+                    uint8_t * at = ring + st * L::STAGE + L::STAGE / 2 + place(key);
+                    uint32_t m = 0;
+#pragma unroll 4
+                    for (int c = lane / WK; c < D / 8; c += 32 / WK) m = magnitude(m, *reinterpret_cast<const uint4 *>(at + (c >> 3) * half + (((c + lane) & 7) << 4)));
+                    // another warp may share the tokens and clear them meanwhile: it says so first, so who reads its zeros sees that too
+                    if (not_finite<C>(m) && bit < 512) atomicOr(&bad[bit >> 5], 1u << (bit & 31));
+                    __threadfence_block();
+                    __syncwarp();
+                    const bool clear = bit < 512 && (*const_cast<volatile uint32_t *>(&bad[bit >> 5]) >> (bit & 31) & 1);
+                    if (__any_sync(0xffffffffu, clear)) {
+                        if (lane < WK && clear) {
+#pragma unroll 1
+                            for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4 *>(at + (c >> 3) * half + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
 #pragma unroll
                     for (int x = 0; x < XR; ++x)
 #pragma unroll
@@ -336,6 +371,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
         const bool whole = is_whole(s);
         float4 * pc = reinterpret_cast<float4 *>(piece(a, blockIdx.x, s.t0 == 0));
         named_sync(1, 256);                                      // q is read
+        const bool any_bad = __any_sync(0xffffffffu, bad[lane & 15] != 0);
 #pragma unroll
         for (int h = 0; h < D / W; ++h) {
 #pragma unroll
@@ -362,6 +398,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
                     sum += w * stat[w0 + k][1][r];
                     y.x += w * v.x; y.y += w * v.y; y.z += w * v.z; y.w += w * v.w;
                 }
+                if (any_bad) y = with_bad<T, C, D>(a, s, bad, m, ref, W * h + 4 * q, y);
                 if (whole) {
                     const float inv = sum == 0.f ? 0.f : 1.f / sum;
                     T * dst = row_at<T>(a, a.out, a.out_stride, s, m) + W * h + 4 * q;

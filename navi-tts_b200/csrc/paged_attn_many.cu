@@ -44,6 +44,7 @@ template <class T, int D, int ROWS> struct ManySmem {
 struct ManyControl {
     uint64_t full[8], empty[8], q_full, q_empty, s_full[2], p_full[2][2], o_full[2], drained;
     float stat[2][2][128];
+    uint32_t bad[16];            // tokens from the first masked tile on whose V is not finite
     SegmentRing segs;
     int red[12];
     Share sh;
@@ -375,6 +376,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
 #pragma unroll 1
         for (int sn = 0;; ++sn) {
             const bool got = wait(&S.segs.full[sn % SegmentRing::N], (sn / SegmentRing::N) & 1);
+            if (tid < 16) S.bad[tid] = 0;
             // after an abort all warps leave together
             if (named_sync_or(1, 256, !got)) break;
             const Segment & it = S.segs.s[sn % SegmentRing::N];
@@ -384,20 +386,37 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
             const int m = (two ? wg * 128 : 0) + r, j = by_group(a, it.m0 + min(m, it.m - 1));
             // every row of the warp sees the tokens before `open`
             const int open = ctx + (a.mask ? 0 : by_group(a, it.m0 + min((two ? wg * 128 : 0) + (warp & 3) * 32, it.m - 1)) + 1);
+            const int open0 = ctx + (a.mask ? 0 : by_group(a, it.m0) + 1), bad0 = open0 / KT * KT;   // the same for the item; its first masked tile
             float top = -INFINITY, sum = 0.f;
             bool any = false;                             // this warpgroup has had a tile
             for (int x = two ? 0 : wg; x < nt; x += two ? 1 : 2, ++ns) {
                 if (!wait(&S.s_full[wg], ns & 1)) break;
                 fence_after_sync();
                 const int key0 = (t0 + x) * KT, left = n_keys - key0;
-                if (left < KT) {                      // V rows past the last token: zeros, whatever the page holds there
+                if (key0 + KT > open0) {              // some of these tokens are not seen by every row of the item
                     const int idx = base + 2 * x + 1, st = idx % L::STAGES;
                     wait(&S.full[st], (idx / L::STAGES) & 1);
-                    for (int k = r; k < (KT - left) * (D / 8); k += 128) {
-                        const int key = left + k / (D / 8), c = k % (D / 8);
-                        *reinterpret_cast<uint4 *>(ring + st * L::STAGE + (c >> 3) * (KT * 128) + key * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                    // V rows past the last token, whatever the page holds there, and those that are not finite: zeros. A thread a row
+                    uint8_t * row = ring + st * L::STAGE + r * 128;
+                    bool clear = r >= left;
+                    if (!clear) {
+                        uint32_t m = 0;
+#pragma unroll
+                        for (int c = 0; c < D / 8; ++c) m = magnitude(m, *reinterpret_cast<const uint4 *>(row + (c >> 3) * (KT * 128) + (((c + r) & 7) << 4)));
+                        // the other warpgroup may share the tile and clear the row meanwhile: it says so first, so who reads
+                        // its zeros sees that too
+                        const int bit = key0 - bad0 + r;
+                        if (bit < 512) {
+                            if (not_finite<C>(m)) atomicOr(&S.bad[bit >> 5], 1u << (bit & 31));
+                            __threadfence_block();
+                            clear = *const_cast<volatile uint32_t *>(&S.bad[bit >> 5]) >> (bit & 31) & 1;
+                        }
                     }
-                    fence_proxy_async_smem();
+                    if (clear) {
+#pragma unroll 1
+                        for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4 *>(row + (c >> 3) * (KT * 128) + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                        fence_proxy_async_smem();
+                    }
                 }
                 uint32_t s[KT];
                 tmem_ld<64>(s_at, s);
@@ -481,6 +500,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 float4 * pc = reinterpret_cast<float4 *>(piece(a, blockIdx.x, it.t0 == 0)) + m;
                 const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
                 const bool live = m < it.m;
+                const bool bad = __any_sync(0xffffffffu, S.bad[lane & 15] != 0);   // tokens of this segment whose V was cleared
                 T * dst = row_at<T>(a, a.out, a.out_stride, it, live ? m : 0);
                 const bool wide = (reinterpret_cast<uintptr_t>(dst) & 31) == 0;   // rows are at least 16-byte aligned
                 w0 *= inv;
@@ -500,6 +520,23 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                         for (int k = 0; k < 32; ++k) v[k] += __uint_as_float(o[k]) * w1;
                     }
                     if (!live) continue;
+                    if (bad) {
+#pragma unroll 1
+                        for (int w = 0; w < 16; ++w)
+#pragma unroll 1
+                            for (uint32_t left = S.bad[w]; left; left &= left - 1) {
+                                const int key = bad0 + 32 * w + __ffs(left) - 1;
+                                if (!(seen_bits(a, it, j, key - ctx, n_keys - key) & 1)) continue;
+                                const T * q = row_at<const T>(a, a.q, a.q_stride, it, m);
+                                const C * kr = token_at<C, D>(a, it, a.k, key), * vr = token_at<C, D>(a, it, a.v, key) + c;
+                                float z = 0.f;
+#pragma unroll 1
+                                for (int d = 0; d < D; ++d) z += static_cast<float>(q[d]) * static_cast<float>(kr[d]);
+                                const float u = exp2_fast(fmaf(z, a.scale, top == -INFINITY ? 0.f : -top)) * inv;
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) v[k] += u * static_cast<float>(vr[k]);
+                            }
+                    }
                     if (!whole) {
 #pragma unroll
                         for (int k = 0; k < 32; k += 4) pc[(c + k) / 4 * ROWS] = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);

@@ -398,6 +398,41 @@ def test_attend_large_and_infinite_scores(dev):
     assert (out.cpu().double().view(T, H, D) - want).abs().max() < 2.0 ** -8 * c.v[0].nan_to_num(0).abs().max()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("H,G,D", [(4, 2, 128), (2, 2, 64)])
+@pytest.mark.parametrize("parent", ["tree", None])
+@pytest.mark.parametrize("ctx,new", [([20, 0], [5, 3]), ([37, 130], [14, 9]), ([100, 3], [33, 64]), ([5, 250], [150, 40])])
+def test_attend_values_that_are_not_finite_stay_with_those_who_look(dev, dtype, H, G, D, parent, ctx, new):
+    """K and V of a new row that hold NaN or infinity: only rows that see it (its descendants, the later
+    rows of a chain) are affected, in the dims that they concern; its siblings' results are as without it."""
+    tt, _, kt, kcode = TYPES[dtype]
+    c = Cache(dev, rows=2, blocks=20, G=G, D=D, kt=kt, code=kcode)
+    planned(c, [0, 0], ctx, None)
+    g = planned(c, ctx, new, parent)
+    fill_tokens(c, g, torch.Generator().manual_seed(4), kt)
+    for i, j, pool, dims, what in ((0, 2, "v", slice(None), math.nan), (1, 1, "v", slice(3, 7), math.inf), (0, new[0] - 1, "v", slice(0, 1), -math.inf),
+                                   (1, new[1] - 1, "k", slice(None), math.nan)):
+        slot = g.s.slot[g.s.cu[i] + j]
+        getattr(c, pool)[0][slot // 16, 0, slot % 16, dims] = what
+    gen = torch.Generator().manual_seed(1)
+    T = g.rows
+    q = torch.randn(T, H * D, generator=gen).to(tt)
+    qd, out = q.cuda(), torch.zeros(T, H * D, dtype=tt, device="cuda")
+    a = engine.AttendArgs(q=qd.data_ptr(), out=out.data_ptr(), dtype=TYPES[dtype][1], n_head=H, scale=D ** -0.5)
+    c.h.attend(g.c, 0, a, stream=0)
+    torch.cuda.synchronize()
+    want, _ = op.attend(c.t, g.s, q.double().reshape(T, H, D), c.k[0].cpu().double(), c.v[0].cpu().double(), D ** -0.5)
+    got = out.cpu().double().reshape(T, H, D)
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+    assert torch.equal(got[got.isinf()], want[want.isinf()])
+    fine = want.isfinite()
+    assert fine.any() and not fine.all()
+    # the scores of standard normal values are below 8; the tolerance of the finite ones as in check_attend
+    vmax, L = 6.0, max(x + n for x, n in zip(ctx, new))
+    tol = vmax * (2.0 ** -19 * 8 * 12 + 2.0 ** -20 + L * 2.0 ** -24 + (0 if dtype == "f32" else U[dtype]))
+    assert ((got - want)[fine].abs() <= tol + U[dtype] * want[fine].abs()).all()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 def test_attend_strides_table_rows_and_no_lse(dev, dtype):
     c = Cache(dev, rows=6, blocks=8)
