@@ -37,11 +37,14 @@ void Pages::attend(const navi_step & s, int layer, const navi_attend_args & q, c
     if (a.group > 1) a.group_mul = static_cast<uint32_t>(((1ull << 32) + static_cast<uint64_t>(a.group) - 1) / static_cast<uint64_t>(a.group));
     if ((a.group & (a.group - 1)) != 0 && (most + 512) * a.group * a.group >= 1ll << 32) fail("pages attend: too many rows for this many heads to a KV head", NAVI_E_SHAPE);
     // the list of key tiles that the blocks divide
-    const int64_t rows = most * a.group <= attn::FEW_ROWS ? 16 : 128, items = (most * a.group + rows - 1) / rows * d_.n_kv_head * s.n_req, tiles = (static_cast<int64_t>(d_.max_blocks) * d_.page_size + attn::KT - 1) / attn::KT + 2;
+    const int64_t rows = most * a.group <= attn::FEW_ROWS_SHORT ? 16 : 128, items = (most * a.group + rows - 1) / rows * d_.n_kv_head * s.n_req, tiles = (static_cast<int64_t>(d_.max_blocks) * d_.page_size + attn::KT - 1) / attn::KT + 2;
     if (items * tiles >= 1ll << 31) fail("pages attend: requests x heads x tokens pass 31 bits of key tiles", NAVI_E_SHAPE);
     const int64_t m = most * a.group;
     const size_t at = static_cast<size_t>(2 * layer);
-    if (m <= attn::FEW_ROWS) return attn::attend_few(a, page_maps_[at], page_maps_[at + 1], q.dtype, d_.dtype, static_cast<int>(m), sms, stream);
+    if (m <= attn::FEW_ROWS || (m <= attn::FEW_ROWS_SHORT && s.n_req * d_.n_kv_head < sms)) return attn::attend_few(a, page_maps_[at], page_maps_[at + 1], q.dtype, d_.dtype, static_cast<int>(m), sms, stream);
+    // q by TMA where an item has two tiles of it, by a warp's loads where it has one: 48 trees of up to 33 rows
+    // 101 us by loads and 105 by TMA. 8 chunks of 1000 rows went from 246 to 210 us in the step that brought
+    // TMA and, with it, the waits before a pair of products.
     CUtensorMap qm{};
     if (q.dtype != NAVI_F32 && m > 128 && a.group <= 128 && (a.group & (a.group - 1)) == 0) {
         a.q_boxes = 1;

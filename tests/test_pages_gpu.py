@@ -360,6 +360,20 @@ def test_attend_long(dev, dtype, ctx):
     assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [8, 9, 16, 17])
+@pytest.mark.parametrize("B", [70, 74, 80])
+def test_attend_small_trees_of_many_requests(dev, dtype, rows, B):
+    """16 to 34 rows x heads, on both sides of as many items as a B200 has multiprocessors (148 = 74 x 2)."""
+    tt, _, kt, kcode = TYPES[dtype]
+    ctx, new = [(37 * r) % 210 for r in range(B)], [rows - (r * 5) % (rows + 1) for r in range(B)]
+    c = Cache(dev, rows=B, blocks=16, G=2, kt=kt, code=kcode)
+    planned(c, [0] * B, ctx, None)
+    g = planned(c, ctx, new)
+    fill_tokens(c, g, torch.Generator().manual_seed(B), kt)
+    check_attend(c, g, dtype, 4)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_attend_rows_that_see_nothing(dev, dtype):
     """A mask without a bit and no cached token; refused requests; a token's scores of -inf."""
