@@ -15,7 +15,7 @@ struct AttendArgs;
 //   17 to 32: few while the step has fewer items (requests x KV heads) than the GPU has multiprocessors,
 //     else many. Four trees of up to 16 rows, two heads each, KV 200 to 2048, f32: few 20.6 us,
 //     many 25.7. 48 such requests, KV 255 to 8191: f16 103 and 95 us, f32 134 and 122.
-//   above: many. 48 trees of up to 33 rows, KV 255 to 8191, f16: 97 to 102 us; the simple kernel before it
+//   above: many. 48 trees of up to 33 rows, KV 255 to 8191, f16: 97 to 104 us; the simple kernel before it
 //     (mma.sync tiles of 64 rows, a block each) 394.
 constexpr int FEW_ROWS = 16, FEW_ROWS_SHORT = 32;
 

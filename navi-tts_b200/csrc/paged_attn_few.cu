@@ -35,7 +35,7 @@ template <class C> __device__ __forceinline__ void mma(float (&c)[4], const uint
 // terms and each step's contribution are summed apart and added in f32. 16-bit rows are exact, and
 // p is rounded once to the type that the result has.
 //
-// Measured on one B200: one request of 200,003 tokens, 5 rows, bf16: 129 to 132 us, 6.2 to 6.3 TB/s (a copy
+// Measured on one B200: one request of 200,003 tokens, 5 rows, bf16: 129 to 133 us, 6.2 to 6.3 TB/s (a copy
 // reaches 6.54). 48 single rows over pages of 16: 84 us with a page as one box, 92.7 with one for each 64
 // dims. The tile's rows: 48 single rows, KV 255 to 8191, f32: 88 us in tiles of 8, 150 in tiles of 32; 30
 // such, KV 255 to 2000, f16: 31 and 39. Four single rows at KV 512 take 11 us, of which the data are 1.3; what

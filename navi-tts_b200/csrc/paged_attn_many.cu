@@ -31,7 +31,7 @@ using namespace navi::umma;
 // Measured on one B200: 8 chunks of 1000 bf16 rows over 511 to 4097 tokens: 211 to 222 us, 680 to 720 TFLOP/s;
 // a plain matrix product reaches 1669. 128 rows x 128 keys take about 2000 cycles in the loop, their two products
 // alone 1025 to 1136 in a loop of nothing else. 48 trees of up to 33 f16 rows over 255 to 8191 tokens in pages of
-// 16: 97 to 102 us, 4.5 to 4.7 TB/s. Weights go over in two halves (48 trees 96 us; whole 97). Tried and slower:
+// 16: 97 to 104 us, 4.4 to 4.7 TB/s. Weights go over in two halves (48 trees 96 us; whole 97). Tried and slower:
 // S in units of 64 keys with two buffers a warpgroup (279 us for the chunks, 210 then: an MMA of 64 columns
 // takes as long as one of 128), an MMA warp for each warpgroup (222 us, 204 then).
 constexpr int LAZY = 8;
