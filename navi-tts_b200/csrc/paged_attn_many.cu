@@ -480,8 +480,9 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
             }
             base += 2 * nt;
-            // which warpgroup's sums there are; both read both where they took the key tiles in turn
-            const bool use0 = two ? wg == 0 : nt > 0, use1 = two ? wg == 1 : nt > 1;
+            // which warpgroup's sums there are: none where the rows see no key (a request that is not served); both
+            // read both where they took the key tiles in turn
+            const bool use0 = nt > 0 && (!two || wg == 0), use1 = two ? nt > 0 && wg == 1 : nt > 1;
             if (use0) wait(&S.o_full[0], no0 & 1);
             if (use1) wait(&S.o_full[1], no1 & 1);
             no0 += nt > 0;

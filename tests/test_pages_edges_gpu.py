@@ -1,0 +1,64 @@
+"""Edges of the paged cache's calls (navi_pages_*): requests that are refused, the ends of the types'
+ranges, shared buffers, graphs. Against the plain 64-bit restatement of oracle/pages.py, as
+test_pages_gpu.py, whose caches and steps are used. navi_pages_check follows each attend, so that a wait
+that ran out fails the test even where the results are right."""
+import math
+import random
+
+import pytest
+import torch
+
+from navi_b200 import capi, engine
+from oracle import pages as op
+from test_pages_gpu import TYPES, U, Cache, GpuStep, check_attend, fill_tokens, i32, planned, tree
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    d = engine.Device(0)
+    yield d
+    d.close()
+
+
+# ---- requests that are not served ------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("group,n", [(1, 129), (1, 256), (1, 300), (2, 65), (2, 128), (2, 150), (3, 43), (3, 86), (3, 100)])
+@pytest.mark.parametrize("why", ["full", "shape", "parent"])
+@pytest.mark.parametrize("first", [True, False])
+def test_attend_refused_requests_of_many_rows(dev, dtype, group, n, why, first):
+    """129, about 256 and 300 rows x heads of a request that is not served, before or after one that is:
+    0 and -inf for it, its neighbour as without it."""
+    if why == "parent" and n > 256:
+        pytest.skip("a tree has at most 256 rows")
+    _, _, kt, kcode = TYPES[dtype]
+    need, ctx1, served = -(-n // 16), 70, 9                  # pages of 16; the other request has 70 + 9 tokens, or 16 + 9
+    if why == "full":
+        served = 140
+        blocks, n_pages = max(need, 14), 5 + need - 1 if first else 14
+    elif why == "shape":
+        ctx1, blocks, n_pages = 16, need - 1, 64
+    else:
+        blocks, n_pages = max(need, 5), 64
+    c = Cache(dev, rows=2, blocks=blocks, n_pages=n_pages, G=1, kt=kt, code=kcode)
+    planned(c, [0], [ctx1], None, req=[1])
+    order = [0, 1] if first else [1, 0]
+    ctx, new = [0 if r == 0 else ctx1 for r in order], [n if r == 0 else served for r in order]
+    par = None
+    if why == "parent":
+        rng = random.Random(n)
+        trees = {0: tree(rng, n), 1: tree(rng, served)}
+        trees[0][n - 1] = n - 1                             # not below its row
+        par = sum((trees[r] for r in order), [])
+    g = planned(c, ctx, new, par, req=order)
+    status = g.status.tolist()
+    assert status[order.index(0)] == {"full": capi.NAVI_E_KV_FULL, "shape": capi.NAVI_E_SHAPE, "parent": capi.NAVI_E_ARG}[why]
+    # a later request that needs pages waits for the one that does not fit
+    assert status[order.index(1)] == (capi.NAVI_E_KV_FULL if why == "full" and first else capi.NAVI_OK)
+    fill_tokens(c, g, torch.Generator().manual_seed(n), kt)
+    out, lse = check_attend(c, g, dtype, group)
+    c.h.check(stream=0)
+    a = 0 if first else served
+    assert (out[a:a + n] == 0).all() and (lse[a:a + n] == -math.inf).all()
