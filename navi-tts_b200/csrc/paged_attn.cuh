@@ -83,6 +83,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+// The weights of a softmax enter the product with V as values of the cache's type. bf16 has f32's range; f16 would lose
+// what is 2^-25 of the largest weight, whose sum over a long tail of keys counts (and which the sum of the
+// weights, in f32, has). So with f16 the largest weight is 2^LIFT and not 1: the reference that scores are taken
+// against is LIFT lower, in log2, which cancels in the division, in the join of pieces and in the log of the sum.
+// Rounded up, the reference is never below max scale - LIFT, so that no weight passes 2^LIFT however large the scores.
+__device__ __forceinline__ float reference(float best, float scale, float lift) { return __fmaf_ru(best, scale, -lift); }
+
 // Lets a kernel have `bytes` of dynamic shared memory, asking the runtime once a kernel and device.
 template <class... A> void allow_smem(void (*kernel)(A...), int bytes) {
     static std::mutex lock;

@@ -30,16 +30,19 @@ template <class C> __device__ __forceinline__ void mma(float (&c)[4], const uint
 // so up to 32 rows the bound is HBM.
 //
 // f32 rows enter the products as two f16 terms, q = hi + lo and p = hi + lo, against the exact cache
-// values, about 22 bits. With 8 rows the high terms are rows 0..7 of the 16 that a product has
-// and the low ones rows 8..15, so that they cost nothing. The tensor cores' sums truncate: the low
+// values: about 22 bits of q, and of weights down to 2^-17 of the largest (smaller ones to 2^-39 of
+// it). With 8 rows the high terms are rows 0..7 of the 16 that a product has and the low ones rows
+// 8..15, so that they cost nothing. The tensor cores' sums truncate: the low
 // terms and each step's contribution are summed apart and added in f32. 16-bit rows are exact, and
-// p is rounded once to the type that the result has.
+// p is rounded once to the type that the result has: 8 bits of bf16, 11 of f16 down to 2^-28 of the largest weight.
 //
 // Measured on one B200: one request of 200,003 tokens, 5 rows, bf16: 129 to 133 us, 6.2 to 6.3 TB/s (a copy
 // reaches 6.54). 48 single rows over pages of 16: 84 us with a page as one box, 92.7 with one for each 64
 // dims. The tile's rows: 48 single rows, KV 255 to 8191, f32: 88 us in tiles of 8, 150 in tiles of 32; 30
 // such, KV 255 to 2000, f16: 31 and 39. Four single rows at KV 512 take 11 us, of which the data are 1.3; what
 // is left is launch and one trip to L2 after another: the work list, q and pages, the tile, the join.
+template <class C> constexpr float LIFT = std::is_same_v<C, __half> ? 14.f : 0.f;   // f16 holds 65504
+
 template <int D> struct FewSmem {
     static constexpr int STAGE = KT * D * 4;                    // K and V of a tile
     static constexpr int STAGES = D == 128 ? 3 : 6;
@@ -292,7 +295,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
 #pragma unroll
                     for (int y = 0; y < 2 * KS; ++y) m[x] = fmaxf(m[x], fmaxf(sc[y][2 * x], sc[y][2 * x + 1]));
                     m[x] = fmaxf(m[x], __shfl_xor_sync(0xffffffffu, m[x], 1));
-                    m[x] = fmaxf(m[x], __shfl_xor_sync(0xffffffffu, m[x], 2)) * a.scale;
+                    m[x] = reference(fmaxf(m[x], __shfl_xor_sync(0xffffffffu, m[x], 2)), a.scale, LIFT<C>);
                     more = more || m[x] > mx[x];
                 }
                 if (__any_sync(0xffffffffu, more)) {

@@ -23,7 +23,8 @@ using namespace navi::umma;
 //   S(0) S(1) | P V(0) S(2) | P V(1) S(3) | ...     each P V after its warpgroup has written P
 // A commit covers all that was issued before it, so when S(n) is there P V(n - 2), the last to
 // touch this warpgroup's O, is done too, and the warpgroup may rescale O. It does so only where
-// a row's maximum grew by more than 2^8: weights up to 2^8 are as exact, and sums are f32.
+// a row's maximum grew by more than 2^LAZY: bf16 weights up to 2^8 are as exact, and sums are f32. f16 weights
+// are 2^14 at first and up to 2^15 (LIFT + LAZY, of 65504), so that a long tail keeps its weights: see reference().
 //
 // f32 rows: q and p as two f16 terms each against the exact cache values, as in the kernel for few
 // rows. Two tiles of q do not fit then, so their items have 128 rows.
@@ -34,7 +35,11 @@ using namespace navi::umma;
 // 16: 97 to 104 us, 4.4 to 4.7 TB/s. Weights go over in two halves (48 trees 96 us; whole 97). Tried and slower:
 // S in units of 64 keys with two buffers a warpgroup (279 us for the chunks, 210 then: an MMA of 64 columns
 // takes as long as one of 128), an MMA warp for each warpgroup (222 us, 204 then).
-constexpr int LAZY = 8;
+// f16: LAZY 1, 2, 3, 5 and 8 with LIFT to match (15 - LAZY): 48 trees 99.8, 99.0, 98.6, 98.1 and 98.0 us, 8 chunks of
+// f16 rows 219, 224, 218, 221 and 216, of f32 rows 431, 429 to 435, 417, 429 and 436 (410 to 419 without LIFT): the
+// closest was taken.
+template <class C> constexpr float LIFT = std::is_same_v<C, __half> ? 14.f : 0.f;
+template <class C> constexpr float LAZY = std::is_same_v<C, __half> ? 1.f : 8.f;
 constexpr int EXTRA = 1;                                        // what an item costs beside its key tiles, in key tiles. 48 trees with 0 to 3: 102, 102, 108, 113 us; 8 chunks 217, 210, 211, 209
 
 template <class T, int D, int ROWS> struct ManySmem {
@@ -439,10 +444,10 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int k = 0; k < KT; k += 2) mx[k / 2 & 3] = max3(mx[k / 2 & 3], __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
-                const float best = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale;
+                const float best = reference(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), a.scale, LIFT<C>);
                 if (!any) {
                     top = best;
-                } else if (__any_sync(0xffffffffu, best > top + LAZY)) {
+                } else if (__any_sync(0xffffffffu, best > top + LAZY<C>)) {
                     const float now = fmaxf(best, top), w = now == -INFINITY ? 1.f : exp2_fast(top - now);
                     top = now;
                     sum *= w;

@@ -62,3 +62,43 @@ def test_attend_refused_requests_of_many_rows(dev, dtype, group, n, why, first):
     c.h.check(stream=0)
     a = 0 if first else served
     assert (out[a:a + n] == 0).all() and (lse[a:a + n] == -math.inf).all()
+
+
+# ---- the ends of the types' ranges ------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("new,H", [(1, 2), (5, 2), (12, 2), (40, 2), (90, 2)])
+@pytest.mark.parametrize("ctx,nats", [(700, 10.0), (8192, 18.0), (8192, 20.0), (60000, 17.0)])
+def test_attend_long_tail_under_a_few_large_weights(dev, dtype, new, H, ctx, nats):
+    """Every 16th key far above the others, and V zero there: the result is the others' sum alone, which a
+    weight that is dropped or rounded to a multiple of 2^-24 of the largest would show.
+
+    Weights: 2^-25 of f16's terms against 2^(13 - nats log2 e) at the least (an f16 cache), their one rounding
+    (16-bit rows), scores of up to 60 in f32 (60 x 2^-23 twice, and the same of log2 e), sums over the keys of
+    relative 2^-23 a 16-key step."""
+    tt, _, kt, kcode = TYPES[dtype]
+    D, page = 128, 64
+    c = Cache(dev, rows=1, blocks=-(-(ctx + new) // page), page=page, G=1, D=D, kt=kt, code=kcode, fill=0)
+    planned(c, [0], [ctx], None)
+    g = planned(c, [ctx], [new])
+    c.v[..., 0::2], c.v[..., 1::2] = 1.0, 1.5
+    scale, q0, top = D ** -0.5, 8.0, 64.0                   # scores up to 45
+    low = float(torch.tensor(top - nats / (scale * q0)).to(kt))
+    c.k[..., 0] = low
+    where = torch.tensor(c.t.table[0])[:-(-ctx // page)].cuda()
+    keys = torch.arange(0, ctx, 16, device="cuda")
+    c.k[0, where[keys // page], 0, keys % page, 0] = top
+    c.v[0, where[keys // page], 0, keys % page] = 0.0
+    q = torch.zeros(new, H, D)
+    q[..., 0] = q0
+    qd, out = q.to(tt).cuda(), torch.zeros(new, H, D, dtype=tt, device="cuda")
+    c.h.attend(g.c, 0, engine.AttendArgs(q=qd.data_ptr(), out=out.data_ptr(), dtype=TYPES[dtype][1], n_head=H, scale=scale), stream=0)
+    c.h.check(stream=0)
+    gap = (top - low) * q0 * scale
+    many = torch.tensor([len(a) for a in g.s.anc]).double() + ctx - len(keys)
+    share = many * math.exp(-gap) / (many * math.exp(-gap) + len(keys))
+    want = share[:, None, None] * torch.where(torch.arange(D) % 2 == 0, 1.0, 1.5).double()
+    rel = 2.0 ** (gap * math.log2(math.e) - 13 - 25) if kt == torch.float16 else 0.0
+    rel += 4 * 60 * 2.0 ** -23 + (ctx + new) / 16 * 2.0 ** -23 + (0 if dtype == "f32" else U[dtype])
+    tiny = 2.0 ** -25 if dtype == "f16" else 0.0            # f16's own smallest step in the result
+    assert ((out.cpu().double() - want).abs() <= (rel + U[dtype]) * want + tiny).all(), ((out.cpu().double() / want - 1).abs().max(), rel)
