@@ -76,6 +76,25 @@ template <class C> __device__ __forceinline__ void split_pair(float x, float y, 
     const float2 b = unpack<C>(hi);
     lo = pack<C>(x - b.x, y - b.y);
 }
+// A row of f32 q is brought to magnitudes of up to 2^15 by a power of two before the split, and its scores back by the
+// inverse in their scale: f16 would take values from 65520 on as infinity and keep few bits of small ones.
+// From the row's largest magnitude: the exponent field of that power, 2^(field - 127), 14..253 (127 if it is not finite).
+__device__ __forceinline__ uint32_t row_field(float largest) {
+    const uint32_t e = __float_as_uint(largest) >> 23;
+    return e == 255 ? 127 : min(268 - e, 253u);
+}
+__device__ __forceinline__ float row_up(uint32_t field) { return __uint_as_float(field << 23); }
+// The scale of such a row's scores. It stays above 0 and finite, as a score of -inf or 0 times it has to stay what it is.
+__device__ __forceinline__ float row_scale(float scale, uint32_t field) {
+    return fminf(fmaxf(scale * __uint_as_float((254 - field) << 23), 1.17549435e-38f), 3.40282347e38f);
+}
+__device__ __forceinline__ float largest4(float4 v) { return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))); }
+// The largest over N neighbouring lanes (N a power of two, lanes from a multiple of N on).
+template <int N> __device__ __forceinline__ float lanes_max(float x) {
+#pragma unroll
+    for (int o = 1; o < N; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
+}
 // 2^x by the hardware's approximation (two units of the last place); 2^-inf = 0
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;

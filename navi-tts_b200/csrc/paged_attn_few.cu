@@ -83,6 +83,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
     __shared__ __align__(8) uint64_t full[L::STAGES], empty[L::STAGES];
     __shared__ __align__(8) SegmentRing segs;
     __shared__ float stat[8][2][MR];
+    __shared__ float q_scale[SPLIT ? ROWS : 1];   // f32 rows: each row's scale of the scores
     __shared__ uint32_t bad[16];   // tokens from the item's first masked tile on whose V is not finite
     __shared__ int red[9];
     __shared__ Share share;
@@ -178,34 +179,42 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
         if (named_sync_or(1, 256, !got)) break;
         const Segment & s = segs.s[sn % SegmentRing::N];
         if (s.nt < 0) break;
-        // q into shared memory, a thread 8 values
+        // q into shared memory, a thread 8 values, whole rows a warp
 #pragma unroll 1
         for (int x = tid; x < ROWS * (D / 8); x += 256) {
             const int m = x / (D / 8), c = x % (D / 8);
             uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+            float4 f = make_float4(0.f, 0.f, 0.f, 0.f), g = f;   // f32 rows
             if (m < s.m) {
                 const T * src = row_at<const T>(a, a.q, a.q_stride, s, m) + c * 8;
                 if constexpr (SPLIT) {
-                    const float4 f = *reinterpret_cast<const float4 *>(src), g = *reinterpret_cast<const float4 *>(src + 4);
-                    split_pair<C>(f.x, f.y, hi.x, lo.x);
-                    split_pair<C>(f.z, f.w, hi.y, lo.y);
-                    split_pair<C>(g.x, g.y, hi.z, lo.z);
-                    split_pair<C>(g.z, g.w, hi.w, lo.w);
+                    f = *reinterpret_cast<const float4 *>(src);
+                    g = *reinterpret_cast<const float4 *>(src + 4);
                 } else {
                     hi = *reinterpret_cast<const uint4 *>(src);
                 }
+            }
+            if constexpr (SPLIT) {
+                const uint32_t field = row_field(lanes_max<D / 8>(fmaxf(largest4(f), largest4(g))));
+                const float up = row_up(field);
+                split_pair<C>(f.x * up, f.y * up, hi.x, lo.x);
+                split_pair<C>(f.z * up, f.w * up, hi.y, lo.y);
+                split_pair<C>(g.x * up, g.y * up, hi.z, lo.z);
+                split_pair<C>(g.z * up, g.w * up, hi.w, lo.w);
+                if (c == 0) q_scale[m] = row_scale(a.scale, field);
             }
             uint8_t * dst = qs + m * (D * 2) + ((c ^ (m & 7)) << 4);
             *reinterpret_cast<uint4 *>(dst) = hi;
             if constexpr (SPLIT || EIGHT) *reinterpret_cast<uint4 *>(dst + (EIGHT ? 8 : ROWS) * D * 2) = lo;
         }
         named_sync(1, 256);
-        float o[D / 8][2 * XR], mx[XR], l[XR];
+        float o[D / 8][2 * XR], mx[XR], l[XR], scale[XR];
         int row[XR];
 #pragma unroll
         for (int x = 0; x < XR; ++x) {
             mx[x] = -INFINITY;
             l[x] = 0.f;
+            scale[x] = SPLIT ? q_scale[SPLIT ? rt * 16 + gq + 8 * x : 0] : a.scale;
             row[x] = by_group(a, s.m0 + min(rt * 16 + gq + 8 * x, s.m - 1));
         }
 #pragma unroll
@@ -295,7 +304,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
 #pragma unroll
                     for (int y = 0; y < 2 * KS; ++y) m[x] = fmaxf(m[x], fmaxf(sc[y][2 * x], sc[y][2 * x + 1]));
                     m[x] = fmaxf(m[x], __shfl_xor_sync(0xffffffffu, m[x], 1));
-                    m[x] = reference(fmaxf(m[x], __shfl_xor_sync(0xffffffffu, m[x], 2)), a.scale, LIFT<C>);
+                    m[x] = reference(fmaxf(m[x], __shfl_xor_sync(0xffffffffu, m[x], 2)), scale[x], LIFT<C>);
                     more = more || m[x] > mx[x];
                 }
                 if (__any_sync(0xffffffffu, more)) {
@@ -321,7 +330,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
 #pragma unroll
                         for (int y = 0; y < 2; ++y) {
                             const float * v = sc[2 * k + y] + 2 * x;
-                            const float p0 = exp2_fast(fmaf(v[0], a.scale, -ref)), p1 = exp2_fast(fmaf(v[1], a.scale, -ref));
+                            const float p0 = exp2_fast(fmaf(v[0], scale[x], -ref)), p1 = exp2_fast(fmaf(v[1], scale[x], -ref));
                             l[x] += p0 + p1;
                             if constexpr (TERMS) split_pair<C>(p0, p1, ph[k][2 * y + x], pl[k][2 * y + x]);
                             else if constexpr (SPLIT) split_pair<C>(p0, p1, ph[k][2 * y], ph[k][2 * y + 1]);

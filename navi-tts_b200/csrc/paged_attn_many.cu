@@ -27,7 +27,8 @@ using namespace navi::umma;
 // are 2^14 at first and up to 2^15 (LIFT + LAZY, of 65504), so that a long tail keeps its weights: see reference().
 //
 // f32 rows: q and p as two f16 terms each against the exact cache values, as in the kernel for few
-// rows. Two tiles of q do not fit then, so their items have 128 rows.
+// rows. Two tiles of q do not fit then, so their items have 128 rows. Bringing each row of q to f16's range costs
+// 4 to 5 % there (48 trees of up to 33 f32 rows 125 -> 132 us, 8 chunks 422 -> 434).
 //
 // Measured on one B200: 8 chunks of 1000 bf16 rows over 511 to 4097 tokens: 211 to 222 us, 680 to 720 TFLOP/s;
 // a plain matrix product reaches 1669. 128 rows x 128 keys take about 2000 cycles in the loop, their two products
@@ -54,8 +55,9 @@ template <class T, int D, int ROWS> struct ManySmem {
 };
 
 struct ManyControl {
-    uint64_t full[8], empty[8], q_full, q_empty, s_full[2], p_full[2][2], o_full[2], drained;
+    uint64_t full[8], empty[8], q_full, q_empty, s_full[2], p_full[2][2], o_full[2], drained, q_scaled[2];
     float stat[2][2][128];
+    uint8_t q_field[2][128];     // f32 rows: row_field of this segment's and the next one's
     uint32_t bad[16];            // tokens from the first masked tile on whose V is not finite
     SegmentRing segs;
     int red[12];
@@ -135,6 +137,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
             mbar_init(&S.p_full[g][0], 128);
             mbar_init(&S.p_full[g][1], 128);
             mbar_init(&S.o_full[g], 1);
+            mbar_init(&S.q_scaled[g], 64);
         }
         mbar_init(&S.drained, 1);
         S.segs.init(11);
@@ -360,11 +363,15 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                             const int m = m1 + k * STEP;
                             uint8_t * dst = qs + (m >> 7) * L::QTILE + (c >> 3) * (128 * 128) + (m & 127) * 128 + (((c & 7) ^ (m & 7)) << 4);
                             if constexpr (SPLIT) {
+                                const float4 f = *reinterpret_cast<const float4 *>(&v[k]), g = *reinterpret_cast<const float4 *>(&w[k]);
+                                const uint32_t field = row_field(lanes_max<CH>(fmaxf(largest4(f), largest4(g))));
+                                const float up = row_up(field);
                                 uint4 hi, lo;
-                                split_pair<C>(__uint_as_float(v[k].x), __uint_as_float(v[k].y), hi.x, lo.x);
-                                split_pair<C>(__uint_as_float(v[k].z), __uint_as_float(v[k].w), hi.y, lo.y);
-                                split_pair<C>(__uint_as_float(w[k].x), __uint_as_float(w[k].y), hi.z, lo.z);
-                                split_pair<C>(__uint_as_float(w[k].z), __uint_as_float(w[k].w), hi.w, lo.w);
+                                split_pair<C>(f.x * up, f.y * up, hi.x, lo.x);
+                                split_pair<C>(f.z * up, f.w * up, hi.y, lo.y);
+                                split_pair<C>(g.x * up, g.y * up, hi.z, lo.z);
+                                split_pair<C>(g.z * up, g.w * up, hi.w, lo.w);
+                                if (c == 0) S.q_field[(nq - 1) & 1][m] = static_cast<uint8_t>(field);
                                 *reinterpret_cast<uint4 *>(dst) = hi;
                                 *reinterpret_cast<uint4 *>(dst + L::QTILE) = lo;
                             } else {
@@ -374,6 +381,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                     }
                     fence_proxy_async_smem();
                     mbar_arrive(&S.q_full);
+                    if constexpr (SPLIT) mbar_arrive(&S.q_scaled[(nq - 1) & 1]);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&S.segs.empty[sn % SegmentRing::N]);
@@ -399,8 +407,12 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
             // every row of the warp sees the tokens before `open`
             const int open = ctx + (a.mask ? 0 : by_group(a, it.m0 + min((two ? wg * 128 : 0) + (warp & 3) * 32, it.m - 1)) + 1);
             const int open0 = ctx + (a.mask ? 0 : by_group(a, it.m0) + 1), bad0 = open0 / KT * KT;   // the same for the item; its first masked tile
-            float top = -INFINITY, sum = 0.f;
+            float top = -INFINITY, sum = 0.f, scale = a.scale;
             bool any = false;                             // this warpgroup has had a tile
+            if (SPLIT && wg < nt) {   // this place is next written two segments on, behind the weights of this one
+                wait(&S.q_scaled[no0 & 1], (no0 >> 1) & 1);
+                scale = row_scale(a.scale, S.q_field[no0 & 1][r]);
+            }
             for (int x = two ? 0 : wg; x < nt; x += two ? 1 : 2, ++ns) {
                 if (!wait(&S.s_full[wg], ns & 1)) break;
                 fence_after_sync();
@@ -444,7 +456,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int k = 0; k < KT; k += 2) mx[k / 2 & 3] = max3(mx[k / 2 & 3], __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
-                const float best = reference(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), a.scale, LIFT<C>);
+                const float best = reference(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), scale, LIFT<C>);
                 if (!any) {
                     top = best;
                 } else if (__any_sync(0xffffffffu, best > top + LAZY<C>)) {
@@ -462,7 +474,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 }
                 any = true;
                 const float ref = top == -INFINITY ? 0.f : top;
-                const float2 scale2 = make_float2(a.scale, a.scale), ref2 = make_float2(-ref, -ref);
+                const float2 scale2 = make_float2(scale, scale), ref2 = make_float2(-ref, -ref);
                 float2 part[2] = {};
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {

@@ -102,3 +102,32 @@ def test_attend_long_tail_under_a_few_large_weights(dev, dtype, new, H, ctx, nat
     rel += 4 * 60 * 2.0 ** -23 + (ctx + new) / 16 * 2.0 ** -23 + (0 if dtype == "f32" else U[dtype])
     tiny = 2.0 ** -25 if dtype == "f16" else 0.0            # f16's own smallest step in the result
     assert ((out.cpu().double() - want).abs() <= (rel + U[dtype]) * want + tiny).all(), ((out.cpu().double() / want - 1).abs().max(), rel)
+
+
+@pytest.mark.parametrize("new,H,D", [(1, 2, 128), (4, 4, 64), (7, 2, 128), (16, 2, 64), (50, 2, 128), (150, 1, 64)])
+@pytest.mark.parametrize("size", [1e5, 1e-4, 1e30, 1e-20])
+@pytest.mark.parametrize("ctx", [90, 1500])
+def test_attend_f32_rows_of_any_size(dev, new, H, D, size, ctx):
+    """f32 q far from 1, its magnitude taken out again by the scale, a row of another magnitude, a row of zeros: the
+    tolerance of standard normal rows (check_attend's), as the scores are theirs."""
+    c = Cache(dev, rows=1, blocks=-(-(ctx + new) // 16), G=1, D=D, fill=0)
+    c.k.normal_(generator=torch.Generator("cuda").manual_seed(1))
+    c.v.normal_(generator=torch.Generator("cuda").manual_seed(2))
+    planned(c, [0], [ctx], None)
+    g = planned(c, [ctx], [new])
+    x = torch.randn(new, H, D, generator=torch.Generator().manual_seed(new))
+    x[0, 0, 1:] *= 2.0 ** -9
+    if new > 2:
+        x[1] *= 2.0 ** -12
+        x[2, H - 1] = 0
+    q = x * size
+    qd, out, lse = q.cuda(), torch.zeros(new, H, D, device="cuda"), torch.zeros(new, H, device="cuda")
+    scale = D ** -0.5 / size
+    c.h.attend(g.c, 0, engine.AttendArgs(q=qd.data_ptr(), out=out.data_ptr(), lse=lse.data_ptr(), dtype=capi.NAVI_F32, n_head=H, scale=scale), stream=0)
+    c.h.check(stream=0)
+    kd, vd = c.k[0].cpu().double(), c.v[0].cpu().double()
+    want, wl = op.attend(c.t, g.s, q.double(), kd, vd, scale)
+    ds = 2.0 ** -20 * scale * float(q.double().abs().sum(2).max()) * float(kd.abs().max())
+    tol = float(vd.abs().max()) * (2 * ds + 2.0 ** -20 + (ctx + new) * 2.0 ** -24)
+    assert ((out.cpu().double() - want).abs() <= tol + 2.0 ** -24 * want.abs()).all(), (out.cpu().double() - want).abs().max()
+    assert ((lse.cpu().double() - wl).abs() <= ds + 2.0 ** -20 + (ctx + new) * 2.0 ** -24 + 2.0 ** -22 * wl.abs()).all()
