@@ -424,7 +424,8 @@ typedef struct navi_step {
     int32_t * row_req;             /* [max_rows]: index 0..n_req-1 of the row's request */
     int32_t * pos;                 /* [max_rows]: ctx_len + depth, the RoPE position */
     int64_t * slot;                /* [max_rows]: page * page_size + offset where the row's K/V go, -1: nowhere */
-    uint64_t * mask;               /* [max_rows][mask_words]: bit a = row a of the request is the row itself or an ancestor */
+    uint64_t * mask;               /* [max_rows][mask_words], NULL with mask_words 0: bit a = row a of the request is the row
+                                      itself or an ancestor */
     int32_t * status;              /* [n_req]: NAVI_OK, or why the request is not served:
                                       NAVI_E_KV_FULL  too few free pages: it waits, and with it every later request that needs pages
                                       NAVI_E_SHAPE    longer than the block table, max_new or max_rows allow

@@ -645,7 +645,7 @@ void Pages::check_step(const navi_step & s, const char * who) const {
     if (s.max_rows > 0 && (!s.row_req || !s.pos || !s.slot)) refuse(": row_req, pos and slot are needed", NAVI_E_ARG);
     if (s.parent) {
         if (s.max_new > NAVI_STEP_MAX_TREE) refuse(": a tree has at most NAVI_STEP_MAX_TREE rows", NAVI_E_SHAPE);
-        if (s.mask_words < 0 || s.mask_words > NAVI_STEP_MAX_TREE / 64 || 64 * s.mask_words < s.max_new || (s.max_new > 0 && !s.mask))
+        if (s.mask_words < 0 || s.mask_words > NAVI_STEP_MAX_TREE / 64 || 64 * s.mask_words < s.max_new || (s.mask_words > 0 && !s.mask))
             refuse(": mask of 64 * mask_words >= max_new bits is needed with parent", NAVI_E_ARG);
     }
 }

@@ -131,3 +131,29 @@ def test_attend_f32_rows_of_any_size(dev, new, H, D, size, ctx):
     tol = float(vd.abs().max()) * (2 * ds + 2.0 ** -20 + (ctx + new) * 2.0 ** -24)
     assert ((out.cpu().double() - want).abs() <= tol + 2.0 ** -24 * want.abs()).all(), (out.cpu().double() - want).abs().max()
     assert ((lse.cpu().double() - wl).abs() <= ds + 2.0 ** -20 + (ctx + new) * 2.0 ** -24 + 2.0 ** -22 * wl.abs()).all()
+
+
+# ---- arguments ----------------------------------------------------------------------------------------
+
+def refused(status, fn, *a, **kw):
+    with pytest.raises(capi.NaviError) as e:
+        fn(*a, **kw)
+    assert e.value.status == status and len(str(e.value)) > 12
+
+
+def step_with(g, **kw):
+    return engine.TreeStep(**{**{n: getattr(g.c.s, n) for n, _ in capi.Step._fields_}, **kw})
+
+
+def test_plan_without_a_mask(dev):
+    """Words of a mask without a mask are refused, whatever max_new says; max_new 0 and no words are a step whose requests
+    with rows are refused, each by its status."""
+    c = Cache(dev, rows=2, blocks=4)
+    g = planned(c, [3, 0], [2, 0])
+    for kw in (dict(max_new=0, mask_words=1, mask=0), dict(max_new=0, mask_words=4, mask=0), dict(max_new=2, mask_words=1, mask=0),
+               dict(max_new=1, mask_words=0, mask=0)):
+        for call in (lambda s: c.h.plan(s, stream=0), lambda s: c.h.commit(s, engine.CommitArgs(width=1), stream=0)):
+            refused(capi.NAVI_E_ARG, call, step_with(g, **kw))
+    c.h.plan(step_with(g, max_new=0, mask_words=0, mask=0), stream=0)
+    torch.cuda.synchronize()
+    assert g.status.tolist() == [capi.NAVI_E_SHAPE, capi.NAVI_OK] and g.slot.tolist() == [-1, -1]
