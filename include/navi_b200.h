@@ -378,7 +378,7 @@ int navi_conv1d(navi_device * dev, const navi_conv_args * a);
  *
  * Every call only enqueues work on `stream` (a cudaStream_t, as everywhere in CUDA NULL is the
  * legacy default stream; navi_device_stream gives the engine's) and returns. A device's first
- * plan or attend on each stream takes that stream's scratch (make it before capturing the
+ * plan, attend or in-place commit on each stream takes that stream's scratch (make it before capturing the
  * stream); nothing else allocates. The calls of one cache are ordered by the caller: on one
  * stream, or by events between streams. */
 #define NAVI_PAGES_MAX_LAYERS 128
@@ -480,6 +480,8 @@ typedef struct navi_commit_args {
     int32_t * path;                /* device [max_rows]: of each request its accepted rows in order, then -1 */
     int32_t * new_len;             /* device [n_req]: ctx_len + accepted */
     int32_t * next_token;          /* device [n_req][width]: the model's choice after the branch */
+                                   /* The outcome does not overlap the ids above, but next_token may be root_target, and
+                                      new_len the step's ctx_len */
 } navi_commit_args;
 /* From the root down, the lowest-numbered child whose ids equal the model's choice is accepted.
  * The accepted rows' K and V move to the tokens ctx_len .. new_len - 1 in every layer, in place.

@@ -13,6 +13,7 @@
 #include <cstring>
 #include <string>
 #include <type_traits>
+#include <utility>
 
 namespace navi {
 
@@ -455,6 +456,7 @@ struct CommitArgs {
     navi_step s;
     navi_commit_args c;
     uint8_t * k[NAVI_PAGES_MAX_LAYERS], * v[NAVI_PAGES_MAX_LAYERS];
+    int * walked;                       // next_token is root_target: the blocks of a request that have walked; else nullptr
     int n_layer, n_kv, shift, chunks;   // chunks: 16-byte pieces of one head's row
     int n_pages;
 };
@@ -516,10 +518,23 @@ __global__ void __launch_bounds__(COMMIT_THREADS) k_pages_commit(const __grid_co
     }
     __syncthreads();
     const int k0 = moved, k1 = count;
+    const int32_t * nx = k1 > 0 ? a.c.targets + static_cast<size_t>(r0 + path[k1 - 1]) * W : a.c.root_target + static_cast<size_t>(i) * W;
+    int32_t * next = a.c.next_token + static_cast<size_t>(i) * W;
+    if (a.walked && tid >= COMMIT_THREADS - 32) {   // over the ids that the other blocks compare: by the last of them, when all have
+        const int lane = tid & 31;
+        int last = 0;
+        if (lane == 0) {
+            __threadfence();
+            last = atomicAdd(a.walked + i, 1) == static_cast<int>(gridDim.y) - 1;
+            if (last) a.walked[i] = 0;
+        }
+        if (__shfl_sync(0xffffffffu, last, 0))
+            for (int x = lane; x < W; x += 32) next[x] = nx[x];
+    }
     if (blockIdx.y == 0) {
         for (int j = tid; j < n; j += COMMIT_THREADS) a.c.path[r0 + j] = j < k1 ? path[j] : -1;
-        const int32_t * nx = k1 > 0 ? a.c.targets + static_cast<size_t>(r0 + path[k1 - 1]) * W : a.c.root_target + static_cast<size_t>(i) * W;
-        for (int x = tid; x < W; x += COMMIT_THREADS) a.c.next_token[static_cast<size_t>(i) * W + x] = nx[x];
+        if (!a.walked)
+            for (int x = tid; x < W; x += COMMIT_THREADS) next[x] = nx[x];
         if (tid == 0) {
             a.c.accepted[i] = k1;
             a.c.new_len[i] = a.s.ctx_len[i] + k1;
@@ -565,6 +580,11 @@ CUtensorMap pool_map(void * pool, const navi_pages_desc & d, bool whole) {
     const cuuint64_t dims[2] = {64 * halves, rows}, strides[1] = {row};
     const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(d.page_size)};
     return swizzled_map(pool, d.dtype, 2, dims, strides, box);
+}
+
+bool overlap(const void * a, size_t na, const void * b, size_t nb) {
+    const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return na > 0 && nb > 0 && x < y + nb && y < x + na;
 }
 
 bool aligned16(const void * p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -701,8 +721,18 @@ void Pages::commit(const navi_step & s, const navi_commit_args & c, cudaStream_t
     if (!s.parent) fail("pages commit: the step has no parent (there is no tree to walk)", NAVI_E_ARG);
     if (!c.root_target || !c.accepted || !c.new_len || !c.next_token) fail("pages commit: NULL argument", NAVI_E_ARG);
     if (s.max_rows > 0 && (!c.tokens || !c.targets || !c.path)) fail("pages commit: NULL argument", NAVI_E_ARG);
+    // Blocks of a request read its ids while another of them writes the outcome
+    const size_t ids = static_cast<size_t>(s.max_rows) * c.width, reqs = static_cast<size_t>(s.n_req);
+    const std::pair<const int32_t *, size_t> in[] = {{c.tokens, ids}, {c.targets, ids}, {c.root_target, reqs * c.width}},
+                                             out[] = {{c.next_token, reqs * c.width}, {c.accepted, reqs}, {c.path, static_cast<size_t>(s.max_rows)}, {c.new_len, reqs}};
+    const bool in_place = c.next_token == c.root_target;
+    for (const auto & o : out)
+        for (const auto & i : in)
+            if (overlap(o.first, o.second * 4, i.first, i.second * 4) && !(in_place && o.first == c.next_token && i.first == c.root_target))
+                fail("pages commit: the outcome overlaps the ids (next_token may be root_target)", NAVI_E_ARG);
     NAVI_CUDA(cudaSetDevice(dev_->info().ordinal));
     CommitArgs a{};
+    if (in_place) a.walked = PagesScratch(dev_->scratch(stream, PagesScratch::bytes(dev_->info().multiprocessors)), dev_->info().multiprocessors).broken;
     a.s = s;
     a.c = c;
     for (int l = 0; l < d_.n_layer; ++l) {

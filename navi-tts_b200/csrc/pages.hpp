@@ -51,7 +51,7 @@ private:
 struct PagesScratch {
     static constexpr size_t TICKETS = 64;                            // launch-wide counters
     static constexpr size_t PIECE_FLOATS = 256 * (128 + 2);          // attend: one block's unfinished item
-    int * tickets, * broken, * arrived, * err;                       // broken: plan, a request with a bad parent
+    int * tickets, * broken, * arrived, * err;                       // broken: plan, a request with a bad parent; commit, blocks
     float * pieces;                                                  // two a block
 
     // `blocks`: the most blocks of a launch that leave pieces (one a multiprocessor)

@@ -10,7 +10,7 @@ import torch
 
 from navi_b200 import capi, engine
 from oracle import pages as op
-from test_pages_gpu import TYPES, U, Cache, GpuStep, check_attend, fill_tokens, i32, planned, tree
+from test_pages_gpu import TYPES, U, Cache, GpuStep, check_attend, drafts, fill_tokens, i32, planned, tree
 
 pytestmark = pytest.mark.gpu
 
@@ -157,3 +157,45 @@ def test_plan_without_a_mask(dev):
     c.h.plan(step_with(g, max_new=0, mask_words=0, mask=0), stream=0)
     torch.cuda.synchronize()
     assert g.status.tolist() == [capi.NAVI_E_SHAPE, capi.NAVI_OK] and g.slot.tolist() == [-1, -1]
+
+
+# ---- shared buffers -------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("width", [1, 5, 16, 40])
+@pytest.mark.parametrize("B", [1, 3, 200])
+def test_commit_in_place(dev, width, B):
+    """One step's next_token is the next one's root_target, its new_len the next one's ctx_len: both in the same buffer.
+    Few requests have hundreds of blocks, which all read the root's ids."""
+    rng = random.Random(width * B)
+    ctx, new = [rng.randrange(60) for _ in range(B)], [rng.randrange(13) for _ in range(B)]
+    c = Cache(dev, rows=B, blocks=5, G=2, D=64, L=28, fill=0)
+    planned(c, [0] * B, ctx, None)
+    g = planned(c, ctx, new)
+    for rep in range(8):
+        tok, tgt, root = drafts(rng, g.s, width, (0.0, 0.9, 1.0)[rep % 3], vocab=3 if width == 1 else 50)
+        T = max(g.s.cu[-1], 1)
+        ids, tg, nx = i32(sum(tok, []) or [0]), i32(sum(tgt, []) or [0]), i32(sum(root, []))
+        acc, path, nl = i32([-7] * B), i32([-7] * T), g.ctx.clone()
+        c.k.normal_(generator=torch.Generator("cuda").manual_seed(rep))
+        c.v.normal_(generator=torch.Generator("cuda").manual_seed(rep + 100))
+        kw, vw = c.k.cpu().clone(), c.v.cpu().clone()
+        c.h.commit(step_with(g, ctx_len=nl.data_ptr()), engine.CommitArgs(width=width, tokens=ids.data_ptr(), targets=tg.data_ptr(), root_target=nx.data_ptr(),
+                                                                          accepted=acc.data_ptr(), path=path.data_ptr(), new_len=nl.data_ptr(),
+                                                                          next_token=nx.data_ptr()), stream=0)
+        torch.cuda.synchronize()
+        paths, nxt = op.commit(16, g.s, tok, tgt, root, [x for l in range(28) for x in (kw[l], vw[l])])
+        assert acc.tolist() == [len(p) for p in paths] and nl.tolist() == [x + len(p) for x, p in zip(ctx, paths)]
+        assert nx.view(B, width).tolist() == nxt
+        assert torch.equal(c.k.cpu(), kw) and torch.equal(c.v.cpu(), vw)
+
+
+def test_commit_refuses_an_outcome_over_the_ids(dev):
+    c = Cache(dev, rows=2, blocks=4)
+    g = planned(c, [3, 0], [2, 4])
+    x = i32([0] * 256)
+    p = lambda n: x[n:].data_ptr()  # noqa: E731
+    good = dict(width=2, tokens=p(0), targets=p(16), root_target=p(32), accepted=p(48), path=p(64), new_len=p(80), next_token=p(96))
+    for kw in (dict(next_token=p(33)), dict(next_token=p(1)), dict(next_token=p(15)), dict(path=p(20)), dict(accepted=p(35)), dict(new_len=p(11))):
+        refused(capi.NAVI_E_ARG, c.h.commit, g.c, engine.CommitArgs(**{**good, **kw}), stream=0)
+    c.h.commit(g.c, engine.CommitArgs(**good), stream=0)
+    torch.cuda.synchronize()
