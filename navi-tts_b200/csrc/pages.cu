@@ -648,6 +648,8 @@ std::unique_ptr<Pages> Pages::create(const Device & dev, const navi_pages_desc &
         NAVI_CUDA(cudaMemcpy(p->d_.free_pages, ids.data(), ids.size() * 4, cudaMemcpyHostToDevice));
         NAVI_CUDA(cudaMemcpy(p->d_.n_free, &d.n_pages, 4, cudaMemcpyHostToDevice));
     }
+    // the zeros are written on the legacy stream, for which other streams (the engine's) do not wait
+    if (!p->owned_.empty()) NAVI_CUDA(cudaStreamSynchronize(cudaStreamLegacy));
     return p;
 }
 

@@ -2,6 +2,7 @@
 ranges, shared buffers, graphs. Against the plain 64-bit restatement of oracle/pages.py, as
 test_pages_gpu.py, whose caches and steps are used. navi_pages_check follows each attend, so that a wait
 that ran out fails the test even where the results are right."""
+import ctypes
 import math
 import random
 
@@ -199,3 +200,46 @@ def test_commit_refuses_an_outcome_over_the_ids(dev):
         refused(capi.NAVI_E_ARG, c.h.commit, g.c, engine.CommitArgs(**{**good, **kw}), stream=0)
     c.h.commit(g.c, engine.CommitArgs(**good), stream=0)
     torch.cuda.synchronize()
+
+
+# ---- pools that the library allocates --------------------------------------------------------------------
+
+@pytest.mark.parametrize("tables", ["own", "library"])
+def test_rows_stored_right_after_create_stay(dev, tables):
+    """Pools of 8 GB are zeroed before create returns: rows stored at once, on a stream that waits for no other, are there."""
+    if torch.cuda.mem_get_info()[0] < 30 << 30:
+        pytest.skip("needs 30 GB free")
+    G, D, page, L, blocks = 8, 128, 16, 2, 4
+    n_pages = (2 << 30) // (G * D * page * 2)
+    H, T = 1, 3 * page
+    s = op.Step([0], [T], None)
+    g = GpuStep(s)
+    qkv = torch.randn(T, (H + 2 * G) * D, generator=torch.Generator().manual_seed(0)).half().cuda()
+    q = torch.zeros(T, H * D, dtype=torch.float16, device="cuda")
+    t = op.Tables.fresh(n_pages, page, 1, blocks)           # page 0 on top; own tables: the last page, which is zeroed last
+    if tables == "own":
+        t.free.sort()
+    table, held, free, n_free = i32([0] * blocks), i32([0]), i32(t.free), i32([n_pages])
+    op.plan(t, s)
+    torch.cuda.synchronize()
+    p = lambda x: x.data_ptr()  # noqa: E731
+    d = capi.PagesDesc(L, n_pages, page, G, D, capi.NAVI_F16, 1, blocks)
+    if tables == "own":
+        d.table, d.held, d.free_pages, d.n_free = p(table), p(held), p(free), p(n_free)
+    kv = engine.PagedKv(dev, d)
+    kv.plan(g.c)                                            # on the engine's stream
+    a = engine.StoreArgs(qkv=p(qkv), q_out=p(q), dtype=capi.NAVI_F16, n_head=H)
+    for l in range(L - 1, -1, -1):
+        kv.store(g.c, l, a)
+    kv.check()
+    desc = kv.desc()
+    cudart = ctypes.CDLL("libcudart.so.12")
+    for l in range(L):
+        for pool, first in ((desc.k, H), (desc.v, H + G)):
+            for b in range(3):
+                got = torch.empty(G, page, D, dtype=torch.float16, device="cuda")
+                src = pool[l] + t.table[0][b] * G * page * D * 2
+                assert cudart.cudaMemcpy(ctypes.c_void_p(p(got)), ctypes.c_void_p(src), ctypes.c_size_t(got.numel() * 2), 3) == 0
+                want = qkv[b * page:(b + 1) * page].view(page, H + 2 * G, D)[:, first:first + G].transpose(0, 1)
+                assert torch.equal(got, want)
+    kv.close()
