@@ -377,10 +377,13 @@ int navi_conv1d(navi_device * dev, const navi_conv_args * a);
  *   navi_pages_commit   the branch that agrees with the model's choices, its K/V moved to the front
  *
  * Every call only enqueues work on `stream` (a cudaStream_t, as everywhere in CUDA NULL is the
- * legacy default stream; navi_device_stream gives the engine's) and returns. A device's first
- * plan, attend or in-place commit on each stream takes that stream's scratch (make it before capturing the
- * stream); nothing else allocates. The calls of one cache are ordered by the caller: on one
- * stream, or by events between streams. */
+ * legacy default stream; navi_device_stream gives the engine's) and returns. Nothing allocates
+ * but a device's first plan, attend or in-place commit on each stream (39 MB of scratch, kept until the device
+ * closes; a stream that is destroyed, when its calls have ended, leaves it to the next of its handle). Calls may be
+ * captured: the first on each stream of a capture takes scratch for the graph, so that graphs captured on one stream,
+ * and calls on it, may run side by side; it goes to a later capture when the graph and its executables
+ * are gone. Two executables of one graph share it and must not run at once. The calls of one cache
+ * are ordered by the caller: on one stream, or by events between streams. */
 #define NAVI_PAGES_MAX_LAYERS 128
 enum { NAVI_F32 = 0, NAVI_F16 = 1, NAVI_BF16 = 2 };   /* the .navi type codes */
 #define NAVI_PAGES_MAX_REQUESTS 8192
@@ -488,8 +491,8 @@ typedef struct navi_commit_args {
  * The step needs parent; a request that is not served accepts nothing. */
 int navi_pages_commit(navi_pages * p, const navi_step * s, const navi_commit_args * a, void * stream);
 
-/* Waits for `stream`. NAVI_E_TIMEOUT when a kernel of these calls on it gave up a wait for a copy
- * or a matrix product since the last check (its results are then void); the waits are bounded, so
+/* Waits for `stream`. NAVI_E_TIMEOUT when a kernel of these calls on it, or of captured ones on any, gave up a
+ * wait for a copy or a matrix product since the last check (its results are then void); the waits are bounded, so
  * no call hangs the device. */
 int navi_pages_check(navi_pages * p, void * stream);
 

@@ -26,7 +26,7 @@ struct AttendArgs {
     const uint8_t * k, * v;      // the layer's pools, for what does not come by TMA
     const int32_t * table, * req, * ctx_len, * cu_rows, * status;
     const uint64_t * mask;       // nullptr: a chain
-    float * pieces;              // the stream's scratch: unfinished sums, arrival counters, error word
+    float * pieces;              // the stream's or graph's scratch: unfinished sums, arrival counters, error word
     int * arrived, * err;
     int64_t q_stride, out_stride;
     float scale;                 // times log2(e)
@@ -129,7 +129,7 @@ template <class... A> void allow_smem(void (*kernel)(A...), int bytes) {
 // after EXTRA units that stand for what an item costs beside its tiles.
 // Lengths are on the device and ragged, so the blocks divide the list evenly themselves,
 // whatever request the units belong to. An item that falls to several blocks leaves its pieces
-// (the sums and each row's maximum and sum, f32) in the stream's scratch, and the block that
+// (the sums and each row's maximum and sum, f32) in the scratch, and the block that
 // arrives last joins them in the blocks' order, so the result does not depend on who was last. A
 // block has at most two such pieces: slot 0 for one that begins inside an item, slot 1 for one
 // that begins with the item and ends inside it. Arrivals are counted in key tiles at the item's

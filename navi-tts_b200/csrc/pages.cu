@@ -756,12 +756,20 @@ void Pages::commit(const navi_step & s, const navi_commit_args & c, cudaStream_t
 void Pages::check(cudaStream_t stream) const {
     NAVI_CUDA(cudaSetDevice(dev_->info().ordinal));
     const int sms = dev_->info().multiprocessors;
-    const PagesScratch sc(dev_->scratch(stream, PagesScratch::bytes(sms)), sms);
-    int err = 0;
-    NAVI_CUDA(cudaMemcpyAsync(&err, sc.err, sizeof(int), cudaMemcpyDeviceToHost, stream));
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    NAVI_CUDA(cudaStreamIsCapturing(stream, &capturing));
+    if (capturing != cudaStreamCaptureStatusNone) fail("pages check: the stream is being captured", NAVI_E_ARG);
+    std::vector<void *> blocks = dev_->captured_scratch();
+    blocks.push_back(dev_->scratch(stream, PagesScratch::bytes(sms)));
+    std::vector<int> err(blocks.size(), 0);
+    for (size_t k = 0; k < blocks.size(); ++k)
+        NAVI_CUDA(cudaMemcpyAsync(&err[k], PagesScratch(blocks[k], sms).err, sizeof(int), cudaMemcpyDeviceToHost, stream));
     NAVI_CUDA(cudaStreamSynchronize(stream));
-    if (!err) return;
-    NAVI_CUDA(cudaMemsetAsync(sc.tickets, 0, PagesScratch::ints(sms) * sizeof(int), stream));   // counters of blocks that gave up
+    if (std::all_of(err.begin(), err.end(), [](int e) { return e == 0; })) return;
+    NAVI_CUDA(cudaDeviceSynchronize());
+    for (size_t k = 0; k < blocks.size(); ++k)   // counters of blocks that gave up
+        if (err[k]) NAVI_CUDA(cudaMemsetAsync(PagesScratch(blocks[k], sms).tickets, 0, PagesScratch::ints(sms) * sizeof(int), stream));
+    NAVI_CUDA(cudaStreamSynchronize(stream));
     fail("pages: a wait for a copy or a matrix product passed its deadline", NAVI_E_TIMEOUT);
 }
 

@@ -30,7 +30,7 @@ public:
     void store(const navi_step & s, int layer, const navi_store_args & a, cudaStream_t stream) const;
     void attend(const navi_step & s, int layer, const navi_attend_args & a, cudaStream_t stream) const;
     void commit(const navi_step & s, const navi_commit_args & a, cudaStream_t stream) const;
-    // Waits for the stream; throws NAVI_E_TIMEOUT when a kernel on it gave up a wait since the last check.
+    // Waits for the stream; throws NAVI_E_TIMEOUT when a kernel on it, or of a graph, gave up a wait since the last check.
     void check(cudaStream_t stream) const;
 
 private:
@@ -46,7 +46,7 @@ private:
     int shift_ = 0;                 // log2(page_size)
 };
 
-// The scratch of one stream (Device::scratch), laid out for every operator that hands work from
+// A block of scratch (Device::scratch), laid out for every operator that hands work from
 // one block to another. All counters are zero between launches.
 struct PagesScratch {
     static constexpr size_t TICKETS = 64;                            // launch-wide counters

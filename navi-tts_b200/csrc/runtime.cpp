@@ -7,8 +7,10 @@
 #include <sys/stat.h>
 #include <unistd.h>
 
+#include <algorithm>
 #include <cerrno>
 #include <cstring>
+#include <mutex>
 #include <set>
 
 namespace navi {
@@ -426,7 +428,36 @@ Validation validate(const NaviFile & f, const Params & p) {
 
 // ---- device ---------------------------------------------------------------------------------------------
 
+struct Device::Scratch {
+    struct Held {
+        unsigned long long capture;   // 0: calls on the stream itself
+        cudaStream_t stream;
+        void * block;
+    };
+    struct Return {
+        std::shared_ptr<Scratch> scratch;
+        unsigned long long capture;
+        cudaStream_t stream;
+    };
+    std::mutex lock;                  // graphs give back from a thread of the driver's
+    std::vector<Held> held;
+    std::vector<void *> idle, all;    // given back; every block there is
+
+    static void CUDART_CB give_back(void * p) {
+        const std::unique_ptr<Return> r(static_cast<Return *>(p));
+        Scratch & s = *r->scratch;
+        const std::lock_guard<std::mutex> hold(s.lock);
+        for (auto h = s.held.begin(); h != s.held.end(); ++h)
+            if (h->capture == r->capture && h->stream == r->stream) {
+                s.idle.push_back(h->block);
+                s.held.erase(h);
+                return;
+            }
+    }
+};
+
 Device::Device(int ordinal) {
+    scratch_ = std::make_shared<Scratch>();
     int n = 0;
     NAVI_CUDA(cudaGetDeviceCount(&n));
     if (ordinal < 0 || ordinal >= n) fail("no CUDA device " + std::to_string(ordinal) + " (" + std::to_string(n) + " visible)", NAVI_E_ARG);
@@ -456,23 +487,73 @@ Device::Device(int ordinal) {
 Device::~Device() {
     if (stream_) {
         cudaSetDevice(info_.ordinal);
-        for (const auto & s : scratch_) cudaFree(s.second);
+        std::vector<void *> blocks;
+        {
+            const std::lock_guard<std::mutex> hold(scratch_->lock);
+            blocks.swap(scratch_->all);
+            scratch_->held.clear();
+            scratch_->idle.clear();
+        }
+        for (void * b : blocks) cudaFree(b);
         cudaStreamDestroy(stream_);
     }
 }
 
 void * Device::scratch(cudaStream_t stream, size_t bytes) const {
-    for (const auto & s : scratch_)
-        if (s.first == stream) return s.second;
-    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    NAVI_CUDA(cudaStreamIsCapturing(stream, &cap));
-    if (cap != cudaStreamCaptureStatusNone)
-        fail("the stream's scratch must be taken by a call made before the stream is captured", NAVI_E_ARG);
-    void * p = nullptr;
-    NAVI_CUDA(cudaMalloc(&p, bytes));
-    NAVI_CUDA(cudaMemsetAsync(p, 0, bytes, stream));
-    scratch_.emplace_back(stream, p);
-    return p;
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    cudaGraph_t graph = nullptr;
+    NAVI_CUDA(cudaStreamGetCaptureInfo_v2(stream, &status, &id, &graph, nullptr, nullptr));
+    if (status == cudaStreamCaptureStatusInvalidated) fail("the capture of the stream has failed", NAVI_E_CUDA);
+    if (status == cudaStreamCaptureStatusNone) id = 0;
+    Scratch & sc = *scratch_;
+    void * block = nullptr;
+    {
+        const std::lock_guard<std::mutex> hold(sc.lock);
+        for (const Scratch::Held & h : sc.held)
+            if (h.capture == id && h.stream == stream) return h.block;
+        if (!sc.idle.empty()) {
+            block = sc.idle.back();
+            sc.idle.pop_back();
+        }
+    }
+    // a capture by this thread forbids it to allocate or wait, even where the captured stream has no part in that
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    NAVI_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+    cudaStream_t aside = nullptr;
+    cudaError_t e = block ? cudaSuccess : cudaMalloc(&block, bytes);
+    if (e == cudaSuccess) {
+        const std::lock_guard<std::mutex> hold(sc.lock);
+        if (std::find(sc.all.begin(), sc.all.end(), block) == sc.all.end()) sc.all.push_back(block);
+    }
+    if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&aside, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMemsetAsync(block, 0, bytes, aside);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(aside);
+    if (aside) cudaStreamDestroy(aside);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    // the graph keeps a reference to what gives its block back
+    if (e == cudaSuccess && id) {
+        auto * back = new Scratch::Return{scratch_, id, stream};
+        cudaUserObject_t object = nullptr;
+        e = cudaUserObjectCreate(&object, back, Scratch::give_back, 1, cudaUserObjectNoDestructorSync);
+        if (e != cudaSuccess) delete back;
+        else if ((e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove)) != cudaSuccess) cudaUserObjectRelease(object, 1);
+    }
+    const std::lock_guard<std::mutex> hold(sc.lock);
+    if (e != cudaSuccess) {
+        if (block) sc.idle.push_back(block);
+        cuda_check(e, "scratch", __FILE__, __LINE__);
+    }
+    sc.held.push_back({id, stream, block});
+    return block;
+}
+
+std::vector<void *> Device::captured_scratch() const {
+    const std::lock_guard<std::mutex> hold(scratch_->lock);
+    std::vector<void *> blocks;
+    for (const Scratch::Held & h : scratch_->held)
+        if (h.capture) blocks.push_back(h.block);
+    return blocks;
 }
 
 void Device::make_current() const { NAVI_CUDA(cudaSetDevice(info_.ordinal)); }

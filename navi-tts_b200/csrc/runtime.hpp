@@ -147,15 +147,19 @@ public:
     const DeviceInfo & info() const { return info_; }
     cudaStream_t stream() const { return stream_; }
     void make_current() const;
-    // `bytes` of device memory for the launches of one stream to hand work to one another: a block
-    // per stream, zeroed when it is taken at the stream's first call and kept until the device
-    // closes. Every caller asks for the same size.
+    // `bytes` of device memory for launches that follow one another to hand work on: a block for
+    // each stream, kept until the device closes, and one for each stream of a capture, since the
+    // graph runs wherever it is replayed; that one goes to a later capture when the graph and what
+    // was instantiated from it are gone. Zeroed when it is taken. Every caller asks for the same size.
     void * scratch(cudaStream_t stream, size_t bytes) const;
+    // The blocks that captures hold.
+    std::vector<void *> captured_scratch() const;
 
 private:
     DeviceInfo info_;
     cudaStream_t stream_ = nullptr;
-    mutable std::vector<std::pair<cudaStream_t, void *>> scratch_;
+    struct Scratch;
+    std::shared_ptr<Scratch> scratch_;   // shared with the graphs that hold blocks of it
 };
 
 // ---- weights arena (reference: runtime/weights/device_weights.cpp:18-72) ----------------------------

@@ -243,3 +243,118 @@ def test_rows_stored_right_after_create_stay(dev, tables):
                 want = qkv[b * page:(b + 1) * page].view(page, H + 2 * G, D)[:, first:first + G].transpose(0, 1)
                 assert torch.equal(got, want)
     kv.close()
+
+
+# ---- graphs ------------------------------------------------------------------------------------------------
+
+class Whole:
+    """plan, store, attend and commit of a drafted step over a cache of its own, with buffers that stay."""
+
+    def __init__(self, dev, seed, H=4, G=2, D=128):
+        rng = random.Random(seed)
+        self.H, self.G, self.D = H, G, D
+        self.ctx, self.new = [2900, 1500 + seed, 20], [9, 1 + seed % 3, 4]
+        self.c = Cache(dev, rows=3, blocks=200, n_pages=320, G=G, D=D, seed=seed, fill=0)
+        self.c.k.normal_(generator=torch.Generator("cuda").manual_seed(seed))
+        self.c.v.normal_(generator=torch.Generator("cuda").manual_seed(seed + 1))
+        planned(self.c, [0] * 3, self.ctx, None)
+        self.s = op.Step(self.ctx, self.new, sum((tree(rng, n) for n in self.new), []))
+        self.g = GpuStep(self.s)
+        T = sum(self.new)
+        gen = torch.Generator().manual_seed(seed)
+        self.qkv = torch.randn(T, (H + 2 * G) * D, generator=gen).half().cuda()
+        self.q, self.out = (torch.zeros(T, H * D, dtype=torch.float16, device="cuda") for _ in range(2))
+        self.tok = i32(rng.randrange(2) for _ in range(T))
+        self.tgt, self.root = i32(rng.randrange(2) for _ in range(T)), i32(rng.randrange(2) for _ in self.ctx)
+        self.acc, self.path, self.nl, self.nx = i32([-7] * 3), i32([-7] * T), i32([-7] * 3), i32([-7] * 3)
+        p = lambda x: x.data_ptr()  # noqa: E731
+        self.sa = engine.StoreArgs(qkv=p(self.qkv), q_out=p(self.q), dtype=capi.NAVI_F16, n_head=H)
+        self.aa = engine.AttendArgs(q=p(self.q), out=p(self.out), dtype=capi.NAVI_F16, n_head=H, scale=D ** -0.5)
+        self.ca = engine.CommitArgs(width=1, tokens=p(self.tok), targets=p(self.tgt), root_target=p(self.root), accepted=p(self.acc),
+                                    path=p(self.path), new_len=p(self.nl), next_token=p(self.nx))
+        self.state = [self.c.k, self.c.v, self.c.table, self.c.held, self.c.free, self.c.n_free]
+        self.before = [x.clone() for x in self.state]
+
+    def run(self, stream):
+        self.c.h.plan(self.g.c, stream=stream)
+        self.c.h.store(self.g.c, 0, self.sa, stream=stream)
+        for _ in range(6):                                  # many pieces to join
+            self.c.h.attend(self.g.c, 0, self.aa, stream=stream)
+        self.c.h.commit(self.g.c, self.ca, stream=stream)
+
+    def again(self):
+        """The cache as it was, the results cleared; on the current stream."""
+        for x, y in zip(self.state, self.before):
+            x.copy_(y)
+        for x in (self.out, self.q, self.acc, self.path, self.nl, self.nx, self.g.slot):
+            x.zero_()
+
+    def results(self):
+        return [x.clone() for x in (self.out, self.q, self.acc, self.path, self.nl, self.nx, self.g.slot, self.c.k, self.c.v, self.c.table)]
+
+
+def test_graphs_of_one_stream_side_by_side(dev):
+    """Two steps captured on one stream, the first calls on it, replayed on two others while a third step is called on the
+    stream itself: each as when it runs alone."""
+    steps = [Whole(dev, k) for k in range(3)]
+    wants = []
+    for w in steps:
+        w.run(0)
+        w.c.h.check(stream=0)
+        wants.append(w.results())
+        w.again()
+    # the first one's attention against the oracle; the others by it
+    w = steps[0]
+    op.plan(w.c.t, w.s)
+    cap, streams = torch.cuda.Stream(), [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    graphs = []
+    for w in steps[:2]:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=cap):
+            w.run(cap.cuda_stream)
+        graphs.append(gr)
+    for rep in range(10):
+        for w in steps:
+            w.again()
+        torch.cuda.synchronize()
+        for st, gr in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                gr.replay()
+        steps[2].run(cap.cuda_stream)
+        torch.cuda.synchronize()
+        for w, want in zip(steps, wants):
+            assert all(torch.equal(x, y) for x, y in zip(w.results(), want))
+    w.c.h.check(stream=cap.cuda_stream)
+    s, w = steps[0].s, steps[0]
+    w.again()
+    kd, vd = w.c.k[0].cpu().double(), w.c.v[0].cpu().double()
+    T = s.cu[-1]
+    q = op.store(16, s, w.qkv.cpu(), w.H, w.G, kd, vd)
+    want, _ = op.attend(w.c.t, s, q, kd, vd, w.D ** -0.5)
+    # check_attend's tolerance: scores by f32 sums of exact products, f16 weights and result, the sums over the keys
+    ds = 2.0 ** -20 * w.D ** -0.5 * float(q.abs().sum(2).max()) * float(kd.abs().max())
+    tol = float(vd.abs().max()) * (2 * ds + 2.0 ** -20 + 3000 * 2.0 ** -24 + U["f16"])
+    assert ((wants[0][0].cpu().double().view(T, w.H, w.D) - want).abs() <= tol + U["f16"] * want.abs()).all()
+    # the scratch of graphs that are gone serves the next ones: 20 captures take no more memory than two
+    del gr, graphs
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    for _ in range(20):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=cap):
+            steps[0].run(cap.cuda_stream)
+        gr.replay()
+        torch.cuda.synchronize()
+        gr.reset()
+    assert free - torch.cuda.mem_get_info()[0] < 10 * (39 << 20)
+
+
+def test_check_refuses_a_stream_that_is_captured(dev):
+    w = Whole(dev, 5)
+    st, gr = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=st):
+        refused(capi.NAVI_E_ARG, w.c.h.check, stream=st.cuda_stream)
+        w.run(st.cuda_stream)
+    gr.replay()
+    w.c.h.check(stream=0)
