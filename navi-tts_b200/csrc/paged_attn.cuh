@@ -19,6 +19,9 @@ namespace navi::attn {
 
 using namespace navi::dev;
 
+// The kernels may be resident while plan and store still write what they read, before griddep_wait: no
+// load here is of the kind that takes its data for constant over the kernel's life (ld.global.nc, __ldg).
+
 struct AttendArgs {
     const void * q;
     void * out;
@@ -467,8 +470,8 @@ __device__ __forceinline__ uint32_t seen_bits(const AttendArgs & a, const Segmen
     } else {
         const uint64_t * m = a.mask + static_cast<size_t>(it.row0 + j) * a.mask_words;
         const int w = at >> 6;               // floor: -1 for the bits before row 0, all seen
-        const uint64_t lo = w < 0 ? ~0ull : w < a.mask_words ? __ldg(m + w) : 0ull;
-        const uint64_t hi = w + 1 < a.mask_words ? __ldg(m + w + 1) : 0ull;
+        const uint64_t lo = w < 0 ? ~0ull : w < a.mask_words ? m[w] : 0ull;
+        const uint64_t hi = w + 1 < a.mask_words ? m[w + 1] : 0ull;
         const int s = at & 63;
         b = static_cast<uint32_t>(s ? (lo >> s) | (hi << (64 - s)) : lo);
     }
@@ -483,7 +486,7 @@ __device__ __forceinline__ int tile_pages(const AttendArgs & a, const Segment & 
 // past them keep what they held. The bytes (tile_pages * page * D * 2) arrive on a barrier. Every lane
 // reads its page's id a tile ahead, so the ids cost one latency together and not one each.
 __device__ __forceinline__ int page_at(const AttendArgs & a, const Segment & s, int t, int p) {
-    return p < tile_pages(a, s, t) ? min(max(__ldg(a.table + static_cast<size_t>(s.table) * a.max_blocks + (t * KT >> a.shift) + p), 0), a.n_pages - 1) : -1;
+    return p < tile_pages(a, s, t) ? min(max(a.table[static_cast<size_t>(s.table) * a.max_blocks + (t * KT >> a.shift) + p], 0), a.n_pages - 1) : -1;
 }
 
 // ---- values that are not finite where a row does not look --------------------------------------
@@ -508,7 +511,7 @@ template <class C> __device__ __forceinline__ bool not_finite(uint32_t m) {
 }
 // Token `key` of the segment's request and KV head in a pool.
 template <class C, int D> __device__ __forceinline__ const C * token_at(const AttendArgs & a, const Segment & s, const uint8_t * pool, int key) {
-    const int page = min(max(__ldg(a.table + static_cast<size_t>(s.table) * a.max_blocks + (key >> a.shift)), 0), a.n_pages - 1);
+    const int page = min(max(a.table[static_cast<size_t>(s.table) * a.max_blocks + (key >> a.shift)], 0), a.n_pages - 1);
     return reinterpret_cast<const C *>(pool) + (((static_cast<size_t>(page) * a.n_kv + s.g) << a.shift) + (key & ((1 << a.shift) - 1))) * D;
 }
 

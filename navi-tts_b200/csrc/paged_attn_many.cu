@@ -354,8 +354,8 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                             if constexpr (SPLIT) w[k] = v[k];
                             if (m < it.m) {
                                 const uint4 * src = reinterpret_cast<const uint4 *>(row_at<const T>(a, a.q, a.q_stride, it, m) + c * 8);
-                                v[k] = __ldg(src);
-                                if constexpr (SPLIT) w[k] = __ldg(src + 1);
+                                v[k] = src[0];
+                                if constexpr (SPLIT) w[k] = src[1];
                             }
                         }
 #pragma unroll

@@ -68,3 +68,16 @@ def test_tree_is_its_branches():
     for a, b in ((k2, k), (v2, v)):
         for x in L:
             assert torch.equal(a[x // 16, :, x % 16], b[x // 16, :, x % 16])
+
+
+def test_kernels_launched_early_read_nothing_as_constant():
+    """plan, store, attend and commit may be resident while the launch before them still writes what they read: loads
+    through the read-only path (__ldg, ld.global.nc, restrict pointers) are for data that nobody writes meanwhile."""
+    import pathlib
+    import re
+    src = pathlib.Path(__file__).resolve().parent.parent / "navi-tts_b200" / "csrc"
+    files = sorted(src.glob("paged_attn*")) + [src / "pages.cu"]
+    assert len(files) == 6
+    for f in files:
+        code = re.sub(r"//.*", "", f.read_text())
+        assert not re.search(r"__ldg|global\.nc|__restrict__", code), f.name
