@@ -503,8 +503,8 @@ int navi_pages_check(navi_pages * p, void * stream);
  * rows and d_logits [s->max_rows][vocab] (or NULL) their codec logits. The rows of the batch share one pass over
  * the weights, which is what a drafted step saves. navi_pages_commit then keeps the branch that
  * agrees. The cache is f16 with the talker's layers, KV heads and head_dim; s->max_rows <=
- * max_prompt_tokens; a row past the talker's max_positions is not stored. Runs on the engine's
- * stream and waits for it. navi_talker_last_ms gives the device time. */
+ * max_prompt_tokens; a request with a row at the talker's max_positions or past it gets NAVI_E_SHAPE (a tree
+ * after it took its pages, which the next plan gives back). Runs on the engine's stream and waits for it. navi_talker_last_ms gives the device time. */
 int navi_talker_step(navi_talker * t, navi_pages * p, const navi_step * s, const float * d_rows, float * d_hidden, float * d_logits);
 
 /* Inspection of the last frame (host copies): the talker's post-norm hidden [hidden],

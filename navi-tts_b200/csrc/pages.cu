@@ -47,6 +47,7 @@ struct PlanArgs {
     int32_t * table, * held, * free_pages, * n_free;
     int * ticket, * broken;
     int n_pages, shift, max_blocks, max_requests;
+    int positions;   // no row may be at this position or past it
 };
 
 constexpr int PLAN_THREADS = 256;
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_pages_plan(const __grid_consta
             int status = NAVI_OK, g = 0, u = 0;
             const long long need = (static_cast<long long>(max(ctx, 0)) + max(n, 0) + (1 << a.shift) - 1) >> a.shift;
             if (n < 0 || ctx < 0 || tr < 0 || tr >= a.max_requests || held < 0 || held > MB) status = NAVI_E_ARG;
-            else if (n > a.s.max_new || need > MB || row > cap) status = NAVI_E_SHAPE;
+            else if (n > a.s.max_new || need > MB || row > cap || (!a.s.parent && n > 0 && ctx > a.positions - n)) status = NAVI_E_SHAPE;
             else {
                 g = max(static_cast<int>(need) - held, 0);
                 u = max(held - static_cast<int>(need), 0);
@@ -262,7 +263,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_pages_plan(const __grid_consta
             const int page = blk < held ? table_row(i)[blk] : taken_page(cg[i] + blk - held);
             if (page >= 0 && page < a.n_pages) slot = (static_cast<int64_t>(page) << a.shift) + ((ctx + j) & ((1 << a.shift) - 1));
         }
-        if (!whole) a.broken[i] = 1;
+        if (a.s.parent && (!whole || ctx + depth >= a.positions)) atomicMax(a.broken + i, whole ? 1 : 2);
         a.s.row_req[r] = i;
         a.s.pos[r] = ctx + depth;
         a.s.slot[r] = slot;
@@ -283,9 +284,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_pages_plan(const __grid_consta
     for (int i = tid; i < B; i += PLAN_THREADS) {
         int status = st[i];
         if (status == NAVI_OK) a.held[a.s.req ? a.s.req[i] : i] = need_of(i);
-        if (a.s.parent && __ldcg(a.broken + i)) {
+        if (const int why = a.s.parent ? __ldcg(a.broken + i) : 0; why) {   // 2: a parent, 1: a position
             a.broken[i] = 0;
-            if (status == NAVI_OK) status = NAVI_E_ARG;
+            if (status == NAVI_OK) status = why == 2 ? NAVI_E_ARG : NAVI_E_SHAPE;
         }
         a.s.status[i] = status;
     }
@@ -672,13 +673,13 @@ void Pages::check_step(const navi_step & s, const char * who) const {
     }
 }
 
-void Pages::plan(const navi_step & s, cudaStream_t stream) const {
+void Pages::plan(const navi_step & s, cudaStream_t stream, int positions) const {
     check_step(s, "pages plan");
     if (s.n_req == 0) return;
     NAVI_CUDA(cudaSetDevice(dev_->info().ordinal));
     const int sms = dev_->info().multiprocessors;
     const PagesScratch sc(dev_->scratch(stream, PagesScratch::bytes(sms)), sms);
-    PlanArgs a{s, d_.table, d_.held, d_.free_pages, d_.n_free, sc.tickets, sc.broken, d_.n_pages, shift_, d_.max_blocks, d_.max_requests};
+    PlanArgs a{s, d_.table, d_.held, d_.free_pages, d_.n_free, sc.tickets, sc.broken, d_.n_pages, shift_, d_.max_blocks, d_.max_requests, positions};
     const size_t smem = (4 * static_cast<size_t>(s.n_req) + 1) * sizeof(int);
     static_assert((4 * static_cast<size_t>(NAVI_PAGES_MAX_REQUESTS) + 1) * sizeof(int) < 200 * 1024);
     if (smem > 40 * 1024)

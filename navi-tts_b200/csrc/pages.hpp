@@ -9,6 +9,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <climits>
 #include <cstdint>
 #include <memory>
 #include <vector>
@@ -26,7 +27,8 @@ public:
     Pages(const Pages &) = delete;
 
     const navi_pages_desc & desc() const { return d_; }
-    void plan(const navi_step & s, cudaStream_t stream) const;
+    // A request with a row at `positions` or past it is not served (NAVI_E_SHAPE).
+    void plan(const navi_step & s, cudaStream_t stream, int positions = INT_MAX) const;
     void store(const navi_step & s, int layer, const navi_store_args & a, cudaStream_t stream) const;
     void attend(const navi_step & s, int layer, const navi_attend_args & a, cudaStream_t stream) const;
     void commit(const navi_step & s, const navi_commit_args & a, cudaStream_t stream) const;
@@ -51,7 +53,7 @@ private:
 struct PagesScratch {
     static constexpr size_t TICKETS = 64;                            // launch-wide counters
     static constexpr size_t PIECE_FLOATS = 256 * (128 + 2);          // attend: one block's unfinished item
-    int * tickets, * broken, * arrived, * err;                       // broken: plan, a request with a bad parent; commit, blocks
+    int * tickets, * broken, * arrived, * err;                       // broken: plan, requests whose tree is refused; commit, blocks
     float * pieces;                                                  // two a block
 
     // `blocks`: the most blocks of a launch that leave pieces (one a multiprocessor)

@@ -641,7 +641,7 @@ void Talker::step(const Pages & pages, const navi_step & s, const float * rows, 
     const int T = s.max_rows, H = I.H;
     if (T > I.max_prompt) fail("talker: more rows than max_prompt_tokens", NAVI_E_ARG);
     if (s.n_req > 0 && T > 0 && (!rows || !hidden)) fail("talker: NULL rows", NAVI_E_ARG);
-    pages.plan(s, I.stream);
+    pages.plan(s, I.stream, I.kv.max_pos);
     if (s.n_req == 0 || T == 0) return;
     NAVI_CUDA(cudaEventRecord(I.ev0, I.stream));
     NAVI_CUDA(cudaMemcpyAsync(I.x, rows, static_cast<size_t>(T) * H * sizeof(float), cudaMemcpyDeviceToDevice, I.stream));
