@@ -393,6 +393,7 @@ struct Talker::Impl {
     std::vector<std::pair<int, cudaGraphExec_t>> graphs;
     std::vector<int> uncapturable;
     void enqueue_prefill(int T);
+    void enqueue_step(const Pages & pages, const navi_step & s, const float * rows, float * hidden, float * logits);
     void finish_layer(int l, int T);
     void check_waits();
     void capture_prefill(int T);
@@ -638,12 +639,26 @@ void Talker::step(const Pages & pages, const navi_step & s, const float * rows, 
     const navi_pages_desc & d = pages.desc();
     if (d.n_layer != tp.n_layer || d.n_kv_head != I.NKV || d.head_dim != tp.head_dim || d.dtype != NAVI_F16)
         fail("talker: the paged cache's layers, KV heads, head_dim or type are not the talker's", NAVI_E_SHAPE);
-    const int T = s.max_rows, H = I.H;
+    const int T = s.max_rows;
     if (T > I.max_prompt) fail("talker: more rows than max_prompt_tokens", NAVI_E_ARG);
     if (s.n_req > 0 && T > 0 && (!rows || !hidden)) fail("talker: NULL rows", NAVI_E_ARG);
-    pages.plan(s, I.stream, I.kv.max_pos);
-    if (s.n_req == 0 || T == 0) return;
     NAVI_CUDA(cudaEventRecord(I.ev0, I.stream));
+    pages.plan(s, I.stream, I.kv.max_pos);
+    if (s.n_req > 0 && T > 0) I.enqueue_step(pages, s, rows, hidden, logits);
+    NAVI_CUDA(cudaEventRecord(I.ev1, I.stream));
+    NAVI_CUDA(cudaEventSynchronize(I.ev1));
+    float ms = 0.f;
+    NAVI_CUDA(cudaEventElapsedTime(&ms, I.ev0, I.ev1));
+    I.last_ms = ms;
+    I.check_waits();
+    pages.check(I.stream);
+}
+
+// The layers and the codec head over a planned step's rows.
+void Talker::Impl::enqueue_step(const Pages & pages, const navi_step & s, const float * rows, float * hidden, float * logits) {
+    Impl & I = *this;
+    const auto & tp = I.p.talker;
+    const int T = s.max_rows, H = I.H;
     NAVI_CUDA(cudaMemcpyAsync(I.x, rows, static_cast<size_t>(T) * H * sizeof(float), cudaMemcpyDeviceToDevice, I.stream));
     navi_store_args st{};
     st.qkv = I.qkv;
@@ -673,13 +688,6 @@ void Talker::step(const Pages & pages, const navi_step & s, const float * rows, 
     }
     NAVI_CUDA(navi::dev::launch_pdl(k_rmsnorm, dim3(T), dim3(256), 0, I.stream, I.x, I.final_norm, H, tp.rms_eps, hidden));
     if (logits) I.gemm(I.head, nullptr, hidden, H, T, H, I.TV, logits, I.TV, EPI_NONE);
-    NAVI_CUDA(cudaEventRecord(I.ev1, I.stream));
-    NAVI_CUDA(cudaEventSynchronize(I.ev1));
-    float ms = 0.f;
-    NAVI_CUDA(cudaEventElapsedTime(&ms, I.ev0, I.ev1));
-    I.last_ms = ms;
-    I.check_waits();
-    pages.check(I.stream);
 }
 
 // What follows attention in layer l, over the T rows in x and att: O, the norms, the MLP, and the next

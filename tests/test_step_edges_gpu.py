@@ -1,5 +1,7 @@
 """Edges of navi_talker_step: the end of the talker's positions, steps without rows, cached prompts of requests
 that are refused. Rows that are served are compared with the CPU oracle's prefill as in test_step_gpu.py."""
+import ctypes
+
 import pytest
 import torch
 
@@ -59,3 +61,20 @@ def test_requests_at_the_end_of_the_positions(small_navi):
     S.check(h[0], lg[0], torch.cat([hist[0], x[:1]]))
     _, _, st, _ = S.step_any(rows_of(3, S.H, 80), [62], [3])
     assert st == [capi.NAVI_E_SHAPE]
+
+
+@pytest.mark.parametrize("requests", [0, 3])
+def test_a_step_without_rows_waits_too(small_navi, requests):
+    """A step that only gives pages back, or does nothing, has ended when the call returns; its time is its own."""
+    S = Session(small_navi)
+    cudart = ctypes.CDLL("libcudart.so.12")
+    S.step(rows_of(200, S.H, 1), [0, 0, 0], [100, 60, 40])
+    before = S.tal.last_ms()
+    z, st, cu = i32([0] * 8), i32([-7] * 4), i32([0] * 4)
+    torch.cuda.synchronize()
+    p = z.data_ptr()
+    s = engine.TreeStep(n_req=requests, max_rows=0, max_new=0, ctx_len=p, n_new=p, cu_rows=cu.data_ptr(), status=st.data_ptr())
+    S.tal.step(S.pages, s, 0, 0)
+    assert cudart.cudaStreamQuery(ctypes.c_void_p(S.dev.stream)) == 0
+    assert st.tolist()[:requests] == [capi.NAVI_OK] * requests
+    assert 0 <= S.tal.last_ms() < before
