@@ -439,7 +439,9 @@ typedef struct navi_step {
  * the stack (n_new = 0 after a drafted step gives back what the drafts took, ctx_len = 0 frees a
  * request), the first request's first page on top; then requests take pages from the top in their
  * order, so that a step that grows and one that undoes it leave the stack as it was. A request
- * that is not served keeps its pages, and its rows get slot -1. */
+ * that is not served keeps its pages, and its rows get slot -1. But a parent that is not below its row is
+ * found when the pages are dealt out already: such a request has taken them until a later plan gives them back (n_new =
+ * 0), and its rows whose own ancestors are sound have slots, which store fills; attend and commit refuse them all. */
 int navi_pages_plan(navi_pages * p, const navi_step * s, void * stream);
 
 typedef struct navi_store_args {

@@ -358,3 +358,24 @@ def test_check_refuses_a_stream_that_is_captured(dev):
         w.run(st.cuda_stream)
     gr.replay()
     w.c.h.check(stream=0)
+
+
+def test_a_bad_parent_takes_pages_until_the_next_plan(dev):
+    """What the header says of it: pages taken, slots for the rows above the bad one, nothing attended or accepted; a
+    plan without rows gives the pages back."""
+    c = Cache(dev, rows=2, blocks=4, n_pages=5, fill=0)
+    planned(c, [0, 0], [10, 3], None)
+    stack = c.free.tolist()[:c.n_free.item()]
+    g = planned(c, [10, 3], [30, 2], [-1] + list(range(28)) + [29] + [-1, 0])
+    assert g.status.tolist() == [capi.NAVI_E_ARG, capi.NAVI_OK] and c.held.tolist() == [3, 1]
+    assert all(x >= 0 for x in g.slot.tolist()[:29]) and g.slot.tolist()[29] == -1
+    out, lse = check_attend(c, g, "f16", 2)
+    assert (out[:30] == 0).all() and (lse[:30] == -math.inf).all()
+    ids, acc, path, nl, nx = i32([1] * 32), i32([-7] * 2), i32([-7] * 32), i32([-7] * 2), i32([-7] * 2)
+    root = i32([1, 1])
+    c.h.commit(g.c, engine.CommitArgs(width=1, tokens=ids.data_ptr(), targets=ids.data_ptr(), root_target=root.data_ptr(), accepted=acc.data_ptr(),
+                                      path=path.data_ptr(), new_len=nl.data_ptr(), next_token=nx.data_ptr()), stream=0)
+    c.h.check(stream=0)
+    assert acc.tolist() == [0, 2] and nl.tolist() == [10, 5] and path.tolist() == [-1] * 30 + [0, 1]
+    planned(c, [10, 3], [0, 0], None)
+    assert c.free.tolist()[:c.n_free.item()] == stack and c.held.tolist() == [1, 1]
