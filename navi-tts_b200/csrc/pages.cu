@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(COMMIT_THREADS) k_pages_commit(const __grid_co
     griddep_wait();
     griddep_launch_dependents();
     const int i = blockIdx.x, tid = threadIdx.x, W = a.c.width;
-    const int r0 = a.s.cu_rows[i], n = min(a.s.cu_rows[i + 1] - r0, NAVI_STEP_MAX_TREE);
+    const int r0 = a.s.cu_rows[i], rows = a.s.cu_rows[i + 1] - r0, n = min(rows, NAVI_STEP_MAX_TREE);   // more rows: not served
     const bool served = a.s.status[i] == NAVI_OK;
     for (int j = tid; j <= n; j += COMMIT_THREADS) child[j] = INT_MAX;
     __syncthreads();
@@ -533,7 +533,7 @@ __global__ void __launch_bounds__(COMMIT_THREADS) k_pages_commit(const __grid_co
             for (int x = lane; x < W; x += 32) next[x] = nx[x];
     }
     if (blockIdx.y == 0) {
-        for (int j = tid; j < n; j += COMMIT_THREADS) a.c.path[r0 + j] = j < k1 ? path[j] : -1;
+        for (int j = tid; j < rows; j += COMMIT_THREADS) a.c.path[r0 + j] = j < k1 ? path[j] : -1;
         if (!a.walked)
             for (int x = tid; x < W; x += COMMIT_THREADS) next[x] = nx[x];
         if (tid == 0) {

@@ -379,3 +379,18 @@ def test_a_bad_parent_takes_pages_until_the_next_plan(dev):
     assert acc.tolist() == [0, 2] and nl.tolist() == [10, 5] and path.tolist() == [-1] * 30 + [0, 1]
     planned(c, [10, 3], [0, 0], None)
     assert c.free.tolist()[:c.n_free.item()] == stack and c.held.tolist() == [1, 1]
+
+
+@pytest.mark.parametrize("n", [257, 300, 700])
+def test_commit_path_of_a_refused_tree_of_many_rows(dev, n):
+    """A tree of more rows than a tree may have is refused; path is -1 in all of its rows."""
+    c = Cache(dev, rows=2, blocks=60, fill=0)
+    g = planned(c, [0, 0], [n, 2], [x - 1 for x in range(n)] + [-1, 0], max_new=256)
+    assert g.status.tolist() == [capi.NAVI_E_SHAPE, capi.NAVI_OK]
+    ids, acc, path, nl, nx = i32([1] * (n + 2)), i32([-7] * 2), i32([-7] * (n + 4)), i32([-7] * 2), i32([-7] * 2)
+    root = i32([1, 1])
+    c.h.commit(g.c, engine.CommitArgs(width=1, tokens=ids.data_ptr(), targets=ids.data_ptr(), root_target=root.data_ptr(), accepted=acc.data_ptr(),
+                                      path=path.data_ptr(), new_len=nl.data_ptr(), next_token=nx.data_ptr()), stream=0)
+    torch.cuda.synchronize()
+    assert acc.tolist() == [0, 2] and nl.tolist() == [0, 2] and nx.tolist() == [1, 1]
+    assert path.tolist() == [-1] * n + [0, 1] + [-7] * 2
