@@ -399,7 +399,8 @@ typedef struct navi_pages_desc {
     int dtype;                     /* of the cache: NAVI_F16 or NAVI_BF16 */
     int max_requests, max_blocks;  /* the block table's rows (<= NAVI_PAGES_MAX_REQUESTS) and columns */
     void ** k, ** v;               /* host arrays of n_layer device pools [n_pages][n_kv_head][page_size][head_dim],
-                                      16-byte aligned; both NULL: the library allocates them (zeroed) */
+                                      16-byte aligned; both NULL: the library allocates them (zeroed). A layer's entry
+                                      may be NULL: store, attend and commit refuse it */
     int32_t * table;               /* device [max_requests][max_blocks] */
     int32_t * held;                /* device [max_requests]: pages that each request holds */
     int32_t * free_pages;          /* device [n_pages]: the stack of free pages, its top at n_free - 1 */

@@ -14,7 +14,7 @@ namespace navi {
 
 void Pages::attend(const navi_step & s, int layer, const navi_attend_args & q, cudaStream_t stream) const {
     check_step(s, "pages attend");
-    if (layer < 0 || layer >= d_.n_layer) fail("pages attend: layer outside the cache", NAVI_E_ARG);
+    check_layer(layer, "pages attend");
     if (q.n_head < 1 || q.n_head > 4096 || q.n_head % d_.n_kv_head) fail("pages attend: n_head must be a positive multiple of n_kv_head", NAVI_E_ARG);
     if (!(q.dtype == d_.dtype || (q.dtype == NAVI_F32 && d_.dtype == NAVI_F16))) fail("pages attend: rows are of the cache's type, or NAVI_F32 for an f16 cache", NAVI_E_ARG);
     if (!(q.scale > 0.f) || q.scale > 1e30f) fail("pages attend: scale must be positive and finite", NAVI_E_ARG);

@@ -673,6 +673,11 @@ void Pages::check_step(const navi_step & s, const char * who) const {
     }
 }
 
+void Pages::check_layer(int layer, const char * who) const {
+    if (layer < 0 || layer >= d_.n_layer) fail(std::string(who) + ": layer outside the cache", NAVI_E_ARG);
+    if (!k_[static_cast<size_t>(layer)] || !v_[static_cast<size_t>(layer)]) fail(std::string(who) + ": the layer has no pool", NAVI_E_ARG);
+}
+
 void Pages::plan(const navi_step & s, cudaStream_t stream, int positions) const {
     check_step(s, "pages plan");
     if (s.n_req == 0) return;
@@ -691,7 +696,7 @@ void Pages::plan(const navi_step & s, cudaStream_t stream, int positions) const 
 
 void Pages::store(const navi_step & s, int layer, const navi_store_args & q, cudaStream_t stream) const {
     check_step(s, "pages store");
-    if (layer < 0 || layer >= d_.n_layer) fail("pages store: layer outside the cache", NAVI_E_ARG);
+    check_layer(layer, "pages store");
     if (q.n_head < 0 || q.n_head > 4096) fail("pages store: n_head outside 0..4096", NAVI_E_ARG);
     if (!(q.dtype == d_.dtype || (q.dtype == NAVI_F32 && d_.dtype == NAVI_F16))) fail("pages store: rows are of the cache's type, or NAVI_F32 for an f16 cache", NAVI_E_ARG);
     if (q.rope && q.rope_positions < 1) fail("pages store: rope_positions must be positive", NAVI_E_ARG);
@@ -722,6 +727,7 @@ void Pages::commit(const navi_step & s, const navi_commit_args & c, cudaStream_t
     if (c.width < 1) fail("pages commit: width must be positive", NAVI_E_ARG);
     if (s.n_req == 0) return;
     if (!s.parent) fail("pages commit: the step has no parent (there is no tree to walk)", NAVI_E_ARG);
+    for (int l = 0; l < d_.n_layer; ++l) check_layer(l, "pages commit");
     if (!c.root_target || !c.accepted || !c.new_len || !c.next_token) fail("pages commit: NULL argument", NAVI_E_ARG);
     if (s.max_rows > 0 && (!c.tokens || !c.targets || !c.path)) fail("pages commit: NULL argument", NAVI_E_ARG);
     // Blocks of a request read its ids while another of them writes the outcome

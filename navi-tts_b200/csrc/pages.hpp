@@ -39,6 +39,8 @@ private:
     Pages() = default;
     // Throws NAVI_E_ARG / NAVI_E_SHAPE for a step that no call can take.
     void check_step(const navi_step & s, const char * who) const;
+    // Throws NAVI_E_ARG for a layer that the cache has not, or has no pool of.
+    void check_layer(int layer, const char * who) const;
 
     const Device * dev_ = nullptr;
     navi_pages_desc d_{};

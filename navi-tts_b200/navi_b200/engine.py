@@ -280,6 +280,8 @@ class PagedKv:
     def wrap(dev: Device, k_ptrs, v_ptrs, n_pages: int, page_size: int, n_kv_head: int, head_dim: int, dtype: int, max_requests: int,
              max_blocks: int, table: int, held: int, free_pages: int, n_free: int, keepalive=None) -> "PagedKv":
         n = len(k_ptrs)
+        if len(v_ptrs) != n:
+            raise ValueError(f"{n} K pools and {len(v_ptrs)} V pools")
         ka, va = (c_void_p * n)(*k_ptrs), (c_void_p * n)(*v_ptrs)
         return PagedKv(dev, capi.PagesDesc(n, n_pages, page_size, n_kv_head, head_dim, dtype, max_requests, max_blocks, ka, va, table, held,
                                            free_pages, n_free), keepalive)

@@ -81,3 +81,9 @@ def test_kernels_launched_early_read_nothing_as_constant():
     for f in files:
         code = re.sub(r"//.*", "", f.read_text())
         assert not re.search(r"__ldg|global\.nc|__restrict__", code), f.name
+
+
+def test_wrap_needs_a_v_pool_for_each_k_pool():
+    for k, v in (([16], []), ([], [16]), ([16, 32], [48])):
+        with pytest.raises(ValueError, match="pools"):
+            engine.PagedKv.wrap(None, k, v, 4, 16, 2, 128, capi.NAVI_F16, 2, 2, 16, 16, 16, 16)

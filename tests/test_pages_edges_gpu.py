@@ -394,3 +394,24 @@ def test_commit_path_of_a_refused_tree_of_many_rows(dev, n):
     torch.cuda.synchronize()
     assert acc.tolist() == [0, 2] and nl.tolist() == [0, 2] and nx.tolist() == [1, 1]
     assert path.tolist() == [-1] * n + [0, 1] + [-7] * 2
+
+
+def test_layers_without_a_pool_are_refused(dev):
+    """Tables without pools serve plan alone; a layer with one of two pools none of the others."""
+    x = torch.zeros(1 << 16, dtype=torch.float16, device="cuda")
+    table, held, free, n_free = i32([0] * 8), i32([0] * 2), i32(range(4)), i32([4])
+    p = lambda t: t.data_ptr()  # noqa: E731
+    s = op.Step([0, 0], [3, 2], [-1, 0, 1, -1, 0])
+    g = GpuStep(s)
+    ids = i32([0] * 64)
+    co = engine.CommitArgs(width=1, tokens=p(ids), targets=p(ids), root_target=p(ids), accepted=p(ids[16:]), path=p(ids[24:]), new_len=p(ids[32:]),
+                           next_token=p(ids[40:]))
+    for k, v in (([0, 0], [0, 0]), ([p(x), 0], [p(x), p(x)]), ([p(x), p(x)], [p(x), 0])):
+        kv = engine.PagedKv.wrap(dev, k, v, n_pages=4, page_size=16, n_kv_head=2, head_dim=128, dtype=capi.NAVI_F16, max_requests=2, max_blocks=4,
+                                 table=p(table), held=p(held), free_pages=p(free), n_free=p(n_free))
+        kv.plan(g.c, stream=0)
+        torch.cuda.synchronize()
+        assert g.status.tolist() == [0, 0]
+        refused(capi.NAVI_E_ARG, kv.store, g.c, 1, engine.StoreArgs(qkv=p(x), q_out=p(x), dtype=capi.NAVI_F16, n_head=2), stream=0)
+        refused(capi.NAVI_E_ARG, kv.attend, g.c, 1, engine.AttendArgs(q=p(x), out=p(x[8192:]), dtype=capi.NAVI_F16, n_head=2, scale=1.0), stream=0)
+        refused(capi.NAVI_E_ARG, kv.commit, g.c, co, stream=0)
