@@ -448,7 +448,8 @@ int navi_pages_plan(navi_pages * p, const navi_step * s, void * stream);
 typedef struct navi_store_args {
     const void * qkv;              /* device rows [n_head q heads | n_kv_head k heads | n_kv_head v heads] x head_dim */
     int64_t qkv_stride;            /* elements between rows; 0: dense */
-    void * q_out;                  /* device rows [n_head][head_dim]; may be the q part of qkv; NULL with n_head 0 */
+    void * q_out;                  /* device rows [n_head][head_dim]; may be the q part of qkv (with its stride), or lie
+                                      between its rows; NULL with n_head 0 */
     int64_t q_out_stride;          /* 0: dense */
     int dtype;                     /* of qkv and q_out: NAVI_F32, or the cache's own */
     int n_head;                    /* q heads in a row, 0 for rows of K and V alone */

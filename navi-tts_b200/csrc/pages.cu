@@ -707,6 +707,15 @@ void Pages::store(const navi_step & s, int layer, const navi_store_args & q, cud
     if (!q.qkv || (q.n_head > 0 && !q.q_out)) fail("pages store: NULL rows", NAVI_E_ARG);
     if (in < static_cast<int64_t>(heads) * D || out < static_cast<int64_t>(q.n_head) * D) fail("pages store: a row stride is shorter than the row", NAVI_E_ARG);
     if (!aligned16(q.qkv) || !aligned16(q.q_out) || in * elt % 16 || out * elt % 16) fail("pages store: rows must be 16-byte aligned", NAVI_E_ARG);
+    // q over its own rows, or between them; any other overlap would write rows that are still to be read
+    const bool same_rows = q.q_out == q.qkv && (in == out || s.max_rows == 1);
+    if (q.n_head > 0 && !same_rows &&
+        overlap(q.qkv, static_cast<size_t>((s.max_rows - 1) * in + static_cast<int64_t>(heads) * D) * elt, q.q_out,
+                static_cast<size_t>((s.max_rows - 1) * out + static_cast<int64_t>(q.n_head) * D) * elt)) {
+        const int64_t apart = (reinterpret_cast<intptr_t>(q.q_out) - reinterpret_cast<intptr_t>(q.qkv)) / elt, at = (apart % in + in) % in;
+        if (in != out || at < static_cast<int64_t>(heads) * D || at + static_cast<int64_t>(q.n_head) * D > in)
+            fail("pages store: q_out overlaps qkv otherwise than row for row (q_out_stride of rows in place is theirs)", NAVI_E_ARG);
+    }
     NAVI_CUDA(cudaSetDevice(dev_->info().ordinal));
     StoreArgs a{q.qkv, q.q_out, in, out, s.cu_rows, s.pos, s.slot, q.q_norm, q.k_norm, q.rope, static_cast<uint8_t *>(k_[static_cast<size_t>(layer)]),
                 static_cast<uint8_t *>(v_[static_cast<size_t>(layer)]), q.eps, s.n_req, s.max_rows, q.n_head, d_.n_kv_head, shift_, d_.n_pages, q.rope_positions, 1};

@@ -415,3 +415,30 @@ def test_layers_without_a_pool_are_refused(dev):
         refused(capi.NAVI_E_ARG, kv.store, g.c, 1, engine.StoreArgs(qkv=p(x), q_out=p(x), dtype=capi.NAVI_F16, n_head=2), stream=0)
         refused(capi.NAVI_E_ARG, kv.attend, g.c, 1, engine.AttendArgs(q=p(x), out=p(x[8192:]), dtype=capi.NAVI_F16, n_head=2, scale=1.0), stream=0)
         refused(capi.NAVI_E_ARG, kv.commit, g.c, co, stream=0)
+
+
+def test_store_refuses_q_over_other_rows(dev):
+    """q in place of its rows or between them, not over rows that are still to be read: the default stride of rows in place."""
+    c = Cache(dev, rows=2, blocks=4, fill=0)
+    g = planned(c, [3, 0], [2, 4])
+    H, G, D, T = 4, 2, 128, 6
+    W = (H + 2 * G) * D
+    x = torch.randn(T + 2, W + H * D, generator=torch.Generator().manual_seed(0)).cuda()
+    p, f, one = x.data_ptr(), 4, x.shape[1]
+    base = dict(qkv=p, dtype=capi.NAVI_F32, n_head=H)
+    for kw in (dict(q_out=p), dict(q_out=p + f * D, qkv_stride=one, q_out_stride=one), dict(q_out=p + f * one, qkv_stride=one, q_out_stride=one),
+               dict(q_out=p + f * (W - D), qkv_stride=one, q_out_stride=one), dict(q_out=p + f * W, qkv_stride=one),
+               dict(q_out=p + f * (W + D), qkv_stride=one, q_out_stride=one), dict(q_out=p, qkv_stride=one, q_out_stride=one - 4)):
+        refused(capi.NAVI_E_ARG, c.h.store, g.c, 0, engine.StoreArgs(**base, **kw), stream=0)
+    kw, vw = c.k[0].cpu().double(), c.v[0].cpu().double()
+    want = op.store(16, g.s, x[:T, :W].cpu(), H, G, kw, vw)
+    for off in (W, 0):                                      # between the rows, then in place
+        c.h.store(g.c, 0, engine.StoreArgs(**base, q_out=p + f * off, qkv_stride=one, q_out_stride=one), stream=0)
+        torch.cuda.synchronize()
+        assert (x[:T, off:off + H * D].cpu().double().view(T, H, D) - want).abs().max() < 1e-6
+    g1 = planned(c, [0], [1], req=[1])
+    y = x[T:, :].contiguous()
+    want = y[:1, :H * D].clone()
+    c.h.store(g1.c, 0, engine.StoreArgs(qkv=y.data_ptr(), q_out=y.data_ptr(), dtype=capi.NAVI_F32, n_head=H), stream=0)   # one row: no other
+    torch.cuda.synchronize()
+    assert torch.equal(y[:1, :H * D], want)
