@@ -18,7 +18,7 @@ void Pages::attend(const navi_step & s, int layer, const navi_attend_args & q, c
     if (q.n_head < 1 || q.n_head > 4096 || q.n_head % d_.n_kv_head) fail("pages attend: n_head must be a positive multiple of n_kv_head", NAVI_E_ARG);
     if (!(q.dtype == d_.dtype || (q.dtype == NAVI_F32 && d_.dtype == NAVI_F16))) fail("pages attend: rows are of the cache's type, or NAVI_F32 for an f16 cache", NAVI_E_ARG);
     if (!(q.scale > 0.f) || q.scale > 1e30f) fail("pages attend: scale must be positive and finite", NAVI_E_ARG);
-    if (s.n_req == 0 || s.max_rows == 0 || s.max_new == 0) return;
+    if (s.n_req == 0 || s.max_rows == 0) return;
     const int D = d_.head_dim;
     const int64_t elt = q.dtype == NAVI_F32 ? 4 : 2, dense = static_cast<int64_t>(q.n_head) * D, in = q.q_stride ? q.q_stride : dense,
                   out = q.out_stride ? q.out_stride : dense;
@@ -35,10 +35,13 @@ void Pages::attend(const navi_step & s, int layer, const navi_attend_args & q, c
                  d_.n_pages, d_.max_blocks, d_.max_requests};
     const int64_t most = std::min(s.max_new, s.max_rows);
     if (a.group > 1) a.group_mul = static_cast<uint32_t>(((1ull << 32) + static_cast<uint64_t>(a.group) - 1) / static_cast<uint64_t>(a.group));
-    if ((a.group & (a.group - 1)) != 0 && (most + 512) * a.group * a.group >= 1ll << 32) fail("pages attend: too many rows for this many heads to a KV head", NAVI_E_SHAPE);
-    // the list of key tiles that the blocks divide
+    // a request that is not served may have all of max_rows: its rows are counted too, and written
+    const int64_t all = static_cast<int64_t>(s.max_rows) + 512;
+    if (all * a.group > INT32_MAX || ((a.group & (a.group - 1)) != 0 && all * a.group * a.group >= 1ll << 32))
+        fail("pages attend: too many rows for this many heads to a KV head", NAVI_E_SHAPE);
+    // the list of key tiles that the blocks divide: of requests that are served, and a tile for each 8 rows x heads that are not
     const int64_t rows = most * a.group <= attn::FEW_ROWS_SHORT ? 16 : 128, items = (most * a.group + rows - 1) / rows * d_.n_kv_head * s.n_req, tiles = (static_cast<int64_t>(d_.max_blocks) * d_.page_size + attn::KT - 1) / attn::KT + 2;
-    if (items * tiles >= 1ll << 31) fail("pages attend: requests x heads x tokens pass 31 bits of key tiles", NAVI_E_SHAPE);
+    if (items * tiles + (all * a.group / 8 + s.n_req) * 2 * d_.n_kv_head >= 1ll << 31) fail("pages attend: requests x heads x tokens pass 31 bits of key tiles", NAVI_E_SHAPE);
     const int64_t m = most * a.group;
     const size_t at = static_cast<size_t>(2 * layer);
     if (m <= attn::FEW_ROWS || (m <= attn::FEW_ROWS_SHORT && s.n_req * d_.n_kv_head < sms)) return attn::attend_few(a, page_maps_[at], page_maps_[at + 1], q.dtype, d_.dtype, static_cast<int>(m), sms, stream);

@@ -442,3 +442,32 @@ def test_store_refuses_q_over_other_rows(dev):
     c.h.store(g1.c, 0, engine.StoreArgs(qkv=y.data_ptr(), q_out=y.data_ptr(), dtype=capi.NAVI_F32, n_head=H), stream=0)   # one row: no other
     torch.cuda.synchronize()
     assert torch.equal(y[:1, :H * D], want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("parent", ["tree", None])
+@pytest.mark.parametrize("new", [[1, 2], [70, 3], [200, 300]])
+def test_attend_with_max_new_zero(dev, dtype, parent, new):
+    """No request may have rows: those that have are refused, and their rows get 0 and -inf as any refused request's."""
+    _, _, kt, kcode = TYPES[dtype]
+    c = Cache(dev, rows=2, blocks=20, G=1, kt=kt, code=kcode)
+    rng = random.Random(1)
+    s = op.Step([0, 0], new, sum((tree(rng, n) for n in new), []) if parent else None, max_new=0)
+    g = GpuStep(s, words=0)
+    c.h.plan(g.c, stream=0)
+    op.plan(c.t, s)
+    torch.cuda.synchronize()
+    assert g.status.tolist() == [capi.NAVI_E_SHAPE] * 2
+    out, lse = check_attend(c, g, dtype, 2)
+    c.h.check(stream=0)
+    assert (out == 0).all() and (lse == -math.inf).all()
+
+
+def test_attend_refuses_more_rows_than_its_counts_hold(dev):
+    """Room for rows whose number times the heads passes 31 bits, or the exact quotients of 32; nothing is launched."""
+    c = Cache(dev, rows=1, blocks=4, G=1)
+    g = planned(c, [0], [3])
+    x = torch.zeros(1 << 14, device="cuda")
+    for rows, H in ((1 << 30, 2), (1 << 24, 128), (1 << 29, 3), (5_000_000, 31)):
+        refused(capi.NAVI_E_SHAPE, c.h.attend, step_with(g, max_rows=rows, max_new=4),
+                0, engine.AttendArgs(q=x.data_ptr(), out=x.data_ptr() + 32768, dtype=capi.NAVI_F32, n_head=H, scale=0.1), stream=0)
