@@ -87,7 +87,8 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
     __shared__ uint32_t bad[16];   // tokens from the item's first masked tile on whose V is not finite
     __shared__ int red[9];
     __shared__ Share share;
-    __shared__ int abort_flag, is_last;
+    __shared__ volatile int abort_flag;
+    __shared__ int is_last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, tq = lane & 3;
     if (tid == 0) {
         abort_flag = 0;
@@ -145,7 +146,8 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
                 page = next;
             }
         }
-        // after an abort the copies still under way land before the block's shared memory goes
+        // after an abort, whoever raised it, the copies still under way land before the block's shared memory goes
+        named_sync(2, 288);
         if (abort_flag)
             for (int k = max(n - L::STAGES, 0); k < n; ++k) mbar_drain(&full[k % L::STAGES], (k / L::STAGES) & 1);
         return;
@@ -442,6 +444,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
         __syncwarp();
         if (lane == 0) mbar_arrive(&segs.empty[sn % SegmentRing::N]);
     }
+    named_sync(2, 288);
 }
 
 template <class T, class C, int D> void few(const AttendArgs & a, const CUtensorMap & k, const CUtensorMap & v, int rows, int sms, cudaStream_t stream) {

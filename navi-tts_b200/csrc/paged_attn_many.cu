@@ -63,7 +63,8 @@ struct ManyControl {
     int red[12];
     Share sh;
     uint32_t tmem_at;
-    int abort_flag, is_last;
+    volatile int abort_flag;
+    int is_last;
 };
 
 // K-major rows (Q, K): desc_kmajor_sw128 of umma.cuh. V is the B operand with its rows along the
@@ -156,6 +157,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
     if (!one) share_of_block<ROWS, EXTRA, 384>(a, S.sh, S.red);
     const uint32_t tmem = S.tmem_at;
     const Wait wait{&S.abort_flag, a.err};
+    int issued = 0;              // by this warp: tiles of K and V, or q of so many segments by TMA
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
@@ -205,9 +207,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                     page = next;
                 }
             }
-            // after an abort the copies still under way land before the block's shared memory goes
-            if (S.abort_flag)
-                for (int k = max(n - L::STAGES, 0); k < n; ++k) mbar_drain(&S.full[k % L::STAGES], (k / L::STAGES) & 1);
+            issued = n;
         } else if (warp == 9) {
             constexpr uint32_t ID_S = idesc<C>(128, KT, false), ID_O = idesc<C>(128, D, true);
             const uint32_t leader = lane == 0, tm = static_cast<uint32_t>(uniform(static_cast<int>(tmem)));
@@ -331,6 +331,7 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                 if (named_sync_or(2, 64, !ok) || it.nt < 0) break;   // after an abort both warps leave together
                 if (has && a.q_boxes) {
                     ++nq;
+                    issued = nq;
                     if (tid == 320) {
                         const int tiles = it.m > 128 ? 2 : 1;
                         mbar_arrive_expect_tx(&S.q_full, static_cast<uint32_t>(tiles * L::QTILE));
@@ -609,6 +610,12 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
     __syncwarp();
     fence_before_sync();
     __syncthreads();
+    // after an abort, whoever raised it, the copies still under way land before the block's shared memory goes
+    if (S.abort_flag) {
+        if (warp == 8)
+            for (int k = max(issued - L::STAGES, 0); k < issued; ++k) mbar_drain(&S.full[k % L::STAGES], (k / L::STAGES) & 1);
+        if (warp == 10 && issued > 0) mbar_drain(&S.q_full, (issued - 1) & 1);
+    }
     if (warp == 9) {
         fence_after_sync();
         tmem_dealloc(tmem, 512);

@@ -87,3 +87,14 @@ def test_wrap_needs_a_v_pool_for_each_k_pool():
     for k, v in (([16], []), ([], [16]), ([16, 32], [48])):
         with pytest.raises(ValueError, match="pools"):
             engine.PagedKv.wrap(None, k, v, 4, 16, 2, 128, capi.NAVI_F16, 2, 2, 16, 16, 16, 16)
+
+
+def test_copies_land_before_a_block_that_gave_up_ends():
+    """A wait of any warp may give up after the warp that copies has left its loop: the copies under way (K and V, and q
+    by TMA in the kernel for many rows) are waited for behind the last barrier of the block."""
+    import pathlib
+    src = pathlib.Path(__file__).resolve().parent.parent / "navi-tts_b200" / "csrc"
+    few, many = ((src / f).read_text() for f in ("paged_attn_few.cu", "paged_attn_many.cu"))
+    assert few.index("named_sync(2, 288);") < few.index("mbar_drain(") and few.count("named_sync(2, 288);") == 2
+    last = many.rindex("__syncthreads();")
+    assert many.index("mbar_drain(&S.full[") > last and many.index("mbar_drain(&S.q_full") > last
