@@ -34,7 +34,10 @@ template <class C> __device__ __forceinline__ void mma(float (&c)[4], const uint
 // it). With 8 rows the high terms are rows 0..7 of the 16 that a product has and the low ones rows
 // 8..15, so that they cost nothing. The tensor cores' sums truncate: the low
 // terms and each step's contribution are summed apart and added in f32. 16-bit rows are exact, and
-// p is rounded once to the type that the result has: 8 bits of bf16, 11 of f16 down to 2^-28 of the largest weight.
+// their p is two terms too in tiles of 8. With more rows it is rounded once to the type that the
+// result has, 8 bits of bf16, 11 of f16 down to 2^-28 of the largest weight, about the result's own rounding:
+// a second term there is products of its own (5 rows of two heads over 200,003 bf16 tokens 132 -> 135.5 us, 48 f16
+// trees of up to 8 such rows 99 -> 107), in tiles of 8 none (48 single f16 rows 89.5 -> 87.7 us, without the spills).
 //
 // Measured on one B200: one request of 200,003 tokens, 5 rows, bf16: 129 to 133 us, 6.2 to 6.3 TB/s (a copy
 // reaches 6.54). 48 single rows over pages of 16: 84 us with a page as one box, 92.7 with one for each 64
@@ -335,7 +338,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
                             const float p0 = exp2_fast(fmaf(v[0], scale[x], -ref)), p1 = exp2_fast(fmaf(v[1], scale[x], -ref));
                             l[x] += p0 + p1;
                             if constexpr (TERMS) split_pair<C>(p0, p1, ph[k][2 * y + x], pl[k][2 * y + x]);
-                            else if constexpr (SPLIT) split_pair<C>(p0, p1, ph[k][2 * y], ph[k][2 * y + 1]);
+                            else if constexpr (EIGHT) split_pair<C>(p0, p1, ph[k][2 * y], ph[k][2 * y + 1]);
                             else ph[k][2 * y + x] = pack<C>(p0, p1);
                         }
                 }
@@ -361,7 +364,7 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
 #pragma unroll
                         for (int y = 0; y < 2; ++y)
 #pragma unroll
-                            for (int e = 0; e < 2 * XR; ++e) o[2 * dp + y][e] += SPLIT && EIGHT ? c[y][e] + c[y][2 + e] : c[y][e];
+                            for (int e = 0; e < 2 * XR; ++e) o[2 * dp + y][e] += EIGHT ? c[y][e] + c[y][2 + e] : c[y][e];
                     } else {
 #pragma unroll
                         for (int k = 0; k < KS; ++k) {

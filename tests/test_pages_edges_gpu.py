@@ -471,3 +471,27 @@ def test_attend_refuses_more_rows_than_its_counts_hold(dev):
     for rows, H in ((1 << 30, 2), (1 << 24, 128), (1 << 29, 3), (5_000_000, 31)):
         refused(capi.NAVI_E_SHAPE, c.h.attend, step_with(g, max_rows=rows, max_new=4),
                 0, engine.AttendArgs(q=x.data_ptr(), out=x.data_ptr() + 32768, dtype=capi.NAVI_F32, n_head=H, scale=0.1), stream=0)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("H,G,D,new", [(4, 2, 128, [1, 1, 1]), (4, 2, 64, [4, 1, 3]), (8, 1, 128, [1, 0, 1]), (3, 3, 64, [8, 5, 7])])
+def test_attend_16_bit_rows_of_tiles_of_8_keep_their_weights(dev, dtype, H, G, D, new):
+    """Up to 8 rows x heads: weights enter the product as two terms (2^-16 of each with bf16, 2^-22 with f16), so the error is
+    that of f32 rows and the result's one rounding."""
+    tt, code, kt, kcode = TYPES[dtype]
+    ctx = [1500, 3, 700]
+    c = Cache(dev, rows=3, blocks=100, G=G, D=D, kt=kt, code=kcode, fill=0)
+    c.k.normal_(generator=torch.Generator("cuda").manual_seed(1))
+    c.v.normal_(generator=torch.Generator("cuda").manual_seed(2))
+    planned(c, [0] * 3, ctx, None)
+    g = planned(c, ctx, new)
+    T = sum(new)
+    q = (torch.randn(T, H, D, generator=torch.Generator().manual_seed(3)) * 2).to(tt)
+    qd, out = q.cuda(), torch.zeros(T, H, D, dtype=tt, device="cuda")
+    c.h.attend(g.c, 0, engine.AttendArgs(q=qd.data_ptr(), out=out.data_ptr(), dtype=code, n_head=H, scale=D ** -0.5), stream=0)
+    c.h.check(stream=0)
+    kd, vd = c.k[0].cpu().double(), c.v[0].cpu().double()
+    want, _ = op.attend(c.t, g.s, q.double(), kd, vd, D ** -0.5)
+    ds = 2.0 ** -20 * D ** -0.5 * float(q.double().abs().sum(2).max()) * float(kd.abs().max())
+    tol = float(vd.abs().max()) * (2 * ds + 2.0 ** -20 + 1510 * 2.0 ** -24) + (2.0 ** -16 if dtype == "bf16" else 2.0 ** -22) * float(vd.abs().max())
+    assert ((out.cpu().double() - want).abs() <= tol + U[dtype] * want.abs()).all(), ((out.cpu().double() - want).abs().max(), tol)
