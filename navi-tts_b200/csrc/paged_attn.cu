@@ -29,10 +29,35 @@ void Pages::attend(const navi_step & s, int layer, const navi_attend_args & q, c
     NAVI_CUDA(cudaSetDevice(dev_->info().ordinal));
     const int sms = dev_->info().multiprocessors;
     const PagesScratch sc(dev_->scratch(stream, PagesScratch::bytes(sms)), sms);
-    attn::AttendArgs a{q.q, q.out, q.lse, static_cast<const uint8_t *>(k_[static_cast<size_t>(layer)]),
-                       static_cast<const uint8_t *>(v_[static_cast<size_t>(layer)]), d_.table, s.req, s.ctx_len, s.cu_rows, s.status, s.parent ? s.mask : nullptr, sc.pieces, sc.arrived, sc.err,
-                 in, out, q.scale * 1.4426950408889634f, 0, s.n_req, s.max_rows, s.mask_words, q.n_head, d_.n_kv_head, q.n_head / d_.n_kv_head, 0, D, shift_,
-                 d_.n_pages, d_.max_blocks, d_.max_requests};
+    attn::AttendArgs a{};
+    a.q = q.q;
+    a.out = q.out;
+    a.lse = q.lse;
+    a.k = static_cast<const uint8_t *>(k_[static_cast<size_t>(layer)]);
+    a.v = static_cast<const uint8_t *>(v_[static_cast<size_t>(layer)]);
+    a.table = d_.table;
+    a.req = s.req;
+    a.ctx_len = s.ctx_len;
+    a.cu_rows = s.cu_rows;
+    a.status = s.status;
+    a.mask = s.parent ? s.mask : nullptr;
+    a.pieces = sc.pieces;
+    a.arrived = sc.arrived;
+    a.err = sc.err;
+    a.q_stride = in;
+    a.out_stride = out;
+    a.scale = q.scale * 1.4426950408889634f;
+    a.n_req = s.n_req;
+    a.max_rows = s.max_rows;
+    a.mask_words = s.mask_words;
+    a.n_head = q.n_head;
+    a.n_kv = d_.n_kv_head;
+    a.group = q.n_head / d_.n_kv_head;
+    a.head_dim = D;
+    a.shift = shift_;
+    a.n_pages = d_.n_pages;
+    a.max_blocks = d_.max_blocks;
+    a.max_requests = d_.max_requests;
     const int64_t most = std::min(s.max_new, s.max_rows);
     if (a.group > 1) a.group_mul = static_cast<uint32_t>(((1ull << 32) + static_cast<uint64_t>(a.group) - 1) / static_cast<uint64_t>(a.group));
     // a request that is not served may have all of max_rows: its rows are counted too, and written

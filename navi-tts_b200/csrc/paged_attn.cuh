@@ -515,18 +515,14 @@ template <class C, int D> __device__ __forceinline__ const C * token_at(const At
     return reinterpret_cast<const C *>(pool) + (((static_cast<size_t>(page) * a.n_kv + s.g) << a.shift) + (key & ((1 << a.shift) - 1))) * D;
 }
 
-// y += 2^(scale q k - ref) v[dim .. dim + 3] of row m of the segment and token `key`.
-template <class T, class C, int D> __device__ __forceinline__ void add_token(const AttendArgs & a, const Segment & s, int m, int key, float ref, int dim, float4 & y) {
+// The weight 2^(scale q k - ref) of row m of the segment and token `key`.
+template <class T, class C, int D> __device__ __forceinline__ float token_weight(const AttendArgs & a, const Segment & s, int m, int key, float ref) {
     const T * q = row_at<const T>(a, a.q, a.q_stride, s, m);
-    const C * k = token_at<C, D>(a, s, a.k, key), * v = token_at<C, D>(a, s, a.v, key) + dim;
+    const C * k = token_at<C, D>(a, s, a.k, key);
     float z = 0.f;
 #pragma unroll 1
     for (int d = 0; d < D; ++d) z += static_cast<float>(q[d]) * static_cast<float>(k[d]);
-    const float w = exp2_fast(fmaf(z, a.scale, -ref));
-    y.x += w * static_cast<float>(v[0]);
-    y.y += w * static_cast<float>(v[1]);
-    y.z += w * static_cast<float>(v[2]);
-    y.w += w * static_cast<float>(v[3]);
+    return exp2_fast(fmaf(z, a.scale, -ref));
 }
 
 // The ring of segments: one warp fills it, every other role reads it.

@@ -62,7 +62,13 @@ __device__ __noinline__ float4 with_bad(const AttendArgs & a, const Segment & s,
 #pragma unroll 1
         for (uint32_t left = bad[w]; left; left &= left - 1) {
             const int key = bad0 + 32 * w + __ffs(left) - 1;
-            if (seen_bits(a, s, j, key - s.ctx, s.n_keys - key) & 1) add_token<T, C, D>(a, s, m, key, ref, dim, y);
+            if (!(seen_bits(a, s, j, key - s.ctx, s.n_keys - key) & 1)) continue;
+            const float w = token_weight<T, C, D>(a, s, m, key, ref);
+            const C * v = token_at<C, D>(a, s, a.v, key) + dim;
+            y.x += w * static_cast<float>(v[0]);
+            y.y += w * static_cast<float>(v[1]);
+            y.z += w * static_cast<float>(v[2]);
+            y.w += w * static_cast<float>(v[3]);
         }
     return y;
 }

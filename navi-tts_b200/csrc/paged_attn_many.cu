@@ -553,12 +553,8 @@ __global__ void __launch_bounds__(384, 1) k_attend_many(const __grid_constant__ 
                             for (uint32_t left = S.bad[w]; left; left &= left - 1) {
                                 const int key = bad0 + 32 * w + __ffs(left) - 1;
                                 if (!(seen_bits(a, it, j, key - ctx, n_keys - key) & 1)) continue;
-                                const T * q = row_at<const T>(a, a.q, a.q_stride, it, m);
-                                const C * kr = token_at<C, D>(a, it, a.k, key), * vr = token_at<C, D>(a, it, a.v, key) + c;
-                                float z = 0.f;
-#pragma unroll 1
-                                for (int d = 0; d < D; ++d) z += static_cast<float>(q[d]) * static_cast<float>(kr[d]);
-                                const float u = exp2_fast(fmaf(z, a.scale, top == -INFINITY ? 0.f : -top)) * inv;
+                                const float u = token_weight<T, C, D>(a, it, m, key, top == -INFINITY ? 0.f : top) * inv;
+                                const C * vr = token_at<C, D>(a, it, a.v, key) + c;
 #pragma unroll
                                 for (int k = 0; k < 32; ++k) v[k] += u * static_cast<float>(vr[k]);
                             }

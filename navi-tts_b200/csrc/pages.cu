@@ -684,7 +684,7 @@ void Pages::plan(const navi_step & s, cudaStream_t stream, int positions) const 
     NAVI_CUDA(cudaSetDevice(dev_->info().ordinal));
     const int sms = dev_->info().multiprocessors;
     const PagesScratch sc(dev_->scratch(stream, PagesScratch::bytes(sms)), sms);
-    PlanArgs a{s, d_.table, d_.held, d_.free_pages, d_.n_free, sc.tickets, sc.broken, d_.n_pages, shift_, d_.max_blocks, d_.max_requests, positions};
+    PlanArgs a{s, d_.table, d_.held, d_.free_pages, d_.n_free, sc.ticket, sc.broken, d_.n_pages, shift_, d_.max_blocks, d_.max_requests, positions};
     const size_t smem = (4 * static_cast<size_t>(s.n_req) + 1) * sizeof(int);
     static_assert((4 * static_cast<size_t>(NAVI_PAGES_MAX_REQUESTS) + 1) * sizeof(int) < 200 * 1024);
     if (smem > 40 * 1024)
@@ -784,7 +784,7 @@ void Pages::check(cudaStream_t stream) const {
     if (std::all_of(err.begin(), err.end(), [](int e) { return e == 0; })) return;
     NAVI_CUDA(cudaDeviceSynchronize());
     for (size_t k = 0; k < blocks.size(); ++k)   // counters of blocks that gave up
-        if (err[k]) NAVI_CUDA(cudaMemsetAsync(PagesScratch(blocks[k], sms).tickets, 0, PagesScratch::ints(sms) * sizeof(int), stream));
+        if (err[k]) NAVI_CUDA(cudaMemsetAsync(PagesScratch(blocks[k], sms).ticket, 0, PagesScratch::ints(sms) * sizeof(int), stream));
     NAVI_CUDA(cudaStreamSynchronize(stream));
     fail("pages: a wait for a copy or a matrix product passed its deadline", NAVI_E_TIMEOUT);
 }

@@ -53,17 +53,16 @@ private:
 // A block of scratch (Device::scratch), laid out for every operator that hands work from
 // one block to another. All counters are zero between launches.
 struct PagesScratch {
-    static constexpr size_t TICKETS = 64;                            // launch-wide counters
     static constexpr size_t PIECE_FLOATS = 256 * (128 + 2);          // attend: one block's unfinished item
-    int * tickets, * broken, * arrived, * err;                       // broken: plan, requests whose tree is refused; commit, blocks
+    int * ticket, * broken, * arrived, * err;                        // ticket: plan, blocks that have finished; broken: plan, requests whose tree is refused; commit, blocks
     float * pieces;                                                  // two a block
 
     // `blocks`: the most blocks of a launch that leave pieces (one a multiprocessor)
-    static size_t ints(int blocks) { return (TICKETS + NAVI_PAGES_MAX_REQUESTS + static_cast<size_t>(blocks) + 1 + 63) / 64 * 64; }
+    static size_t ints(int blocks) { return (1 + NAVI_PAGES_MAX_REQUESTS + static_cast<size_t>(blocks) + 1 + 63) / 64 * 64; }
     static size_t bytes(int blocks) { return ints(blocks) * sizeof(int) + 2 * static_cast<size_t>(blocks) * PIECE_FLOATS * sizeof(float); }
     PagesScratch(void * p, int blocks)
-        : tickets(static_cast<int *>(p)), broken(tickets + TICKETS), arrived(broken + NAVI_PAGES_MAX_REQUESTS), err(arrived + blocks),
-          pieces(reinterpret_cast<float *>(tickets + ints(blocks))) {}
+        : ticket(static_cast<int *>(p)), broken(ticket + 1), arrived(broken + NAVI_PAGES_MAX_REQUESTS), err(arrived + blocks),
+          pieces(reinterpret_cast<float *>(ticket + ints(blocks))) {}
 };
 
 } // namespace navi
