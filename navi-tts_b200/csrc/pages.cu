@@ -47,6 +47,8 @@ struct PlanArgs {
     int32_t * table, * held, * free_pages, * n_free;
     int * ticket, * broken;
     int n_pages, shift, max_blocks, max_requests;
+};
+struct PlanLimited : PlanArgs {
     int positions;   // no row may be at this position or past it
 };
 
@@ -96,7 +98,9 @@ __device__ __forceinline__ int owner(const int * a, int n, int e) {
 // inputs (asked for together, the parents of the block's rows with them), one for the pages, one to count
 // the blocks. A plan and the plan that undoes it, launched in a row: 9 us for four single rows, 12 for 64
 // trees of up to 61 rows (899 in all), 18 for a thousand prompts (218,522 rows).
-__global__ void __launch_bounds__(PLAN_THREADS) k_pages_plan(const __grid_constant__ PlanArgs a) {
+// Args: PlanArgs, or PlanLimited for a talker's step.
+template <class Args> __global__ void __launch_bounds__(PLAN_THREADS) k_pages_plan(const __grid_constant__ Args a) {
+    constexpr bool LIMIT = std::is_same_v<Args, PlanLimited>;
     extern __shared__ int plan_smem[];
     __shared__ long long red64[PLAN_THREADS / 32];
     __shared__ int par[2 * PLAN_THREADS];
@@ -138,13 +142,17 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_pages_plan(const __grid_consta
         long long row = block_scan(rows, red64, total);
         if (tid == 0) cu[B] = static_cast<int>(min(total, cap));
         long long grow = 0, surplus = 0;
+        const auto past = [&](int n, int ctx) {   // a chain's last row
+            if constexpr (LIMIT) return !a.s.parent && n > 0 && ctx > a.positions - n;
+            return false;
+        };
         const auto sort = [&](int i, int n, int ctx, int tr, int held) {
             cu[i] = static_cast<int>(min(row, cap));
             row += max(n, 0);
             int status = NAVI_OK, g = 0, u = 0;
             const long long need = (static_cast<long long>(max(ctx, 0)) + max(n, 0) + (1 << a.shift) - 1) >> a.shift;
             if (n < 0 || ctx < 0 || tr < 0 || tr >= a.max_requests || held < 0 || held > MB) status = NAVI_E_ARG;
-            else if (n > a.s.max_new || need > MB || row > cap || (!a.s.parent && n > 0 && ctx > a.positions - n)) status = NAVI_E_SHAPE;
+            else if (n > a.s.max_new || need > MB || row > cap || past(n, ctx)) status = NAVI_E_SHAPE;
             else {
                 g = max(static_cast<int>(need) - held, 0);
                 u = max(held - static_cast<int>(need), 0);
@@ -263,7 +271,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_pages_plan(const __grid_consta
             const int page = blk < held ? table_row(i)[blk] : taken_page(cg[i] + blk - held);
             if (page >= 0 && page < a.n_pages) slot = (static_cast<int64_t>(page) << a.shift) + ((ctx + j) & ((1 << a.shift) - 1));
         }
-        if (a.s.parent && (!whole || ctx + depth >= a.positions)) atomicMax(a.broken + i, whole ? 1 : 2);
+        if constexpr (LIMIT) {
+            if (a.s.parent && (!whole || ctx + depth >= a.positions)) atomicMax(a.broken + i, whole ? 1 : 2);
+        } else {
+            if (!whole) a.broken[i] = 2;
+        }
         a.s.row_req[r] = i;
         a.s.pos[r] = ctx + depth;
         a.s.slot[r] = slot;
@@ -284,9 +296,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_pages_plan(const __grid_consta
     for (int i = tid; i < B; i += PLAN_THREADS) {
         int status = st[i];
         if (status == NAVI_OK) a.held[a.s.req ? a.s.req[i] : i] = need_of(i);
-        if (const int why = a.s.parent ? __ldcg(a.broken + i) : 0; why) {   // 2: a parent, 1: a position
-            a.broken[i] = 0;
-            if (status == NAVI_OK) status = why == 2 ? NAVI_E_ARG : NAVI_E_SHAPE;
+        if (a.s.parent) {
+            if (const int why = __ldcg(a.broken + i); why) {   // 2: a parent, 1: a position
+                a.broken[i] = 0;
+                if (status == NAVI_OK) status = LIMIT && why == 1 ? NAVI_E_SHAPE : NAVI_E_ARG;
+            }
         }
         a.s.status[i] = status;
     }
@@ -457,7 +471,7 @@ struct CommitArgs {
     navi_step s;
     navi_commit_args c;
     uint8_t * k[NAVI_PAGES_MAX_LAYERS], * v[NAVI_PAGES_MAX_LAYERS];
-    int * walked;                       // next_token is root_target: the blocks of a request that have walked; else nullptr
+    int * walked;                       // IN_PLACE: the blocks of a request that have walked
     int n_layer, n_kv, shift, chunks;   // chunks: 16-byte pieces of one head's row
     int n_pages;
 };
@@ -472,7 +486,8 @@ constexpr int COMMIT_THREADS = 256;
 // trips to L2 (parents, ids, choices, slots) and then by the moves: four trees 7 us, as long as a launch;
 // 64 trees through 28 layers 10.6 to 11.8 us, 3.5 to 3.9 TB/s. 16 bytes at a time with four moves ahead took
 // it from 29 to 17.0 us, twice the blocks (8 for 4 times the multiprocessors) to 11.5; 16 times takes 12.1.
-__global__ void __launch_bounds__(COMMIT_THREADS) k_pages_commit(const __grid_constant__ CommitArgs a) {
+// IN_PLACE: next_token is root_target.
+template <bool IN_PLACE> __global__ void __launch_bounds__(COMMIT_THREADS) k_pages_commit(const __grid_constant__ CommitArgs a) {
     __shared__ int child[NAVI_STEP_MAX_TREE + 1];
     __shared__ int path[NAVI_STEP_MAX_TREE];
     __shared__ int64_t from[NAVI_STEP_MAX_TREE], to[NAVI_STEP_MAX_TREE];
@@ -480,7 +495,7 @@ __global__ void __launch_bounds__(COMMIT_THREADS) k_pages_commit(const __grid_co
     griddep_wait();
     griddep_launch_dependents();
     const int i = blockIdx.x, tid = threadIdx.x, W = a.c.width;
-    const int r0 = a.s.cu_rows[i], rows = a.s.cu_rows[i + 1] - r0, n = min(rows, NAVI_STEP_MAX_TREE);   // more rows: not served
+    const int r0 = a.s.cu_rows[i], n = min(a.s.cu_rows[i + 1] - r0, NAVI_STEP_MAX_TREE);
     const bool served = a.s.status[i] == NAVI_OK;
     for (int j = tid; j <= n; j += COMMIT_THREADS) child[j] = INT_MAX;
     __syncthreads();
@@ -521,7 +536,7 @@ __global__ void __launch_bounds__(COMMIT_THREADS) k_pages_commit(const __grid_co
     const int k0 = moved, k1 = count;
     const int32_t * nx = k1 > 0 ? a.c.targets + static_cast<size_t>(r0 + path[k1 - 1]) * W : a.c.root_target + static_cast<size_t>(i) * W;
     int32_t * next = a.c.next_token + static_cast<size_t>(i) * W;
-    if (a.walked && tid >= COMMIT_THREADS - 32) {   // over the ids that the other blocks compare: by the last of them, when all have
+    if (IN_PLACE && tid >= COMMIT_THREADS - 32) {   // over the ids that the other blocks compare: by the last of them, when all have
         const int lane = tid & 31;
         int last = 0;
         if (lane == 0) {
@@ -533,8 +548,10 @@ __global__ void __launch_bounds__(COMMIT_THREADS) k_pages_commit(const __grid_co
             for (int x = lane; x < W; x += 32) next[x] = nx[x];
     }
     if (blockIdx.y == 0) {
-        for (int j = tid; j < rows; j += COMMIT_THREADS) a.c.path[r0 + j] = j < k1 ? path[j] : -1;
-        if (!a.walked)
+        for (int j = tid; j < n; j += COMMIT_THREADS) a.c.path[r0 + j] = j < k1 ? path[j] : -1;
+        if (n == NAVI_STEP_MAX_TREE)   // more rows are not served
+            for (int j = r0 + n + tid; j < a.s.cu_rows[i + 1]; j += COMMIT_THREADS) a.c.path[j] = -1;
+        if constexpr (!IN_PLACE)
             for (int x = tid; x < W; x += COMMIT_THREADS) next[x] = nx[x];
         if (tid == 0) {
             a.c.accepted[i] = k1;
@@ -684,14 +701,18 @@ void Pages::plan(const navi_step & s, cudaStream_t stream, int positions) const 
     NAVI_CUDA(cudaSetDevice(dev_->info().ordinal));
     const int sms = dev_->info().multiprocessors;
     const PagesScratch sc(dev_->scratch(stream, PagesScratch::bytes(sms)), sms);
-    PlanArgs a{s, d_.table, d_.held, d_.free_pages, d_.n_free, sc.ticket, sc.broken, d_.n_pages, shift_, d_.max_blocks, d_.max_requests, positions};
+    PlanArgs a{s, d_.table, d_.held, d_.free_pages, d_.n_free, sc.ticket, sc.broken, d_.n_pages, shift_, d_.max_blocks, d_.max_requests};
     const size_t smem = (4 * static_cast<size_t>(s.n_req) + 1) * sizeof(int);
     static_assert((4 * static_cast<size_t>(NAVI_PAGES_MAX_REQUESTS) + 1) * sizeof(int) < 200 * 1024);
-    if (smem > 40 * 1024)
-        NAVI_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(&k_pages_plan), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>((4 * NAVI_PAGES_MAX_REQUESTS + 1) * sizeof(int))));
     const int blocks = std::clamp((s.max_rows + PLAN_THREADS - 1) / PLAN_THREADS, 1, 2 * sms);
-    NAVI_CUDA(launch_pdl(k_pages_plan, dim3(static_cast<unsigned>(blocks)), dim3(PLAN_THREADS), smem, stream, a));
+    const auto go = [&](auto kernel, const auto & args) {
+        if (smem > 40 * 1024)
+            NAVI_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           static_cast<int>((4 * NAVI_PAGES_MAX_REQUESTS + 1) * sizeof(int))));
+        NAVI_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(blocks)), dim3(PLAN_THREADS), smem, stream, args));
+    };
+    if (positions == INT_MAX) go(k_pages_plan<PlanArgs>, a);
+    else go(k_pages_plan<PlanLimited>, PlanLimited{a, positions});
 }
 
 void Pages::store(const navi_step & s, int layer, const navi_store_args & q, cudaStream_t stream) const {
@@ -766,7 +787,8 @@ void Pages::commit(const navi_step & s, const navi_commit_args & c, cudaStream_t
     if (items > INT32_MAX / 2) fail("pages commit: too many heads", NAVI_E_SHAPE);
     const int most = static_cast<int>((items + COMMIT_THREADS - 1) / COMMIT_THREADS);
     const int z = std::clamp(8 * dev_->info().multiprocessors / s.n_req, 1, std::min(most, 65535));
-    NAVI_CUDA(launch_pdl(k_pages_commit, dim3(static_cast<unsigned>(s.n_req), static_cast<unsigned>(z)), dim3(COMMIT_THREADS), 0, stream, a));
+    NAVI_CUDA(launch_pdl(in_place ? k_pages_commit<true> : k_pages_commit<false>, dim3(static_cast<unsigned>(s.n_req), static_cast<unsigned>(z)), dim3(COMMIT_THREADS),
+                         0, stream, a));
 }
 
 void Pages::check(cudaStream_t stream) const {

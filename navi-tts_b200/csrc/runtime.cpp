@@ -503,9 +503,9 @@ void * Device::scratch(cudaStream_t stream, size_t bytes) const {
     cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
     unsigned long long id = 0;
     cudaGraph_t graph = nullptr;
-    NAVI_CUDA(cudaStreamGetCaptureInfo_v2(stream, &status, &id, &graph, nullptr, nullptr));
+    NAVI_CUDA(cudaStreamIsCapturing(stream, &status));
     if (status == cudaStreamCaptureStatusInvalidated) fail("the capture of the stream has failed", NAVI_E_CUDA);
-    if (status == cudaStreamCaptureStatusNone) id = 0;
+    if (status == cudaStreamCaptureStatusActive) NAVI_CUDA(cudaStreamGetCaptureInfo_v2(stream, &status, &id, &graph, nullptr, nullptr));
     Scratch & sc = *scratch_;
     void * block = nullptr;
     {

@@ -495,3 +495,19 @@ def test_attend_16_bit_rows_of_tiles_of_8_keep_their_weights(dev, dtype, H, G, D
     ds = 2.0 ** -20 * D ** -0.5 * float(q.double().abs().sum(2).max()) * float(kd.abs().max())
     tol = float(vd.abs().max()) * (2 * ds + 2.0 ** -20 + 1510 * 2.0 ** -24) + (2.0 ** -16 if dtype == "bf16" else 2.0 ** -22) * float(vd.abs().max())
     assert ((out.cpu().double() - want).abs() <= tol + U[dtype] * want.abs()).all(), ((out.cpu().double() - want).abs().max(), tol)
+
+
+# ---- pages of 64 ---------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("H,G,D", [(4, 2, 128), (2, 2, 64)])
+@pytest.mark.parametrize("parent", ["tree", None])
+@pytest.mark.parametrize("ctx,new", [([0, 63, 64], [1, 1, 1]), ([129, 65, 0], [12, 3, 64]), ([200], [190])])
+def test_attend_pages_of_64(dev, dtype, H, G, D, parent, ctx, new):
+    _, _, kt, kcode = TYPES[dtype]
+    c = Cache(dev, rows=len(ctx), blocks=7, page=64, G=G, D=D, kt=kt, code=kcode)
+    planned(c, [0] * len(ctx), ctx, None)
+    g = planned(c, ctx, new, parent)
+    fill_tokens(c, g, torch.Generator().manual_seed(7), kt)
+    check_attend(c, g, dtype, H)
+    c.h.check(stream=0)
