@@ -475,7 +475,9 @@ typedef struct navi_attend_args {
 /* out = softmax(scale q k) v over the request's ctx_len cached tokens and, of the step's rows, those in
  * the row's mask (parent) or up to the row itself (no parent). q head h reads KV head
  * h / (n_head / n_kv_head). A row that sees no key, and every row of a request that is not
- * served, gets out 0 and lse -inf. */
+ * served, gets out 0 and lse -inf. Infinity or NaN in K or V reaches only the rows that see its token; infinity in a
+ * cached V comes out as infinity or, from f32 rows of more than 8 rows x heads to a KV head, as NaN. The kernel is
+ * chosen by max_new (and max_rows): keep it tight (48 single rows: 86 us with 1, 117 with 16). */
 int navi_pages_attend(navi_pages * p, const navi_step * s, int layer, const navi_attend_args * a, void * stream);
 
 typedef struct navi_commit_args {

@@ -370,7 +370,8 @@ __global__ void __launch_bounds__(288, 1) k_attend_few(const __grid_constant__ A
 #pragma unroll
                         for (int y = 0; y < 2; ++y)
 #pragma unroll
-                            for (int e = 0; e < 2 * XR; ++e) o[2 * dp + y][e] += EIGHT ? c[y][e] + c[y][2 + e] : c[y][e];
+                            for (int e = 0; e < 2 * XR; ++e)   // a value of infinity is in the high terms' sum; the low ones' may be 0 or less
+                                o[2 * dp + y][e] += !EIGHT || !(fabsf(c[y][e]) < INFINITY) ? c[y][e] : c[y][e] + c[y][2 + e];
                     } else {
 #pragma unroll
                         for (int k = 0; k < KS; ++k) {

@@ -511,3 +511,28 @@ def test_attend_pages_of_64(dev, dtype, H, G, D, parent, ctx, new):
     fill_tokens(c, g, torch.Generator().manual_seed(7), kt)
     check_attend(c, g, dtype, H)
     c.h.check(stream=0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("H,D,new", [(4, 128, [1, 2]), (2, 64, [3, 5]), (8, 128, [2, 0])])
+def test_attend_infinite_cached_values_stay_infinite(dev, dtype, H, D, new):
+    """Infinity in a cached V (what an f16 cache makes of a value past its range) in tiles of 8 rows: that infinity in its
+    dim, all else as without it. Scores are small, so that no weight is lost."""
+    tt, code, kt, kcode = TYPES[dtype]
+    ctx = [600, 90]
+    c = Cache(dev, rows=2, blocks=50, G=2, D=D, kt=kt, code=kcode, fill=0)
+    c.k.normal_(generator=torch.Generator("cuda").manual_seed(1))
+    c.v.normal_(generator=torch.Generator("cuda").manual_seed(2))
+    planned(c, [0, 0], ctx, None)
+    g = planned(c, ctx, new)
+    for i, x, dim, what in ((0, 5, 3, math.inf), (0, 130, 7, -math.inf), (0, 300, 40, math.inf), (1, 0, 1, math.inf)):
+        c.v[0][c.t.table[i][x // 16], :, x % 16, dim] = what
+    T = sum(new)
+    q = (torch.randn(T, H, D, generator=torch.Generator().manual_seed(3))).to(tt)
+    qd, out = q.cuda(), torch.zeros(T, H, D, dtype=tt, device="cuda")
+    c.h.attend(g.c, 0, engine.AttendArgs(q=qd.data_ptr(), out=out.data_ptr(), dtype=code, n_head=H, scale=D ** -0.5), stream=0)
+    c.h.check(stream=0)
+    want, _ = op.attend(c.t, g.s, q.double(), c.k[0].cpu().double(), c.v[0].cpu().double(), D ** -0.5)
+    got = out.cpu().double()
+    assert want.isinf().any() and torch.equal(got.isinf(), want.isinf()) and torch.equal(got[got.isinf()], want[want.isinf()])
+    assert not got.isnan().any() and (got - want)[want.isfinite()].abs().max() < 4 * U[dtype] + 2.0 ** -14
