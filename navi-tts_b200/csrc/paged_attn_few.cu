@@ -39,9 +39,9 @@ template <class C> __device__ __forceinline__ void mma(float (&c)[4], const uint
 // a second term there is products of its own (5 rows of two heads over 200,003 bf16 tokens 132 -> 135.5 us, 48 f16
 // trees of up to 8 such rows 99 -> 107), in tiles of 8 none (48 single f16 rows 89.5 -> 87.7 us, without the spills).
 //
-// Measured on one B200: one request of 200,003 tokens, 5 rows, bf16: 129 to 133 us, 6.2 to 6.3 TB/s (a copy
-// reaches 6.54). 48 single rows over pages of 16: 84 us with a page as one box, 92.7 with one for each 64
-// dims. The tile's rows: 48 single rows, KV 255 to 8191, f32: 88 us in tiles of 8, 150 in tiles of 32; 30
+// Measured on one B200: one request of 200,003 tokens, 5 rows, bf16: 129 to 135 us, 6.1 to 6.3 TB/s (a copy
+// reaches 6.54). 48 single f16 rows over pages of 16: 84 to 88 us; with a box for each 64 dims of a page 92.7 where
+// one box took 84.3. The tile's rows: 48 single rows, KV 255 to 8191, f32: 88 us in tiles of 8, 150 in tiles of 32; 30
 // such, KV 255 to 2000, f16: 31 and 39. Four single rows at KV 512 take 11 us, of which the data are 1.3; what
 // is left is launch and one trip to L2 after another: the work list, q and pages, the tile, the join.
 template <class C> constexpr float LIFT = std::is_same_v<C, __half> ? 14.f : 0.f;   // f16 holds 65504

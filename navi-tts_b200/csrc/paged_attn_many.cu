@@ -30,11 +30,12 @@ using namespace navi::umma;
 // rows. Two tiles of q do not fit then, so their items have 128 rows. Bringing each row of q to f16's range costs
 // 4 to 5 % there (48 trees of up to 33 f32 rows 125 -> 132 us, 8 chunks 422 -> 434).
 //
-// Measured on one B200: 8 chunks of 1000 bf16 rows over 511 to 4097 tokens: 211 to 222 us, 680 to 720 TFLOP/s;
+// Measured on one B200: 8 chunks of 1000 bf16 rows over 511 to 4097 tokens: 199 to 224 us, 675 to 760 TFLOP/s;
 // a plain matrix product reaches 1669. 128 rows x 128 keys take about 2000 cycles in the loop, their two products
 // alone 1025 to 1136 in a loop of nothing else. 48 trees of up to 33 f16 rows over 255 to 8191 tokens in pages of
-// 16: 97 to 104 us, 4.4 to 4.7 TB/s. Weights go over in two halves (48 trees 96 us; whole 97). Tried and slower:
-// S in units of 64 keys with two buffers a warpgroup (279 us for the chunks, 210 then: an MMA of 64 columns
+// 16: 98 to 108 us, 4.2 to 4.6 TB/s; counters for both: the tensor pipe 41 and 26 % of the cycles, ex2's pipe 42 and
+// 26 %, so each waits for the other. The f32 variants spill 20 to 28 bytes a thread. Weights go over in two halves
+// (48 trees 96 us; whole 97). Tried and slower: S in units of 64 keys with two buffers a warpgroup (279 us for the chunks, 210 then: an MMA of 64 columns
 // takes as long as one of 128), an MMA warp for each warpgroup (222 us, 204 then).
 // f16: LAZY 1, 2, 3, 5 and 8 with LIFT to match (15 - LAZY): 48 trees 99.8, 99.0, 98.6, 98.1 and 98.0 us, 8 chunks of
 // f16 rows 219, 224, 218, 221 and 216, of f32 rows 431, 429 to 435, 417, 429 and 436 (410 to 419 without LIFT): the

@@ -96,7 +96,7 @@ __device__ __forceinline__ int owner(const int * a, int n, int e) {
 // one that this very call gives back; it is read where it still stands, in its owner's table
 // row, whose entries past the need nobody writes. What bounds it is a chain of trips to L2: one for the
 // inputs (asked for together, the parents of the block's rows with them), one for the pages, one to count
-// the blocks. A plan and the plan that undoes it, launched in a row: 9 us for four single rows, 12 for 64
+// the blocks. A plan and the plan that undoes it, launched in a row: 9 to 11 us for four single rows, 12 for 64
 // trees of up to 61 rows (899 in all), 18 for a thousand prompts (218,522 rows).
 // Args: PlanArgs, or PlanLimited for a talker's step.
 template <class Args> __global__ void __launch_bounds__(PLAN_THREADS) k_pages_plan(const __grid_constant__ Args a) {
@@ -484,7 +484,7 @@ constexpr int COMMIT_THREADS = 256;
 // The k-th accepted row is row path[k] >= k, so a thread that owns 16 bytes of a token's row and
 // goes through the path in order never writes a place that a later step still has to read. Bound by the walk's
 // trips to L2 (parents, ids, choices, slots) and then by the moves: four trees 7 us, as long as a launch;
-// 64 trees through 28 layers 10.6 to 11.8 us, 3.5 to 3.9 TB/s. 16 bytes at a time with four moves ahead took
+// 64 trees through 28 layers 10.6 to 12.4 us, 3.3 to 3.9 TB/s. 16 bytes at a time with four moves ahead took
 // it from 29 to 17.0 us, twice the blocks (8 for 4 times the multiprocessors) to 11.5; 16 times takes 12.1.
 // IN_PLACE: next_token is root_target.
 template <bool IN_PLACE> __global__ void __launch_bounds__(COMMIT_THREADS) k_pages_commit(const __grid_constant__ CommitArgs a) {
